@@ -33,7 +33,7 @@ extern "C" {
 #endif
 
 /* Element types of tensors crossing this ABI. */
-enum omni_b200_dtype { OMNI_B200_F32 = 0, OMNI_B200_BF16 = 1, OMNI_B200_F16 = 2 };
+enum omni_b200_dtype { OMNI_B200_F32 = 0, OMNI_B200_BF16 = 1, OMNI_B200_F16 = 2, OMNI_B200_E4M3 = 3 };
 
 OMNI_B200_API const char *omni_b200_last_error(void);
 OMNI_B200_API const char *omni_b200_version(void);
@@ -163,6 +163,52 @@ OMNI_B200_API int omni_b200_vq_argmin_noalloc(const void *x, const void *codeboo
                                               const void *cbnorm, void *ids, size_t rows,
                                               size_t dim, size_t codes, int profile,
                                               int ids_u16, void *stream);
+
+/* ---- 8-bit transformer layers --------------------------------------------
+ * No counterpart in the reference (its layers run in fp32 or bf16).
+ *
+ * e4m3 tensors carry fp32 scales, one for each group of 128 columns (of a
+ * weight: each block of 128 rows x 128 columns; the last group or block may be
+ * smaller).  With amax the largest magnitude of a group, NaN left out,
+ *   scale = max(amax / 448, 2^-126),   q = e4m3(x * (1 / scale)),
+ * rounded to nearest even; q * scale stands for x.  A NaN becomes e4m3's NaN;
+ * a group that holds an infinity gets an infinite scale and stands for NaN.
+ * Strides count elements of the tensor they belong to; columns are contiguous.
+ * rows == 0 (m == 0) does nothing.
+ *
+ * omni_b200_rms_norm: per row of x [rows, cols],
+ *   h = x + residual (or x),   out = h / sqrt(mean(h^2) + eps) * weight,
+ * all in fp32.  residual != NULL also needs residual_out, which receives h
+ * rounded to dtype; residual_out may be the same tensor as x or residual, and
+ * out (of dtype) the same as any of them, with that tensor's stride; other
+ * overlaps are not allowed.  dtype F32, BF16 or F16 is the type of x, residual,
+ * weight [cols] and residual_out.  out_dtype is dtype, with scales NULL, or
+ * E4M3, with scales [rows, ceil(cols / 128)].  cols <= 2^24.
+ *
+ * omni_b200_quantize_e4m3: x [rows, cols] to q and scales.  block_rows 1: scales
+ * [rows, ceil(cols / 128)]; block_rows 128 (weights): scales
+ * [ceil(rows / 128), ceil(cols / 128)], rows <= 8388480. */
+OMNI_B200_API int omni_b200_rms_norm(const void *x, const void *residual, const void *weight,
+                                     void *residual_out, void *out, float *scales, size_t rows,
+                                     size_t cols, size_t x_stride, size_t residual_stride,
+                                     size_t residual_out_stride, size_t out_stride, float eps,
+                                     int dtype, int out_dtype, void *stream);
+OMNI_B200_API int omni_b200_quantize_e4m3(const void *x, void *q, float *scales, size_t rows,
+                                          size_t cols, size_t x_stride, size_t q_stride,
+                                          int block_rows, int dtype, void *stream);
+
+/* out[m, n] = sum over groups g of a_scales[m, g] * w_scales[n / 128, g] *
+ *             (sum over the k of g of a[m, k] * w[n, k])   (+ bias[n])
+ * a [m, k] and w [n, k] are e4m3 as above (a in groups of 128 columns, w in 128
+ * x 128 blocks), 16-byte aligned with row strides lda and ldw >= k that are
+ * multiples of 16.  The sums are fp32, rounded once to out_dtype (F32, BF16 or
+ * F16) [m, n] with row stride ldo; bias (NULL: none) is [n] of out_dtype.  k is
+ * at most 2^24, n at most 2^22.  out overlaps no input.  No workspace; the
+ * same call gives the same bits. */
+OMNI_B200_API int omni_b200_linear_e4m3(const void *a, const float *a_scales, const void *w,
+                                        const float *w_scales, const void *bias, void *out,
+                                        size_t m, size_t n, size_t k, size_t lda, size_t ldw,
+                                        size_t ldo, int out_dtype, void *stream);
 
 /* ---- Diagnostics (failure detection without a GPU fault) ----------------
  * Every pipeline wait in this library's kernels is bounded: a wait that has

@@ -1,0 +1,84 @@
+// e4m3.cuh -- element conversions shared by the 8-bit layer kernels.
+//
+// Quantisation of a group with largest magnitude amax:
+//   scale = max(amax / 448, 2^-126),  q = e4m3(x * (1 / scale)),
+// so x ~ q * scale.  448 is e4m3's largest value.  The floor 2^-126 keeps
+// 1 / scale finite for a group of zeros (whose q are zeros).  A NaN does not
+// take part in amax and becomes e4m3's NaN; an infinity makes the scale
+// infinite, and the group then stands for NaN.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace omni_b200 {
+
+constexpr int kGroup = 128; // columns (of weights: columns and rows) that share a scale
+constexpr float kE4m3Max = 448.f;
+constexpr float kMinScale = 1.17549435e-38f; // 2^-126
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// Eight consecutive elements as they lie in memory (16 bytes of a 2-byte type,
+// 32 of fp32), and as fp32.
+template <typename T> struct Vec8 {
+    uint4 w[sizeof(T) / 2];
+};
+template <typename T> __device__ __forceinline__ Vec8<T> load8(const T *p) {
+    Vec8<T> v;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+        v.w[i] = reinterpret_cast<const uint4 *>(p)[i];
+    return v;
+}
+template <typename T> __device__ __forceinline__ void store8(T *p, const Vec8<T> &v) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+        reinterpret_cast<uint4 *>(p)[i] = v.w[i];
+}
+template <typename T> __device__ __forceinline__ void unpack8(const Vec8<T> &v, float (&f)[8]) {
+    const T *e = reinterpret_cast<const T *>(v.w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        f[i] = to_float(e[i]);
+}
+template <typename T> __device__ __forceinline__ Vec8<T> pack8(const float (&f)[8]) {
+    Vec8<T> v;
+    T *e = reinterpret_cast<T *>(v.w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        e[i] = from_float<T>(f[i]);
+    return v;
+}
+
+// Two e4m3 values in 16 bits, `lo` in the low byte (round to nearest even,
+// beyond 448 to 448, NaN to NaN).
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint2 e4m3x8(const float (&f)[8], float inv) {
+    uint2 r;
+    r.x = e4m3x2(f[0] * inv, f[1] * inv) | (e4m3x2(f[2] * inv, f[3] * inv) << 16);
+    r.y = e4m3x2(f[4] * inv, f[5] * inv) | (e4m3x2(f[6] * inv, f[7] * inv) << 16);
+    return r;
+}
+__device__ __forceinline__ float amax8(const float (&f)[8]) {
+    const float a = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
+    const float b = fmaxf(fmaxf(fabsf(f[4]), fabsf(f[5])), fmaxf(fabsf(f[6]), fabsf(f[7])));
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float group_scale(float amax) {
+    return fmaxf(__fdiv_rn(amax, kE4m3Max), kMinScale);
+}
+
+} // namespace omni_b200

@@ -1,0 +1,354 @@
+// rms_norm.cu -- root-mean-square norm with the residual's addition, and the
+// quantisation to e4m3 with a scale for each 128 columns (rows) or each 128 x
+// 128 block (weights).
+//
+// Per row, in fp32 (inputs are widened, the sum is not rounded before the norm
+// reads it):
+//   h = x + residual,  y = h * rsqrt(mean(h^2) + eps) * weight,
+// residual_out = h and out = y, each rounded once to the element type, or out =
+// the groups of e4m3.cuh.  A row is read once: its elements stay in registers
+// between the sum of squares and the scaling (vector kernel), so the bound is
+// the memory traffic of the inputs and outputs.
+//
+// rows_kernel: TPR threads own a row, 8 consecutive elements each per step
+// (16-byte loads of 2-byte types), VPT steps.  A group of 128 columns is then
+// 16 neighbouring lanes, so its largest magnitude takes four shuffles and no
+// shared memory.  The grid is persistent: the weight is read once per CTA.
+// rows_scalar_kernel serves columns and pitches that 16-byte loads cannot, and
+// rows wider than the registers hold; it reads its row twice (the second time
+// from L2).
+#include "e4m3.cuh"
+#include "layer.h"
+
+#include <algorithm>
+
+namespace omni_b200 {
+namespace {
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+// Over the 16 lanes of a half warp.
+__device__ __forceinline__ float half_warp_max(float v) {
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1)
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+    return v;
+}
+
+template <typename T, bool NORM, bool QUANT, int TPR, int VPT, int ROWS>
+__global__ void __launch_bounds__(TPR *ROWS) rows_kernel(const RowsArgs a) {
+    constexpr int WARPS = TPR / 32; // warps of a row
+    __shared__ float part[2][WARPS];
+    static_assert(ROWS == 1 || TPR == 32, "a row of one warp, or a CTA for each row");
+    const int t = threadIdx.x % TPR;
+    const T *x = static_cast<const T *>(a.x), *res = static_cast<const T *>(a.residual);
+    T *res_out = static_cast<T *>(a.residual_out);
+    const int groups = (a.cols + kGroup - 1) / kGroup;
+    Vec8<T> w[NORM ? VPT : 1];
+    if constexpr (NORM) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * TPR + t) * 8;
+            if (c < a.cols)
+                w[i] = load8(static_cast<const T *>(a.weight) + c);
+        }
+    }
+    int turn = 0;
+    const long long step = static_cast<long long>(gridDim.x) * ROWS;
+    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / TPR; row < a.rows; row += step) {
+        float h[VPT][8];
+        {
+            Vec8<T> xv[VPT], rv[NORM ? VPT : 1];
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int c = (i * TPR + t) * 8;
+                if (c < a.cols) {
+                    xv[i] = load8(x + row * a.x_stride + c);
+                    if (NORM && res)
+                        rv[NORM ? i : 0] = load8(res + row * a.residual_stride + c);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int c = (i * TPR + t) * 8;
+                if (c < a.cols) {
+                    unpack8(xv[i], h[i]);
+                    if (NORM && res) {
+                        float r[8];
+                        unpack8(rv[NORM ? i : 0], r);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            h[i][e] += r[e];
+                        store8(res_out + row * a.residual_out_stride + c, pack8<T>(h[i]));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        h[i][e] = 0.f;
+                }
+            }
+        }
+        if constexpr (NORM) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    sum = fmaf(h[i][e], h[i][e], sum);
+            sum = warp_sum(sum);
+            if constexpr (WARPS > 1) {
+                // Two buffers: a warp may write the next row's part while
+                // another still reads this row's.
+                if (t % 32 == 0)
+                    part[turn][t / 32] = sum;
+                __syncthreads();
+                sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < WARPS; ++k)
+                    sum += part[turn][k];
+                turn ^= 1;
+            }
+            const float rstd = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int c = (i * TPR + t) * 8;
+                if (c < a.cols) {
+                    float wf[8];
+                    unpack8(w[i], wf);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        h[i][e] = h[i][e] * rstd * wf[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * TPR + t) * 8;
+            if constexpr (QUANT) {
+                const float scale = group_scale(half_warp_max(amax8(h[i])));
+                if (c < a.cols) {
+                    uint8_t *q = static_cast<uint8_t *>(a.out) + row * a.out_stride + c;
+                    *reinterpret_cast<uint2 *>(q) = e4m3x8(h[i], __frcp_rn(scale));
+                    if (t % 16 == 0)
+                        a.scales[row * groups + c / kGroup] = scale;
+                }
+            } else if (c < a.cols) {
+                store8(static_cast<T *>(a.out) + row * a.out_stride + c, pack8<T>(h[i]));
+            }
+        }
+    }
+}
+
+// One CTA per row; a warp takes a group of 128 columns, four elements a lane.
+// Each element is written by the thread that read it last, so that an output
+// may be the same tensor as x or the residual.
+template <typename T, bool NORM, bool QUANT>
+__global__ void __launch_bounds__(256) rows_scalar_kernel(const RowsArgs a) {
+    __shared__ float part[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int groups = (a.cols + kGroup - 1) / kGroup;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+        const T *res = NORM && a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
+        float rstd = 1.f;
+        if constexpr (NORM) {
+            float sum = 0.f;
+            for (int c = threadIdx.x; c < a.cols; c += 256) {
+                const float h = to_float(x[c]) + (res ? to_float(res[c]) : 0.f);
+                sum = fmaf(h, h, sum);
+            }
+            sum = warp_sum(sum);
+            if (lane == 0)
+                part[warp] = sum;
+            __syncthreads();
+            sum = 0.f;
+            for (int k = 0; k < 8; ++k)
+                sum += part[k];
+            __syncthreads(); // before the next row's parts, and before a row that is written in place
+            rstd = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
+        }
+        for (int g = warp; g < groups; g += 8) {
+            float y[4], amax = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = g * kGroup + e * 32 + lane;
+                y[e] = 0.f;
+                if (c < a.cols) {
+                    y[e] = to_float(x[c]);
+                    if constexpr (NORM) {
+                        if (res) {
+                            y[e] += to_float(res[c]);
+                            static_cast<T *>(a.residual_out)[row * a.residual_out_stride + c] = from_float<T>(y[e]);
+                        }
+                        y[e] = y[e] * rstd * to_float(static_cast<const T *>(a.weight)[c]);
+                    }
+                }
+                amax = fmaxf(amax, fabsf(y[e]));
+            }
+            float scale = 1.f, inv = 1.f;
+            if constexpr (QUANT) {
+                amax = half_warp_max(amax);
+                scale = group_scale(fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16)));
+                inv = __frcp_rn(scale);
+                if (lane == 0)
+                    a.scales[row * groups + g] = scale;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = g * kGroup + e * 32 + lane;
+                if (c >= a.cols)
+                    continue;
+                if constexpr (QUANT)
+                    static_cast<uint8_t *>(a.out)[row * a.out_stride + c] = static_cast<uint8_t>(e4m3x2(y[e] * inv, 0.f));
+                else
+                    static_cast<T *>(a.out)[row * a.out_stride + c] = from_float<T>(y[e]);
+            }
+        }
+    }
+}
+
+// One CTA per 128 x 128 block: thread = 8 columns of every 16th row, its 64
+// elements in registers between the largest magnitude and the conversion.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) quantize_blocks_kernel(const T *x, uint8_t *q, float *scales, long long rows,
+                                                              int cols, long long x_stride, long long q_stride) {
+    __shared__ float part[8];
+    const int c = blockIdx.x * kGroup + (threadIdx.x % 16) * 8;
+    const long long r0 = static_cast<long long>(blockIdx.y) * kGroup + threadIdx.x / 16;
+    float f[8][8], amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long r = r0 + i * 16;
+        if (VEC && r < rows && c < cols) {
+            unpack8(load8(x + r * x_stride + c), f[i]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                f[i][e] = !VEC && r < rows && c + e < cols ? to_float(x[r * x_stride + c + e]) : 0.f;
+        }
+        amax = fmaxf(amax, amax8(f[i]));
+    }
+    amax = half_warp_max(amax);
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
+    if (threadIdx.x % 32 == 0)
+        part[threadIdx.x / 32] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        amax = fmaxf(amax, part[k]);
+    const float scale = group_scale(amax), inv = __frcp_rn(scale);
+    if (threadIdx.x == 0)
+        scales[static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x] = scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long r = r0 + i * 16;
+        if (r >= rows || c >= cols)
+            continue;
+        uint8_t *to = q + r * q_stride + c;
+        const uint2 v = e4m3x8(f[i], inv);
+        if constexpr (VEC) {
+            *reinterpret_cast<uint2 *>(to) = v;
+        } else {
+            for (int e = 0; e < 8 && c + e < cols; ++e)
+                to[e] = static_cast<uint8_t>((e < 4 ? v.x >> (8 * e) : v.y >> (8 * (e - 4))) & 0xffu);
+        }
+    }
+}
+
+int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
+        n = 148;
+    return n;
+}
+
+template <typename T, bool NORM, bool QUANT, int TPR, int VPT, int ROWS>
+int launch_rows(const RowsArgs &a, cudaStream_t stream) {
+    // Up to 2048 threads an SM; what the registers do not hold at once waits.
+    const long long ctas = (a.rows + ROWS - 1) / ROWS;
+    const long long most = static_cast<long long>(sm_count()) * (2048 / (TPR * ROWS));
+    rows_kernel<T, NORM, QUANT, TPR, VPT, ROWS>
+        <<<static_cast<unsigned>(std::min(ctas, most)), TPR * ROWS, 0, stream>>>(a);
+    return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T, bool NORM, bool QUANT> int launch_typed(const RowsArgs &a, cudaStream_t stream) {
+    constexpr int kAlign = 16 / sizeof(T); // elements of 16 bytes
+    const uintptr_t base = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.residual) |
+                           reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.residual_out);
+    const uintptr_t out = reinterpret_cast<uintptr_t>(a.out);
+    const bool vec = base % 16 == 0 && a.cols % 8 == 0 && a.x_stride % kAlign == 0 &&
+                     (!a.residual || (a.residual_stride % kAlign == 0 && a.residual_out_stride % kAlign == 0)) &&
+                     (QUANT ? out % 8 == 0 && a.out_stride % 8 == 0 : out % 16 == 0 && a.out_stride % kAlign == 0);
+    const int vecs = a.cols / 8;
+    if (!vec || vecs > 2048) {
+        const unsigned grid = static_cast<unsigned>(std::min<long long>(a.rows, 8ll * sm_count()));
+        rows_scalar_kernel<T, NORM, QUANT><<<grid, 256, 0, stream>>>(a);
+        return static_cast<int>(cudaGetLastError());
+    }
+    if (vecs <= 32)
+        return launch_rows<T, NORM, QUANT, 32, 1, 4>(a, stream);
+    if (vecs <= 64)
+        return launch_rows<T, NORM, QUANT, 32, 2, 4>(a, stream);
+    if (vecs <= 128)
+        return launch_rows<T, NORM, QUANT, 32, 4, 4>(a, stream);
+    if (vecs <= 256)
+        return launch_rows<T, NORM, QUANT, 128, 2, 1>(a, stream);
+    if (vecs <= 512)
+        return launch_rows<T, NORM, QUANT, 128, 4, 1>(a, stream);
+    if (vecs <= 1024)
+        return launch_rows<T, NORM, QUANT, 256, 4, 1>(a, stream);
+    return launch_rows<T, NORM, QUANT, 512, 4, 1>(a, stream);
+}
+
+template <typename T> int launch_dtype(const RowsArgs &a, cudaStream_t stream) {
+    if (!a.norm)
+        return launch_typed<T, false, true>(a, stream);
+    return a.quantize ? launch_typed<T, true, true>(a, stream) : launch_typed<T, true, false>(a, stream);
+}
+
+template <typename T>
+int launch_blocks(const T *x, uint8_t *q, float *scales, long long rows, int cols, long long x_stride,
+                  long long q_stride, cudaStream_t stream) {
+    const dim3 grid((cols + kGroup - 1) / kGroup, static_cast<unsigned>((rows + kGroup - 1) / kGroup));
+    const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 &&
+                     cols % 8 == 0 && x_stride % (16 / static_cast<int>(sizeof(T))) == 0 && q_stride % 8 == 0;
+    if (vec)
+        quantize_blocks_kernel<T, true><<<grid, 256, 0, stream>>>(x, q, scales, rows, cols, x_stride, q_stride);
+    else
+        quantize_blocks_kernel<T, false><<<grid, 256, 0, stream>>>(x, q, scales, rows, cols, x_stride, q_stride);
+    return static_cast<int>(cudaGetLastError());
+}
+
+} // namespace
+
+int rows_launch(const RowsArgs &a, cudaStream_t stream) {
+    switch (a.dtype) {
+    case kF32:
+        return launch_dtype<float>(a, stream);
+    case kBF16:
+        return launch_dtype<__nv_bfloat16>(a, stream);
+    default:
+        return launch_dtype<__half>(a, stream);
+    }
+}
+
+int quantize_blocks_launch(const void *x, void *q, float *scales, long long rows, int cols, long long x_stride,
+                           long long q_stride, int dtype, cudaStream_t stream) {
+    uint8_t *to = static_cast<uint8_t *>(q);
+    switch (dtype) {
+    case kF32:
+        return launch_blocks(static_cast<const float *>(x), to, scales, rows, cols, x_stride, q_stride, stream);
+    case kBF16:
+        return launch_blocks(static_cast<const __nv_bfloat16 *>(x), to, scales, rows, cols, x_stride, q_stride, stream);
+    default:
+        return launch_blocks(static_cast<const __half *>(x), to, scales, rows, cols, x_stride, q_stride, stream);
+    }
+}
+
+} // namespace omni_b200

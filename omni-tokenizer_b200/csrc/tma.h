@@ -24,4 +24,8 @@ int make_map_2d(CUtensorMap *map, const void *base, int cols, long long rows, in
 // (box_w * 4 bytes = 32, 64 or 128 selects the swizzle).
 int make_map_2d_f32(CUtensorMap *map, const void *base, int cols, long long rows, int box_w,
                     int box_rows);
+// Row-major matrix of 1-, 2- or 4-byte elements (type: its tensor-map type) with
+// rows `pitch` bytes apart; 128-byte swizzle, box of box_w columns x box_rows rows.
+int make_map_pitched(CUtensorMap *map, const void *base, CUtensorMapDataType type, int elem_bytes, long long cols,
+                     long long rows, long long pitch, int box_w, int box_rows);
 } // namespace omni_b200

@@ -15,7 +15,7 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, E4M3 = 0, 1, 2, 3
 
 # omni_status (include/omni/omni.h)
 OK, INVALID_ARGUMENT, IO_ERROR, INVALID_MODEL, UNSUPPORTED, OUT_OF_MEMORY, CANCELLED, INTERNAL_ERROR = range(8)
@@ -52,6 +52,18 @@ SIGNATURES = {
          C.c_int, _P, C.c_size_t, _P],
     ),
     "omni_b200_gelu": (C.c_int, [_P, C.c_size_t, C.c_int, _P]),
+    "omni_b200_rms_norm": (
+        C.c_int,
+        [_P, _P, _P, _P, _P, _P, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_float,
+         C.c_int, C.c_int, _P],
+    ),
+    "omni_b200_quantize_e4m3": (
+        C.c_int, [_P, _P, _P, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_int, C.c_int, _P],
+    ),
+    "omni_b200_linear_e4m3": (
+        C.c_int,
+        [_P, _P, _P, _P, _P, _P, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_int, _P],
+    ),
     "omni_b200_squares": (C.c_int, [_P, _P, C.c_size_t, C.c_size_t, C.c_int, C.c_int, _P]),
     "omni_b200_vq_argmin": (
         C.c_int,
@@ -235,3 +247,161 @@ def attention_rows(q, k, v, heads, block=0, valid=None, fused=False, out_dtype=N
             batch, heads, hd, block, valid, None if lengths is None else lengths.data_ptr(), int(fused),
             _dtype_code(q), _dtype_code(out), ws.data_ptr(), ws_bytes, _stream_ptr(stream)))
     return out
+
+
+# -------------------------------------------------------- 8-bit layer operators
+def _refuse(message):
+    raise NativeError(INVALID_ARGUMENT, message)
+
+
+def _element_code(what, t):
+    """Type code of a 2-d tensor of one of the element types."""
+    import torch
+
+    if t.dim() != 2 or t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        _refuse(f"{what}: need a [rows, cols] tensor of float32, bfloat16 or float16")
+    return _dtype_code(t)
+
+
+def _checked(what, tensors, like):
+    """Every tensor on like's device and with contiguous columns."""
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda or t.device != like.device:
+            _refuse(f"{what}: every tensor must be on the same CUDA device")
+        if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+            _refuse(f"{what}: columns must be contiguous")
+
+
+def _row_stride(t):
+    """Elements between rows; a single row's stride does not matter."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _call(name, device, stream, *args):
+    """Calls an entry point on `device` and its current stream (or `stream`)."""
+    import torch
+
+    lib = library()
+    if device.index == torch.cuda.current_device():
+        s = stream if stream is not None else torch.cuda.current_stream()
+        lib.check(getattr(lib.lib, name)(*args, s.cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            s = stream if stream is not None else torch.cuda.current_stream()
+            lib.check(getattr(lib.lib, name)(*args, s.cuda_stream))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _empty_e4m3(rows, cols, device):
+    """[rows, cols] of e4m3 whose row stride is a multiple of 16, as linear_e4m3 reads it."""
+    import torch
+
+    if cols % 16 == 0:
+        return torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=device)
+    return torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=device)[:, :cols]
+
+
+def _norm(what, x, weight, residual, residual_out, out, scales, eps, out_dtype, stream):
+    import torch
+
+    rows, cols = x.shape
+    if weight.shape != (cols,) or weight.dtype != x.dtype:
+        _refuse(f"{what}: weight must be [{cols}] of x's type")
+    if residual is None:
+        if residual_out is not None:
+            _refuse(f"{what}: residual_out needs a residual")
+    else:
+        if residual_out is None:
+            residual_out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        for t in (residual, residual_out):
+            if t.shape != x.shape or t.dtype != x.dtype:
+                _refuse(f"{what}: residual and residual_out must have x's shape and type")
+    _checked(what, (x, weight, residual, residual_out, out, scales), x)
+    _call("omni_b200_rms_norm", x.device, stream, x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(residual_out),
+          out.data_ptr(), _ptr(scales), rows, cols, _row_stride(x), 0 if residual is None else _row_stride(residual),
+          0 if residual is None else _row_stride(residual_out), _row_stride(out), eps, _dtype_code(x), out_dtype)
+    return residual_out
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None, stream=None):
+    """Root-mean-square norm of the rows of x [rows, cols] (+ residual).
+
+    Returns (y, h): y = h / sqrt(mean(h^2) + eps) * weight in x's type, h = x + residual
+    (None without a residual).  residual_out may be x or residual, out any of them."""
+    import torch
+
+    code = _element_code("rms_norm", x)
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    elif out.shape != x.shape or out.dtype != x.dtype:
+        _refuse("rms_norm: out must have x's shape and type")
+    return out, _norm("rms_norm", x, weight, residual, residual_out, out, None, eps, code, stream)
+
+
+def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, residual_out=None, stream=None):
+    """rms_norm with its output in e4m3 and an fp32 scale for each 128 columns.
+
+    Returns (q, scales, h); q and scales are what linear_e4m3 takes."""
+    import torch
+
+    _element_code("rms_norm_e4m3", x)
+    q = _empty_e4m3(*x.shape, x.device)
+    scales = torch.empty((x.shape[0], (x.shape[1] + 127) // 128), dtype=torch.float32, device=x.device)
+    return q, scales, _norm("rms_norm_e4m3", x, weight, residual, residual_out, q, scales, eps, E4M3, stream)
+
+
+def quantize_e4m3(x, block_rows=1, stream=None):
+    """x [rows, cols] in e4m3: (q, scales), a scale for each 128 columns of a row
+    (block_rows=1) or each 128 x 128 block (block_rows=128, weights)."""
+    import torch
+
+    code = _element_code("quantize_e4m3", x)
+    rows, cols = x.shape
+    if block_rows not in (1, 128):
+        _refuse("quantize_e4m3: block_rows must be 1 or 128")
+    _checked("quantize_e4m3", (x,), x)
+    q = _empty_e4m3(rows, cols, x.device)
+    scales = torch.empty(((rows + block_rows - 1) // block_rows, (cols + 127) // 128), dtype=torch.float32,
+                         device=x.device)
+    _call("omni_b200_quantize_e4m3", x.device, stream, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols,
+          _row_stride(x), _row_stride(q), block_rows, code)
+    return q, scales
+
+
+def linear_e4m3(a, a_scales, w, w_scales, bias=None, out_dtype=None, out=None, stream=None):
+    """a [m, k] times w [n, k] transposed, both e4m3 with scales (quantize_e4m3 with
+    block_rows 1 and 128), plus bias [n]: [m, n] of out_dtype (bfloat16)."""
+    import torch
+
+    if a.dim() != 2 or w.dim() != 2:
+        _refuse("linear_e4m3: a and w must be matrices")
+    (m, k), n = a.shape, w.shape[0]
+    if a.dtype != torch.float8_e4m3fn or w.dtype != torch.float8_e4m3fn or w.shape != (n, k):
+        _refuse("linear_e4m3: a [m, k] and w [n, k] must be float8_e4m3fn")
+    groups = (k + 127) // 128
+    for t, rows in ((a_scales, m), (w_scales, (n + 127) // 128)):
+        if t.dtype != torch.float32 or t.shape != (rows, groups) or not t.is_contiguous():
+            _refuse(f"linear_e4m3: scales must be contiguous float32 [{rows}, {groups}]")
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype or torch.bfloat16, device=a.device)
+    elif out.shape != (m, n) or (out_dtype is not None and out.dtype != out_dtype):
+        _refuse("linear_e4m3: out must be [m, n] of out_dtype")
+    if out.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        _refuse("linear_e4m3: out must be float32, bfloat16 or float16")
+    if bias is not None and (bias.shape != (n,) or bias.dtype != out.dtype):
+        _refuse(f"linear_e4m3: bias must be [{n}] of the output's type")
+    _checked("linear_e4m3", (a, a_scales, w, w_scales, bias, out), a)
+    _call("omni_b200_linear_e4m3", a.device, stream, a.data_ptr(), a_scales.data_ptr(), w.data_ptr(),
+          w_scales.data_ptr(), _ptr(bias), out.data_ptr(), m, n, k, _pitch(a, 16), _pitch(w, 16), _row_stride(out),
+          _dtype_code(out))
+    return out
+
+
+def _pitch(t, multiple):
+    """Row stride of a matrix; a single row counts as one padded to `multiple`."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + multiple - 1) // multiple * multiple

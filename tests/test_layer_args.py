@@ -1,0 +1,105 @@
+"""Refusals of the 8-bit layer entry points, which answer before they touch a
+device: bad arguments are refused on a machine without one."""
+
+import ctypes as C
+
+import pytest
+
+from tests.conftest import load_package
+
+ob = load_package()
+E4M3, BF16, F32, F16 = 3, 1, 0, 2
+# Addresses that nothing reads: a refused call launches nothing.
+X, R, W, H, O, S = (0x10000 * i for i in range(1, 7))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    path = ob.native.PKG / "libomni_b200.so"
+    if not path.is_file():
+        pytest.skip("library not built")
+    return ob.library().lib
+
+
+def _norm(lib, **k):
+    a = dict(x=X, residual=R, weight=W, residual_out=H, out=O, scales=None, rows=4, cols=256, xs=256, rs=256, hs=256,
+             os=256, eps=1e-6, dtype=BF16, out_dtype=BF16)
+    a.update(k)
+    return lib.omni_b200_rms_norm(*a.values(), None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(x=None), dict(weight=None), dict(out=None), dict(residual=None), dict(residual_out=None), dict(dtype=E4M3),
+    dict(dtype=-1), dict(out_dtype=F32), dict(out_dtype=E4M3), dict(scales=S), dict(cols=0), dict(cols=(1 << 24) + 1),
+    dict(xs=255), dict(rs=255), dict(hs=0), dict(os=100), dict(xs=(1 << 40) + 8), dict(eps=-1.0),
+    dict(eps=float("nan")), dict(eps=float("inf")), dict(x=X + 1), dict(out=O + 1), dict(weight=W + 1),
+    dict(out_dtype=E4M3, scales=S + 2), dict(rows=(1 << 40) + 1),
+])
+def test_rms_norm_refuses(lib, bad):
+    assert _norm(lib, **bad) == 1
+    assert b"rms_norm" in lib.omni_b200_last_error()
+
+
+@pytest.mark.parametrize("bad", [
+    dict(x=None), dict(q=None), dict(scales=None), dict(dtype=E4M3), dict(cols=0), dict(block=64), dict(block=0),
+    dict(xs=100), dict(qs=255), dict(x=X + 1), dict(scales=S + 1), dict(rows=8388481, block=128),
+])
+def test_quantize_refuses(lib, bad):
+    a = dict(x=X, q=O, scales=S, rows=4, cols=256, xs=256, qs=256, block=1, dtype=BF16)
+    a.update(bad)
+    assert lib.omni_b200_quantize_e4m3(*a.values(), None) == 1
+    assert b"quantize_e4m3" in lib.omni_b200_last_error()
+
+
+@pytest.mark.parametrize("status,bad", [
+    (1, dict(a=None)), (1, dict(sa=None)), (1, dict(w=None)), (1, dict(sw=None)), (1, dict(out=None)),
+    (1, dict(n=0)), (1, dict(k=0)), (1, dict(lda=255)), (1, dict(lda=264)), (1, dict(ldw=240)), (1, dict(ldw=257)),
+    (1, dict(ldo=127)), (1, dict(a=X + 8)), (1, dict(w=W + 4)), (1, dict(out=O + 1)), (1, dict(bias=R + 1)),
+    (1, dict(sa=S + 2)), (1, dict(dtype=E4M3)), (1, dict(n=(1 << 22) + 1, ldo=1 << 23)),
+    (1, dict(m=(1 << 30) + 1)), (4, dict(m=1 << 30, n=1 << 22, ldo=1 << 22)),
+])
+def test_linear_refuses(lib, status, bad):
+    a = dict(a=X, sa=S, w=W, sw=H, bias=None, out=O, m=4, n=128, k=256, lda=256, ldw=256, ldo=128, dtype=BF16)
+    a.update(bad)
+    assert lib.omni_b200_linear_e4m3(*a.values(), None) == status
+    assert b"linear_e4m3" in lib.omni_b200_last_error()
+
+
+def test_no_rows_is_no_work(lib):
+    """Without rows nothing is launched and no pointer is looked at."""
+    assert _norm(lib, rows=0, x=None, out=None, weight=None, residual=None, residual_out=None) == 0
+    assert lib.omni_b200_quantize_e4m3(None, None, None, 0, 128, 128, 128, 1, BF16, None) == 0
+    assert lib.omni_b200_linear_e4m3(None, None, None, None, None, None, 0, 8, 16, 16, 16, 8, BF16, None) == 0
+
+
+def test_helpers_refuse():
+    torch = pytest.importorskip("torch")
+    x, w = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(256, dtype=torch.bfloat16)
+    refused = pytest.raises(ob.NativeError)
+    for call in (lambda: ob.rms_norm(x, w), lambda: ob.rms_norm_e4m3(x, w), lambda: ob.quantize_e4m3(x)):
+        with refused as e:  # tensors of the host
+            call()
+        assert e.value.status == 1
+    q, s = torch.zeros(4, 256).to(torch.float8_e4m3fn), torch.zeros(4, 2)
+    for call in (
+        lambda: ob.rms_norm(x, w.float()),
+        lambda: ob.rms_norm(x, w[:128]),
+        lambda: ob.rms_norm(x, w, residual=x[:2]),
+        lambda: ob.rms_norm(x, w, residual=x.float()),
+        lambda: ob.rms_norm(x, w, residual_out=x),
+        lambda: ob.rms_norm(x, w, out=x.float()),
+        lambda: ob.rms_norm(x.int(), w.int()),
+        lambda: ob.quantize_e4m3(x, block_rows=32),
+        lambda: ob.quantize_e4m3(x.double()),
+        lambda: ob.linear_e4m3(x, s, q, s[:1]),
+        lambda: ob.linear_e4m3(q, s, q[:, :128], s[:1]),
+        lambda: ob.linear_e4m3(q, s[:3], q, s[:1]),
+        lambda: ob.linear_e4m3(q, s.double(), q, s[:1]),
+        lambda: ob.linear_e4m3(q, s, q, s[:1], bias=w),
+        lambda: ob.linear_e4m3(q, s, q, s[:1], out=x),
+        lambda: ob.linear_e4m3(q, s, q, s[:1], out_dtype=torch.float64),
+        lambda: ob.linear_e4m3(q, s, q, s[:1]),
+    ):
+        with refused as e:
+            call()
+        assert e.value.status == 1
