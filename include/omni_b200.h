@@ -210,6 +210,32 @@ OMNI_B200_API int omni_b200_linear_e4m3(const void *a, const float *a_scales, co
                                         size_t m, size_t n, size_t k, size_t lda, size_t ldw,
                                         size_t ldo, int out_dtype, void *stream);
 
+/* Sliding-window attention with first tokens that stay visible, grouped heads
+ * and keys that outnumber the queries (prompts, encoders, the next tokens of a
+ * sequence against its cache).  q and out are [batch, heads, q_len, head_dim], k
+ * and v [batch, kv_heads, kv_len, head_dim]; query head h reads key head
+ * h / (heads / kv_heads).  Sequence b holds n = lengths[b] keys (NULL: kv_len) and
+ * m = q_lengths[b] queries (NULL: q_len), its last ones: query i stands at
+ * position p = n - m + i and sees the keys s with
+ *   0 <= s < n,  s <= p + right,  and (window <= 0, or s > p - window, or s < sinks):
+ * `window` keys up to its own position, the first `sinks` keys, and `right` keys
+ * past it (0: causal).  out = softmax(scale * q . k) v over these, zeros where
+ * there are none; scale <= 0 selects head_dim^-1/2.  Rows i >= m of out stay as
+ * they are.  lengths and q_lengths are DEVICE int32[batch], clamped to
+ * [0, kv_len] and [0, q_len].  Keys and values at s >= n are not used, whatever
+ * they hold; those below n must be finite, also where a mask hides them.
+ * strides: HOST int64[12], the (batch, head, token) strides of q, k, v and out in
+ * elements, columns contiguous; NULL: contiguous tensors of the shapes above.
+ * dtype BF16 or F16, out_dtype F32 or dtype.  head_dim is a multiple of 8 in
+ * [8, 128]; q, k, v are 16-byte aligned and their strides multiples of 8.  out
+ * overlaps no input.  No workspace; the same call gives the same bits. */
+OMNI_B200_API int omni_b200_attention_window(const void *q, const void *k, const void *v, void *out,
+                                             int batch, int heads, int kv_heads, int q_len,
+                                             int kv_len, int head_dim, const int64_t *strides,
+                                             const int32_t *lengths, const int32_t *q_lengths,
+                                             int window, int right, int sinks, float scale,
+                                             int dtype, int out_dtype, void *stream);
+
 /* ---- Diagnostics (failure detection without a GPU fault) ----------------
  * Every pipeline wait in this library's kernels is bounded: a wait that has
  * not completed after 2 s records a bit in the current device's kernel error

@@ -7,7 +7,7 @@ bench.py or __graft_entry__.py, or bind libomni_b200.so directly with ctypes
 """
 
 from .native import (  # noqa: F401
-    NativeError, Library, Context, library, attention_bhld, attention_rows, gelu_, linear_e4m3, quantize_e4m3, rms_norm,
-    rms_norm_e4m3)
+    NativeError, Library, Context, library, attention_bhld, attention_rows, attention_window, gelu_, linear_e4m3,
+    quantize_e4m3, rms_norm, rms_norm_e4m3)
 
 __version__ = "0.1.0"

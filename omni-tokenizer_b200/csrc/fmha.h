@@ -43,6 +43,10 @@ struct FmhaParams {
     float *split_m, *split_l, *split_o; // [part][256], [part][256], [part][256][HDP]
     float scale_log2;
     int *err;
+    // Sliding window (win != 0): L counts queries, kv_len keys; `group` query
+    // heads share a key head.
+    int win, window, right, sinks, kv_len, group;
+    const int *q_lengths; // [batch] queries of each sequence, or nullptr: L
 };
 
 // Parameters of the fp32 split-precision kernel (fmha_f32_sm100.cu): tensor
@@ -85,7 +89,28 @@ struct FmhaArgs {
     // bytes, 256-byte aligned), or nullptr: no split.
     void *split_ws = nullptr;
     size_t split_ws_bytes = 0;
+    // Sliding window (omni_b200_attention_window): window <= 0 is no window.
+    int win = 0, window = 0, right = 0, sinks = 0;
+    const int *q_lengths = nullptr;
 };
+
+// omni_b200_attention_window: q and out [batch, heads, q_len, head_dim], k and v
+// [batch, kv_heads, kv_len, head_dim] with strides in elements (batch, head, token).
+struct WindowArgs {
+    const void *q = nullptr, *k = nullptr, *v = nullptr;
+    void *out = nullptr;
+    int batch = 0, heads = 0, kv_heads = 0, q_len = 0, kv_len = 0, hd = 0;
+    long long qs[3] = {}, ks[3] = {}, vs[3] = {}, os[3] = {};
+    const int *lengths = nullptr, *q_lengths = nullptr;
+    int window = 0, right = 0, sinks = 0;
+    bool bf16 = true;
+    int out_dtype = kOutBF16;
+    float scale = 0.f; // 0: hd^-1/2
+    int *err = nullptr;
+};
+int attention_window(const WindowArgs &a, cudaStream_t stream);
+// Its kernel for few query rows (window_tokens.cu).
+int window_tokens_launch(const WindowArgs &a, cudaStream_t stream);
 
 // Returns 0 on success, a CUDA error code, or a negative/1000+ code for an
 // unsupported shape / tensor-map failure.

@@ -1,7 +1,8 @@
-// layer_api.cu -- extern "C" entry points of the 8-bit layer operators declared
-// in include/omni_b200.h.
+// layer_api.cu -- extern "C" entry points of the 8-bit layer operators and the
+// windowed attention declared in include/omni_b200.h.
 #include "omni_b200.h"
 
+#include "fmha.h"
 #include "layer.h"
 
 #include <cmath>
@@ -150,6 +151,75 @@ int omni_b200_linear_e4m3(const void *a, const float *a_scales, const void *w, c
     if (!l.err)
         return ctx_fail(7, "linear_e4m3: no CUDA device");
     return launch_status(linear_e4m3_launch(l, static_cast<cudaStream_t>(stream)), "linear_e4m3");
+}
+
+int omni_b200_attention_window(const void *q, const void *k, const void *v, void *out, int batch, int heads,
+                               int kv_heads, int q_len, int kv_len, int head_dim, const int64_t *strides,
+                               const int32_t *lengths, const int32_t *q_lengths, int window, int right, int sinks,
+                               float scale, int dtype, int out_dtype, void *stream) {
+    ctx_clear();
+    constexpr int kMost = 1 << 30;
+    if (dtype != OMNI_B200_BF16 && dtype != OMNI_B200_F16)
+        return ctx_fail(1, "attention_window: dtype must be BF16 or F16");
+    if (out_dtype != dtype && out_dtype != OMNI_B200_F32)
+        return ctx_fail(1, "attention_window: out_dtype must be dtype or F32");
+    if (batch < 0 || q_len < 0 || heads <= 0 || kv_heads <= 0 || kv_len <= 0 || q_len > kMost || kv_len > kMost)
+        return ctx_fail(1, "attention_window: sizes must be positive and at most 2^30");
+    if (heads % kv_heads)
+        return ctx_fail(1, "attention_window: heads must be a multiple of kv_heads");
+    if (head_dim <= 0 || head_dim > 128 || head_dim % 8)
+        return ctx_fail(4, "attention_window: head_dim must be a multiple of 8 in [8, 128]");
+    if (window > kMost || right < 0 || right > kMost || sinks < 0 || sinks > kMost)
+        return ctx_fail(1, "attention_window: window, right and sinks must be at most 2^30, right and sinks not negative");
+    if (std::isnan(scale) || std::isinf(scale))
+        return ctx_fail(1, "attention_window: scale must be finite");
+    if (static_cast<double>(batch) * heads * ((q_len + 255) / 256) > kMost)
+        return ctx_fail(4, "attention_window: more than 2^30 blocks of queries");
+    if (batch == 0 || q_len == 0)
+        return 0;
+    if (!q || !k || !v || !out)
+        return ctx_fail(1, "attention_window: null tensor pointer");
+    WindowArgs a;
+    const int of_heads[4] = {heads, kv_heads, kv_heads, heads}, of_len[4] = {q_len, kv_len, kv_len, q_len};
+    long long *to[4] = {a.qs, a.ks, a.vs, a.os};
+    for (int i = 0; i < 4; ++i) {
+        const int sizes[3] = {batch, of_heads[i], of_len[i]};
+        const long long plain[3] = {static_cast<long long>(of_heads[i]) * of_len[i] * head_dim,
+                                    static_cast<long long>(of_len[i]) * head_dim, head_dim};
+        for (int d = 0; d < 3; ++d) {
+            // The stride of a single element is never used.
+            to[i][d] = strides && sizes[d] > 1 ? strides[3 * i + d] : plain[d];
+            if (to[i][d] < head_dim || to[i][d] > (1ll << 38) || (i < 3 && to[i][d] % 8))
+                return ctx_fail(1, "attention_window: strides must be at least head_dim, at most 2^38, and those of "
+                                   "q, k and v multiples of 8");
+        }
+    }
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16))
+        return ctx_fail(1, "attention_window: q, k and v must be 16-byte aligned");
+    if (!aligned(out, type_bytes(out_dtype)) || !aligned(lengths, 4) || !aligned(q_lengths, 4))
+        return ctx_fail(1, "attention_window: a pointer is not aligned to its element type");
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = out;
+    a.batch = batch;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.q_len = q_len;
+    a.kv_len = kv_len;
+    a.hd = head_dim;
+    a.lengths = lengths;
+    a.q_lengths = q_lengths;
+    a.window = window;
+    a.right = right;
+    a.sinks = sinks;
+    a.bf16 = dtype == OMNI_B200_BF16;
+    a.out_dtype = out_dtype;
+    a.scale = scale;
+    a.err = kernel_error_word();
+    if (!a.err)
+        return ctx_fail(7, "attention_window: no CUDA device");
+    return launch_status(attention_window(a, static_cast<cudaStream_t>(stream)), "attention_window");
 }
 
 } // extern "C"

@@ -64,6 +64,11 @@ SIGNATURES = {
         C.c_int,
         [_P, _P, _P, _P, _P, _P, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_int, _P],
     ),
+    "omni_b200_attention_window": (
+        C.c_int,
+        [_P, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, _P, C.c_int, C.c_int, C.c_int,
+         C.c_float, C.c_int, C.c_int, _P],
+    ),
     "omni_b200_squares": (C.c_int, [_P, _P, C.c_size_t, C.c_size_t, C.c_int, C.c_int, _P]),
     "omni_b200_vq_argmin": (
         C.c_int,
@@ -405,3 +410,41 @@ def linear_e4m3(a, a_scales, w, w_scales, bias=None, out_dtype=None, out=None, s
 def _pitch(t, multiple):
     """Row stride of a matrix; a single row counts as one padded to `multiple`."""
     return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + multiple - 1) // multiple * multiple
+
+
+_STRIDES = C.c_int64 * 12
+
+
+def attention_window(q, k, v, window=0, sinks=0, right=0, lengths=None, q_lengths=None, scale=0.0, out=None,
+                     out_dtype=None, stream=None):
+    """Sliding-window attention: q [B, H, Lq, D] over k, v [B, Hkv, Lk, D] (any strides
+    with contiguous columns), bfloat16 or float16.
+
+    Sequence b holds lengths[b] keys (None: Lk) and q_lengths[b] queries (None: Lq), its
+    last ones (CUDA int32 tensors).  The query at position p sees `window` keys up to its
+    own (window <= 0: all), the first `sinks` keys, and `right` keys past it.  Rows past a
+    sequence's queries are left as they are in `out`, undefined in a new one."""
+    import torch
+
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        _refuse("attention_window: q must be [B, H, Lq, D], k and v [B, Hkv, Lk, D]")
+    B, H, Lq, D = q.shape
+    if k.shape[0] != B or k.shape[3] != D:
+        _refuse("attention_window: q, k and v must agree in batch and head dimension")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        _refuse("attention_window: q, k and v must all be bfloat16, or all float16")
+    for t in (lengths, q_lengths):
+        if t is not None and (t.shape != (B,) or t.dtype != torch.int32 or not t.is_contiguous()):
+            _refuse("attention_window: lengths and q_lengths must be contiguous int32 [B]")
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+    elif out.shape != q.shape or (out_dtype is not None and out.dtype != out_dtype):
+        _refuse("attention_window: out must have q's shape and out_dtype")
+    if out.dtype not in (q.dtype, torch.float32):
+        _refuse("attention_window: the output's type must be q's, or float32")
+    _checked("attention_window", (q, k, v, lengths, q_lengths, out), q)
+    strides = _STRIDES(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3])
+    _call("omni_b200_attention_window", q.device, stream, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B,
+          H, k.shape[1], Lq, k.shape[2], D, strides, _ptr(lengths), _ptr(q_lengths), window, right, sinks, scale,
+          _dtype_code(q), _dtype_code(out))
+    return out

@@ -103,3 +103,63 @@ def test_helpers_refuse():
         with refused as e:
             call()
         assert e.value.status == 1
+
+
+def _window(lib, strides=None, **k):
+    a = dict(q=X, k=R, v=W, out=O, batch=2, heads=4, kv_heads=2, q_len=3, kv_len=40, hd=64, strides=None, lengths=None,
+             q_lengths=None, window=8, right=0, sinks=1, scale=0.0, dtype=BF16, out_dtype=BF16)
+    a.update(k)
+    if strides is not None:
+        a["strides"] = (C.c_int64 * 12)(*strides)
+    return lib.omni_b200_attention_window(*a.values(), None)
+
+
+_PLAIN = [768, 192, 64, 5120, 2560, 64, 5120, 2560, 64, 768, 192, 64]
+
+
+def _with(i, value):
+    return dict(strides=_PLAIN[:i] + [value] + _PLAIN[i + 1:])
+
+
+@pytest.mark.parametrize("status,bad", [
+    (1, dict(q=None)), (1, dict(k=None)), (1, dict(v=None)), (1, dict(out=None)), (1, dict(batch=-1)),
+    (1, dict(heads=0)), (1, dict(kv_heads=0)), (1, dict(kv_heads=3)), (1, dict(q_len=-1)), (1, dict(kv_len=0)),
+    (1, dict(kv_len=(1 << 30) + 1)), (4, dict(hd=0)), (4, dict(hd=60)), (4, dict(hd=136)), (1, dict(window=2**31 - 1)),
+    (1, dict(right=-1)), (1, dict(right=2**31 - 1)), (1, dict(sinks=-1)), (1, dict(sinks=2**31 - 1)),
+    (1, dict(scale=float("nan"))), (1, dict(scale=float("inf"))), (1, dict(dtype=F32)), (1, dict(dtype=E4M3)),
+    (1, dict(out_dtype=F16)), (1, dict(q=X + 2)), (1, dict(k=R + 8)), (1, dict(v=W + 8)), (1, dict(out=O + 1)),
+    (1, dict(lengths=S + 1)), (1, dict(q_lengths=S + 2)), (4, dict(batch=1 << 20, heads=1 << 12)),
+    (1, _with(0, 0)), (1, _with(1, 63)), (1, _with(2, 68)), (1, _with(4, -64)), (1, _with(8, 0)), (1, _with(11, 32)),
+    (1, _with(5, (1 << 38) + 8)),
+])
+def test_window_refuses(lib, status, bad):
+    assert _window(lib, **bad) == status
+    assert b"attention_window" in lib.omni_b200_last_error()
+
+
+def test_window_without_queries_is_no_work(lib):
+    assert _window(lib, batch=0, q=None, k=None, v=None, out=None) == 0
+    assert _window(lib, q_len=0, q=None, k=None, v=None, out=None) == 0
+
+
+def test_window_helper_refuses():
+    torch = pytest.importorskip("torch")
+    q, k = torch.zeros(2, 4, 3, 64, dtype=torch.bfloat16), torch.zeros(2, 2, 40, 64, dtype=torch.bfloat16)
+    n = torch.zeros(2, dtype=torch.int32)
+    for call in (
+        lambda: ob.attention_window(q, k, k),  # tensors of the host
+        lambda: ob.attention_window(q[0], k, k),
+        lambda: ob.attention_window(q, k, k[:, :1]),
+        lambda: ob.attention_window(q[:1], k, k),
+        lambda: ob.attention_window(q[..., :32], k, k),
+        lambda: ob.attention_window(q.half(), k, k),
+        lambda: ob.attention_window(q.float(), k.float(), k.float()),
+        lambda: ob.attention_window(q, k, k, lengths=n.long()),
+        lambda: ob.attention_window(q, k, k, q_lengths=n[:1]),
+        lambda: ob.attention_window(q, k, k, out=q[:, :2]),
+        lambda: ob.attention_window(q, k, k, out=q, out_dtype=torch.float32),
+        lambda: ob.attention_window(q, k, k, out_dtype=torch.float16),
+    ):
+        with pytest.raises(ob.NativeError) as e:
+            call()
+        assert e.value.status == 1

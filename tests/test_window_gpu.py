@@ -1,0 +1,249 @@
+"""attention_window on the GPU against softmax attention in 64 bits.
+
+Tolerance, from arithmetic.  With A = the softmax-weighted mean of |v|, for each
+output element:
+  * the weights are rounded to the operand type for the product with v and their
+    sum may be taken before or after that: 2 * eps / 2 * A;
+  * scores are fp32 sums of exact products: at most D * 2^-24 of the sum of
+    magnitudes, below 2^-12 in the exponent for these inputs, so 2^-12 * A with
+    the exponential's own 2^-22;
+  * fp16 weights below 2^-14 of the row's largest lose at most 2^-25 each, times
+    the largest |v|;
+  * the output's rounding, half a step.
+Keys and values past a sequence's length are NaN in every test, rows past its
+queries must stay as they were.
+"""
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+KEPT = 123.0
+
+
+@pytest.fixture(scope="module")
+def ob():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from tests.conftest import load_package
+
+    return load_package()
+
+
+def _tensor(shape, layout, dtype, gen):
+    b, h, n, d = shape
+    if layout == "heads":
+        return torch.randn(b, h, n, d, generator=gen).to(dtype).cuda()
+    if layout == "tokens":
+        return torch.randn(b, n, h, d, generator=gen).to(dtype).cuda().transpose(1, 2)
+    # rows of a wider matrix, as a joint projection leaves them
+    wide = torch.full((b, n, h * d + 40), KEPT, dtype=dtype)
+    wide[..., 16:16 + h * d] = torch.randn(b, n, h * d, generator=gen).to(dtype)
+    return wide.cuda()[..., 16:16 + h * d].unflatten(2, (h, d)).transpose(1, 2)
+
+
+def _inputs(B, H, Hkv, Lq, Lk, D, dtype, layout, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [_tensor((B, h, n, D), layout, dtype, g) for h, n in ((H, Lq), (Hkv, Lk), (Hkv, Lk))]
+
+
+def _reference(q, k, v, window, right, sinks, lengths, q_lengths, scale=0.0):
+    """(out, A, most |v|, seen) in 64 bits; rows without keys are zeros."""
+    B, H, Lq, D = q.shape
+    Hkv, Lk = k.shape[1:3]
+    group = H // Hkv
+    out = torch.zeros(B, H, Lq, D, dtype=torch.float64, device=q.device)
+    mean = torch.zeros_like(out)
+    for b in range(B):
+        n, m = (Lk if lengths is None else lengths[b]), (Lq if q_lengths is None else q_lengths[b])
+        if n == 0 or m == 0:
+            continue
+        p = torch.arange(n - m, n, device=q.device)[:, None]
+        s = torch.arange(n, device=q.device)[None]
+        seen = s <= p + right
+        if window > 0:
+            seen &= (s > p - window) | (s < sinks)
+        kk = k[b, :, :n].double().repeat_interleave(group, 0)
+        vv = v[b, :, :n].double().repeat_interleave(group, 0)
+        e = q[b, :, :m].double() @ kk.transpose(1, 2) * (scale if scale > 0 else D**-0.5)
+        w = torch.nan_to_num(torch.softmax(e.masked_fill(~seen, -math.inf), dim=2))
+        out[b, :, :m], mean[b, :, :m] = w @ vv, w @ vv.abs()
+    return out, mean
+
+
+def _check(got, q, k, v, window, right, sinks, lengths, q_lengths, scale=0.0):
+    want, mean = _reference(q, k, v, window, right, sinks, lengths, q_lengths, scale)
+    eps = torch.finfo(q.dtype).eps
+    tol = mean * (eps + 2.0**-12) + want.abs() * torch.finfo(got.dtype).eps / 2 * (1 + 2.0**-8) + 1e-30
+    if q.dtype == F16:
+        keys = k.shape[2] if window <= 0 else min(k.shape[2], window + right + sinks)
+        most = max(float(v[b, :, :n].abs().max()) if n else 0.0
+                   for b, n in enumerate(lengths or [k.shape[2]] * q.shape[0]))
+        tol = tol + keys * 2.0**-25 * most
+        if got.dtype == F16:
+            tol = tol + 2.0**-25
+    for b in range(q.shape[0]):
+        m = q.shape[2] if q_lengths is None else q_lengths[b]
+        err = (got[b, :, :m].double() - want[b, :, :m]).abs()
+        assert bool((err <= tol[b, :, :m]).all()), (
+            f"sequence {b}: worst {float((err / tol[b, :, :m]).nan_to_num(1e9).max()):.3f} of the tolerance")
+        if q_lengths is not None:
+            assert bool((got[b, :, m:] == KEPT).all()), f"sequence {b}: rows past its queries changed"
+
+
+def _run(ob, q, k, v, lengths=None, q_lengths=None, out_dtype=None, out=None, **kw):
+    k, v = k.clone(), v.clone()
+    if lengths is not None:
+        for b, n in enumerate(lengths):
+            k[b, :, n:] = float("nan")
+            v[b, :, n:] = float("nan")
+    i32 = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    if out is None:
+        out = torch.full(q.shape, KEPT, dtype=out_dtype or q.dtype, device="cuda")
+    got = ob.attention_window(q, k, v, lengths=i32(lengths), q_lengths=i32(q_lengths), out=out, **kw)
+    ob.library().sync_check()
+    assert got is out
+    return got
+
+
+# B, H, Hkv, Lq, Lk, D, window, right, sinks
+TOKENS = [
+    (1, 1, 1, 1, 1, 64, 0, 0, 0),
+    (1, 2, 1, 1, 17, 8, 5, 0, 2),
+    (2, 4, 2, 1, 300, 64, 100, 0, 4),
+    (1, 16, 2, 1, 2048, 128, 512, 0, 4),
+    (3, 6, 2, 2, 129, 72, 40, 0, 1),
+    (2, 8, 1, 7, 500, 96, 64, 0, 130),
+    (1, 5, 5, 4, 700, 80, 0, 0, 3),
+    (2, 3, 3, 16, 40, 32, 7, 3, 2),
+    (1, 64, 1, 1, 1000, 16, 33, 0, 0),
+    (1, 1, 1, 60, 61, 24, 10, 100, 5),
+    (1, 4, 4, 1, 16000, 128, 0, 0, 0),
+    (20, 32, 8, 1, 260, 128, 1, 0, 0),
+]
+PROMPTS = [
+    (1, 1, 1, 65, 65, 64, 0, 0, 0),
+    (1, 2, 1, 257, 257, 64, 100, 0, 4),
+    (2, 4, 2, 300, 700, 128, 128, 0, 1),
+    (1, 3, 3, 1000, 1000, 72, 129, 0, 130),
+    (1, 2, 2, 515, 515, 96, 60, 59, 5),
+    (1, 4, 1, 200, 3000, 80, 500, 0, 300),
+    (2, 1, 1, 130, 128, 32, 20, 0, 2),
+    (1, 2, 2, 400, 400, 16, 0, 50, 0),
+    (1, 8, 2, 128, 128, 8, 1, 0, 0),
+    (1, 2, 2, 300, 1500, 40, 64, 2000, 7),
+    (1, 2, 1, 1200, 1200, 128, 0, 0, 0),
+    (3, 40, 8, 600, 600, 64, 300, 10, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("layout", ["heads", "tokens", "rows"])
+@pytest.mark.parametrize("case", TOKENS + PROMPTS, ids=lambda c: "-".join(map(str, c)))
+def test_window(ob, case, layout, dtype):
+    B, H, Hkv, Lq, Lk, D, window, right, sinks = case
+    q, k, v = _inputs(B, H, Hkv, Lq, Lk, D, dtype, layout, seed=sum(case))
+    mask = dict(window=window, right=right, sinks=sinks)
+    for out_dtype in (dtype, F32):
+        got = _run(ob, q, k, v, out_dtype=out_dtype, **mask)
+        _check(got, q, k, v, window, right, sinks, None, None)
+    assert torch.equal(got, _run(ob, q, k, v, out_dtype=F32, **mask))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("case", [
+    (6, 4, 2, 1, 300, 64, 100, 0, 4), (6, 6, 2, 5, 200, 72, 30, 4, 70), (6, 2, 1, 16, 90, 128, 0, 0, 0),
+    (6, 2, 2, 300, 300, 64, 50, 0, 4), (6, 4, 1, 280, 900, 128, 200, 20, 150), (6, 2, 2, 520, 640, 96, 0, 0, 0),
+    (6, 3, 3, 333, 400, 32, 17, 5, 3),
+], ids=lambda c: "-".join(map(str, c)))
+def test_window_lengths(ob, case, dtype):
+    """Sequences of several lengths: empty, one key, queries that outnumber the keys
+    (rows with no key give zeros), lengths inside and at the ends of tiles."""
+    B, H, Hkv, Lq, Lk, D, window, right, sinks = case
+    q, k, v = _inputs(B, H, Hkv, Lq, Lk, D, dtype, "heads", seed=sum(case) + 1)
+    lengths = [Lk, 0, 1, min(Lk, 129), Lk - 1, min(Lk, 128)]
+    mask = dict(window=window, right=right, sinks=sinks)
+    for q_lengths in (None, [Lq, Lq, Lq, max(1, Lq // 2), 0, min(Lq, 128)]):
+        for out_dtype in (dtype, F32):
+            got = _run(ob, q, k, v, lengths, q_lengths, out_dtype=out_dtype, **mask)
+            _check(got, q, k, v, window, right, sinks, lengths, q_lengths)
+    # Lengths beyond the tensors count as their sizes, negative ones as none.
+    far = _run(ob, q, k, v, [Lk] * 5 + [0], [Lq] * 6, **mask)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    clamped = ob.attention_window(q, k, v, lengths=torch.tensor([Lk + 99] * 5 + [-3], **i32),
+                                  q_lengths=torch.tensor([2**31 - 1] * 6, **i32), **mask)
+    ob.library().sync_check()
+    assert torch.equal(far, clamped)
+
+
+@pytest.mark.parametrize("Lq", [1, 300])
+def test_window_scale_and_large_scores(ob, Lq):
+    """Scores of a few hundred: the maximum is subtracted before the exponential."""
+    q, k, v = _inputs(1, 2, 2, Lq, 600, 64, BF16, "heads", seed=3)
+    for scale in (0.01, 2.0):
+        got = _run(ob, q, k, v, window=100, sinks=3, scale=scale, out_dtype=F32)
+        want, mean = _reference(q, k, v, 100, 0, 3, None, None, scale)
+        # Score errors grow with the scores: fp32 sums of 64 products of up to 16,
+        # times the scale, against 2^-24: below 64 * 2^-24 * 1024 * scale.
+        tol = mean * (2 * 2.0**-8 + 2.0**-8 * scale) + want.abs() * 2.0**-20
+        assert bool(((got.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("Lq", [1, 200])
+def test_window_writes_its_rows_only(ob, Lq):
+    """An output inside a larger tensor: what lies around it stays."""
+    q, k, v = _inputs(2, 4, 2, Lq, 256, 64, BF16, "tokens", seed=5)
+    want = _run(ob, q, k, v, window=60, sinks=2)
+    wide = torch.full((2, Lq + 2, 4, 80), KEPT, dtype=BF16, device="cuda")
+    inner = wide[:, 1:Lq + 1, :, 8:72].transpose(1, 2)
+    _run(ob, q, k, v, window=60, sinks=2, out=inner)
+    assert torch.equal(inner, want)
+    inner.fill_(KEPT)
+    assert bool((wide == KEPT).all())
+
+
+@pytest.mark.parametrize("Lq", [2, 300])
+def test_window_captured_on_two_streams(ob, Lq):
+    """Two captured calls with inputs of their own, replayed together and again with
+    other lengths, give what plain calls give."""
+    graphs = []
+    for seed in (1, 2):
+        q, k, v = _inputs(3, 4, 2, Lq, 700, 64, BF16, "heads", seed=seed)
+        lengths = torch.tensor([700, 350, 301], dtype=torch.int32, device="cuda")
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=stream):
+            ob.attention_window(q, k, v, window=128, sinks=4, lengths=lengths, out=out)
+        graphs.append((graph, stream, q, k, v, lengths, out))
+    for turn in range(2):
+        for graph, stream, *_, lengths, out in graphs:
+            lengths.copy_(torch.tensor([699 - 90 * turn, 500, 320], dtype=torch.int32))
+        torch.cuda.synchronize()
+        for graph, stream, *_ in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, stream, q, k, v, lengths, out in graphs:
+            assert torch.equal(out, ob.attention_window(q, k, v, window=128, sinks=4, lengths=lengths))
+    ob.library().sync_check()
+
+
+def test_window_of_everything_is_plain_attention(ob):
+    """No window and full lookahead is what attention_bhld computes."""
+    q, k, v = _inputs(2, 3, 3, 500, 500, 64, BF16, "heads", seed=9)
+    plain = ob.attention_bhld(q, k, v, out_dtype=F32)
+    got = ob.attention_window(q, k, v, right=500, out_dtype=F32)
+    ob.library().sync_check()
+    assert torch.allclose(got, plain, rtol=0, atol=2.0**-8 * float(v.abs().max()))
+
+
+def test_window_empty_calls(ob):
+    q, k, v = _inputs(2, 2, 1, 4, 8, 64, BF16, "heads", seed=1)
+    assert ob.attention_window(q[:0], k[:0], v[:0]).shape == (0, 2, 4, 64)
+    assert ob.attention_window(q[:, :, :0], k, v).shape == (2, 2, 0, 64)
+    ob.library().sync_check()
