@@ -255,28 +255,50 @@ def attention_rows(q, k, v, heads, block=0, valid=None, fused=False, out_dtype=N
 
 
 # -------------------------------------------------------- 8-bit layer operators
+# A call with one token is over in a few microseconds on the device, so these
+# helpers keep the host's part short: types and the device's stream are looked up
+# without building tensors' device objects or importing per call.
+class _Torch:
+    """torch's names that the helpers use, looked up at their first call."""
+
+    def __getattr__(self, name):
+        import torch
+
+        self.codes = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+        self.e4m3, self.f32, self.bf16, self.i32 = torch.float8_e4m3fn, torch.float32, torch.bfloat16, torch.int32
+        self.empty, self.empty_like, self.cuda = torch.empty, torch.empty_like, torch.cuda
+        self.current_device, self.raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
+        if name not in self.__dict__:
+            raise AttributeError(name)
+        return self.__dict__[name]
+
+
+_t = _Torch()
+
+
 def _refuse(message):
     raise NativeError(INVALID_ARGUMENT, message)
 
 
 def _element_code(what, t):
     """Type code of a 2-d tensor of one of the element types."""
-    import torch
-
-    if t.dim() != 2 or t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    code = _t.codes.get(t.dtype)
+    if code is None or t.dim() != 2:
         _refuse(f"{what}: need a [rows, cols] tensor of float32, bfloat16 or float16")
-    return _dtype_code(t)
+    return code
 
 
-def _checked(what, tensors, like):
-    """Every tensor on like's device and with contiguous columns."""
+def _checked(what, *tensors):
+    """The device of the first tensor: every one must be there and have contiguous columns."""
+    device = tensors[0].get_device()
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda or t.device != like.device:
+        if device < 0 or t.get_device() != device:
             _refuse(f"{what}: every tensor must be on the same CUDA device")
-        if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        if not t.is_contiguous() and t.shape[-1] > 1 and t.stride(-1) != 1:
             _refuse(f"{what}: columns must be contiguous")
+    return device
 
 
 def _row_stride(t):
@@ -284,52 +306,57 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _call(name, device, stream, *args):
-    """Calls an entry point on `device` and its current stream (or `stream`)."""
-    import torch
+def _pitch(t):
+    """Row stride of an e4m3 matrix; a single row counts as one padded to 16."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
-    lib = library()
-    if device.index == torch.cuda.current_device():
-        s = stream if stream is not None else torch.cuda.current_stream()
-        lib.check(getattr(lib.lib, name)(*args, s.cuda_stream))
+
+def _call(name, device, stream, *args):
+    """Calls an entry point on `device` and on `stream`, or that device's current one."""
+    lib = _LIB or library()
+    fn = getattr(lib.lib, name)
+    s = _t.raw_stream(device) if stream is None else stream.cuda_stream
+    if device == _t.current_device():
+        status = fn(*args, s)
     else:
-        with torch.cuda.device(device):
-            s = stream if stream is not None else torch.cuda.current_stream()
-            lib.check(getattr(lib.lib, name)(*args, s.cuda_stream))
+        with _t.cuda.device(device):
+            status = fn(*args, s)
+    if status:
+        lib.check(status)
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _empty_e4m3(rows, cols, device):
-    """[rows, cols] of e4m3 whose row stride is a multiple of 16, as linear_e4m3 reads it."""
-    import torch
-
+def _empty_e4m3(x):
+    """e4m3 of x's shape whose row stride is a multiple of 16, as linear_e4m3 reads it."""
+    rows, cols = x.shape
     if cols % 16 == 0:
-        return torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=device)
-    return torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=device)[:, :cols]
+        return x.new_empty((rows, cols), dtype=_t.e4m3)
+    return x.new_empty((rows, (cols + 15) // 16 * 16), dtype=_t.e4m3)[:, :cols]
 
 
-def _norm(what, x, weight, residual, residual_out, out, scales, eps, out_dtype, stream):
-    import torch
-
+def _norm(what, x, weight, residual, residual_out, out, scales, eps, code, out_code, stream):
     rows, cols = x.shape
     if weight.shape != (cols,) or weight.dtype != x.dtype:
         _refuse(f"{what}: weight must be [{cols}] of x's type")
+    stride = out_stride = 0
     if residual is None:
         if residual_out is not None:
             _refuse(f"{what}: residual_out needs a residual")
     else:
         if residual_out is None:
-            residual_out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        for t in (residual, residual_out):
-            if t.shape != x.shape or t.dtype != x.dtype:
-                _refuse(f"{what}: residual and residual_out must have x's shape and type")
-    _checked(what, (x, weight, residual, residual_out, out, scales), x)
-    _call("omni_b200_rms_norm", x.device, stream, x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(residual_out),
-          out.data_ptr(), _ptr(scales), rows, cols, _row_stride(x), 0 if residual is None else _row_stride(residual),
-          0 if residual is None else _row_stride(residual_out), _row_stride(out), eps, _dtype_code(x), out_dtype)
+            residual_out = x.new_empty((rows, cols))
+        elif residual_out.shape != x.shape or residual_out.dtype != x.dtype:
+            _refuse(f"{what}: residual_out must have x's shape and type")
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            _refuse(f"{what}: residual must have x's shape and type")
+        stride, out_stride = _row_stride(residual), _row_stride(residual_out)
+    device = _checked(what, x, weight, residual, residual_out, out, scales)
+    _call("omni_b200_rms_norm", device, stream, x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(residual_out),
+          out.data_ptr(), _ptr(scales), rows, cols, _row_stride(x), stride, out_stride, _row_stride(out), eps, code,
+          out_code)
     return residual_out
 
 
@@ -338,42 +365,35 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None, st
 
     Returns (y, h): y = h / sqrt(mean(h^2) + eps) * weight in x's type, h = x + residual
     (None without a residual).  residual_out may be x or residual, out any of them."""
-    import torch
-
     code = _element_code("rms_norm", x)
     if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        out = x.new_empty(x.shape)
     elif out.shape != x.shape or out.dtype != x.dtype:
         _refuse("rms_norm: out must have x's shape and type")
-    return out, _norm("rms_norm", x, weight, residual, residual_out, out, None, eps, code, stream)
+    return out, _norm("rms_norm", x, weight, residual, residual_out, out, None, eps, code, code, stream)
 
 
 def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, residual_out=None, stream=None):
     """rms_norm with its output in e4m3 and an fp32 scale for each 128 columns.
 
     Returns (q, scales, h); q and scales are what linear_e4m3 takes."""
-    import torch
-
-    _element_code("rms_norm_e4m3", x)
-    q = _empty_e4m3(*x.shape, x.device)
-    scales = torch.empty((x.shape[0], (x.shape[1] + 127) // 128), dtype=torch.float32, device=x.device)
-    return q, scales, _norm("rms_norm_e4m3", x, weight, residual, residual_out, q, scales, eps, E4M3, stream)
+    code = _element_code("rms_norm_e4m3", x)
+    q = _empty_e4m3(x)
+    scales = x.new_empty((x.shape[0], (x.shape[1] + 127) // 128), dtype=_t.f32)
+    return q, scales, _norm("rms_norm_e4m3", x, weight, residual, residual_out, q, scales, eps, code, E4M3, stream)
 
 
 def quantize_e4m3(x, block_rows=1, stream=None):
     """x [rows, cols] in e4m3: (q, scales), a scale for each 128 columns of a row
     (block_rows=1) or each 128 x 128 block (block_rows=128, weights)."""
-    import torch
-
     code = _element_code("quantize_e4m3", x)
-    rows, cols = x.shape
-    if block_rows not in (1, 128):
+    if block_rows != 1 and block_rows != 128:
         _refuse("quantize_e4m3: block_rows must be 1 or 128")
-    _checked("quantize_e4m3", (x,), x)
-    q = _empty_e4m3(rows, cols, x.device)
-    scales = torch.empty(((rows + block_rows - 1) // block_rows, (cols + 127) // 128), dtype=torch.float32,
-                         device=x.device)
-    _call("omni_b200_quantize_e4m3", x.device, stream, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols,
+    rows, cols = x.shape
+    device = _checked("quantize_e4m3", x)
+    q = _empty_e4m3(x)
+    scales = x.new_empty(((rows + block_rows - 1) // block_rows, (cols + 127) // 128), dtype=_t.f32)
+    _call("omni_b200_quantize_e4m3", device, stream, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols,
           _row_stride(x), _row_stride(q), block_rows, code)
     return q, scales
 
@@ -381,35 +401,26 @@ def quantize_e4m3(x, block_rows=1, stream=None):
 def linear_e4m3(a, a_scales, w, w_scales, bias=None, out_dtype=None, out=None, stream=None):
     """a [m, k] times w [n, k] transposed, both e4m3 with scales (quantize_e4m3 with
     block_rows 1 and 128), plus bias [n]: [m, n] of out_dtype (bfloat16)."""
-    import torch
-
     if a.dim() != 2 or w.dim() != 2:
         _refuse("linear_e4m3: a and w must be matrices")
-    (m, k), n = a.shape, w.shape[0]
-    if a.dtype != torch.float8_e4m3fn or w.dtype != torch.float8_e4m3fn or w.shape != (n, k):
+    (m, k), (n, wk) = a.shape, w.shape
+    if a.dtype != _t.e4m3 or w.dtype != _t.e4m3 or wk != k:
         _refuse("linear_e4m3: a [m, k] and w [n, k] must be float8_e4m3fn")
     groups = (k + 127) // 128
-    for t, rows in ((a_scales, m), (w_scales, (n + 127) // 128)):
-        if t.dtype != torch.float32 or t.shape != (rows, groups) or not t.is_contiguous():
+    for s, rows in ((a_scales, m), (w_scales, (n + 127) // 128)):
+        if s.dtype != _t.f32 or s.shape != (rows, groups) or not s.is_contiguous():
             _refuse(f"linear_e4m3: scales must be contiguous float32 [{rows}, {groups}]")
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype or torch.bfloat16, device=a.device)
+        out = a.new_empty((m, n), dtype=out_dtype or _t.bf16)
     elif out.shape != (m, n) or (out_dtype is not None and out.dtype != out_dtype):
         _refuse("linear_e4m3: out must be [m, n] of out_dtype")
-    if out.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        _refuse("linear_e4m3: out must be float32, bfloat16 or float16")
+    code = _element_code("linear_e4m3 output", out)
     if bias is not None and (bias.shape != (n,) or bias.dtype != out.dtype):
         _refuse(f"linear_e4m3: bias must be [{n}] of the output's type")
-    _checked("linear_e4m3", (a, a_scales, w, w_scales, bias, out), a)
-    _call("omni_b200_linear_e4m3", a.device, stream, a.data_ptr(), a_scales.data_ptr(), w.data_ptr(),
-          w_scales.data_ptr(), _ptr(bias), out.data_ptr(), m, n, k, _pitch(a, 16), _pitch(w, 16), _row_stride(out),
-          _dtype_code(out))
+    device = _checked("linear_e4m3", a, a_scales, w, w_scales, bias, out)
+    _call("omni_b200_linear_e4m3", device, stream, a.data_ptr(), a_scales.data_ptr(), w.data_ptr(),
+          w_scales.data_ptr(), _ptr(bias), out.data_ptr(), m, n, k, _pitch(a), _pitch(w), _row_stride(out), code)
     return out
-
-
-def _pitch(t, multiple):
-    """Row stride of a matrix; a single row counts as one padded to `multiple`."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + multiple - 1) // multiple * multiple
 
 
 _STRIDES = C.c_int64 * 12
@@ -424,27 +435,28 @@ def attention_window(q, k, v, window=0, sinks=0, right=0, lengths=None, q_length
     last ones (CUDA int32 tensors).  The query at position p sees `window` keys up to its
     own (window <= 0: all), the first `sinks` keys, and `right` keys past it.  Rows past a
     sequence's queries are left as they are in `out`, undefined in a new one."""
-    import torch
-
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         _refuse("attention_window: q must be [B, H, Lq, D], k and v [B, Hkv, Lk, D]")
     B, H, Lq, D = q.shape
-    if k.shape[0] != B or k.shape[3] != D:
+    Bk, Hkv, Lk, Dk = k.shape
+    if Bk != B or Dk != D:
         _refuse("attention_window: q, k and v must agree in batch and head dimension")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    code = _t.codes.get(dtype, F32)
+    if code == F32 or k.dtype != dtype or v.dtype != dtype:
         _refuse("attention_window: q, k and v must all be bfloat16, or all float16")
-    for t in (lengths, q_lengths):
-        if t is not None and (t.shape != (B,) or t.dtype != torch.int32 or not t.is_contiguous()):
+    for n in (lengths, q_lengths):
+        if n is not None and (n.shape != (B,) or n.dtype != _t.i32 or not n.is_contiguous()):
             _refuse("attention_window: lengths and q_lengths must be contiguous int32 [B]")
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+        out = q.new_empty(q.shape, dtype=out_dtype or dtype)
     elif out.shape != q.shape or (out_dtype is not None and out.dtype != out_dtype):
         _refuse("attention_window: out must have q's shape and out_dtype")
-    if out.dtype not in (q.dtype, torch.float32):
+    if out.dtype != dtype and out.dtype != _t.f32:
         _refuse("attention_window: the output's type must be q's, or float32")
-    _checked("attention_window", (q, k, v, lengths, q_lengths, out), q)
+    device = _checked("attention_window", q, k, v, lengths, q_lengths, out)
     strides = _STRIDES(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3])
-    _call("omni_b200_attention_window", q.device, stream, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B,
-          H, k.shape[1], Lq, k.shape[2], D, strides, _ptr(lengths), _ptr(q_lengths), window, right, sinks, scale,
-          _dtype_code(q), _dtype_code(out))
+    _call("omni_b200_attention_window", device, stream, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B, H,
+          Hkv, Lq, Lk, D, strides, _ptr(lengths), _ptr(q_lengths), window, right, sinks, scale, code,
+          _t.codes[out.dtype])
     return out
