@@ -68,14 +68,42 @@ __device__ __forceinline__ float2 unpair(uint64_t v) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
     return r;
 }
-// sum += d * s.  volatile: the sums of one TMEM load are taken before the next
+// sum += d * f.  volatile: the sums of one TMEM load are taken before a later
 // load's registers are filled.
-__device__ __forceinline__ void add_scaled(uint64_t &sum, uint32_t d0, uint32_t d1, uint64_t s) {
+__device__ __forceinline__ void add_scaled(uint64_t &sum, uint32_t d0, uint32_t d1, uint64_t f) {
     asm volatile("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\tfma.rn.f32x2 %0, d, %3, %0;\n\t}"
                  : "+l"(sum)
-                 : "r"(d0), "r"(d1), "l"(s));
+                 : "r"(d0), "r"(d1), "l"(f));
 }
-
+__device__ __forceinline__ float shared_f32(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 shared_f32x4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+// Arrives without release: for a thread whose reads so far are complete (their
+// values are in registers) and that has written nothing.  The release form would
+// wait for every load in flight.
+__device__ __forceinline__ void arrive_relaxed(uint64_t *bar) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.relaxed.cta.shared::cta.b64 st, [%0];\n\t}" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// 4 bytes from global to shared memory, asynchronously.
+__device__ __forceinline__ void copy_async_4(float *dst, const float *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// Arrives on `bar` when this thread's copies so far have landed.
+__device__ __forceinline__ void copy_async_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// 16 bytes to shared memory by a 32-bit address: the sums leave few registers.
+__device__ __forceinline__ void put16(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 __device__ __forceinline__ float bias_at(const LinearParams &p, int n) {
     if (!p.bias || n >= p.n)
         return 0.f;
@@ -93,6 +121,20 @@ __device__ __forceinline__ void store_one(const LinearParams &p, long long at, f
     else
         static_cast<__half *>(p.out)[at] = __float2half_rn(v);
 }
+// A box's elements to rows r0.. and columns col.. of out, one warp.
+__device__ __forceinline__ void store_box(const LinearParams &p, const uint8_t *box, int r0, int col, int size) {
+    const int width = min(128 / size, p.n - col), rows = min(32, p.m - r0);
+    for (int r = 0; r < rows; ++r)
+        for (int j = lane_id(); j < width; j += 32) {
+            const int at = j * size;
+            const uint8_t *from = box + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15);
+            const long long to = (r0 + r) * p.ldo + col + j;
+            if (size == 4)
+                static_cast<uint32_t *>(p.out)[to] = *reinterpret_cast<const uint32_t *>(from);
+            else
+                static_cast<uint16_t *>(p.out)[to] = *reinterpret_cast<const uint16_t *>(from);
+        }
+}
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, int dtype) {
     if (dtype == kBF16) {
         const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -106,12 +148,23 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, int dtype) {
 // Persistent CTAs, tiles of 128 rows x 256 columns of out.  Warps 0-7 add up:
 // warp w owns TMEM lane quarter w % 4 (32 rows, a row per lane) and columns
 // [128 (w / 4), +128), which lie in one block of w, so a thread's 128 sums all
-// take the same factor.  Warp 8 loads, warp 9 issues the products.  Registers:
-// 384 x 168 at launch = 256 x 224 (sums) + 128 x 56 (control).
-constexpr int kBigM = 128, kBigN = 256, kBigStages = 4, kBigThreads = 384;
+// take the same factor.  Warp 8 loads, warps 9 and 10 issue the products.  Registers:
+// 384 x 168 at launch = 256 x 216 (sums) + 128 x 72 (control).
+constexpr int kBigM = 128, kBigN = 256, kBigStages = 3, kBigThreads = 384;
+constexpr int kSumWarps = 8, kLoadWarp = 8, kIssueWarp = 9;
 constexpr int kBigStageBytes = (kBigM + kBigN) * kRowBytes;
-constexpr int kStagingBytes = 8 * 32 * 128; // a 32-row x 128-byte output box per warp
-constexpr int kBigSmem = kBigStages * kBigStageBytes + kStagingBytes + 256 + 1024;
+// Two output boxes of 32 rows x 128 bytes per warp: all of a warp's 2-byte
+// outputs, so that a tile waits for no store of its own.
+constexpr int kBoxBytes = 32 * 128;
+// The scales of a group: 128 of a's rows and two of w's blocks.  Loading stage n
+// of the ring follows product n - 3, which follows the sums of group n - 5, so
+// eight slots need no barrier of their own.
+constexpr int kScaleSlots = 8, kSlotFloats = kBigM + 4;
+static_assert(kScaleSlots >= kBigStages + 2, "a slot is read before it is written again");
+constexpr int kBigSmem =
+    kBigStages * kBigStageBytes + kSumWarps * 2 * kBoxBytes + kScaleSlots * kSlotFloats * 4 +
+    kSumWarps * 512 + 256 + 1024;
+static_assert(kBigSmem <= 227 * 1024, "shared memory of a CTA");
 constexpr int kBand = 16; // row tiles of a band
 
 // Tile order: bands of 16 row tiles, rows first, so that the tiles that run
@@ -128,28 +181,29 @@ __global__ void __launch_bounds__(kBigThreads, 1) linear_e4m3_big(const __grid_c
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t *staging = smem + kBigStages * kBigStageBytes;
-    uint64_t *full = reinterpret_cast<uint64_t *>(staging + kStagingBytes);
-    uint64_t *empty = full + kBigStages;
-    uint64_t *acc_full = empty + kBigStages; // [2]
-    uint64_t *acc_empty = acc_full + 2;      // [2]
-    uint64_t *drain = acc_empty + 2;
-    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(drain + 1);
+    float *scales = reinterpret_cast<float *>(staging + kSumWarps * 2 * kBoxBytes);
+    float *bias_lines = scales + kScaleSlots * kSlotFloats; // [warp][128]
+    uint64_t *full = reinterpret_cast<uint64_t *>(bias_lines + kSumWarps * 128);
+    // Product n is done: its accumulator is full, and its stage n % 3 free.
+    uint64_t *done = full + kBigStages;
+    uint64_t *acc_empty = done + kBigStages; // [2]
+    uint64_t *drain = acc_empty + 2;         // [2]
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(drain + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tiles = p.m_tiles * p.n_tiles;
     int *err = p.err;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kBigStages; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+            mbar_init(&full[s], 33); // 32 lanes' copies of the scales, and the tensor copies' bytes
+            mbar_init(&done[s], 2);  // the product's end, and its issuer, which saw the scales
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 8);
+            mbar_init(&acc_empty[i], kSumWarps);
+            mbar_init(&drain[i], 1);
         }
-        mbar_init(drain, 1);
         fence_mbarrier_init();
     }
-    if (warp == 9) {
+    if (warp == kIssueWarp) {
         tmem_alloc(tmem_holder, 512);
         tmem_relinquish();
     }
@@ -158,17 +212,22 @@ __global__ void __launch_bounds__(kBigThreads, 1) linear_e4m3_big(const __grid_c
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
 
-    if (warp >= 8) {
-        reg_dec<56>();
-        if (warp == 8) {
+    if (warp >= kLoadWarp) {
+        reg_dec<72>();
+        if (warp == kLoadWarp) {
             int n = 0;
             bool ok = true;
             for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
                 int mt, nt;
                 tile_at(p, tile, mt, nt);
+                // Rows and columns past the end: their operands are zero fill.
+                const float *sa[4], *sw = p.sw + static_cast<long long>(min(nt * 2 + (lane & 1), (p.n - 1) / 128)) * p.groups;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    sa[i] = p.sa + static_cast<long long>(min(mt * kBigM + i * 32 + lane, p.m - 1)) * p.groups;
                 for (int g = 0; g < p.groups; ++g, ++n) {
                     const int st = n % kBigStages;
-                    if (!(ok = warp_wait(&empty[st], ((n / kBigStages) & 1) ^ 1, err, kErrWaitEmpty)))
+                    if (!(ok = warp_wait(&done[st], ((n / kBigStages) & 1) ^ 1, err, kErrWaitEmpty)))
                         break;
                     if (elect_one()) {
                         uint8_t *to = smem + st * kBigStageBytes;
@@ -176,149 +235,168 @@ __global__ void __launch_bounds__(kBigThreads, 1) linear_e4m3_big(const __grid_c
                         tma_load_2d(to, &p.ta, &full[st], g * kRowBytes, mt * kBigM);
                         tma_load_2d(to + kBigM * kRowBytes, &p.tw, &full[st], g * kRowBytes, nt * kBigN);
                     }
+                    float *slot = scales + (n % kScaleSlots) * kSlotFloats;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        copy_async_4(slot + i * 32 + lane, sa[i] + g);
+                    if (lane < 2)
+                        copy_async_4(slot + kBigM + lane, sw + g);
+                    copy_async_arrive(&full[st]);
                     __syncwarp();
                 }
             }
             for (int j = max(0, n - kBigStages); j < n; ++j)
                 drain_wait(&full[j % kBigStages], (j / kBigStages) & 1, err);
-        } else if (warp == 9) {
+        } else if (warp < kIssueWarp + 2) {
+            // One warp alone cannot issue as fast as the products run (its waits
+            // and commits cost it about 600 clocks a group, a product 512), so
+            // each of two owns an accumulator and takes every other group.
             constexpr uint32_t idesc = make_idesc_e4m3(kBigM, kBigN);
             const uint32_t leader = elect_one() ? 1u : 0u;
             const uint32_t base = smem_u32(smem);
-            int n = 0;
-            bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-                for (int g = 0; g < p.groups; ++g, ++n) {
-                    const int st = n % kBigStages, buf = n & 1;
-                    if (!(ok = warp_wait(&acc_empty[buf], ((n >> 1) & 1) ^ 1, err, kErrWaitAcc)))
-                        break;
-                    if (!(ok = warp_wait(&full[st], (n / kBigStages) & 1, err, kErrWaitK)))
-                        break;
-                    tc_fence_after();
-                    const uint32_t at = base + st * kBigStageBytes;
-                    const uint64_t ad = make_smem_desc(at, 16, 8 * kRowBytes, kLayoutSW128);
-                    const uint64_t wd = make_smem_desc(at + kBigM * kRowBytes, 16, 8 * kRowBytes, kLayoutSW128);
+            const int buf = warp - kIssueWarp;
+            int total = 0;
+            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x)
+                total += p.groups;
+            for (int n = buf; n < total; n += 2) {
+                const int st = n % kBigStages;
+                if (!warp_wait(&acc_empty[buf], ((n >> 1) & 1) ^ 1, err, kErrWaitAcc) ||
+                    !warp_wait(&full[st], (n / kBigStages) & 1, err, kErrWaitK))
+                    break;
+                tc_fence_after();
+                const uint32_t at = base + st * kBigStageBytes;
+                const uint64_t ad = make_smem_desc(at, 16, 8 * kRowBytes, kLayoutSW128);
+                const uint64_t wd = make_smem_desc(at + kBigM * kRowBytes, 16, 8 * kRowBytes, kLayoutSW128);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_ss_f8_if(leader, tmem + buf * kBigN, ad + 2 * k, wd + 2 * k, idesc, k > 0 ? 1u : 0u);
-                    tc_commit_if(leader, &empty[st]);
-                    tc_commit_if(leader, &acc_full[buf]);
-                    __syncwarp();
-                }
+                for (int k = 0; k < 4; ++k)
+                    umma_ss_f8_if(leader, tmem + buf * kBigN, ad + 2 * k, wd + 2 * k, idesc, k > 0 ? 1u : 0u);
+                tc_commit_if(leader, &done[st]);
+                if (leader)
+                    mbar_arrive(&done[st]);
+                __syncwarp();
             }
-            tc_commit_if(leader, drain);
-            drain_wait(drain, 0, err);
+            tc_commit_if(leader, &drain[buf]);
+            drain_wait(&drain[buf], 0, err);
         }
         __syncwarp();
     } else {
-        reg_inc<224>();
+        reg_inc<216>();
         const int quarter = warp & 3, half = warp >> 2;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
-        uint8_t *box = staging + warp * 4096;
+        const uint32_t box = smem_u32(staging) + warp * 2 * kBoxBytes;
+        const uint32_t biases = smem_u32(bias_lines);
+        const uint32_t own_scale = smem_u32(scales) + (quarter * 32 + lane) * 4, block_scale = smem_u32(scales) + (kBigM + half) * 4;
         int n = 0;
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
             int mt, nt;
             tile_at(p, tile, mt, nt);
-            const int row = mt * kBigM + quarter * 32 + lane;
+            const int r0 = mt * kBigM + quarter * 32;
             const int col = nt * kBigN + half * 128;
-            // Rows and blocks past the end have scale 0 (their operands are zero fill).
-            const bool real = row < p.m && col < p.n;
-            const float *sa = p.sa + static_cast<long long>(real ? row : 0) * p.groups;
-            const float *sw = p.sw + static_cast<long long>(real ? col / 128 : 0) * p.groups;
-            uint64_t acc[64]; // 128 sums, starting at the bias
+            // Bias of columns col + 4 lane.., wanted when the sums are complete.
+            float bias[4] = {0.f, 0.f, 0.f, 0.f};
+            if (p.bias) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    bias[e] = bias_at(p, col + 4 * lane + e);
+            }
+            uint64_t acc[64]; // 128 sums
 #pragma unroll
             for (int c = 0; c < 64; ++c)
-                acc[c] = pair(bias_at(p, col + 2 * c), bias_at(p, col + 2 * c + 1));
-            float a_next = __ldg(sa), w_next = __ldg(sw);
+                acc[c] = 0;
             for (int g = 0; g < p.groups; ++g, ++n) {
-                const float f = a_next * w_next;
-                const uint64_t s = pair(f, f);
-                if (g + 1 < p.groups) {
-                    a_next = __ldg(sa + g + 1);
-                    w_next = __ldg(sw + g + 1);
-                }
                 const int buf = n & 1;
-                if (!(ok = warp_wait(&acc_full[buf], (n >> 1) & 1, err, kErrWaitS)))
+                if (!(ok = warp_wait(&done[n % kBigStages], (n / kBigStages) & 1, err, kErrWaitS)))
                     break;
                 tc_fence_after();
+                const uint32_t slot = (n % kScaleSlots) * (kSlotFloats * 4);
+                const float s = shared_f32(own_scale + slot) * shared_f32(block_scale + slot);
+                const uint64_t f = pair(s, s);
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t d[32];
-                    tmem_ld32(lanes + buf * kBigN + c, d);
+                for (int c = 0; c < 128; c += 16) {
+                    uint32_t d[16];
+                    tmem_ld16(lanes + buf * kBigN + c, d);
                     tmem_wait_ld();
+                    if (c == 112) { // all of it is in registers: the next product may start
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0)
+                            arrive_relaxed(&acc_empty[buf]);
+                    }
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2)
-                        add_scaled(acc[(c + e) / 2], d[e], d[e + 1], s);
+                    for (int e = 0; e < 16; e += 2)
+                        add_scaled(acc[(c + e) / 2], d[e], d[e + 1], f);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0)
-                    mbar_arrive(&acc_empty[buf]);
             }
             if (!ok)
                 break;
-            // A box of 32 rows x 128 bytes at a time, each lane its row, in the
-            // 128-byte swizzle of the store's tensor map; rows that TMA cannot
-            // address leave the box by plain stores.
-            const int r0 = mt * kBigM + quarter * 32;
-            auto reuse = [&]() {
-                if (lane == 0)
-                    tma_store_wait_read();
+            // Boxes of 32 rows x 128 bytes, each lane its row, in the 128-byte swizzle
+            // of the store's tensor map; rows that TMA cannot address leave the box
+            // by plain stores.
+            const int size = p.out_dtype == kF32 ? 4 : 2, width = 128 / size;
+            const uint32_t line = biases + warp * 512; // the bias in column order
+            if (p.bias) {
                 __syncwarp();
-            };
-            auto flush = [&](int c, int size) {
+                put16(line + lane * 16, __float_as_uint(bias[0]), __float_as_uint(bias[1]), __float_as_uint(bias[2]),
+                      __float_as_uint(bias[3]));
+            }
+#pragma unroll
+            for (int c = 0; c < 128; c += 16) {
+                // 16 columns: half a box of fp32, a quarter of one of 2-byte elements.
+                const int in = c % width, which = (c / width) & 1;
+                if (size == 4 ? c % 64 == 0 : c == 0) { // both boxes are free again
+                    if (lane == 0)
+                        tma_store_wait_read();
+                    __syncwarp();
+                }
+                float v[16];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float2 x = unpair(acc[c / 2 + e]);
+                    v[2 * e] = x.x;
+                    v[2 * e + 1] = x.y;
+                }
+                if (p.bias) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const float4 b = shared_f32x4(line + (c + e) * 4);
+                        v[e] += b.x;
+                        v[e + 1] += b.y;
+                        v[e + 2] += b.z;
+                        v[e + 3] += b.w;
+                    }
+                }
+                const uint32_t row = box + which * kBoxBytes + lane * 128;
+                auto place = [&](int j) { return row + ((j ^ (lane & 7)) << 4); };
+                if (size == 4) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        put16(place(j + in / 4), __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                              __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        put16(place(j + in / 8), pack16(v[8 * j], v[8 * j + 1], p.out_dtype),
+                              pack16(v[8 * j + 2], v[8 * j + 3], p.out_dtype),
+                              pack16(v[8 * j + 4], v[8 * j + 5], p.out_dtype),
+                              pack16(v[8 * j + 6], v[8 * j + 7], p.out_dtype));
+                }
+                if (in + 16 < width)
+                    continue;
+                const int at = col + c + 16 - width; // the box's first column
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (r0 >= p.m || c >= p.n)
-                    return;
+                if (r0 >= p.m || at >= p.n)
+                    continue;
+                uint8_t *from = staging + (warp * 2 + which) * kBoxBytes;
                 if (p.o_tma) {
                     if (lane == 0) {
-                        tma_store_2d(&p.to, box, c, r0);
+                        tma_store_2d(&p.to, from, at, r0);
                         tma_store_commit();
                     }
-                    return;
-                }
-                const int width = min(128 / size, p.n - c);
-                for (int r = 0; r < 32 && r0 + r < p.m; ++r)
-                    for (int j = lane; j < width; j += 32) {
-                        const uint8_t *from = box + r * 128 + ((((j * size) >> 4) ^ (r & 7)) << 4) + ((j * size) & 15);
-                        const long long at = (r0 + r) * p.ldo + c + j;
-                        if (size == 4)
-                            static_cast<uint32_t *>(p.out)[at] = *reinterpret_cast<const uint32_t *>(from);
-                        else
-                            static_cast<uint16_t *>(p.out)[at] = *reinterpret_cast<const uint16_t *>(from);
-                    }
-                __syncwarp();
-            };
-            if (p.out_dtype == kF32) {
-#pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    reuse();
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float2 v0 = unpair(acc[c / 2 + j * 2]), v1 = unpair(acc[c / 2 + j * 2 + 1]);
-                        *reinterpret_cast<float4 *>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                            make_float4(v0.x, v0.y, v1.x, v1.y);
-                    }
-                    flush(col + c, 4);
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < 128; c += 64) {
-                    reuse();
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 v = unpair(acc[c / 2 + j * 4 + e]);
-                            w[e] = pack16(v.x, v.y, p.out_dtype);
-                        }
-                        *reinterpret_cast<uint4 *>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                            make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                    flush(col + c, 2);
+                } else {
+                    store_box(p, from, r0, at, size);
+                    __syncwarp();
                 }
             }
         }
@@ -329,7 +407,7 @@ __global__ void __launch_bounds__(kBigThreads, 1) linear_e4m3_big(const __grid_c
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 9)
+    if (warp == kIssueWarp)
         tmem_dealloc(tmem, 512);
 }
 

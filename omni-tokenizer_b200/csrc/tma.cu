@@ -93,11 +93,11 @@ int make_map_2d(CUtensorMap *map, const void *base, int cols, long long rows, in
 }
 
 int make_map_pitched(CUtensorMap *map, const void *base, CUtensorMapDataType type, int elem_bytes, long long cols,
-                     long long rows, long long pitch, int box_w, int box_rows) {
+                     long long rows, long long pitch, int box_w, int box_rows, int swizzle_bytes) {
     const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
     const uint64_t strides[1] = {static_cast<uint64_t>(pitch)};
     const uint32_t box[2] = {static_cast<uint32_t>(box_w), static_cast<uint32_t>(box_rows)};
-    return encode_typed(map, base, type, elem_bytes, 2, dims, strides, box, 128);
+    return encode_typed(map, base, type, elem_bytes, 2, dims, strides, box, swizzle_bytes);
 }
 
 } // namespace omni_b200

@@ -25,7 +25,7 @@ int make_map_2d(CUtensorMap *map, const void *base, int cols, long long rows, in
 int make_map_2d_f32(CUtensorMap *map, const void *base, int cols, long long rows, int box_w,
                     int box_rows);
 // Row-major matrix of 1-, 2- or 4-byte elements (type: its tensor-map type) with
-// rows `pitch` bytes apart; 128-byte swizzle, box of box_w columns x box_rows rows.
+// rows `pitch` bytes apart; box of box_w columns x box_rows rows.
 int make_map_pitched(CUtensorMap *map, const void *base, CUtensorMapDataType type, int elem_bytes, long long cols,
-                     long long rows, long long pitch, int box_w, int box_rows);
+                     long long rows, long long pitch, int box_w, int box_rows, int swizzle_bytes = 128);
 } // namespace omni_b200
