@@ -8,15 +8,17 @@
 // here the tensor work stays far below the loads.)
 //
 // Keys go to the warps 16 at a time; each warp keeps its own running maximum,
-// sum and output, and nothing is shared until the end.  The fragments come
-// straight from global memory with 16-byte loads, without shared memory, by a
-// choice of index order:
+// sum and output and copies its keys and values to a ring of its own in shared
+// memory (cp.async, two chunks ahead, no barrier between warps).  The fragments
+// leave it by 16-byte loads, by a choice of index order:
 //   q k^T sums over the head dimension in any order: in each 32 columns, lane
 //     quad index c = lane % 4 holds columns 8c..8c+7 of q and of k, and takes
 //     them as the k-indexes (2c, 2c+1, 2c+8, 2c+9) of two mma steps;
 //   p v gives its columns in any order: column index n = lane / 4 of mma j
 //     stands for column 8n + j (of each 64), so lane / 4 loads columns 8n..8n+7
 //     of its four keys and pairs them up with byte permutes.
+// Rows are 128 or 256 bytes apart; the 16-byte pieces of a row are permuted by
+// the row number so that the eight lanes of a load phase meet all 32 banks.
 // A cluster of CTAs splits the keys of one tile of rows, so that few sequences
 // still load with many SMs; the parts meet in distributed shared memory, in rank
 // order (no atomics).
@@ -29,7 +31,7 @@
 namespace omni_b200 {
 namespace {
 
-constexpr int kWarps = 4, kChunk = 16;
+constexpr int kWarps = 4, kChunk = 16, kStages = 3, kMaxParts = 16;
 
 struct TokensParams {
     const uint16_t *q, *k, *v;
@@ -64,6 +66,15 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack_pair(float lo, flo
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 __device__ __forceinline__ uint4 load16(const uint16_t *p) { return *reinterpret_cast<const uint4 *>(p); }
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+// 16 bytes to shared memory, zeros where `real` is false (nothing is read then).
+__device__ __forceinline__ void copy_async_16(uint32_t to, const uint16_t *from, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
+}
 // Low and high halves of two words: (x.lo, y.lo) and (x.hi, y.hi).
 __device__ __forceinline__ uint32_t lows(uint32_t x, uint32_t y) { return __byte_perm(x, y, 0x5410); }
 __device__ __forceinline__ uint32_t highs(uint32_t x, uint32_t y) { return __byte_perm(x, y, 0x7632); }
@@ -82,14 +93,23 @@ __device__ __forceinline__ float peer_load(uint32_t at) {
     return v;
 }
 
+template <int DK> struct TokensShape {
+    static constexpr int DV = (DK + 1) / 2;         // 64-column steps of v
+    static constexpr int PITCH = DV * 128;          // bytes of a row
+    static constexpr int TILE = kChunk * PITCH;     // a chunk's keys, or values
+    static constexpr int RING = kWarps * kStages * 2 * TILE;
+    static constexpr int D = DK * 32;
+    // The parts' place at the end, over the ring: m, l of the warps and the CTA, outputs.
+    static constexpr int PARTS = (2 * kWarps + 2) * 16 * 4 + kWarps * 16 * (D + 4) * 4;
+    static constexpr int SMEM = RING > PARTS ? RING : PARTS;
+};
+
 // DK: 32-column steps of the head dimension; columns past hd are zeros.
 template <int DK, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32, 3) window_tokens_kernel(const __grid_constant__ TokensParams p) {
-    constexpr int DV = (DK + 1) / 2; // 64-column steps of v
-    constexpr int D = DK * 32;
-    __shared__ float part_m[kWarps][16], part_l[kWarps][16];
-    __shared__ float cta_m[16], cta_l[16];
-    __shared__ float part_o[kWarps][16][D + 4];
+__global__ void __launch_bounds__(kWarps * 32, 2) window_tokens_kernel(const __grid_constant__ TokensParams p) {
+    using S = TokensShape<DK>;
+    constexpr int DV = S::DV, D = S::D;
+    extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int parts = p.parts, pair = blockIdx.x / parts, part = blockIdx.x - pair * parts;
     const int b = pair / p.kv_heads, kvh = pair - b * p.kv_heads;
@@ -111,14 +131,15 @@ __global__ void __launch_bounds__(kWarps * 32, 3) window_tokens_kernel(const __g
 
     // This thread's rows g and g + 8: their keys [.., limit) with [sinks, floor) hidden.
     int limit[2], floor_[2];
+    const int limit_all = min(n, first + p.right + 1), floor_all = p.window > 0 ? last - p.window + 1 : 0;
     uint32_t qa[DK * 2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int r = row0 + g + 8 * h;
         const bool real = g + 8 * h < rows;
         const int pos = pos0 + r / p.group;
-        limit[h] = real ? min(n, pos + p.right + 1) : 0;
-        floor_[h] = p.window > 0 ? pos - p.window + 1 : 0;
+        limit[h] = real ? min(n, pos + p.right + 1) : n; // a row that is none: anything finite
+        floor_[h] = real && p.window > 0 ? pos - p.window + 1 : 0;
         const uint16_t *q = p.q + b * p.qs[0] + (kvh * p.group + r % p.group) * p.qs[1] + (r / p.group) * p.qs[2];
 #pragma unroll
         for (int d = 0; d < DK; ++d) {
@@ -141,52 +162,58 @@ __global__ void __launch_bounds__(kWarps * 32, 3) window_tokens_kernel(const __g
         key = i < sink_chunks ? i * kChunk : low + (i - sink_chunks) * kChunk;
         end = i < sink_chunks ? sink : high;
     };
-    uint4 kf[2][DK], vf[DV][4];
-    auto load_k = [&](int i) {
+    const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * S::TILE;
+    auto fetch = [&](int i, int stage) {
         int key, end;
         chunk_at(i, key, end);
+        const uint32_t to = ring + stage * 2 * S::TILE;
+        constexpr int P = DK * 4; // pieces of a row
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int s = key + t * 8 + g;
-            const uint16_t *at = kb + s * p.ks[2] + c * 8;
-#pragma unroll
-            for (int d = 0; d < DK; ++d)
-                kf[t][d] = s < end && d * 32 + c * 8 < p.hd ? load16(at + d * 32) : make_uint4(0u, 0u, 0u, 0u);
-        }
-    };
-    auto load_v = [&](int i) {
-        int key, end;
-        chunk_at(i, key, end);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int s = key + c * 2 + (e & 1) + (e >> 1) * 8;
-            const uint16_t *at = vb + s * p.vs[2] + g * 8;
-#pragma unroll
-            for (int d = 0; d < DV; ++d)
-                vf[d][e] = s < end && d * 64 + g * 8 < p.hd ? load16(at + d * 64) : make_uint4(0u, 0u, 0u, 0u);
+        for (int x = lane; x < kChunk * P; x += 32) {
+            const int row = x / P, j = x - row * P;
+            const bool real = key + row < end && j * 8 < p.hd;
+            const long long s = real ? key + row : 0;
+            const int at = real ? j * 8 : 0;
+            const uint32_t piece = row * S::PITCH + (j & ~7) * 16;
+            copy_async_16(to + piece + (((j & 7) ^ ((row & 1) << 2 | ((row >> 1) & 3))) << 4), kb + s * p.ks[2] + at, real);
+            copy_async_16(to + S::TILE + piece + (((j & 7) ^ (row & 7)) << 4), vb + s * p.vs[2] + at, real);
         }
     };
     int i = part * kWarps + warp;
-    if (i < chunks) {
-        load_k(i);
-        load_v(i);
+#pragma unroll
+    for (int k = 0; k < kStages - 1; ++k) {
+        if (i + k * stride < chunks)
+            fetch(i + k * stride, k);
+        asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    for (; i < chunks; i += stride) {
+    for (int stage = 0; i < chunks; i += stride, stage = stage + 1 == kStages ? 0 : stage + 1) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp(); // this chunk has landed for every lane, and every lane is done with the last one
+        if (i + (kStages - 1) * stride < chunks)
+            fetch(i + (kStages - 1) * stride, stage == 0 ? kStages - 1 : stage - 1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const uint32_t kt = ring + stage * 2 * S::TILE, vt = kt + S::TILE;
         float s[2][4];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            float s2[4] = {0.f, 0.f, 0.f, 0.f}; // a second chain of dependent products
             s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+            const uint32_t row = kt + (t * 8 + g) * S::PITCH, turn = (g & 1) << 2 | ((g >> 1) & 3);
 #pragma unroll
             for (int d = 0; d < DK; ++d) {
-                mma16816<BF16>(s[t], qa[2 * d], kf[t][d].x, kf[t][d].y);
-                mma16816<BF16>(s[t], qa[2 * d + 1], kf[t][d].z, kf[t][d].w);
+                const int j = d * 4 + c;
+                const uint4 k = shared16(row + (j & ~7) * 16 + (((j & 7) ^ turn) << 4));
+                mma16816<BF16>(s[t], qa[2 * d], k.x, k.y);
+                mma16816<BF16>(s2, qa[2 * d + 1], k.z, k.w);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                s[t][e] += s2[e];
         }
-        const bool more = i + stride < chunks;
-        if (more)
-            load_k(i + stride);
         int key, end;
         chunk_at(i, key, end);
+        // A chunk that every row sees whole needs no mask.
+        const bool whole = key + kChunk <= min(end, limit_all) && (key >= floor_all || key + kChunk <= p.sinks);
         // s[t][2h + e]: row g + 8h, key + 8t + 2c + e.
         float grown[2];
 #pragma unroll
@@ -198,14 +225,14 @@ __global__ void __launch_bounds__(kWarps * 32, 3) window_tokens_kernel(const __g
                 for (int e = 0; e < 2; ++e) {
                     const int at = key + t * 8 + c * 2 + e;
                     float &x = s[t][2 * h + e];
-                    const bool seen = at < end && at < limit[h] && (at >= floor_[h] || at < p.sinks);
+                    const bool seen = whole || (at < end && at < limit[h] && (at >= floor_[h] || at < p.sinks));
                     x = seen ? x * p.scale_log2 : -INFINITY;
                     mx = fmaxf(mx, x);
                 }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             mx = fmaxf(mx, top[h]);
-            grown[h] = mx > top[h] ? exp2f(top[h] - mx) : 1.f;
+            grown[h] = mx > top[h] ? ex2_approx(top[h] - mx) : 1.f;
             top[h] = mx;
             const float ref = mx == -INFINITY ? 0.f : mx;
             sum[h] *= grown[h];
@@ -214,7 +241,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) window_tokens_kernel(const __g
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     float &x = s[t][2 * h + e];
-                    x = exp2f(x - ref);
+                    x = ex2_approx(x - ref);
                     sum[h] += x;
                 }
         }
@@ -231,16 +258,25 @@ __global__ void __launch_bounds__(kWarps * 32, 3) window_tokens_kernel(const __g
                                 pack_pair<BF16>(s[1][0], s[1][1]), pack_pair<BF16>(s[1][2], s[1][3])};
 #pragma unroll
         for (int d = 0; d < DV; ++d) {
-            const uint32_t *x0 = &vf[d][0].x, *x1 = &vf[d][1].x, *x2 = &vf[d][2].x, *x3 = &vf[d][3].x;
+            uint4 v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = c * 2 + (e & 1) + (e >> 1) * 8;
+                v[e] = shared16(vt + row * S::PITCH + d * 128 + ((g ^ (row & 7)) << 4));
+            }
+            const uint32_t *x0 = &v[0].x, *x1 = &v[1].x, *x2 = &v[2].x, *x3 = &v[3].x;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 mma16816<BF16>(o[d * 8 + 2 * j], pa, lows(x0[j], x1[j]), lows(x2[j], x3[j]));
                 mma16816<BF16>(o[d * 8 + 2 * j + 1], pa, highs(x0[j], x1[j]), highs(x2[j], x3[j]));
             }
         }
-        if (more)
-            load_v(i + stride);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads(); // the ring becomes the parts' place
+    float(*part_m)[16] = reinterpret_cast<float(*)[16]>(smem), (*part_l)[16] = part_m + kWarps;
+    float *cta_m = part_l[kWarps], *cta_l = cta_m + 16;
+    float(*part_o)[16][D + 4] = reinterpret_cast<float(*)[16][D + 4]>(cta_l + 16);
 
     // The warps' parts, then the CTAs': out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
 #pragma unroll
@@ -321,7 +357,19 @@ __global__ void __launch_bounds__(kWarps * 32, 3) window_tokens_kernel(const __g
 }
 
 template <int DK, bool BF16> int launch_dk(const TokensParams &p, dim3 grid, cudaStream_t stream) {
+    static std::atomic<unsigned long long> done{0};
+    const cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(window_tokens_kernel<DK, BF16>),
+                                         TokensShape<DK>::SMEM, done);
+    if (e != cudaSuccess)
+        return static_cast<int>(e);
+    if (p.parts > 8) { // clusters above 8 CTAs need the kernel's consent
+        const cudaError_t w = cudaFuncSetAttribute(window_tokens_kernel<DK, BF16>,
+                                                   cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (w != cudaSuccess)
+            return static_cast<int>(w);
+    }
     cudaLaunchConfig_t cfg{};
+    cfg.dynamicSmemBytes = TokensShape<DK>::SMEM;
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kWarps * 32);
     cfg.stream = stream;
@@ -377,15 +425,17 @@ int window_tokens_launch(const WindowArgs &a, cudaStream_t stream) {
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess)
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    // CTAs that split the keys of one tile: until three fit on every SM, with two
-    // chunks left for each warp.
+    // CTAs that split the keys of one tile: until two are on every SM, with two
+    // chunks left for each warp.  Measured, 4101 keys x 128: 512 tiles 168 us with
+    // one part, 180 with two; 128 tiles 36 and 28 us (four: 30); 32 tiles 38 us
+    // with two parts, 23 with four, 20 with eight.
     const int tiles = (p.group * a.q_len + 15) / 16;
     const long long ctas = static_cast<long long>(tiles) * a.batch * a.kv_heads;
     long long keys = a.kv_len;
     if (a.window > 0)
         keys = std::min(keys, static_cast<long long>(a.window) + a.q_len + a.sinks);
     int parts = 1;
-    while (parts < 8 && ctas * parts * 2 <= 3ll * sms && keys >= 2ll * parts * 2 * kWarps * kChunk)
+    while (parts < kMaxParts && ctas * parts * 2 <= 2ll * sms && keys >= 2ll * parts * 2 * kWarps * kChunk)
         parts *= 2;
     p.parts = parts;
     const dim3 grid(static_cast<unsigned>(parts) * a.batch * a.kv_heads, tiles);
