@@ -21,6 +21,7 @@ struct RowsArgs {
     int dtype = kBF16;
     bool norm = false;      // false: quantise x as it is
     bool quantize = false;  // e4m3 output with scales, else dtype
+    int *err = nullptr;     // the device's error word
 };
 int rows_launch(const RowsArgs &a, cudaStream_t stream);
 

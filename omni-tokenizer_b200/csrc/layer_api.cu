@@ -74,6 +74,9 @@ int omni_b200_rms_norm(const void *x, const void *residual, const void *weight, 
     a.dtype = dtype;
     a.norm = true;
     a.quantize = quantize;
+    a.err = kernel_error_word();
+    if (!a.err)
+        return ctx_fail(7, "rms_norm: no CUDA device");
     return launch_status(rows_launch(a, static_cast<cudaStream_t>(stream)), "rms_norm");
 }
 
@@ -109,6 +112,9 @@ int omni_b200_quantize_e4m3(const void *x, void *q, float *scales, size_t rows, 
     a.out_stride = static_cast<long long>(q_stride);
     a.dtype = dtype;
     a.quantize = true;
+    a.err = kernel_error_word();
+    if (!a.err)
+        return ctx_fail(7, "quantize_e4m3: no CUDA device");
     return launch_status(rows_launch(a, static_cast<cudaStream_t>(stream)), "quantize_e4m3");
 }
 

@@ -14,11 +14,15 @@
 // (16-byte loads of 2-byte types), VPT steps.  A group of 128 columns is then
 // 16 neighbouring lanes, so its largest magnitude takes four shuffles and no
 // shared memory.  The grid is persistent: the weight is read once per CTA.
+// rows_stream_kernel: many rows.  The same thread layout, rows through a ring of
+// shared memory that bulk copies fill several rows ahead, so that loads are in
+// flight at all times (rows_kernel's stop at every reduction).
 // rows_scalar_kernel serves columns and pitches that 16-byte loads cannot, and
 // rows wider than the registers hold; it reads its row twice (the second time
 // from L2).
 #include "e4m3.cuh"
 #include "layer.h"
+#include "sm100.cuh"
 
 #include <algorithm>
 
@@ -39,8 +43,31 @@ __device__ __forceinline__ float half_warp_max(float v) {
     return v;
 }
 
+// Thread t's elements of a row to `out`, as they are or in groups of e4m3.
+template <typename T, bool QUANT, int TPR, int VPT>
+__device__ __forceinline__ void write_row(const RowsArgs &a, long long row, int groups, int t, float (&h)[VPT][8]) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int c = (i * TPR + t) * 8;
+        if constexpr (QUANT) {
+            const float scale = group_scale(half_warp_max(amax8(h[i])));
+            if (c < a.cols) {
+                uint8_t *q = static_cast<uint8_t *>(a.out) + row * a.out_stride + c;
+                *reinterpret_cast<uint2 *>(q) = e4m3x8(h[i], __frcp_rn(scale));
+                if (t % 16 == 0)
+                    a.scales[row * groups + c / kGroup] = scale;
+            }
+        } else if (c < a.cols) {
+            store8(static_cast<T *>(a.out) + row * a.out_stride + c, pack8<T>(h[i]));
+        }
+    }
+}
+
+// Without a norm (no reduction to wait for) 64 registers, half the SM's threads,
+// keep most loads in flight: 24000 x 4096 bf16 54 us, with 80 registers 59, 48
+// registers 64.
 template <typename T, bool NORM, bool QUANT, int TPR, int VPT, int ROWS>
-__global__ void __launch_bounds__(TPR *ROWS) rows_kernel(const RowsArgs a) {
+__global__ void __launch_bounds__(TPR *ROWS, NORM ? 1 : 1024 / (TPR * ROWS)) rows_kernel(const RowsArgs a) {
     constexpr int WARPS = TPR / 32; // warps of a row
     __shared__ float part[2][WARPS];
     static_assert(ROWS == 1 || TPR == 32, "a row of one warp, or a CTA for each row");
@@ -125,20 +152,146 @@ __global__ void __launch_bounds__(TPR *ROWS) rows_kernel(const RowsArgs a) {
                 }
             }
         }
+        write_row<T, QUANT, TPR, VPT>(a, row, groups, t, h);
+    }
+}
+
+constexpr int kStreamThreads = 256, kStreamBytes = 96 * 1024, kMaxStages = 8;
+
+__device__ __forceinline__ void bulk_load(uint32_t to, const void *from, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
+                 "l"(from), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// 256 / TPR rows at a time.  Stage: their x, then their residuals, `pitch` bytes
+// each.  Elements go to registers at once, so a stage is filled again while the
+// row is reduced, scaled and written.
+template <typename T, bool NORM, bool QUANT, int TPR, int VPT>
+__global__ void __launch_bounds__(kStreamThreads) rows_stream_kernel(const RowsArgs a, int stages) {
+    constexpr int ROWS = kStreamThreads / TPR, WARPS = TPR / 32;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ uint64_t full[kMaxStages];
+    __shared__ float part[2][kStreamThreads / 32];
+    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+    const bool res = NORM && a.residual != nullptr;
+    const uint32_t pitch = a.cols * sizeof(T), stage_bytes = ROWS * pitch * (res ? 2 : 1);
+    const int groups = (a.cols + kGroup - 1) / kGroup;
+    const long long turns = (a.rows + ROWS - 1) / ROWS;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < stages; ++i)
+            mbar_init(&full[i], 1);
+        fence_mbarrier_init();
+    }
+    __syncthreads();
+    // Rows [turn * ROWS, ..) into a stage (thread 0).
+    int filled = 0;
+    auto fill = [&](long long turn, int stage) {
+        ++filled;
+        const long long row = turn * ROWS;
+        const int rows = static_cast<int>(min(static_cast<long long>(ROWS), a.rows - row));
+        const uint32_t to = smem_u32(ring) + stage * stage_bytes;
+        mbar_arrive_expect_tx(&full[stage], rows * pitch * (res ? 2 : 1));
+        for (int r = 0; r < rows; ++r) {
+            bulk_load(to + r * pitch, static_cast<const T *>(a.x) + (row + r) * a.x_stride, pitch, &full[stage]);
+            if (res)
+                bulk_load(to + (ROWS + r) * pitch, static_cast<const T *>(a.residual) + (row + r) * a.residual_stride,
+                          pitch, &full[stage]);
+        }
+    };
+    if (threadIdx.x == 0)
+        for (int i = 0; i < stages && blockIdx.x + static_cast<long long>(i) * gridDim.x < turns; ++i)
+            fill(blockIdx.x + static_cast<long long>(i) * gridDim.x, i);
+    Vec8<T> w[NORM ? VPT : 1];
+    if constexpr (NORM) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * TPR + t) * 8;
-            if constexpr (QUANT) {
-                const float scale = group_scale(half_warp_max(amax8(h[i])));
-                if (c < a.cols) {
-                    uint8_t *q = static_cast<uint8_t *>(a.out) + row * a.out_stride + c;
-                    *reinterpret_cast<uint2 *>(q) = e4m3x8(h[i], __frcp_rn(scale));
-                    if (t % 16 == 0)
-                        a.scales[row * groups + c / kGroup] = scale;
+            if (c < a.cols)
+                w[i] = load8(static_cast<const T *>(a.weight) + c);
+        }
+    }
+    int n = 0, stage = 0;
+    for (long long turn = blockIdx.x; turn < turns; turn += gridDim.x, ++n) {
+        const bool ok = mbar_wait(&full[stage], (n / stages) & 1, a.err, kErrWaitV);
+        const long long row = turn * ROWS + slot;
+        float h[VPT][8];
+        const uint8_t *from = ring + stage * stage_bytes + slot * pitch;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * TPR + t) * 8;
+            if (c < a.cols) {
+                unpack8(load8(reinterpret_cast<const T *>(from) + c), h[i]);
+                if (res) {
+                    float r[8];
+                    unpack8(load8(reinterpret_cast<const T *>(from + ROWS * pitch) + c), r);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        h[i][e] += r[e];
                 }
-            } else if (c < a.cols) {
-                store8(static_cast<T *>(a.out) + row * a.out_stride + c, pack8<T>(h[i]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    h[i][e] = 0.f;
             }
+        }
+        float sum = 0.f;
+        if constexpr (NORM) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    sum = fmaf(h[i][e], h[i][e], sum);
+            sum = warp_sum(sum);
+            if (WARPS > 1 && threadIdx.x % 32 == 0)
+                part[n & 1][threadIdx.x / 32] = sum;
+        }
+        // Every thread has read the stage (and its row's parts are written).
+        if (!__syncthreads_and(ok))
+            break;
+        const long long next = turn + static_cast<long long>(stages) * gridDim.x;
+        if (threadIdx.x == 0 && next < turns)
+            fill(next, stage);
+        stage = stage + 1 == stages ? 0 : stage + 1;
+        if (row >= a.rows) // whole warps: the last turn's missing rows
+            continue;
+        if (NORM && res) {
+            T *to = static_cast<T *>(a.residual_out) + row * a.residual_out_stride;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int c = (i * TPR + t) * 8;
+                if (c < a.cols)
+                    store8(to + c, pack8<T>(h[i]));
+            }
+        }
+        if constexpr (NORM) {
+            if constexpr (WARPS > 1) {
+                sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < WARPS; ++k)
+                    sum += part[n & 1][slot * WARPS + k];
+            }
+            const float rstd = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                float wf[8];
+                unpack8(w[i], wf);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    h[i][e] = (i * TPR + t) * 8 < a.cols ? h[i][e] * rstd * wf[e] : 0.f;
+            }
+        }
+        write_row<T, QUANT, TPR, VPT>(a, row, groups, t, h);
+    }
+    // After a wait that gave up: every copy lands before the CTA's memory goes.
+    if (threadIdx.x == 0) {
+        for (; n < filled; ++n) {
+            const uint64_t start = globaltimer_ns();
+            while (!mbar_try_wait(smem_u32(&full[n % stages]), (n / stages) & 1))
+                if (globaltimer_ns() - start > kWaitLimitNs) {
+                    atomicOr(a.err, kErrWaitDrain);
+                    break;
+                }
         }
     }
 }
@@ -269,11 +422,37 @@ int sm_count() {
 
 template <typename T, bool NORM, bool QUANT, int TPR, int VPT, int ROWS>
 int launch_rows(const RowsArgs &a, cudaStream_t stream) {
-    // Up to 2048 threads an SM; what the registers do not hold at once waits.
+    // As many CTAs as run at once: every one takes the same number of rows, +-1.
+    static std::atomic<int> resident{0};
+    int each = resident.load(std::memory_order_relaxed);
+    if (!each) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, rows_kernel<T, NORM, QUANT, TPR, VPT, ROWS>,
+                                                          TPR * ROWS, 0) != cudaSuccess ||
+            each < 1)
+            each = 1;
+        resident.store(each, std::memory_order_relaxed);
+    }
     const long long ctas = (a.rows + ROWS - 1) / ROWS;
-    const long long most = static_cast<long long>(sm_count()) * (2048 / (TPR * ROWS));
+    const long long most = static_cast<long long>(sm_count()) * each;
     rows_kernel<T, NORM, QUANT, TPR, VPT, ROWS>
         <<<static_cast<unsigned>(std::min(ctas, most)), TPR * ROWS, 0, stream>>>(a);
+    return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T, bool NORM, bool QUANT, int TPR, int VPT> int launch_stream(const RowsArgs &a, cudaStream_t stream) {
+    constexpr int ROWS = kStreamThreads / TPR;
+    const int stage = ROWS * a.cols * static_cast<int>(sizeof(T)) * (a.residual ? 2 : 1);
+    const int stages = std::max(2, std::min(kMaxStages, kStreamBytes / stage));
+    static std::atomic<unsigned long long> done{0};
+    const cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(rows_stream_kernel<T, NORM, QUANT, TPR, VPT>),
+                                         std::max(kStreamBytes, 2 * 1024 * 8 * static_cast<int>(sizeof(T)) * 2), done);
+    if (e != cudaSuccess)
+        return static_cast<int>(e);
+    const long long turns = (a.rows + ROWS - 1) / ROWS;
+    const int each = 200 * 1024 / (stages * stage); // CTAs on an SM
+    const long long most = static_cast<long long>(sm_count()) * std::max(1, std::min(each, 4));
+    rows_stream_kernel<T, NORM, QUANT, TPR, VPT>
+        <<<static_cast<unsigned>(std::min(turns, most)), kStreamThreads, stages * stage, stream>>>(a, stages);
     return static_cast<int>(cudaGetLastError());
 }
 
@@ -290,6 +469,22 @@ template <typename T, bool NORM, bool QUANT> int launch_typed(const RowsArgs &a,
         const unsigned grid = static_cast<unsigned>(std::min<long long>(a.rows, 8ll * sm_count()));
         rows_scalar_kernel<T, NORM, QUANT><<<grid, 256, 0, stream>>>(a);
         return static_cast<int>(cudaGetLastError());
+    }
+    // Rows enough for every SM to keep its ring busy.  Measured (bf16, residual,
+    // e4m3): 16384 x 8192 151 us against rows_kernel's 173, 16384 x 4096 85 and 101,
+    // 23328 x 1152 40 and 44.  Without a norm rows_kernel is the faster one.
+    if (NORM && vecs <= 1024 && a.rows * vecs >= 64ll * 1024 * 8) {
+        if (vecs <= 32)
+            return launch_stream<T, NORM, QUANT, 32, 1>(a, stream);
+        if (vecs <= 64)
+            return launch_stream<T, NORM, QUANT, 32, 2>(a, stream);
+        if (vecs <= 128)
+            return launch_stream<T, NORM, QUANT, 32, 4>(a, stream);
+        if (vecs <= 256)
+            return launch_stream<T, NORM, QUANT, 64, 4>(a, stream);
+        if (vecs <= 512)
+            return launch_stream<T, NORM, QUANT, 128, 4>(a, stream);
+        return launch_stream<T, NORM, QUANT, 256, 4>(a, stream);
     }
     if (vecs <= 32)
         return launch_rows<T, NORM, QUANT, 32, 1, 4>(a, stream);

@@ -330,3 +330,27 @@ def test_linear_on_two_streams_at_once(ob):
     for i, g in enumerate(got):
         assert torch.equal(g, want[i % 2])
     ob.library().sync_check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,cols", [(32771, 128), (9001, 512), (4099, 1024), (2503, 2048), (1501, 4096), (1031, 8192),
+                                       (3650, 1152), (977, 4304)])
+def test_rms_norm_many_rows(ob, rows, cols, dtype):
+    """Enough rows for the kernel that streams them, the last turn not full; pitched
+    rows, the residual updated in place."""
+    x = _strided(_randn(rows, cols, seed=cols, dtype=dtype), 16)
+    res = _randn(rows, cols, seed=cols + 1, dtype=dtype, scale=3.0)
+    w = _randn(cols, seed=cols, dtype=dtype)
+    h, y = _norm64(x, w, res, 1e-5)
+    q, scales, hq = ob.rms_norm_e4m3(x, w, residual=res, eps=1e-5)
+    _check_quantized(q, scales, y)
+    _check_rounded(hq, h, dtype, 2.0**-24)
+    inplace = _strided(res, 8)
+    got, hout = ob.rms_norm(x, w, residual=inplace, eps=1e-5, residual_out=inplace)
+    _check_rounded(got, y, dtype, 48 * 2.0**-24)
+    assert torch.equal(hout, hq) and bool((inplace._base[:, cols:] == 7).all())
+    got, _ = ob.rms_norm(x, w, eps=1e-5)
+    _check_rounded(got, _norm64(x, w, None, 1e-5)[1], dtype, 48 * 2.0**-24)
+    q, scales = ob.quantize_e4m3(x)
+    _check_quantized(q, scales, x.double())
+    ob.library().sync_check()
