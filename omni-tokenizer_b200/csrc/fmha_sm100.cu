@@ -954,11 +954,36 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
                 const int kv0 = tile_key<MODE>(it, j) + hh * kCols;
                 const bool masked = kv0 + kCols > limit;
                 if constexpr (WIN) {
-                    if (masked || (kv0 < low && kv0 + kCols > p.sinks)) {
+                    // Columns [0, lo) and [hi, 128) are hidden, save the sinks.  A tile
+                    // wholly before the window shows its sinks alone; one whose hidden
+                    // start they cover shows all.  Each bound costs two instructions a
+                    // column only where some row of the warp has it.
+                    int hi = limit - kv0, lo = low - kv0;
+                    const int sk = p.sinks - kv0;
+                    if (lo >= kCols) {
+                        hi = min(hi, sk);
+                        lo = 0;
+                    } else if (sk >= lo) {
+                        lo = 0;
+                    }
+                    if (__any_sync(0xffffffffu, hi < kCols)) {
 #pragma unroll
                         for (int c = 0; c < kCols; ++c)
-                            if (kv0 + c >= limit || (kv0 + c < low && kv0 + c >= p.sinks))
+                            if (c >= hi)
                                 s[c] = -INFINITY;
+                    }
+                    if (__any_sync(0xffffffffu, lo > 0)) {
+                        if (sk <= 0) {
+#pragma unroll
+                            for (int c = 0; c < kCols; ++c)
+                                if (c < lo)
+                                    s[c] = -INFINITY;
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < kCols; ++c)
+                                if (c < lo && c >= sk)
+                                    s[c] = -INFINITY;
+                        }
                     }
                 } else if (masked) {
 #pragma unroll
