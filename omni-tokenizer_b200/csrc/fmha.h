@@ -135,6 +135,7 @@ int attention_rows(const void *q, const void *k, const void *v, void *out, size_
 // Split scratch for attention_rows on 16-bit rows (0 for fp32 or no split).
 size_t attention_rows_split_workspace(size_t n, int batch, int heads, int head_dim, size_t block,
                                       size_t valid, int dtype);
+int fmha_sm_count(); // SMs of the device, looked up once
 bool tma_view_ok(const void *base, const TensorView &v);
 int padded_head_dim(int hd);
 

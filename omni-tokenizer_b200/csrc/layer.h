@@ -7,6 +7,9 @@
 
 namespace omni_b200 {
 
+// SMs of the device (fmha_sm100.cu; looked up once).
+int fmha_sm_count();
+
 // Element types of the layer operators (the values of omni_b200_dtype).
 enum : int { kF32 = 0, kBF16 = 1, kF16 = 2, kE4M3 = 3 };
 

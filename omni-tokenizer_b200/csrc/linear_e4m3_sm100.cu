@@ -612,14 +612,6 @@ template <int T> __global__ void __launch_bounds__(192, 1) linear_e4m3_few(const
     cluster_sync(); // no CTA leaves while another reads its sums
 }
 
-int sm_count() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-        n = 148;
-    return n;
-}
-
 template <int T> int launch_few(LinearParams &p, const LinearArgs &a, int parts, cudaStream_t stream) {
     using S = FewShape<T>;
     int rc = 0;
@@ -683,7 +675,7 @@ int linear_e4m3_launch(const LinearArgs &a, cudaStream_t stream) {
     p.groups = (a.k + kGroup - 1) / kGroup;
     p.out_dtype = a.out_dtype;
     p.err = a.err;
-    const int sms = sm_count();
+    const int sms = fmha_sm_count();
     const long long big = static_cast<long long>((a.m + kBigM - 1) / kBigM) * ((a.n + kBigN - 1) / kBigN);
     if (a.m > 128 && 2 * big >= sms)
         return launch_big(p, a, sms, stream);

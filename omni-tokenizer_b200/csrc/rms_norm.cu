@@ -412,14 +412,6 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T *x, uint8_
     }
 }
 
-int sm_count() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-        n = 148;
-    return n;
-}
-
 template <typename T, bool NORM, bool QUANT, int TPR, int VPT, int ROWS>
 int launch_rows(const RowsArgs &a, cudaStream_t stream) {
     // As many CTAs as run at once: every one takes the same number of rows, +-1.
@@ -433,7 +425,7 @@ int launch_rows(const RowsArgs &a, cudaStream_t stream) {
         resident.store(each, std::memory_order_relaxed);
     }
     const long long ctas = (a.rows + ROWS - 1) / ROWS;
-    const long long most = static_cast<long long>(sm_count()) * each;
+    const long long most = static_cast<long long>(fmha_sm_count()) * each;
     rows_kernel<T, NORM, QUANT, TPR, VPT, ROWS>
         <<<static_cast<unsigned>(std::min(ctas, most)), TPR * ROWS, 0, stream>>>(a);
     return static_cast<int>(cudaGetLastError());
@@ -450,7 +442,7 @@ template <typename T, bool NORM, bool QUANT, int TPR, int VPT> int launch_stream
         return static_cast<int>(e);
     const long long turns = (a.rows + ROWS - 1) / ROWS;
     const int each = 200 * 1024 / (stages * stage); // CTAs on an SM
-    const long long most = static_cast<long long>(sm_count()) * std::max(1, std::min(each, 4));
+    const long long most = static_cast<long long>(fmha_sm_count()) * std::max(1, std::min(each, 4));
     rows_stream_kernel<T, NORM, QUANT, TPR, VPT>
         <<<static_cast<unsigned>(std::min(turns, most)), kStreamThreads, stages * stage, stream>>>(a, stages);
     return static_cast<int>(cudaGetLastError());
@@ -466,7 +458,7 @@ template <typename T, bool NORM, bool QUANT> int launch_typed(const RowsArgs &a,
                      (QUANT ? out % 8 == 0 && a.out_stride % 8 == 0 : out % 16 == 0 && a.out_stride % kAlign == 0);
     const int vecs = a.cols / 8;
     if (!vec || vecs > 2048) {
-        const unsigned grid = static_cast<unsigned>(std::min<long long>(a.rows, 8ll * sm_count()));
+        const unsigned grid = static_cast<unsigned>(std::min<long long>(a.rows, 8ll * fmha_sm_count()));
         rows_scalar_kernel<T, NORM, QUANT><<<grid, 256, 0, stream>>>(a);
         return static_cast<int>(cudaGetLastError());
     }

@@ -422,9 +422,7 @@ int window_tokens_launch(const WindowArgs &a, cudaStream_t stream) {
     p.out_dtype = a.out_dtype;
     const double scale = a.scale > 0 ? a.scale : 1.0 / std::sqrt(static_cast<double>(a.hd));
     p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess)
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int sms = fmha_sm_count();
     // CTAs that split the keys of one tile: until two are on every SM, with two
     // chunks left for each warp.  Measured, 4101 keys x 128: 512 tiles 168 us with
     // one part, 180 with two; 128 tiles 36 and 28 us (four: 30); 32 tiles 38 us

@@ -256,8 +256,8 @@ def attention_rows(q, k, v, heads, block=0, valid=None, fused=False, out_dtype=N
 
 # -------------------------------------------------------- 8-bit layer operators
 # A call with one token is over in a few microseconds on the device, so these
-# helpers keep the host's part short: types and the device's stream are looked up
-# without building tensors' device objects or importing per call.
+# helpers keep the host's part short: every tensor attribute is read once, and the
+# device's stream is looked up without building objects or importing per call.
 class _Torch:
     """torch's names that the helpers use, looked up at their first call."""
 
@@ -266,8 +266,8 @@ class _Torch:
 
         self.codes = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
         self.e4m3, self.f32, self.bf16, self.i32 = torch.float8_e4m3fn, torch.float32, torch.bfloat16, torch.int32
-        self.empty, self.empty_like, self.cuda = torch.empty, torch.empty_like, torch.cuda
-        self.current_device, self.raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
+        self.empty_like, self.cuda, self.current_device = torch.empty_like, torch.cuda, torch.cuda.current_device
+        self.raw_stream = torch._C._cuda_getCurrentRawStream
         if name not in self.__dict__:
             raise AttributeError(name)
         return self.__dict__[name]
@@ -280,35 +280,24 @@ def _refuse(message):
     raise NativeError(INVALID_ARGUMENT, message)
 
 
-def _element_code(what, t):
-    """Type code of a 2-d tensor of one of the element types."""
-    code = _t.codes.get(t.dtype)
-    if code is None or t.dim() != 2:
-        _refuse(f"{what}: need a [rows, cols] tensor of float32, bfloat16 or float16")
-    return code
-
-
-def _checked(what, *tensors):
-    """The device of the first tensor: every one must be there and have contiguous columns."""
+def _device_of(what, *tensors):
+    """The CUDA device that every given tensor is on."""
     device = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if device < 0 or t.get_device() != device:
+        if t is not None and (device < 0 or t.get_device() != device):
             _refuse(f"{what}: every tensor must be on the same CUDA device")
-        if not t.is_contiguous() and t.shape[-1] > 1 and t.stride(-1) != 1:
-            _refuse(f"{what}: columns must be contiguous")
     return device
 
 
-def _row_stride(t):
-    """Elements between rows; a single row's stride does not matter."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _pitch(t):
-    """Row stride of an e4m3 matrix; a single row counts as one padded to 16."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+def _row_stride(what, t, shape):
+    """Elements between the rows of a matrix with contiguous columns; a single row's
+    stride does not matter."""
+    if t.is_contiguous():
+        return shape[1]
+    rows, columns = t.stride()
+    if columns != 1 and shape[1] > 1:
+        _refuse(f"{what}: columns must be contiguous")
+    return rows if shape[0] > 1 else shape[1]
 
 
 def _call(name, device, stream, *args):
@@ -325,38 +314,48 @@ def _call(name, device, stream, *args):
         lib.check(status)
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _matrix(what, t):
+    """(shape, type code) of a matrix of one of the element types."""
+    code, shape = _t.codes.get(t.dtype), t.shape
+    if code is None or len(shape) != 2:
+        _refuse(f"{what}: need a [rows, cols] tensor of float32, bfloat16 or float16")
+    return shape, code
 
 
-def _empty_e4m3(x):
-    """e4m3 of x's shape whose row stride is a multiple of 16, as linear_e4m3 reads it."""
-    rows, cols = x.shape
+def _empty_e4m3(x, rows, cols):
+    """e4m3 [rows, cols] whose row stride is a multiple of 16, as linear_e4m3 reads it."""
     if cols % 16 == 0:
-        return x.new_empty((rows, cols), dtype=_t.e4m3)
-    return x.new_empty((rows, (cols + 15) // 16 * 16), dtype=_t.e4m3)[:, :cols]
+        if x.is_contiguous():
+            return _t.empty_like(x, dtype=_t.e4m3), cols
+        return x.new_empty((rows, cols), dtype=_t.e4m3), cols
+    pitch = (cols + 15) // 16 * 16
+    return x.new_empty((rows, pitch), dtype=_t.e4m3)[:, :cols], pitch
 
 
-def _norm(what, x, weight, residual, residual_out, out, scales, eps, code, out_code, stream):
-    rows, cols = x.shape
-    if weight.shape != (cols,) or weight.dtype != x.dtype:
-        _refuse(f"{what}: weight must be [{cols}] of x's type")
-    stride = out_stride = 0
+def _norm(what, x, shape, code, weight, residual, residual_out, out, out_stride, scales, eps, out_code, stream):
+    rows, cols = shape
+    dtype = x.dtype
+    if weight.shape != (cols,) or weight.dtype != dtype or (cols > 1 and weight.stride(0) != 1):
+        _refuse(f"{what}: weight must be contiguous [{cols}] of x's type")
+    to_ptr = from_ptr = None
+    to_stride = from_stride = 0
     if residual is None:
         if residual_out is not None:
             _refuse(f"{what}: residual_out needs a residual")
     else:
-        if residual_out is None:
-            residual_out = x.new_empty((rows, cols))
-        elif residual_out.shape != x.shape or residual_out.dtype != x.dtype:
-            _refuse(f"{what}: residual_out must have x's shape and type")
-        if residual.shape != x.shape or residual.dtype != x.dtype:
+        if residual.shape != shape or residual.dtype != dtype:
             _refuse(f"{what}: residual must have x's shape and type")
-        stride, out_stride = _row_stride(residual), _row_stride(residual_out)
-    device = _checked(what, x, weight, residual, residual_out, out, scales)
-    _call("omni_b200_rms_norm", device, stream, x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(residual_out),
-          out.data_ptr(), _ptr(scales), rows, cols, _row_stride(x), stride, out_stride, _row_stride(out), eps, code,
-          out_code)
+        if residual_out is None:
+            residual_out, to_stride = _t.empty_like(x) if x.is_contiguous() else x.new_empty(shape), cols
+        elif residual_out.shape != shape or residual_out.dtype != dtype:
+            _refuse(f"{what}: residual_out must have x's shape and type")
+        else:
+            to_stride = _row_stride(what, residual_out, shape)
+        from_stride = _row_stride(what, residual, shape)
+        from_ptr, to_ptr = residual.data_ptr(), residual_out.data_ptr()
+    device = _device_of(what, x, weight, residual, residual_out, out)
+    _call("omni_b200_rms_norm", device, stream, x.data_ptr(), from_ptr, weight.data_ptr(), to_ptr, out.data_ptr(),
+          scales, rows, cols, _row_stride(what, x, shape), from_stride, to_stride, out_stride, eps, code, out_code)
     return residual_out
 
 
@@ -365,61 +364,79 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None, st
 
     Returns (y, h): y = h / sqrt(mean(h^2) + eps) * weight in x's type, h = x + residual
     (None without a residual).  residual_out may be x or residual, out any of them."""
-    code = _element_code("rms_norm", x)
+    shape, code = _matrix("rms_norm", x)
     if out is None:
-        out = x.new_empty(x.shape)
-    elif out.shape != x.shape or out.dtype != x.dtype:
+        out, out_stride = _t.empty_like(x) if x.is_contiguous() else x.new_empty(shape), shape[1]
+    elif out.shape != shape or out.dtype != x.dtype:
         _refuse("rms_norm: out must have x's shape and type")
-    return out, _norm("rms_norm", x, weight, residual, residual_out, out, None, eps, code, code, stream)
+    else:
+        out_stride = _row_stride("rms_norm", out, shape)
+    return out, _norm("rms_norm", x, shape, code, weight, residual, residual_out, out, out_stride, None, eps, code,
+                      stream)
 
 
 def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, residual_out=None, stream=None):
     """rms_norm with its output in e4m3 and an fp32 scale for each 128 columns.
 
     Returns (q, scales, h); q and scales are what linear_e4m3 takes."""
-    code = _element_code("rms_norm_e4m3", x)
-    q = _empty_e4m3(x)
-    scales = x.new_empty((x.shape[0], (x.shape[1] + 127) // 128), dtype=_t.f32)
-    return q, scales, _norm("rms_norm_e4m3", x, weight, residual, residual_out, q, scales, eps, code, E4M3, stream)
+    shape, code = _matrix("rms_norm_e4m3", x)
+    rows, cols = shape
+    q, pitch = _empty_e4m3(x, rows, cols)
+    scales = x.new_empty((rows, (cols + 127) // 128), dtype=_t.f32)
+    return q, scales, _norm("rms_norm_e4m3", x, shape, code, weight, residual, residual_out, q, pitch,
+                            scales.data_ptr(), eps, E4M3, stream)
 
 
 def quantize_e4m3(x, block_rows=1, stream=None):
     """x [rows, cols] in e4m3: (q, scales), a scale for each 128 columns of a row
     (block_rows=1) or each 128 x 128 block (block_rows=128, weights)."""
-    code = _element_code("quantize_e4m3", x)
+    shape, code = _matrix("quantize_e4m3", x)
     if block_rows != 1 and block_rows != 128:
         _refuse("quantize_e4m3: block_rows must be 1 or 128")
-    rows, cols = x.shape
-    device = _checked("quantize_e4m3", x)
-    q = _empty_e4m3(x)
+    rows, cols = shape
+    device = _device_of("quantize_e4m3", x)
+    stride = _row_stride("quantize_e4m3", x, shape)
+    q, pitch = _empty_e4m3(x, rows, cols)
     scales = x.new_empty(((rows + block_rows - 1) // block_rows, (cols + 127) // 128), dtype=_t.f32)
-    _call("omni_b200_quantize_e4m3", device, stream, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols,
-          _row_stride(x), _row_stride(q), block_rows, code)
+    _call("omni_b200_quantize_e4m3", device, stream, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols, stride,
+          pitch, block_rows, code)
     return q, scales
 
 
 def linear_e4m3(a, a_scales, w, w_scales, bias=None, out_dtype=None, out=None, stream=None):
     """a [m, k] times w [n, k] transposed, both e4m3 with scales (quantize_e4m3 with
     block_rows 1 and 128), plus bias [n]: [m, n] of out_dtype (bfloat16)."""
-    if a.dim() != 2 or w.dim() != 2:
-        _refuse("linear_e4m3: a and w must be matrices")
-    (m, k), (n, wk) = a.shape, w.shape
-    if a.dtype != _t.e4m3 or w.dtype != _t.e4m3 or wk != k:
-        _refuse("linear_e4m3: a [m, k] and w [n, k] must be float8_e4m3fn")
+    shape, w_shape = a.shape, w.shape
+    if len(shape) != 2 or len(w_shape) != 2 or a.dtype != _t.e4m3 or w.dtype != _t.e4m3 or w_shape[1] != shape[1]:
+        _refuse("linear_e4m3: a [m, k] and w [n, k] must be float8_e4m3fn matrices")
+    (m, k), n = shape, w_shape[0]
     groups = (k + 127) // 128
-    for s, rows in ((a_scales, m), (w_scales, (n + 127) // 128)):
-        if s.dtype != _t.f32 or s.shape != (rows, groups) or not s.is_contiguous():
-            _refuse(f"linear_e4m3: scales must be contiguous float32 [{rows}, {groups}]")
+    if (a_scales.dtype != _t.f32 or w_scales.dtype != _t.f32 or a_scales.shape != (m, groups)
+            or w_scales.shape != ((n + 127) // 128, groups) or not a_scales.is_contiguous()
+            or not w_scales.is_contiguous()):
+        _refuse(f"linear_e4m3: scales must be contiguous float32 [{m}, {groups}] and [{(n + 127) // 128}, {groups}]")
     if out is None:
-        out = a.new_empty((m, n), dtype=out_dtype or _t.bf16)
+        out = a.new_empty((m, n), dtype=_t.bf16 if out_dtype is None else out_dtype)
+        stride = n
     elif out.shape != (m, n) or (out_dtype is not None and out.dtype != out_dtype):
         _refuse("linear_e4m3: out must be [m, n] of out_dtype")
-    code = _element_code("linear_e4m3 output", out)
-    if bias is not None and (bias.shape != (n,) or bias.dtype != out.dtype):
-        _refuse(f"linear_e4m3: bias must be [{n}] of the output's type")
-    device = _checked("linear_e4m3", a, a_scales, w, w_scales, bias, out)
+    else:
+        stride = _row_stride("linear_e4m3", out, (m, n))
+    dtype = out.dtype
+    code = _t.codes.get(dtype)
+    if code is None:
+        _refuse("linear_e4m3: the output must be float32, bfloat16 or float16")
+    bias_ptr = None
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype != dtype or (n > 1 and bias.stride(0) != 1):
+            _refuse(f"linear_e4m3: bias must be contiguous [{n}] of the output's type")
+        bias_ptr = bias.data_ptr()
+    device = _device_of("linear_e4m3", a, a_scales, w, w_scales, bias, out)
+    # A single row counts as one padded to 16.
+    lda = _row_stride("linear_e4m3", a, shape) if m > 1 else (k + 15) // 16 * 16
+    ldw = _row_stride("linear_e4m3", w, w_shape) if n > 1 else (k + 15) // 16 * 16
     _call("omni_b200_linear_e4m3", device, stream, a.data_ptr(), a_scales.data_ptr(), w.data_ptr(),
-          w_scales.data_ptr(), _ptr(bias), out.data_ptr(), m, n, k, _pitch(a), _pitch(w), _row_stride(out), code)
+          w_scales.data_ptr(), bias_ptr, out.data_ptr(), m, n, k, lda, ldw, stride, code)
     return out
 
 
@@ -435,28 +452,40 @@ def attention_window(q, k, v, window=0, sinks=0, right=0, lengths=None, q_length
     last ones (CUDA int32 tensors).  The query at position p sees `window` keys up to its
     own (window <= 0: all), the first `sinks` keys, and `right` keys past it.  Rows past a
     sequence's queries are left as they are in `out`, undefined in a new one."""
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+    q_shape, k_shape = q.shape, k.shape
+    if len(q_shape) != 4 or len(k_shape) != 4 or v.shape != k_shape:
         _refuse("attention_window: q must be [B, H, Lq, D], k and v [B, Hkv, Lk, D]")
-    B, H, Lq, D = q.shape
-    Bk, Hkv, Lk, Dk = k.shape
+    B, H, Lq, D = q_shape
+    Bk, Hkv, Lk, Dk = k_shape
     if Bk != B or Dk != D:
         _refuse("attention_window: q, k and v must agree in batch and head dimension")
     dtype = q.dtype
     code = _t.codes.get(dtype, F32)
     if code == F32 or k.dtype != dtype or v.dtype != dtype:
         _refuse("attention_window: q, k and v must all be bfloat16, or all float16")
-    for n in (lengths, q_lengths):
-        if n is not None and (n.shape != (B,) or n.dtype != _t.i32 or not n.is_contiguous()):
-            _refuse("attention_window: lengths and q_lengths must be contiguous int32 [B]")
+    pointers = [None, None]
+    for i, n in enumerate((lengths, q_lengths)):
+        if n is not None:
+            if n.shape != (B,) or n.dtype != _t.i32 or not n.is_contiguous():
+                _refuse("attention_window: lengths and q_lengths must be contiguous int32 [B]")
+            pointers[i] = n.data_ptr()
+    out_code = code
     if out is None:
-        out = q.new_empty(q.shape, dtype=out_dtype or dtype)
-    elif out.shape != q.shape or (out_dtype is not None and out.dtype != out_dtype):
+        out = q.new_empty(q_shape, dtype=dtype if out_dtype is None else out_dtype)
+    elif out.shape != q_shape or (out_dtype is not None and out.dtype != out_dtype):
         _refuse("attention_window: out must have q's shape and out_dtype")
-    if out.dtype != dtype and out.dtype != _t.f32:
-        _refuse("attention_window: the output's type must be q's, or float32")
-    device = _checked("attention_window", q, k, v, lengths, q_lengths, out)
-    strides = _STRIDES(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3])
+    if out.dtype != dtype:
+        if out.dtype != _t.f32:
+            _refuse("attention_window: the output's type must be q's, or float32")
+        out_code = F32
+    device = _device_of("attention_window", q, k, v, lengths, q_lengths, out)
+    qb, qh, qt, qd = q.stride()
+    kb, kh, kt, kd = k.stride()
+    vb, vh, vt, vd = v.stride()
+    ob, oh, ot, od = out.stride()
+    if qd != 1 or kd != 1 or vd != 1 or od != 1:
+        _refuse("attention_window: columns must be contiguous")
     _call("omni_b200_attention_window", device, stream, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B, H,
-          Hkv, Lq, Lk, D, strides, _ptr(lengths), _ptr(q_lengths), window, right, sinks, scale, code,
-          _t.codes[out.dtype])
+          Hkv, Lq, Lk, D, _STRIDES(qb, qh, qt, kb, kh, kt, vb, vh, vt, ob, oh, ot), *pointers, window, right, sinks,
+          scale, code, out_code)
     return out
