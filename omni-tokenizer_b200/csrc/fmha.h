@@ -43,10 +43,6 @@ struct FmhaParams {
     float *split_m, *split_l, *split_o; // [part][256], [part][256], [part][256][HDP]
     float scale_log2;
     int *err;
-    // Sliding window (win != 0): L counts queries, kv_len keys; `group` query
-    // heads share a key head.
-    int win, window, right, sinks, kv_len, group;
-    const int *q_lengths; // [batch] queries of each sequence, or nullptr: L
 };
 
 // Parameters of the fp32 split-precision kernel (fmha_f32_sm100.cu): tensor
@@ -89,13 +85,11 @@ struct FmhaArgs {
     // bytes, 256-byte aligned), or nullptr: no split.
     void *split_ws = nullptr;
     size_t split_ws_bytes = 0;
-    // Sliding window (omni_b200_attention_window): window <= 0 is no window.
-    int win = 0, window = 0, right = 0, sinks = 0;
-    const int *q_lengths = nullptr;
 };
 
 // omni_b200_attention_window: q and out [batch, heads, q_len, head_dim], k and v
-// [batch, kv_heads, kv_len, head_dim] with strides in elements (batch, head, token).
+// [batch, kv_heads, kv_len, head_dim] with strides in elements (batch, head, token);
+// window <= 0: none.
 struct WindowArgs {
     const void *q = nullptr, *k = nullptr, *v = nullptr;
     void *out = nullptr;
@@ -109,8 +103,10 @@ struct WindowArgs {
     int *err = nullptr;
 };
 int attention_window(const WindowArgs &a, cudaStream_t stream);
-// Its kernel for few query rows (window_tokens.cu).
+// Its kernels: few query rows for each key head (window_tokens.cu), and blocks of
+// 128 query rows (window_prompt_sm100.cu).
 int window_tokens_launch(const WindowArgs &a, cudaStream_t stream);
+int window_prompt_launch(const WindowArgs &a, cudaStream_t stream);
 
 // Returns 0 on success, a CUDA error code, or a negative/1000+ code for an
 // unsupported shape / tensor-map failure.

@@ -240,57 +240,18 @@ __device__ __forceinline__ void wait_drain(uint64_t *bar, uint32_t parity, int *
     }
 }
 
-// Kernel instances: see fmha_fwd_kernel.
-constexpr int kModePlain = 0, kModeSplit = 1, kModeWindow = 2;
-
 // One work item = 256 query rows of one (batch, head), or (split keys) one
 // part of such an item: KV tiles [kb, kb + T) of the item's T_item tiles.
 struct Item {
     int b, h, q0, valid, T; // T = KV tiles the item (part) needs (0: write zeros)
     int kb;                 // first KV tile
     int part;               // split part slot v (>= 0), or -1: a whole item
-    int rows, pos0;         // window: queries of the sequence, position of its first query
-    int sink_tiles;         // window: the item's KV tiles are [0, sink_tiles) and then [kb, ...)
     bool skip;              // nothing to do (rows past the end / padded-query skip)
 };
 
-// Sliding window (kModeWindow): item r, last query block first, so that with no
-// window the longest items start first, heads and sequences inside.  Query i of
-// a sequence with n keys and m queries stands at position p = n - m + i and sees
-// the keys s < min(n, p + right + 1) with s > p - window or s < sinks, so the
-// item's keys are those its first and last query reach, and the sink tiles
-// before them.
-__device__ __forceinline__ Item decode_window(const FmhaParams &p, int r) {
-    const int per = p.batch * p.heads, block = r / per, bh = r - block * per;
-    Item it;
-    it.q0 = ((p.L + 255) / 256 - 1 - block) * 256;
-    it.b = bh / p.heads;
-    it.h = bh - it.b * p.heads;
-    it.part = -1;
-    const int n = p.lengths ? max(0, min(p.lengths[it.b], p.kv_len)) : p.kv_len;
-    it.valid = n;
-    it.rows = p.q_lengths ? max(0, min(p.q_lengths[it.b], p.L)) : p.L;
-    it.pos0 = n - it.rows;
-    it.skip = it.q0 >= it.rows;
-    const int first = it.pos0 + it.q0, last = it.pos0 + min(it.q0 + 255, it.rows - 1);
-    const int high = max(0, min(n, last + p.right + 1));
-    const int low = p.window > 0 ? max(0, min(first - p.window + 1, high)) : 0;
-    it.sink_tiles = (min(p.sinks, low) + 127) / 128;
-    it.kb = max(low / 128, it.sink_tiles);
-    it.T = it.sink_tiles + max(0, (high + 127) / 128 - it.kb);
-    return it;
-}
-// First key of the item's KV tile j.
-template <int MODE> __device__ __forceinline__ int tile_key(const Item &it, int j) {
-    if (MODE == kModeWindow)
-        return (j < it.sink_tiles ? j : it.kb + j - it.sink_tiles) * 128;
-    return ((MODE == kModeSplit ? it.kb : 0) + j) * 128;
-}
-
 // Item of rank r (sorted order or batch order), all its KV tiles.
 // `tab` is null unless the launch uses the sorted order or split slots.
-template <int MODE> __device__ __forceinline__ Item decode_rank(const FmhaParams &p, const int *tab, int r) {
-    constexpr bool SPLIT = MODE == kModeSplit;
+template <bool SPLIT> __device__ __forceinline__ Item decode_rank(const FmhaParams &p, const int *tab, int r) {
     const int qblocks = (p.L + 255) / 256;
     Item it;
     it.kb = 0;
@@ -337,10 +298,7 @@ template <int MODE> __device__ __forceinline__ Item decode_rank(const FmhaParams
 // order deals rank k*G + c (even k) or k*G + G-1-c (odd k).  Split slots
 // (u >= split_first): the CTA's one part, decoded in the prologue into
 // tab[kSplitSlot..] as (b, h, q0, valid, T, kb, skip).
-template <int MODE> __device__ __forceinline__ Item decode_item(const FmhaParams &p, const int *tab, int u) {
-    constexpr bool SPLIT = MODE == kModeSplit;
-    if (MODE == kModeWindow)
-        return decode_window(p, u);
+template <bool SPLIT> __device__ __forceinline__ Item decode_item(const FmhaParams &p, const int *tab, int u) {
     if (SPLIT && u >= p.split_first) {
         Item it;
         const int v = u - p.split_first;
@@ -361,16 +319,16 @@ template <int MODE> __device__ __forceinline__ Item decode_item(const FmhaParams
         const int G = gridDim.x, k = u / G, c = u - k * G;
         r = k * G + ((k & 1) ? G - 1 - c : c);
     }
-    return decode_rank<MODE>(p, tab, r);
+    return decode_rank<SPLIT>(p, tab, r);
 }
 
 // The first item at or after u (in steps of the grid) that has KV work, or
 // `items` when there is none: the items whose Q, K and V are loaded and whose
 // MMAs are issued.
-template <int MODE>
+template <bool SPLIT>
 __device__ __forceinline__ int next_work_item(const FmhaParams &p, const int *tab, int u, int items) {
     for (; u < items; u += gridDim.x) {
-        const Item it = decode_item<MODE>(p, tab, u);
+        const Item it = decode_item<SPLIT>(p, tab, u);
         if (!it.skip && it.T > 0)
             break;
     }
@@ -378,11 +336,11 @@ __device__ __forceinline__ int next_work_item(const FmhaParams &p, const int *ta
 }
 
 // Loads the two Q tiles of item u into Q slot nq % QBUF once the slot is free.
-template <int HDP, int MODE>
+template <int HDP, bool SPLIT>
 __device__ __forceinline__ bool load_q_tiles(const FmhaParams &p, const int *tab, int u, int nq, uint8_t *sQ,
                                              uint64_t *q_full, uint64_t *q_empty, int *err) {
     using S = FmhaShape<HDP>;
-    const Item it = decode_item<MODE>(p, tab, u);
+    const Item it = decode_item<SPLIT>(p, tab, u);
     const int qs = nq % S::QBUF;
     if (!__all_sync(0xffffffffu,
                     mbar_wait(&q_empty[qs], ((nq / S::QBUF) & 1) ^ 1, err, kErrWaitEmpty)))
@@ -409,12 +367,11 @@ __device__ __forceinline__ void warp_arrive(uint64_t *bar) {
         mbar_arrive(bar);
 }
 
-// kModeSplit: the launch has split slots (p.split_s > 1); kModeWindow: a sliding
-// window.  Separate instances, so that other launches run code without either.
-template <int HDP, bool BF16, int MODE>
+// SPLIT: the launch has split slots (p.split_s > 1); a separate instance so
+// that launches without them run code that has no split branch.
+template <int HDP, bool BF16, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_constant__ FmhaParams p) {
     using S = FmhaShape<HDP>;
-    constexpr bool SPLIT = MODE == kModeSplit, WIN = MODE == kModeWindow;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -489,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
             // Part q of the tail item of rank split_first + w (v = q * tail + w):
             // KV tiles [q T / s, (q + 1) T / s) of the item's T.
             const int v = blockIdx.x, q = v / p.split_tail, w = v - q * p.split_tail;
-            Item it = decode_rank<kModeSplit>(p, tab, p.split_first + w);
+            Item it = decode_rank<true>(p, tab, p.split_first + w);
             const int kb = q * it.T / p.split_s, ke = (q + 1) * it.T / p.split_s;
             *reinterpret_cast<int4 *>(tab + kSplitSlot) = make_int4(it.b, it.h, it.q0, it.valid);
             *reinterpret_cast<int4 *>(tab + kSplitSlot + 4) = make_int4(ke - kb, kb, it.skip ? 1 : 0, 0);
@@ -566,9 +523,9 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
             // K and V loads issued by this CTA (Q tiles are loaded by warp 10).
             int nk = 0, nv = 0;
             bool ok = true;
-            for (int u = next_work_item<MODE>(p, tab, blockIdx.x, items); ok && u < items;
-                 u = next_work_item<MODE>(p, tab, u + gridDim.x, items)) {
-                const Item it = decode_item<MODE>(p, tab, u);
+            for (int u = next_work_item<SPLIT>(p, tab, blockIdx.x, items); ok && u < items;
+                 u = next_work_item<SPLIT>(p, tab, u + gridDim.x, items)) {
+                const Item it = decode_item<SPLIT>(p, tab, u);
                 for (int j = 0; j < it.T; ++j) {
                     const int st = nk % S::STAGES;
                     const uint32_t ph = (nk / S::STAGES) & 1;
@@ -578,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
                     if (elect_one()) {
                         mbar_arrive_expect_tx(&k_full[st], S::TILE_BYTES);
                         load_tile<HDP>(sK + st * S::TILE_BYTES, &p.tk0, &p.tk1, &k_full[st],
-                                       tile_key<MODE>(it, j), WIN ? it.h / p.group : it.h, it.b);
+                                       ((SPLIT ? it.kb : 0) + j) * 128, it.h, it.b);
                     }
                     __syncwarp();
                     ++nk;
@@ -588,10 +545,10 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
                     if (elect_one()) {
                         mbar_arrive_expect_tx(&v_full[st], 128 * 2 * (S::C0 + p.v1_width));
                         uint8_t *vdst = sV + st * S::V_BYTES;
-                        const int row = tile_key<MODE>(it, j), head = WIN ? it.h / p.group : it.h;
-                        tma_load_4d(vdst, &p.tv0, &v_full[st], 0, row, head, it.b);
+                        const int row = ((SPLIT ? it.kb : 0) + j) * 128;
+                        tma_load_4d(vdst, &p.tv0, &v_full[st], 0, row, it.h, it.b);
                         if (S::HDPO > 64 && p.v1_width > 0)
-                            tma_load_4d(vdst + S::V_CH0, &p.tv1, &v_full[st], 64, row, head, it.b);
+                            tma_load_4d(vdst + S::V_CH0, &p.tv1, &v_full[st], 64, row, it.h, it.b);
                     }
                     __syncwarp();
                     ++nv;
@@ -622,27 +579,6 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
             // checked that the allocator returned exactly that address.
             const uint32_t tmem = 0;
             auto commit = [&](uint64_t *bar) { tc_commit_if(leader, bar); };
-            // Window: V rows past the sequence's keys (whatever a cache holds there)
-            // become zeros, since a NaN times P = 0 would not.  The column of ones
-            // stays: TMA does not rewrite it.
-            [[maybe_unused]] auto clear_tail = [&](const Item &it, int j, int st) {
-                const int from = it.valid - tile_key<MODE>(it, j);
-                if (from >= 128)
-                    return;
-                uint8_t *v = sV + st * S::V_BYTES;
-                const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-                for (int x = from * (S::ROW0 / 16) + (threadIdx.x & 31); x < 128 * (S::ROW0 / 16); x += 32)
-                    reinterpret_cast<uint4 *>(v)[x] = zero;
-                if (S::HDPO > 64) {
-                    const int n16 = p.v1_width / 8;
-                    for (int x = from * n16 + (threadIdx.x & 31); x < 128 * n16; x += 32) {
-                        const int row = x / n16, c16 = x - row * n16;
-                        *reinterpret_cast<uint4 *>(v + S::V_CH0 + row * 128 + ((c16 ^ (row & 7)) << 4)) = zero;
-                    }
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-            };
             auto qk = [&](uint32_t qbase, int i, int st) {
                 const uint32_t d = tmem + i * 128;
                 const uint64_t a0 = make_smem_desc(qbase + i * S::TILE_BYTES, 16, 8 * S::ROW0, lay0);
@@ -711,9 +647,9 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
                     commit(&k_empty[st]);
                     return true;
                 };
-                for (int u = next_work_item<MODE>(p, tab, blockIdx.x, items); ok && u < items;) {
-                    const Item it = decode_item<MODE>(p, tab, u);
-                    const int u_next = next_work_item<MODE>(p, tab, u + gridDim.x, items);
+                for (int u = next_work_item<SPLIT>(p, tab, blockIdx.x, items); ok && u < items;) {
+                    const Item it = decode_item<SPLIT>(p, tab, u);
+                    const int u_next = next_work_item<SPLIT>(p, tab, u + gridDim.x, items);
                     const int qs = nq % S::QBUF;
                     const uint32_t qbase = sq + qs * 2 * S::TILE_BYTES;
                     if (!first_s_issued) { // S_i(g0) for the item's first KV tile g0 = kv
@@ -747,8 +683,6 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
                         }
                         if (!(ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (g / S::STAGES) & 1, err, kErrWaitV))))
                             break;
-                        if constexpr (WIN)
-                            clear_tail(it, j, st);
                         for (int i = 0; i < 2; ++i) {
                             if (!(ok = __all_sync(0xffffffffu, mbar_wait(&p_full[i], g & 1, err, kErrWaitP))))
                                 break;
@@ -772,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
                 int nq = 0, kv = 0, n_items = 0;
                 bool ok = true;
                 for (int u = blockIdx.x; ok && u < items; u += gridDim.x) {
-                    const Item it = decode_item<MODE>(p, tab, u);
+                    const Item it = decode_item<SPLIT>(p, tab, u);
                     if (it.skip || it.T == 0)
                         continue;
                     const int qs = nq % S::QBUF;
@@ -798,8 +732,6 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
                         const bool more = j + 1 < it.T;
                         if (!(ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], ph, err, kErrWaitV))))
                             break;
-                        if constexpr (WIN)
-                            clear_tail(it, j, st);
                         if (!(ok = __all_sync(0xffffffffu, mbar_wait(&p_full[0], g & 1, err, kErrWaitP))))
                             break;
                         tc_fence_after();
@@ -845,19 +777,19 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
             // the K/V producer never waits for a Q slot.
             const int i = warp - (kMmaWarp + 1);
             int n_items = 0, nq = 0;
-            int uq = next_work_item<MODE>(p, tab, blockIdx.x, items); // next item whose Q is due
+            int uq = next_work_item<SPLIT>(p, tab, blockIdx.x, items); // next item whose Q is due
             bool ok = true;
             if (i == 0) {
                 for (int k = 0; ok && k < S::QBUF && uq < items; ++k) {
-                    ok = load_q_tiles<HDP, MODE>(p, tab, uq, nq, sQ, q_full, q_empty, err);
+                    ok = load_q_tiles<HDP, SPLIT>(p, tab, uq, nq, sQ, q_full, q_empty, err);
                     ++nq;
-                    uq = next_work_item<MODE>(p, tab, uq + gridDim.x, items);
+                    uq = next_work_item<SPLIT>(p, tab, uq + gridDim.x, items);
                 }
             }
-            for (int u = next_work_item<MODE>(p, tab, blockIdx.x, items); ok && u < items;
-                 u = next_work_item<MODE>(p, tab, u + gridDim.x, items)) {
+            for (int u = next_work_item<SPLIT>(p, tab, blockIdx.x, items); ok && u < items;
+                 u = next_work_item<SPLIT>(p, tab, u + gridDim.x, items)) {
                 if (p.o_tma) {
-                    const Item it = decode_item<MODE>(p, tab, u);
+                    const Item it = decode_item<SPLIT>(p, tab, u);
                     const int qs_out = n_items % S::QBUF;
                     ok = __all_sync(0xffffffffu, mbar_wait(&ebar[i], n_items & 1, err, kErrWaitO));
                     if (!ok)
@@ -881,10 +813,10 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
                     __syncwarp();
                 }
                 if (i == 0 && uq < items) {
-                    if (!(ok = load_q_tiles<HDP, MODE>(p, tab, uq, nq, sQ, q_full, q_empty, err)))
+                    if (!(ok = load_q_tiles<HDP, SPLIT>(p, tab, uq, nq, sQ, q_full, q_empty, err)))
                         break;
                     ++nq;
-                    uq = next_work_item<MODE>(p, tab, uq + gridDim.x, items);
+                    uq = next_work_item<SPLIT>(p, tab, uq + gridDim.x, items);
                 }
             }
             if (i == 0) {
@@ -920,20 +852,15 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
         [[maybe_unused]] int n_sum = 0;
         bool ok = true;
         for (int u = blockIdx.x; ok && u < items; u += gridDim.x) {
-            const Item it = decode_item<MODE>(p, tab, u);
+            const Item it = decode_item<SPLIT>(p, tab, u);
             if (SPLIT && it.part >= 0 && it.part < p.split_tail && threadIdx.x == 0)
                 p.split_hdr[it.part] = make_int4(it.b, it.h, it.q0, it.skip ? 1 : 0); // part 0 of item w
             if (it.skip)
                 continue;
             const int t = it.q0 + i * 128 + r; // query token
             int limit = it.valid;
-            if (!WIN && p.block > 0)
+            if (p.block > 0)
                 limit = min(limit, (t / p.block + 1) * p.block);
-            [[maybe_unused]] int low = 0; // window: keys [sinks, low) are hidden too
-            if constexpr (WIN) {
-                limit = min(limit, it.pos0 + t + p.right + 1);
-                low = p.window > 0 ? it.pos0 + t - p.window + 1 : 0;
-            }
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < it.T; ++j, ++g) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], g & 1, err, kErrWaitS));
@@ -951,41 +878,9 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
                     warp_arrive(&s_free[i]);
                 }
                 float *s = reinterpret_cast<float *>(sraw);
-                const int kv0 = tile_key<MODE>(it, j) + hh * kCols;
+                const int kv0 = ((SPLIT ? it.kb : 0) + j) * 128 + hh * kCols;
                 const bool masked = kv0 + kCols > limit;
-                if constexpr (WIN) {
-                    // Columns [0, lo) and [hi, 128) are hidden, save the sinks.  A tile
-                    // wholly before the window shows its sinks alone; one whose hidden
-                    // start they cover shows all.  Each bound costs two instructions a
-                    // column only where some row of the warp has it.
-                    int hi = limit - kv0, lo = low - kv0;
-                    const int sk = p.sinks - kv0;
-                    if (lo >= kCols) {
-                        hi = min(hi, sk);
-                        lo = 0;
-                    } else if (sk >= lo) {
-                        lo = 0;
-                    }
-                    if (__any_sync(0xffffffffu, hi < kCols)) {
-#pragma unroll
-                        for (int c = 0; c < kCols; ++c)
-                            if (c >= hi)
-                                s[c] = -INFINITY;
-                    }
-                    if (__any_sync(0xffffffffu, lo > 0)) {
-                        if (sk <= 0) {
-#pragma unroll
-                            for (int c = 0; c < kCols; ++c)
-                                if (c < lo)
-                                    s[c] = -INFINITY;
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < kCols; ++c)
-                                if (c < lo && c >= sk)
-                                    s[c] = -INFINITY;
-                        }
-                    }
-                } else if (masked) {
+                if (masked) {
 #pragma unroll
                     for (int c = 0; c < kCols; ++c)
                         if (kv0 + c >= limit)
@@ -1030,10 +925,9 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
                     m = mnew;
                 }
                 float neg_m = -m;
-                if constexpr (SPLIT || WIN) {
-                    // A part past a row's block window, a row whose window starts
-                    // in a later tile: every score of the row is masked so far
-                    // (m = -inf) and P must be 0, not 2^NaN.
+                if constexpr (SPLIT) {
+                    // A part past a row's block window: every score of the row
+                    // is masked so far (m = -inf) and P must be 0, not 2^NaN.
                     neg_m = m == -INFINITY ? 0.f : neg_m;
                 }
                 if (OMNI_FMHA_TURN && (i == 1 || g > 0)) {
@@ -1291,7 +1185,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_fwd_kernel(const __grid_cons
                 warp_arrive(&ebar[i]); // the tile's store warp takes it from here
                 continue;
             }
-            const bool store = t < (WIN ? it.rows : p.L);
+            const bool store = t < p.L;
             const long long base =
                 it.b * p.o_sb + it.h * p.o_sh + static_cast<long long>(t) * p.o_st;
 #pragma unroll
@@ -1496,14 +1390,14 @@ int padded_head_dim(int hd) {
     return -1;
 }
 
-template <int HDP, bool BF16, int MODE> int launch_typed(FmhaParams &p, int grid, cudaStream_t stream) {
+template <int HDP, bool BF16, bool SPLIT> int launch_typed(FmhaParams &p, int grid, cudaStream_t stream) {
     using S = FmhaShape<HDP>;
     static std::atomic<unsigned long long> done{0};
-    const cudaError_t attr = set_smem_limit(reinterpret_cast<const void *>(fmha_fwd_kernel<HDP, BF16, MODE>),
+    const cudaError_t attr = set_smem_limit(reinterpret_cast<const void *>(fmha_fwd_kernel<HDP, BF16, SPLIT>),
                                             S::SMEM_BYTES, done);
     if (attr != cudaSuccess)
         return static_cast<int>(attr);
-    fmha_fwd_kernel<HDP, BF16, MODE><<<grid, kThreads, S::SMEM_BYTES, stream>>>(p);
+    fmha_fwd_kernel<HDP, BF16, SPLIT><<<grid, kThreads, S::SMEM_BYTES, stream>>>(p);
     return static_cast<int>(cudaGetLastError());
 }
 
@@ -1511,12 +1405,9 @@ template <int HDP, bool BF16, int MODE> int launch_typed(FmhaParams &p, int grid
 // split scratch); fmha_launch plans a split for bf16 launches only.
 template <int HDP> int launch_hdp(FmhaParams &p, bool bf16, int grid, cudaStream_t stream) {
     if (p.split_s > 1)
-        return bf16 ? launch_typed<HDP, true, kModeSplit>(p, grid, stream) : -2;
-    if (p.win)
-        return bf16 ? launch_typed<HDP, true, kModeWindow>(p, grid, stream)
-                    : launch_typed<HDP, false, kModeWindow>(p, grid, stream);
-    return bf16 ? launch_typed<HDP, true, kModePlain>(p, grid, stream)
-                : launch_typed<HDP, false, kModePlain>(p, grid, stream);
+        return bf16 ? launch_typed<HDP, true, true>(p, grid, stream) : -2;
+    return bf16 ? launch_typed<HDP, true, false>(p, grid, stream)
+                : launch_typed<HDP, false, false>(p, grid, stream);
 }
 
 int fmha_sm_count() {
@@ -1626,7 +1517,7 @@ int fmha_launch(const FmhaArgs &a, cudaStream_t stream) {
         ov.s_head = a.o_sh;
         ov.s_batch = a.o_sb > 0 ? a.o_sb : a.o_st * a.q.tokens;
         p.o_tma = 0;
-        if (a.out_dtype != kOutF32 && !a.q_lengths && tma_view_ok(a.out, ov) && ov.d % 8 == 0 && ov.d <= hdp) {
+        if (a.out_dtype != kOutF32 && tma_view_ok(a.out, ov) && ov.d % 8 == 0 && ov.d <= hdp) {
             const bool obf = a.out_dtype == kOutBF16;
             if (make_map(&p.to0, a.out, obf, ov, w0, 128) == 0 &&
                 (w1 == 0 || make_map(&p.to1, a.out, obf, ov, w1, 128) == 0))
@@ -1646,13 +1537,6 @@ int fmha_launch(const FmhaArgs &a, cudaStream_t stream) {
     // A window at least as long as the sequence limits nothing: no window
     // (which allows the sorted item order and the key split).
     p.block = a.block >= a.q.tokens ? 0 : a.block;
-    p.win = a.win;
-    p.window = a.window;
-    p.right = a.right;
-    p.sinks = a.sinks;
-    p.kv_len = a.k.tokens;
-    p.group = a.win ? a.q.heads / a.k.heads : 1;
-    p.q_lengths = a.q_lengths;
     p.skip_padded_q = a.skip_padded_q;
     p.out_dtype = a.out_dtype;
     const int esize = a.out_dtype == kOutF32 ? 4 : 2;
@@ -1663,14 +1547,14 @@ int fmha_launch(const FmhaArgs &a, cudaStream_t stream) {
     const double scale = a.scale > 0 ? a.scale : 1.0 / std::sqrt(static_cast<double>(p.hd));
     p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
     p.err = a.err;
-    p.sorted = (!p.win && a.lengths != nullptr && p.block == 0 && a.q.batch > 1 && a.q.batch <= kSortMaxBatch) ? 1 : 0;
+    p.sorted = (a.lengths != nullptr && p.block == 0 && a.q.batch > 1 && a.q.batch <= kSortMaxBatch) ? 1 : 0;
     // Persistent grid: one CTA per SM, each looping over (batch, head, 256-row) items.
     const int sms = fmha_sm_count();
     const long long items = static_cast<long long>(p.batch) * p.heads * ((p.L + 255) / 256);
     int grid_x = static_cast<int>(items < sms ? items : sms);
     // Key split of a partial last round (the whole batch when it has fewer
     // items than SMs); the lengths bound each item's tiles by L.
-    if (a.split_ws && a.bf16 && !p.win) {
+    if (a.split_ws && a.bf16) {
         const int v = a.lengths ? p.L : (p.valid > 0 && p.valid < p.L ? p.valid : p.L);
         const SplitPlan pl = split_plan(items, (v + 127) / 128, p.skip_padded_q);
         if (pl.s > 1 && a.split_ws_bytes >= split_bytes(hdp) &&
@@ -1734,49 +1618,6 @@ int fmha_launch(const FmhaArgs &a, cudaStream_t stream) {
     else
         fmha_split_combine<kSplitMaxParts><<<cgrid, 256, 0, stream>>>(c);
     return static_cast<int>(cudaGetLastError());
-}
-
-// Query rows that share a key head, up to which attention_window takes the
-// kernel for few rows.
-constexpr int kFewRows = 64;
-
-int attention_window(const WindowArgs &a, cudaStream_t stream) {
-    const long long rows = static_cast<long long>(a.heads / a.kv_heads) * a.q_len;
-    if (rows <= kFewRows)
-        return window_tokens_launch(a, stream);
-    FmhaArgs f;
-    f.q_ptr = a.q;
-    f.k_ptr = a.k;
-    f.v_ptr = a.v;
-    auto view = [&](int heads, int tokens, const long long *strides) {
-        TensorView v;
-        v.d = a.hd;
-        v.tokens = tokens;
-        v.heads = heads;
-        v.batch = a.batch;
-        v.s_batch = strides[0];
-        v.s_head = strides[1];
-        v.s_token = strides[2];
-        return v;
-    };
-    f.q = view(a.heads, a.q_len, a.qs);
-    f.k = view(a.kv_heads, a.kv_len, a.ks);
-    f.v = view(a.kv_heads, a.kv_len, a.vs);
-    f.bf16 = a.bf16;
-    f.out = a.out;
-    f.out_dtype = a.out_dtype;
-    f.o_sb = a.os[0];
-    f.o_sh = a.os[1];
-    f.o_st = a.os[2];
-    f.lengths = a.lengths;
-    f.q_lengths = a.q_lengths;
-    f.win = 1;
-    f.window = a.window;
-    f.right = a.right;
-    f.sinks = a.sinks;
-    f.scale = a.scale;
-    f.err = a.err;
-    return fmha_launch(f, stream);
 }
 
 } // namespace omni_b200

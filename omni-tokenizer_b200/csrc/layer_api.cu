@@ -179,7 +179,7 @@ int omni_b200_attention_window(const void *q, const void *k, const void *v, void
         return ctx_fail(1, "attention_window: window, right and sinks must be at most 2^30, right and sinks not negative");
     if (std::isnan(scale) || std::isinf(scale))
         return ctx_fail(1, "attention_window: scale must be finite");
-    if (static_cast<double>(batch) * heads * ((q_len + 255) / 256) > kMost)
+    if (static_cast<double>(batch) * heads * ((q_len + 127) / 128) > kMost)
         return ctx_fail(4, "attention_window: more than 2^30 blocks of queries");
     if (batch == 0 || q_len == 0)
         return 0;
