@@ -8,20 +8,22 @@
 // values, tensor memory and warps of its own: while one waits, another's
 // exponentials use the MUFU (the bound: 16 per clock and SM).  Keys come 64 at a
 // time, starting at the block's first visible key.
-//   NC = 1 (head_dim <= 64): 4 chains, TMEM per chain S [0, 64), O [64, 128).
+//   NC = 1 (head_dim <= 64): 3 chains, TMEM per chain S [0, 64), P [64, 96),
+//     O [96, 160).
 //   NC = 2 (head_dim <= 128): 2 chains, TMEM per chain S0, S1 [0, 128), O
-//     [128, 256); the next scores are computed while the softmax works.
-// P (16-bit pairs) is written over the first 32 columns of its S.
+//     [128, 256); P (16-bit pairs) over the first 32 columns of its S.
+// Either way the next scores are computed while the softmax works on these: with
+// one S as soon as the softmax has it in registers, with two at once.
 //
-// Two barriers tell that O has the product of step g (g & 1): a waiter may be a
-// step behind the products, and one barrier's parity would mistake the step
-// before the last for the one awaited.
-//
-// Per chain: 4 softmax warps (a row per thread = TMEM lane), one warp that loads
-// (TMA, two stages of keys and of values) and one that issues the tensor cores'
-// products.  Exponentials are taken to base 2 with the scale folded in, statistics
-// are fp32; a row keeps a stale maximum until it grows by more than 2^8, so that
-// P <= 2^8 and O is rarely rescaled.
+// Per chain: 4 softmax warps (a row per thread = TMEM lane), one warp that finds the
+// blocks and loads (TMA), and one that issues the tensor cores' products.  The
+// loader publishes each block's description in shared memory, ahead of its use: the
+// divisions and the reads of the lengths stay off the other warps' path.
+// Exponentials are taken to base 2 with the scale folded in, statistics are fp32; a
+// row keeps a stale maximum until it grows by more than 2^8, so that P <= 2^8 and O
+// is rarely rescaled.  Two barriers tell that O has the product of step g (g & 1): a
+// waiter may be a step behind the products, and one barrier's parity would mistake
+// the step before the last for the one awaited.
 //
 // Tiles hold 64 columns (128 bytes, 128-byte swizzle) per row and chunk; columns
 // past head_dim and rows past the tensor are TMA's zero fill.  Rows of v past a
@@ -37,7 +39,6 @@ namespace omni_b200 {
 namespace {
 
 constexpr int kKeys = 64;    // keys of a step
-constexpr int kStages = 2;   // steps of keys and values in flight
 constexpr int kMaxBatch = 496; // sequences that the item table holds
 
 struct PromptParams {
@@ -53,18 +54,18 @@ struct PromptParams {
 };
 
 template <int NC> struct PromptShape {
-    static constexpr int CHAINS = NC == 1 ? 4 : 2;
-    static constexpr int NS = NC; // S buffers
+    static constexpr int CHAINS = NC == 1 ? 3 : 2;
+    static constexpr int STAGES = NC == 1 ? 3 : 2; // of keys, and of values
     static constexpr int SOFT_WARPS = CHAINS * 4, ISSUE_WARP = SOFT_WARPS + CHAINS;
-    static constexpr int THREADS = (SOFT_WARPS + 2 * CHAINS) * 32;
-    // Registers: 768 x 80 at launch = 512 x 96 + 256 x 48; 384 x 168 = 256 x 216 + 128 x 72.
-    static constexpr int SOFT_REGS = NC == 1 ? 96 : 216, CONTROL_REGS = NC == 1 ? 48 : 72;
+    static constexpr int THREADS = (SOFT_WARPS + 2 * CHAINS + 3) / 4 * 128; // whole warpgroups
+    // Registers: 640 x 96 at launch = 384 x 112 + 256 x 72; 384 x 168 = 256 x 216 + 128 x 72.
+    static constexpr int SOFT_REGS = NC == 1 ? 112 : 216, CONTROL_REGS = 72;
     static constexpr int Q_BYTES = NC * 128 * 128, KV_BYTES = NC * kKeys * 128;
-    static constexpr int CHAIN_BYTES = Q_BYTES + 2 * kStages * KV_BYTES;
-    static constexpr uint32_t COLS = 512 / CHAINS, O_COL = 64 * NS;
-    static constexpr int BARS = 18; // per chain
+    static constexpr int CHAIN_BYTES = Q_BYTES + 2 * STAGES * KV_BYTES;
+    static constexpr uint32_t COLS = NC == 1 ? 160 : 256, O_COL = NC == 1 ? 96 : 128;
+    static constexpr int BARS = 26, BLOCK_INTS = 12; // per chain; per published block (two of them)
     static constexpr int TABLE_BYTES = (2 * kMaxBatch + 1) * 4;
-    static constexpr int SMEM = CHAINS * CHAIN_BYTES + CHAINS * BARS * 8 + 16 + TABLE_BYTES + 1024;
+    static constexpr int SMEM = CHAINS * (CHAIN_BYTES + BARS * 8 + 2 * BLOCK_INTS * 4) + 16 + TABLE_BYTES + 1024;
     static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -109,7 +110,6 @@ struct Block {
     int b, h, q0, n, rows, pos0;
     int sink_steps, base, steps;
     bool skip; // no rows
-    __device__ __forceinline__ int key(int j) const { return j < sink_steps ? j * kKeys : base + (j - sink_steps) * kKeys; }
 };
 
 __device__ __forceinline__ int held_keys(const PromptParams &p, int b) {
@@ -164,14 +164,9 @@ __device__ __forceinline__ Block block_at(const PromptParams &p, const int *tabl
     return it;
 }
 
-// The first block at or after u (in steps of `chains`) that has keys, or `blocks`.
-__device__ __forceinline__ int next_block(const PromptParams &p, const int *table, int u, int chains, int blocks, Block &it) {
-    for (; u < blocks; u += chains) {
-        it = block_at(p, table, u, chains);
-        if (!it.skip && it.steps > 0)
-            break;
-    }
-    return u;
+// First key of step j.
+__device__ __forceinline__ int step_key(int j, int sink_steps, int base) {
+    return j * kKeys + (j < sink_steps ? 0 : base - sink_steps * kKeys);
 }
 
 template <int NC, bool BF16>
@@ -181,7 +176,8 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t *all_bars = reinterpret_cast<uint64_t *>(smem + S::CHAINS * S::CHAIN_BYTES);
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(all_bars + S::CHAINS * S::BARS);
-    int *table = reinterpret_cast<int *>(tmem_holder + 4);
+    int *published = reinterpret_cast<int *>(tmem_holder + 4); // [chain][2][BLOCK_INTS]
+    int *table = published + S::CHAINS * 2 * S::BLOCK_INTS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *err = p.err;
 
@@ -210,7 +206,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
         for (int c = 0; c < S::CHAINS; ++c) {
             uint64_t *bar = all_bars + c * S::BARS;
             for (int i = 0; i < S::BARS; ++i)
-                mbar_init(&bar[i], i == 12 || i == 15 ? 4 : 1); // p_full, o_free: one arrive per softmax warp
+                mbar_init(&bar[i], i >= 24 ? 5 : i >= 19 && i < 22 ? 4 : 1);
         }
         fence_mbarrier_init();
     }
@@ -228,23 +224,58 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
     const int chains = gridDim.x * S::CHAINS, mine = chain * gridDim.x + blockIdx.x;
     const int per_block = p.table ? table[kMaxBatch + p.batch] : p.batch * p.heads * ((p.q_len + 127) / 128);
     const int blocks = (per_block + chains - 1) / chains * chains; // whole rounds: their last may be empty
-    uint8_t *sq = smem + chain * S::CHAIN_BYTES, *sk = sq + S::Q_BYTES, *sv = sk + kStages * S::KV_BYTES;
+    uint8_t *sq = smem + chain * S::CHAIN_BYTES, *sk = sq + S::Q_BYTES, *sv = sk + S::STAGES * S::KV_BYTES;
     uint64_t *bar = all_bars + chain * S::BARS;
-    uint64_t *q_full = bar, *q_empty = bar + 1, *k_full = bar + 2, *k_empty = bar + 4, *v_full = bar + 6,
-             *v_empty = bar + 8, *s_full = bar + 10, *p_full = bar + 12, *pv_done = bar + 13, *o_free = bar + 15,
-             *drain = bar + 16;
+    uint64_t *q_full = bar, *q_empty = bar + 1, *k_full = bar + 2, *k_empty = bar + 5, *v_full = bar + 8,
+             *v_empty = bar + 11, *s_full = bar + 14, *pv_done = bar + 16, *drain = bar + 18;
+    uint64_t *p_full = bar + 19, *o_free = bar + 20, *s_free = bar + 21; // an arrive of each softmax warp
+    uint64_t *block_full = bar + 22, *block_empty = bar + 24;            // [2]; read by five warps
+    static_assert(S::STAGES <= 3, "barrier places");
+    int *mine_published = published + chain * 2 * S::BLOCK_INTS;
     const uint32_t tm = tmem + chain * S::COLS;
 
     if (warp >= S::SOFT_WARPS) {
         reg_dec<S::CONTROL_REGS>();
         if (warp < S::ISSUE_WARP) {
-            // ---------------------------------------------------------- loads
-            int n = 0, items = 0;
+            // ------------------------------------------------- blocks and loads
+            int nk = 0, nv = 0, items = 0, listed = 0;
             bool ok = true;
-            Block it;
-            for (int u = next_block(p, table, mine, chains, blocks, it); ok && u < blocks;
-                 u = next_block(p, table, u + chains, chains, blocks, it), ++items) {
-                const int kv_head = it.h / p.group;
+            auto publish = [&](const Block &it) {
+                const int slot = listed & 1;
+                if (!warp_wait(&block_empty[slot], ((listed >> 1) & 1) ^ 1, err, kErrWaitEmpty))
+                    return false;
+                if (lane == 0) {
+                    int *to = mine_published + slot * S::BLOCK_INTS;
+                    to[0] = it.b, to[1] = it.h, to[2] = it.q0, to[3] = it.n, to[4] = it.rows;
+                    to[5] = it.sink_steps, to[6] = it.base, to[7] = it.steps;
+                    mbar_arrive(&block_full[slot]);
+                }
+                __syncwarp();
+                ++listed;
+                return true;
+            };
+            auto load = [&](uint8_t *to, const CUtensorMap *map, uint64_t *full, uint64_t *empty, int &n, int key, int head, int b) {
+                const int st = n % S::STAGES;
+                if (!warp_wait(&empty[st], ((n / S::STAGES) & 1) ^ 1, err, kErrWaitEmpty))
+                    return false;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(&full[st], S::KV_BYTES);
+                    for (int c = 0; c < NC; ++c)
+                        tma_load_4d(to + st * S::KV_BYTES + c * kKeys * 128, map, &full[st], c * 64, key, head, b);
+                }
+                __syncwarp();
+                ++n;
+                return true;
+            };
+            for (int u = mine; ok && u < blocks; u += chains) {
+                const Block it = block_at(p, table, u, chains);
+                if (it.skip)
+                    continue;
+                if (!(ok = publish(it)))
+                    break;
+                if (it.steps == 0)
+                    continue;
+                const int head = it.h / p.group;
                 if (!(ok = warp_wait(q_empty, (items & 1) ^ 1, err, kErrWaitEmpty)))
                     break;
                 if (elect_one()) {
@@ -253,54 +284,43 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                         tma_load_4d(sq + c * 128 * 128, &p.tq, q_full, c * 64, it.q0, it.h, it.b);
                 }
                 __syncwarp();
-                for (int j = 0; j < it.steps; ++j, ++n) {
-                    const int st = n % kStages, key = it.key(j);
-                    const uint32_t ph = ((n / kStages) & 1) ^ 1;
-                    if (!(ok = warp_wait(&k_empty[st], ph, err, kErrWaitEmpty)))
-                        break;
-                    if (elect_one()) {
-                        mbar_arrive_expect_tx(&k_full[st], S::KV_BYTES);
-                        for (int c = 0; c < NC; ++c)
-                            tma_load_4d(sk + st * S::KV_BYTES + c * kKeys * 128, &p.tk, &k_full[st], c * 64, key, kv_head, it.b);
-                    }
-                    __syncwarp();
-                    if (!(ok = warp_wait(&v_empty[st], ph, err, kErrWaitEmpty))) {
-                        // K of this step is in flight: its slot alone is waited for below.
-                        drain_wait(&k_full[st], (n / kStages) & 1, err);
-                        break;
-                    }
-                    if (elect_one()) {
-                        mbar_arrive_expect_tx(&v_full[st], S::KV_BYTES);
-                        for (int c = 0; c < NC; ++c)
-                            tma_load_4d(sv + st * S::KV_BYTES + c * kKeys * 128, &p.tv, &v_full[st], c * 64, key, kv_head, it.b);
-                    }
-                    __syncwarp();
+                ++items;
+                // Keys a step ahead of values: they are wanted a step earlier.
+                ok = load(sk, &p.tk, k_full, k_empty, nk, step_key(0, it.sink_steps, it.base), head, it.b);
+                for (int j = 0; ok && j < it.steps; ++j) {
+                    if (j + 1 < it.steps)
+                        ok = load(sk, &p.tk, k_full, k_empty, nk, step_key(j + 1, it.sink_steps, it.base), head, it.b);
+                    ok = ok && load(sv, &p.tv, v_full, v_empty, nv, step_key(j, it.sink_steps, it.base), head, it.b);
                 }
-                if (!ok) {
-                    drain_wait(q_full, items & 1, err);
-                    break;
-                }
+            }
+            if (ok) {
+                Block end{};
+                end.steps = -1;
+                publish(end);
             }
             // Every copy lands before the CTA ends.
             if (items > 0)
                 drain_wait(q_full, (items - 1) & 1, err);
-            for (int j = max(0, n - kStages); j < n; ++j) {
-                drain_wait(&k_full[j % kStages], (j / kStages) & 1, err);
-                drain_wait(&v_full[j % kStages], (j / kStages) & 1, err);
-            }
-        } else {
+            for (int j = max(0, nk - S::STAGES); j < nk; ++j)
+                drain_wait(&k_full[j % S::STAGES], (j / S::STAGES) & 1, err);
+            for (int j = max(0, nv - S::STAGES); j < nv; ++j)
+                drain_wait(&v_full[j % S::STAGES], (j / S::STAGES) & 1, err);
+        } else if (warp < S::ISSUE_WARP + S::CHAINS) {
             // ------------------------------------------------------- products
             constexpr uint32_t idesc_s = make_idesc_f16(128, kKeys, BF16, false);
             const int ksteps = (p.hd + 15) / 16;
             const uint32_t idesc_o = make_idesc_f16(128, ksteps * 16, BF16, true);
             const uint32_t leader = elect_one() ? 1u : 0u;
             const uint32_t aq = smem_u32(sq), ak = smem_u32(sk), av = smem_u32(sv);
-            int n = 0, items = 0;
+            int n = 0, items = 0, listed = 0;
             bool ok = true;
             // S of step g (of the chain's steps), from its K stage.
             auto scores = [&](int g) {
-                const int st = g % kStages;
-                if (!warp_wait(&k_full[st], (g / kStages) & 1, err, kErrWaitK))
+                const int st = g % S::STAGES;
+                if (!warp_wait(&k_full[st], (g / S::STAGES) & 1, err, kErrWaitK))
+                    return false;
+                // One S: the softmax has the last scores in registers.
+                if (NC == 1 && g > 0 && !warp_wait(s_free, (g - 1) & 1, err, kErrWaitS))
                     return false;
                 tc_fence_after();
                 const uint32_t d = tm + (NC == 2 ? (g & 1) * 64 : 0);
@@ -316,31 +336,37 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                 tc_commit_if(leader, &k_empty[st]);
                 return true;
             };
-            Block it;
-            for (int u = next_block(p, table, mine, chains, blocks, it); ok && u < blocks;
-                 u = next_block(p, table, u + chains, chains, blocks, it), ++items) {
-                if (!(ok = warp_wait(q_full, items & 1, err, kErrWaitQ)))
+            while (true) {
+                const int slot = listed & 1;
+                if (!warp_wait(&block_full[slot], (listed >> 1) & 1, err, kErrWaitQ))
                     break;
-                if (NC == 2 && !(ok = scores(n)))
+                const int *from = mine_published + slot * S::BLOCK_INTS;
+                const int keys = from[3], sink_steps = from[5], base = from[6], steps = from[7];
+                warp_arrive(&block_empty[slot]);
+                ++listed;
+                if (steps < 0)
                     break;
-                if (NC == 2 && it.steps == 1)
+                if (steps == 0)
+                    continue;
+                if (!(ok = warp_wait(q_full, items & 1, err, kErrWaitQ)) || !(ok = scores(n)))
+                    break;
+                if (steps == 1) // every product that reads Q is issued
                     tc_commit_if(leader, q_empty);
-                for (int j = 0; j < it.steps; ++j, ++n) {
-                    const int st = n % kStages;
-                    if (NC == 1 || j + 1 < it.steps) {
-                        const bool last = j + NC == it.steps;
-                        if (!(ok = scores(n + NC - 1)))
+                for (int j = 0; j < steps; ++j, ++n) {
+                    const int st = n % S::STAGES;
+                    if (j + 1 < steps) {
+                        if (!(ok = scores(n + 1)))
                             break;
-                        if (last) // every product that reads Q is issued
+                        if (j + 2 == steps)
                             tc_commit_if(leader, q_empty);
                     }
-                    if (!(ok = warp_wait(&v_full[st], (n / kStages) & 1, err, kErrWaitV)))
+                    if (!(ok = warp_wait(&v_full[st], (n / S::STAGES) & 1, err, kErrWaitV)))
                         break;
-                    const int from = it.n - it.key(j); // V rows from here on are past the sequence
-                    if (from < kKeys) {
-                        for (int x = lane; x < NC * (kKeys - from) * 8; x += 32) {
-                            const int c = x / ((kKeys - from) * 8), y = x - c * (kKeys - from) * 8;
-                            *reinterpret_cast<uint4 *>(sv + st * S::KV_BYTES + c * kKeys * 128 + from * 128 + y * 16) =
+                    const int past = keys - step_key(j, sink_steps, base); // V rows from here on are past the sequence
+                    if (past < kKeys) {
+                        for (int x = lane; x < NC * (kKeys - past) * 8; x += 32) {
+                            const int c = x / ((kKeys - past) * 8), y = x - c * (kKeys - past) * 8;
+                            *reinterpret_cast<uint4 *>(sv + st * S::KV_BYTES + c * kKeys * 128 + past * 128 + y * 16) =
                                 make_uint4(0u, 0u, 0u, 0u);
                         }
                         fence_proxy_async_smem();
@@ -353,7 +379,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                         break;
                     tc_fence_after();
                     const uint64_t v0 = make_smem_desc(av + st * S::KV_BYTES, kKeys * 128, 1024, kLayoutSW128);
-                    const uint32_t a = tm + (NC == 2 ? (n & 1) * 64 : 0);
+                    const uint32_t a = tm + (NC == 2 ? (n & 1) * 64 : 64);
 #pragma unroll
                     for (int k = 0; k < kKeys / 16; ++k)
                         umma_ts_if(leader, tm + S::O_COL, a + k * 8, v0 + static_cast<uint64_t>((k * 16 * 128) >> 4), idesc_o,
@@ -361,6 +387,9 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                     tc_commit_if(leader, &pv_done[n & 1]);
                     tc_commit_if(leader, &v_empty[st]);
                 }
+                if (!ok)
+                    break;
+                ++items;
             }
             tc_commit_if(leader, drain);
             drain_wait(drain, 0, err);
@@ -373,16 +402,25 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
         const uint32_t lanes = tm + (static_cast<uint32_t>(quarter * 32) << 16);
         const float sl2 = p.scale_log2;
         const int chunks = (p.hd + 15) / 16; // of O, 16 columns each
-        int g = 0;
+        int g = 0, listed = 0;
         bool ok = true;
-        for (int u = mine; ok && u < blocks; u += chains) {
-            const Block it = block_at(p, table, u, chains);
-            if (it.skip)
-                continue;
-            const int t = it.q0 + row, pos = it.pos0 + t;
-            const int limit = min(it.n, pos + p.right + 1), low = p.window > 0 ? pos - p.window + 1 : 0;
+        while (true) {
+            const int slot = listed & 1;
+            if (!warp_wait(&block_full[slot], (listed >> 1) & 1, err, kErrWaitQ))
+                break;
+            // What outlives the scores' registers: few values.
+            const int *from = mine_published + slot * S::BLOCK_INTS;
+            const int t = from[2] + row, pos = from[3] - from[4] + t;
+            const int limit = min(from[3], pos + p.right + 1), low = p.window > 0 ? pos - p.window + 1 : 0;
+            const int sink_steps = from[5], start = from[6], steps = from[7];
+            const bool store = t < from[4];
+            const long long base = from[0] * p.o_sb + from[1] * p.o_sh + static_cast<long long>(t) * p.o_st;
+            warp_arrive(&block_empty[slot]);
+            ++listed;
+            if (steps < 0)
+                break;
             float m = -INFINITY, l = 0.f;
-            for (int j = 0; j < it.steps; ++j, ++g) {
+            for (int j = 0; j < steps; ++j, ++g) {
                 const uint32_t ts = lanes + (NC == 2 ? (g & 1) * 64 : 0);
                 if (!(ok = warp_wait(&s_full[NC == 2 ? g & 1 : 0], (NC == 2 ? g >> 1 : g) & 1, err, kErrWaitS)))
                     break;
@@ -391,11 +429,15 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                 tmem_ld32(ts, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
                 tmem_ld32(ts + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
                 tmem_wait_ld();
+                if constexpr (NC == 1) { // the next scores may overwrite these
+                    tc_fence_before();
+                    warp_arrive(s_free);
+                }
                 float *s = reinterpret_cast<float *>(raw);
                 // Columns [0, lo) and [hi, 64) are hidden, save the sinks.  A step wholly
                 // before the window shows its sinks alone; one whose hidden start they
                 // cover shows all.  A bound is tested only where some row has it.
-                const int key = it.key(j), sk = p.sinks - key;
+                const int key = step_key(j, sink_steps, start), sk = p.sinks - key;
                 int hi = limit - key, lo = low - key;
                 if (lo >= kKeys) {
                     hi = min(hi, sk);
@@ -450,12 +492,14 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                     raw[c + 1] = pack_pair<BF16>(x2, x3);
                 }
                 l += (a0 + a1) + (b0 + b1);
-                if (j > 0 && __any_sync(0xffffffffu, grow)) {
-                    // O holds the products up to the last step's, which with one S buffer
-                    // came before this S.
-                    if (NC == 2 && !(ok = warp_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, kErrWaitO)))
+                // The last product is done: its P may be overwritten (one P), O rescaled.
+                const bool rescale = j > 0 && __any_sync(0xffffffffu, grow);
+                if ((NC == 1 && g > 0) || rescale) {
+                    if (!(ok = warp_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, kErrWaitO)))
                         break;
                     tc_fence_after();
+                }
+                if (rescale) {
                     for (int c = 0; c < chunks; ++c) {
                         uint32_t o[16];
                         tmem_ld16(lanes + S::O_COL + c * 16, o);
@@ -467,7 +511,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                     }
                 }
                 __syncwarp();
-                tmem_st32(ts, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
+                tmem_st32(NC == 2 ? ts : lanes + 64, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
                 tmem_wait_st();
                 tc_fence_before();
                 warp_arrive(p_full);
@@ -475,16 +519,14 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
             if (!ok)
                 break;
             const float inv = l > 0.f ? 1.f / l : 0.f;
-            const bool store = t < it.rows;
-            const long long base = it.b * p.o_sb + it.h * p.o_sh + static_cast<long long>(t) * p.o_st;
-            if (it.steps > 0) {
+            if (steps > 0) {
                 if (!(ok = warp_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, kErrWaitO)))
                     break;
                 tc_fence_after();
             }
             for (int c = 0; c < chunks; ++c) {
                 uint32_t o[16];
-                if (it.steps > 0) {
+                if (steps > 0) {
                     tmem_ld16(lanes + S::O_COL + c * 16, o);
                     tmem_wait_ld();
                 } else {
@@ -492,7 +534,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                     for (int e = 0; e < 16; ++e)
                         o[e] = 0u;
                 }
-                if (c + 1 == chunks && it.steps > 0) {
+                if (c + 1 == chunks && steps > 0) {
                     tc_fence_before();
                     warp_arrive(o_free);
                 }
