@@ -39,7 +39,8 @@ namespace omni_b200 {
 namespace {
 
 constexpr int kKeys = 64;    // keys of a step
-constexpr int kMaxBatch = 496; // sequences that the item table holds
+constexpr int kBoxBytes = 32 * 64; // a warp's 32 output rows, 64 bytes at a time
+constexpr int kMaxBatch = 496; // sequences that the table in shared memory holds
 
 struct PromptParams {
     CUtensorMap tq, tk, tv;
@@ -63,9 +64,19 @@ template <int NC> struct PromptShape {
     static constexpr int Q_BYTES = NC * 128 * 128, KV_BYTES = NC * kKeys * 128;
     static constexpr int CHAIN_BYTES = Q_BYTES + 2 * STAGES * KV_BYTES;
     static constexpr uint32_t COLS = NC == 1 ? 160 : 256, O_COL = NC == 1 ? 96 : 128;
+    // Barriers by their byte offsets.  k_*, v_*: one per stage; s_full, pv_done: by the
+    // step's parity; block_*: by the block's.  An arrive of each softmax warp: p_full,
+    // o_free, s_free; of those and the issuer: block_empty.
+    static constexpr uint32_t Q_FULL = 0, Q_EMPTY = 8, K_FULL = 2 * 8, K_EMPTY = 5 * 8, V_FULL = 8 * 8, V_EMPTY = 11 * 8,
+                              S_FULL = 14 * 8, PV_DONE = 16 * 8, DRAIN = 18 * 8, P_FULL = 19 * 8, O_FREE = 20 * 8,
+                              S_FREE = 21 * 8, BLOCK_FULL = 22 * 8, BLOCK_EMPTY = 24 * 8;
+    static_assert(STAGES <= 3, "barrier places");
     static constexpr int BARS = 26, BLOCK_INTS = 12; // per chain; per published block (two of them)
-    static constexpr int TABLE_BYTES = (2 * kMaxBatch + 1) * 4;
-    static constexpr int SMEM = CHAINS * (CHAIN_BYTES + BARS * 8 + 2 * BLOCK_INTS * 4) + 16 + TABLE_BYTES + 1024;
+    static constexpr int TABLE_BYTES = (4 * kMaxBatch + 1) * 4; // keys, rows, and (ragged) seq, pre
+    static constexpr int BOXES_AT = CHAINS * CHAIN_BYTES, BARS_AT = BOXES_AT + SOFT_WARPS * kBoxBytes;
+    static constexpr int TMEM_AT = BARS_AT + CHAINS * BARS * 8, BLOCKS_AT = TMEM_AT + 16;
+    static constexpr int TABLE_AT = BLOCKS_AT + CHAINS * 2 * BLOCK_INTS * 4;
+    static constexpr int SMEM = TABLE_AT + TABLE_BYTES + 1024;
     static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -75,25 +86,73 @@ template <int N> __device__ __forceinline__ void reg_inc() {
 template <int N> __device__ __forceinline__ void reg_dec() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, int *err, int code) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+// Shared memory by 32-bit addresses throughout: the scores leave few registers.
+// Bounded like mbar_wait; the whole warp goes on or gives up together.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int *err, int code) {
+    bool ok = mbar_try_wait(bar, parity);
+    if (__all_sync(0xffffffffu, ok))
+        return true;
+    const uint64_t start = globaltimer_ns();
+    for (uint32_t i = 1; !ok; ++i) {
+        ok = mbar_try_wait(bar, parity);
+        if (!ok && (i & 127u) == 0) {
+            if (*reinterpret_cast<volatile int *>(err) != 0)
+                break;
+            if (globaltimer_ns() - start > kWaitLimitNs) {
+                atomicOr(err, code);
+                break;
+            }
+        }
+    }
+    return __all_sync(0xffffffffu, ok);
 }
 // Bounded by time only: nothing may be in flight when the CTA ends.
-__device__ __forceinline__ void drain_wait(uint64_t *bar, uint32_t parity, int *err) {
-    const uint32_t a = smem_u32(bar);
+__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity, int *err) {
     const uint64_t start = globaltimer_ns();
-    while (!mbar_try_wait(a, parity)) {
+    while (!mbar_try_wait(bar, parity)) {
         if (globaltimer_ns() - start > kWaitLimitNs) {
             atomicOr(err, kErrWaitDrain);
             return;
         }
     }
 }
+__device__ __forceinline__ void arrive(uint32_t bar) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)
+                 : "memory");
+}
 // One arrive per warp, after its lanes.
-__device__ __forceinline__ void warp_arrive(uint64_t *bar) {
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
     __syncwarp();
     if ((threadIdx.x & 31) == 0)
-        mbar_arrive(bar);
+        arrive(bar);
+}
+__device__ __forceinline__ void commit_if(uint32_t issue, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+                 "r"(issue)
+                 : "memory");
+}
+__device__ __forceinline__ void load_4d(uint32_t to, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2, int c3) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(to),
+                 "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+                 : "memory");
+}
+__device__ __forceinline__ int get(uint32_t at) {
+    int v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 get16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void put16(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 template <bool BF16> __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     if constexpr (BF16) {
@@ -112,11 +171,12 @@ struct Block {
     bool skip; // no rows
 };
 
-__device__ __forceinline__ int held_keys(const PromptParams &p, int b) {
-    return p.lengths ? max(0, min(p.lengths[b], p.kv_len)) : p.kv_len;
+// Keys and queries of sequence b, from the table in shared memory while it has room.
+__device__ __forceinline__ int held_keys(const PromptParams &p, const int *table, int b) {
+    return p.batch <= kMaxBatch ? table[b] : p.lengths ? max(0, min(p.lengths[b], p.kv_len)) : p.kv_len;
 }
-__device__ __forceinline__ int held_rows(const PromptParams &p, int b) {
-    return p.q_lengths ? max(0, min(p.q_lengths[b], p.q_len)) : p.q_len;
+__device__ __forceinline__ int held_rows(const PromptParams &p, const int *table, int b) {
+    return p.batch <= kMaxBatch ? table[kMaxBatch + b] : p.q_lengths ? max(0, min(p.q_lengths[b], p.q_len)) : p.q_len;
 }
 
 // Block u of a chain: round k = u / chains goes through the chains forwards and
@@ -127,7 +187,7 @@ __device__ __forceinline__ Block block_at(const PromptParams &p, const int *tabl
     const int k = u / chains, c = u - k * chains, r = k * chains + ((k & 1) ? chains - 1 - c : c);
     Block it;
     if (p.table) {
-        const int *seq = table, *pre = table + kMaxBatch;
+        const int *seq = table + 2 * kMaxBatch, *pre = seq + kMaxBatch;
         if (r >= pre[p.batch]) {
             it.b = it.h = it.q0 = it.n = it.rows = it.pos0 = it.sink_steps = it.base = it.steps = 0;
             it.skip = true;
@@ -151,8 +211,8 @@ __device__ __forceinline__ Block block_at(const PromptParams &p, const int *tabl
         it.b = bh / p.heads;
         it.h = bh - it.b * p.heads;
     }
-    it.n = held_keys(p, it.b);
-    it.rows = held_rows(p, it.b);
+    it.n = held_keys(p, table, it.b);
+    it.rows = held_rows(p, table, it.b);
     it.pos0 = it.n - it.rows;
     it.skip = it.q0 < 0 || it.q0 >= it.rows;
     const int first = it.pos0 + it.q0, last = it.pos0 + min(it.q0 + 127, it.rows - 1);
@@ -169,27 +229,51 @@ __device__ __forceinline__ int step_key(int j, int sink_steps, int base) {
     return j * kKeys + (j < sink_steps ? 0 : base - sink_steps * kKeys);
 }
 
+// Where a chain's tiles, barriers, published blocks and tensor memory lie.  Each
+// role builds its own: values that lived from before the roles part would be
+// spilled.
+template <int NC> struct ChainPlaces {
+    using S = PromptShape<NC>;
+    uint32_t smem, chain;
+    __device__ __forceinline__ ChainPlaces(uint32_t smem, int chain) : smem(smem), chain(chain) {}
+    __device__ __forceinline__ uint32_t q() const { return smem + chain * S::CHAIN_BYTES; }
+    __device__ __forceinline__ uint32_t k() const { return q() + S::Q_BYTES; }
+    __device__ __forceinline__ uint32_t v() const { return k() + S::STAGES * S::KV_BYTES; }
+    __device__ __forceinline__ uint32_t bar() const { return smem + S::BARS_AT + chain * (S::BARS * 8); }
+    __device__ __forceinline__ uint32_t blocks() const { return smem + S::BLOCKS_AT + chain * (2 * S::BLOCK_INTS * 4); }
+    __device__ __forceinline__ uint32_t tmem() const { return get(smem + S::TMEM_AT) + chain * S::COLS; }
+};
+
+// A value that the compiler keeps instead of computing it again at each use.
+__device__ __forceinline__ uint32_t kept(uint32_t v) {
+    asm volatile("" : "+r"(v));
+    return v;
+}
+
 template <int NC, bool BF16>
 __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_kernel(const __grid_constant__ PromptParams p) {
     using S = PromptShape<NC>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint64_t *all_bars = reinterpret_cast<uint64_t *>(smem + S::CHAINS * S::CHAIN_BYTES);
-    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(all_bars + S::CHAINS * S::BARS);
-    int *published = reinterpret_cast<int *>(tmem_holder + 4); // [chain][2][BLOCK_INTS]
-    int *table = published + S::CHAINS * 2 * S::BLOCK_INTS;
+    uint64_t *all_bars = reinterpret_cast<uint64_t *>(smem + S::BARS_AT);
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(smem + S::TMEM_AT);
+    int *table = reinterpret_cast<int *>(smem + S::TABLE_AT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *err = p.err;
 
-    if (p.table) {
-        int *seq = table, *pre = table + kMaxBatch;
+    if (p.batch <= kMaxBatch) {
         for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
-            const int mine = held_keys(p, b);
+            table[b] = p.lengths ? max(0, min(p.lengths[b], p.kv_len)) : p.kv_len;
+            table[kMaxBatch + b] = p.q_lengths ? max(0, min(p.q_lengths[b], p.q_len)) : p.q_len;
+        }
+        __syncthreads();
+    }
+    if (p.table) {
+        int *seq = table + 2 * kMaxBatch, *pre = seq + kMaxBatch;
+        for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
             int rank = 0;
-            for (int o = 0; o < p.batch; ++o) {
-                const int its = held_keys(p, o);
-                rank += its > mine || (its == mine && o < b) ? 1 : 0;
-            }
+            for (int o = 0; o < p.batch; ++o)
+                rank += table[o] > table[b] || (table[o] == table[b] && o < b) ? 1 : 0;
             seq[rank] = b;
         }
         __syncthreads();
@@ -197,7 +281,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
             int sum = 0;
             for (int r = 0; r < p.batch; ++r) {
                 pre[r] = sum;
-                sum += p.heads * ((held_rows(p, seq[r]) + 127) / 128);
+                sum += p.heads * ((table[kMaxBatch + seq[r]] + 127) / 128);
             }
             pre[p.batch] = sum;
         }
@@ -217,81 +301,93 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_holder;
-
-    const int chain = warp < S::SOFT_WARPS ? warp / 4 : (warp - S::SOFT_WARPS) % S::CHAINS;
-    // Chain c of every CTA before chain c + 1 of any: few blocks spread over the SMs.
-    const int chains = gridDim.x * S::CHAINS, mine = chain * gridDim.x + blockIdx.x;
-    const int per_block = p.table ? table[kMaxBatch + p.batch] : p.batch * p.heads * ((p.q_len + 127) / 128);
-    const int blocks = (per_block + chains - 1) / chains * chains; // whole rounds: their last may be empty
-    uint8_t *sq = smem + chain * S::CHAIN_BYTES, *sk = sq + S::Q_BYTES, *sv = sk + S::STAGES * S::KV_BYTES;
-    uint64_t *bar = all_bars + chain * S::BARS;
-    uint64_t *q_full = bar, *q_empty = bar + 1, *k_full = bar + 2, *k_empty = bar + 5, *v_full = bar + 8,
-             *v_empty = bar + 11, *s_full = bar + 14, *pv_done = bar + 16, *drain = bar + 18;
-    uint64_t *p_full = bar + 19, *o_free = bar + 20, *s_free = bar + 21; // an arrive of each softmax warp
-    uint64_t *block_full = bar + 22, *block_empty = bar + 24;            // [2]; read by five warps
-    static_assert(S::STAGES <= 3, "barrier places");
-    int *mine_published = published + chain * 2 * S::BLOCK_INTS;
-    const uint32_t tm = tmem + chain * S::COLS;
 
     if (warp >= S::SOFT_WARPS) {
         reg_dec<S::CONTROL_REGS>();
+        const ChainPlaces<NC> at(smem_u32(smem), (warp - S::SOFT_WARPS) % S::CHAINS);
+        const uint32_t bar = kept(at.bar());
         if (warp < S::ISSUE_WARP) {
             // ------------------------------------------------- blocks and loads
+            // Chain c of every CTA before chain c + 1 of any: few blocks spread over the SMs.
+            const int chains = gridDim.x * S::CHAINS, mine = static_cast<int>(at.chain) * gridDim.x + blockIdx.x;
+            const int listed_blocks = p.table ? table[3 * kMaxBatch + p.batch] : p.batch * p.heads * ((p.q_len + 127) / 128);
+            const int blocks = (listed_blocks + chains - 1) / chains * chains; // whole rounds: their last may be empty
             int nk = 0, nv = 0, items = 0, listed = 0;
             bool ok = true;
             auto publish = [&](const Block &it) {
                 const int slot = listed & 1;
-                if (!warp_wait(&block_empty[slot], ((listed >> 1) & 1) ^ 1, err, kErrWaitEmpty))
+                if (!warp_wait(bar + S::BLOCK_EMPTY + slot * 8, ((listed >> 1) & 1) ^ 1, err, kErrWaitEmpty))
                     return false;
                 if (lane == 0) {
-                    int *to = mine_published + slot * S::BLOCK_INTS;
-                    to[0] = it.b, to[1] = it.h, to[2] = it.q0, to[3] = it.n, to[4] = it.rows;
-                    to[5] = it.sink_steps, to[6] = it.base, to[7] = it.steps;
-                    mbar_arrive(&block_full[slot]);
+                    const uint32_t to = at.blocks() + slot * (S::BLOCK_INTS * 4);
+                    put16(to, it.b, it.h, it.q0, it.n);
+                    put16(to + 16, it.rows, it.sink_steps, it.base, it.steps);
+                    arrive(bar + S::BLOCK_FULL + slot * 8);
                 }
                 __syncwarp();
                 ++listed;
                 return true;
             };
-            auto load = [&](uint8_t *to, const CUtensorMap *map, uint64_t *full, uint64_t *empty, int &n, int key, int head, int b) {
+            auto load = [&](uint32_t to, const CUtensorMap *map, uint32_t full, uint32_t empty, int &n, int key, int head, int b) {
                 const int st = n % S::STAGES;
-                if (!warp_wait(&empty[st], ((n / S::STAGES) & 1) ^ 1, err, kErrWaitEmpty))
+                if (!warp_wait(empty + st * 8, ((n / S::STAGES) & 1) ^ 1, err, kErrWaitEmpty))
                     return false;
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(&full[st], S::KV_BYTES);
+                    arrive_expect_tx(full + st * 8, S::KV_BYTES);
                     for (int c = 0; c < NC; ++c)
-                        tma_load_4d(to + st * S::KV_BYTES + c * kKeys * 128, map, &full[st], c * 64, key, head, b);
+                        load_4d(to + st * S::KV_BYTES + c * kKeys * 128, map, full + st * 8, c * 64, key, head, b);
                 }
                 __syncwarp();
                 ++n;
                 return true;
             };
-            for (int u = mine; ok && u < blocks; u += chains) {
-                const Block it = block_at(p, table, u, chains);
-                if (it.skip)
-                    continue;
-                if (!(ok = publish(it)))
-                    break;
-                if (it.steps == 0)
-                    continue;
+            // The first block at or after u (in steps of `chains`) that has rows.
+            auto find = [&](int &u, Block &it) {
+                for (; u < blocks; u += chains) {
+                    it = block_at(p, table, u, chains);
+                    if (!it.skip)
+                        return true;
+                }
+                return false;
+            };
+            int u = mine;
+            Block it;
+            bool more = find(u, it);
+            ok = !more || publish(it);
+            while (ok && more) {
                 const int head = it.h / p.group;
-                if (!(ok = warp_wait(q_empty, (items & 1) ^ 1, err, kErrWaitEmpty)))
-                    break;
-                if (elect_one()) {
-                    mbar_arrive_expect_tx(q_full, S::Q_BYTES);
-                    for (int c = 0; c < NC; ++c)
-                        tma_load_4d(sq + c * 128 * 128, &p.tq, q_full, c * 64, it.q0, it.h, it.b);
+                if (it.steps > 0) {
+                    if (!(ok = warp_wait(bar + S::Q_EMPTY, (items & 1) ^ 1, err, kErrWaitEmpty)))
+                        break;
+                    if (elect_one()) {
+                        arrive_expect_tx(bar + S::Q_FULL, S::Q_BYTES);
+                        for (int c = 0; c < NC; ++c)
+                            load_4d(at.q() + c * 128 * 128, &p.tq, bar + S::Q_FULL, c * 64, it.q0, it.h, it.b);
+                    }
+                    __syncwarp();
+                    ++items;
+                    // Keys a step ahead of values: they are wanted a step earlier.
+                    if (!(ok = load(at.k(), &p.tk, bar + S::K_FULL, bar + S::K_EMPTY, nk, step_key(0, it.sink_steps, it.base), head, it.b)))
+                        break;
                 }
-                __syncwarp();
-                ++items;
-                // Keys a step ahead of values: they are wanted a step earlier.
-                ok = load(sk, &p.tk, k_full, k_empty, nk, step_key(0, it.sink_steps, it.base), head, it.b);
-                for (int j = 0; ok && j < it.steps; ++j) {
+                // The next block is found while this one's loads are under way.  (Bringing its
+                // queries to L2 here cost more than it saved: 203 against 167 us.)
+                const int look = it.steps > 1 ? 1 : 0;
+                Block next;
+                for (int j = 0; ok && (j < it.steps || j == look); ++j) {
                     if (j + 1 < it.steps)
-                        ok = load(sk, &p.tk, k_full, k_empty, nk, step_key(j + 1, it.sink_steps, it.base), head, it.b);
-                    ok = ok && load(sv, &p.tv, v_full, v_empty, nv, step_key(j, it.sink_steps, it.base), head, it.b);
+                        ok = load(at.k(), &p.tk, bar + S::K_FULL, bar + S::K_EMPTY, nk, step_key(j + 1, it.sink_steps, it.base), head, it.b);
+                    if (ok && j < it.steps)
+                        ok = load(at.v(), &p.tv, bar + S::V_FULL, bar + S::V_EMPTY, nv, step_key(j, it.sink_steps, it.base), head, it.b);
+                    if (!ok || j != look)
+                        continue;
+                    u += chains;
+                    more = find(u, next);
+                    if (!more)
+                        continue;
+                    ok = publish(next);
                 }
+                it = next;
             }
             if (ok) {
                 Block end{};
@@ -300,129 +396,134 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
             }
             // Every copy lands before the CTA ends.
             if (items > 0)
-                drain_wait(q_full, (items - 1) & 1, err);
+                drain_wait(bar + S::Q_FULL, (items - 1) & 1, err);
             for (int j = max(0, nk - S::STAGES); j < nk; ++j)
-                drain_wait(&k_full[j % S::STAGES], (j / S::STAGES) & 1, err);
+                drain_wait(bar + S::K_FULL + j % S::STAGES * 8, (j / S::STAGES) & 1, err);
             for (int j = max(0, nv - S::STAGES); j < nv; ++j)
-                drain_wait(&v_full[j % S::STAGES], (j / S::STAGES) & 1, err);
+                drain_wait(bar + S::V_FULL + j % S::STAGES * 8, (j / S::STAGES) & 1, err);
         } else if (warp < S::ISSUE_WARP + S::CHAINS) {
             // ------------------------------------------------------- products
             constexpr uint32_t idesc_s = make_idesc_f16(128, kKeys, BF16, false);
             const int ksteps = (p.hd + 15) / 16;
             const uint32_t idesc_o = make_idesc_f16(128, ksteps * 16, BF16, true);
             const uint32_t leader = elect_one() ? 1u : 0u;
-            const uint32_t aq = smem_u32(sq), ak = smem_u32(sk), av = smem_u32(sv);
+            const uint32_t tm = kept(at.tmem());
+            const uint64_t dq = make_smem_desc(at.q(), 16, 1024, kLayoutSW128);
+            const uint64_t dk = make_smem_desc(at.k(), 16, 1024, kLayoutSW128);
+            const uint64_t dv = make_smem_desc(at.v(), kKeys * 128, 1024, kLayoutSW128);
             int n = 0, items = 0, listed = 0;
             bool ok = true;
             // S of step g (of the chain's steps), from its K stage.
             auto scores = [&](int g) {
                 const int st = g % S::STAGES;
-                if (!warp_wait(&k_full[st], (g / S::STAGES) & 1, err, kErrWaitK))
+                if (!warp_wait(bar + S::K_FULL + st * 8, (g / S::STAGES) & 1, err, kErrWaitK))
                     return false;
                 // One S: the softmax has the last scores in registers.
-                if (NC == 1 && g > 0 && !warp_wait(s_free, (g - 1) & 1, err, kErrWaitS))
+                if (NC == 1 && g > 0 && !warp_wait(bar + S::S_FREE, (g - 1) & 1, err, kErrWaitS))
                     return false;
                 tc_fence_after();
                 const uint32_t d = tm + (NC == 2 ? (g & 1) * 64 : 0);
+                const uint64_t b = dk + static_cast<uint64_t>(st * (S::KV_BYTES >> 4));
 #pragma unroll
-                for (int k = 0; k < 4 * NC; ++k) {
-                    if (k < ksteps) {
-                        const uint64_t a = make_smem_desc(aq + (k / 4) * 128 * 128, 16, 1024, kLayoutSW128) + 2 * (k % 4);
-                        const uint64_t b = make_smem_desc(ak + st * S::KV_BYTES + (k / 4) * kKeys * 128, 16, 1024, kLayoutSW128) + 2 * (k % 4);
-                        umma_ss_if(leader, d, a, b, idesc_s, k > 0 ? 1u : 0u);
-                    }
-                }
-                tc_commit_if(leader, &s_full[NC == 2 ? g & 1 : 0]);
-                tc_commit_if(leader, &k_empty[st]);
+                for (int k = 0; k < 4 * NC; ++k)
+                    if (k < ksteps)
+                        umma_ss_if(leader, d, dq + (k / 4) * (128 * 128 >> 4) + 2 * (k % 4),
+                                   b + (k / 4) * (kKeys * 128 >> 4) + 2 * (k % 4), idesc_s, k > 0 ? 1u : 0u);
+                commit_if(leader, bar + S::S_FULL + (NC == 2 ? (g & 1) * 8 : 0));
+                commit_if(leader, bar + S::K_EMPTY + st * 8);
                 return true;
             };
             while (true) {
                 const int slot = listed & 1;
-                if (!warp_wait(&block_full[slot], (listed >> 1) & 1, err, kErrWaitQ))
+                if (!warp_wait(bar + S::BLOCK_FULL + slot * 8, (listed >> 1) & 1, err, kErrWaitQ))
                     break;
-                const int *from = mine_published + slot * S::BLOCK_INTS;
-                const int keys = from[3], sink_steps = from[5], base = from[6], steps = from[7];
-                warp_arrive(&block_empty[slot]);
+                const uint32_t from = at.blocks() + slot * (S::BLOCK_INTS * 4);
+                const int keys = get(from + 12), sink_steps = get(from + 20), base = get(from + 24), steps = get(from + 28);
+                warp_arrive(bar + S::BLOCK_EMPTY + slot * 8);
                 ++listed;
                 if (steps < 0)
                     break;
                 if (steps == 0)
                     continue;
-                if (!(ok = warp_wait(q_full, items & 1, err, kErrWaitQ)) || !(ok = scores(n)))
+                if (!(ok = warp_wait(bar + S::Q_FULL, items & 1, err, kErrWaitQ)) || !(ok = scores(n)))
                     break;
                 if (steps == 1) // every product that reads Q is issued
-                    tc_commit_if(leader, q_empty);
+                    commit_if(leader, bar + S::Q_EMPTY);
                 for (int j = 0; j < steps; ++j, ++n) {
                     const int st = n % S::STAGES;
                     if (j + 1 < steps) {
                         if (!(ok = scores(n + 1)))
                             break;
                         if (j + 2 == steps)
-                            tc_commit_if(leader, q_empty);
+                            commit_if(leader, bar + S::Q_EMPTY);
                     }
-                    if (!(ok = warp_wait(&v_full[st], (n / S::STAGES) & 1, err, kErrWaitV)))
+                    if (!(ok = warp_wait(bar + S::V_FULL + st * 8, (n / S::STAGES) & 1, err, kErrWaitV)))
                         break;
                     const int past = keys - step_key(j, sink_steps, base); // V rows from here on are past the sequence
                     if (past < kKeys) {
                         for (int x = lane; x < NC * (kKeys - past) * 8; x += 32) {
                             const int c = x / ((kKeys - past) * 8), y = x - c * (kKeys - past) * 8;
-                            *reinterpret_cast<uint4 *>(sv + st * S::KV_BYTES + c * kKeys * 128 + past * 128 + y * 16) =
-                                make_uint4(0u, 0u, 0u, 0u);
+                            put16(at.v() + st * S::KV_BYTES + c * kKeys * 128 + past * 128 + y * 16, 0u, 0u, 0u, 0u);
                         }
                         fence_proxy_async_smem();
                         __syncwarp();
                     }
-                    if (!(ok = warp_wait(p_full, n & 1, err, kErrWaitP)))
+                    if (!(ok = warp_wait(bar + S::P_FULL, n & 1, err, kErrWaitP)))
                         break;
                     // The first product overwrites O: the last block's rows have been read.
-                    if (j == 0 && items > 0 && !(ok = warp_wait(o_free, (items - 1) & 1, err, kErrWaitO)))
+                    if (j == 0 && items > 0 && !(ok = warp_wait(bar + S::O_FREE, (items - 1) & 1, err, kErrWaitO)))
                         break;
                     tc_fence_after();
-                    const uint64_t v0 = make_smem_desc(av + st * S::KV_BYTES, kKeys * 128, 1024, kLayoutSW128);
+                    const uint64_t v0 = dv + static_cast<uint64_t>(st * (S::KV_BYTES >> 4));
                     const uint32_t a = tm + (NC == 2 ? (n & 1) * 64 : 64);
 #pragma unroll
                     for (int k = 0; k < kKeys / 16; ++k)
                         umma_ts_if(leader, tm + S::O_COL, a + k * 8, v0 + static_cast<uint64_t>((k * 16 * 128) >> 4), idesc_o,
                                    j > 0 || k > 0 ? 1u : 0u);
-                    tc_commit_if(leader, &pv_done[n & 1]);
-                    tc_commit_if(leader, &v_empty[st]);
+                    commit_if(leader, bar + S::PV_DONE + (n & 1) * 8);
+                    commit_if(leader, bar + S::V_EMPTY + st * 8);
                 }
                 if (!ok)
                     break;
                 ++items;
             }
-            tc_commit_if(leader, drain);
-            drain_wait(drain, 0, err);
+            commit_if(leader, bar + S::DRAIN);
+            drain_wait(bar + S::DRAIN, 0, err);
         }
         __syncwarp();
     } else {
         // -------------------------------------------------------------- softmax
         reg_inc<S::SOFT_REGS>();
+        const ChainPlaces<NC> at(smem_u32(smem), warp / 4);
+        const uint32_t bar = kept(at.bar());
         const int quarter = warp & 3, row = quarter * 32 + lane;
-        const uint32_t lanes = tm + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t lanes = kept(at.tmem() + (static_cast<uint32_t>(quarter * 32) << 16));
         const float sl2 = p.scale_log2;
         const int chunks = (p.hd + 15) / 16; // of O, 16 columns each
+        const uint32_t box = kept(at.smem + S::BOXES_AT + warp * kBoxBytes);
         int g = 0, listed = 0;
         bool ok = true;
         while (true) {
             const int slot = listed & 1;
-            if (!warp_wait(&block_full[slot], (listed >> 1) & 1, err, kErrWaitQ))
+            if (!warp_wait(bar + S::BLOCK_FULL + slot * 8, (listed >> 1) & 1, err, kErrWaitQ))
                 break;
             // What outlives the scores' registers: few values.
-            const int *from = mine_published + slot * S::BLOCK_INTS;
-            const int t = from[2] + row, pos = from[3] - from[4] + t;
-            const int limit = min(from[3], pos + p.right + 1), low = p.window > 0 ? pos - p.window + 1 : 0;
-            const int sink_steps = from[5], start = from[6], steps = from[7];
-            const bool store = t < from[4];
-            const long long base = from[0] * p.o_sb + from[1] * p.o_sh + static_cast<long long>(t) * p.o_st;
-            warp_arrive(&block_empty[slot]);
+            const uint32_t from = at.blocks() + slot * (S::BLOCK_INTS * 4);
+            const uint4 who = get16(from), what = get16(from + 16);
+            const int t = static_cast<int>(who.z) + row, keys = who.w, pos = keys - static_cast<int>(what.x) + t;
+            const int limit = min(keys, pos + p.right + 1), low = p.window > 0 ? pos - p.window + 1 : 0;
+            const int sink_steps = what.y, start = what.z, steps = what.w;
+            const int left = static_cast<int>(what.x) - static_cast<int>(who.z) - quarter * 32; // rows of this warp that exist
+            const long long base = static_cast<int>(who.x) * p.o_sb + static_cast<int>(who.y) * p.o_sh +
+                                   static_cast<long long>(t - lane) * p.o_st;
+            warp_arrive(bar + S::BLOCK_EMPTY + slot * 8);
             ++listed;
             if (steps < 0)
                 break;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < steps; ++j, ++g) {
                 const uint32_t ts = lanes + (NC == 2 ? (g & 1) * 64 : 0);
-                if (!(ok = warp_wait(&s_full[NC == 2 ? g & 1 : 0], (NC == 2 ? g >> 1 : g) & 1, err, kErrWaitS)))
+                if (!(ok = warp_wait(bar + S::S_FULL + (NC == 2 ? (g & 1) * 8 : 0), (NC == 2 ? g >> 1 : g) & 1, err, kErrWaitS)))
                     break;
                 tc_fence_after();
                 uint32_t raw[kKeys];
@@ -431,7 +532,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                 tmem_wait_ld();
                 if constexpr (NC == 1) { // the next scores may overwrite these
                     tc_fence_before();
-                    warp_arrive(s_free);
+                    warp_arrive(bar + S::S_FREE);
                 }
                 float *s = reinterpret_cast<float *>(raw);
                 // Columns [0, lo) and [hi, 64) are hidden, save the sinks.  A step wholly
@@ -495,7 +596,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                 // The last product is done: its P may be overwritten (one P), O rescaled.
                 const bool rescale = j > 0 && __any_sync(0xffffffffu, grow);
                 if ((NC == 1 && g > 0) || rescale) {
-                    if (!(ok = warp_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, kErrWaitO)))
+                    if (!(ok = warp_wait(bar + S::PV_DONE + ((g - 1) & 1) * 8, ((g - 1) >> 1) & 1, err, kErrWaitO)))
                         break;
                     tc_fence_after();
                 }
@@ -514,67 +615,78 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                 tmem_st32(NC == 2 ? ts : lanes + 64, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
                 tmem_wait_st();
                 tc_fence_before();
-                warp_arrive(p_full);
+                warp_arrive(bar + S::P_FULL);
             }
             if (!ok)
                 break;
             const float inv = l > 0.f ? 1.f / l : 0.f;
             if (steps > 0) {
-                if (!(ok = warp_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, kErrWaitO)))
+                if (!(ok = warp_wait(bar + S::PV_DONE + ((g - 1) & 1) * 8, ((g - 1) >> 1) & 1, err, kErrWaitO)))
                     break;
                 tc_fence_after();
             }
-            for (int c = 0; c < chunks; ++c) {
-                uint32_t o[16];
-                if (steps > 0) {
-                    tmem_ld16(lanes + S::O_COL + c * 16, o);
-                    tmem_wait_ld();
-                } else {
+            // 64 bytes of each of the warp's rows at a time, through shared memory: a lane
+            // has a row, but the stores take four lanes to a row and write whole sectors.
+            const int size = p.out_dtype == kOutF32 ? 4 : 2, width = 64 / size;
+            for (int c = 0; c < p.hd; c += width) {
+                uint32_t w[16];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h == 1 && size == 4)
+                        break;
+                    uint32_t o[16];
+                    // Columns past head_dim in a 32-column pass: not written below.
+                    if (steps > 0 && c + 16 * h < p.hd) {
+                        tmem_ld16(lanes + S::O_COL + c + 16 * h, o);
+                        tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            o[e] = 0u;
+                    }
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        o[e] = 0u;
-                }
-                if (c + 1 == chunks && steps > 0) {
-                    tc_fence_before();
-                    warp_arrive(o_free);
-                }
-                if (!store)
-                    continue;
-                float v[16];
+                        o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+                    if (size == 4) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    v[e] = __uint_as_float(o[e]) * inv;
-                // head_dim is a multiple of 8.
-#pragma unroll
-                for (int h = 0; h < 16; h += 8) {
-                    const int col = c * 16 + h;
-                    if (col >= p.hd)
-                        continue;
-                    if (p.out_dtype == kOutF32) {
-                        float *out = static_cast<float *>(p.out) + base + col;
-                        if (p.out_vec) {
-                            reinterpret_cast<float4 *>(out)[0] = make_float4(v[h], v[h + 1], v[h + 2], v[h + 3]);
-                            reinterpret_cast<float4 *>(out)[1] = make_float4(v[h + 4], v[h + 5], v[h + 6], v[h + 7]);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                out[e] = v[h + e];
-                        }
+                        for (int e = 0; e < 16; ++e)
+                            w[e] = o[e];
                     } else {
-                        uint16_t *out = static_cast<uint16_t *>(p.out) + base + col;
-                        const uint32_t w[4] = {pack_pair<BF16>(v[h], v[h + 1]), pack_pair<BF16>(v[h + 2], v[h + 3]),
-                                               pack_pair<BF16>(v[h + 4], v[h + 5]), pack_pair<BF16>(v[h + 6], v[h + 7])};
-                        if (p.out_vec) {
-                            *reinterpret_cast<uint4 *>(out) = make_uint4(w[0], w[1], w[2], w[3]);
-                        } else {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                out[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
-                        }
+                        for (int e = 0; e < 8; ++e)
+                            w[8 * h + e] = pack_pair<BF16>(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+                    }
+                }
+                if (c + width >= p.hd && steps > 0) { // O may be overwritten
+                    tc_fence_before();
+                    warp_arrive(bar + S::O_FREE);
+                }
+                __syncwarp(); // the last pass's box has been read
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    put16(box + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4), w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int r = k * 8 + lane / 4, j = lane & 3, col = c + j * (width / 4);
+                    if (r >= left || col >= p.hd)
+                        continue;
+                    const uint4 v = get16(box + r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
+                    const long long place = base + r * p.o_st + col;
+                    if (p.out_vec) {
+                        *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(p.out) + place * size) = v;
+                    } else if (size == 4) {
+                        uint32_t *out = static_cast<uint32_t *>(p.out) + place;
+                        out[0] = v.x, out[1] = v.y, out[2] = v.z, out[3] = v.w;
+                    } else {
+                        uint16_t *out = static_cast<uint16_t *>(p.out) + place;
+                        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            out[e] = static_cast<uint16_t>(x[e / 2] >> (16 * (e & 1)));
                     }
                 }
             }
-            __syncwarp();
         }
         __syncwarp();
     }
@@ -582,7 +694,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
     __syncthreads();
     tc_fence_after();
     if (warp == S::ISSUE_WARP)
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(*tmem_holder, 512);
 }
 
 // (d, token, head, batch) map with boxes of 64 columns x `rows` tokens.
