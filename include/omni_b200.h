@@ -170,7 +170,7 @@ OMNI_B200_API int omni_b200_vq_argmin_noalloc(const void *x, const void *codeboo
  * e4m3 tensors carry fp32 scales, one for each group of 128 columns (of a
  * weight: each block of 128 rows x 128 columns; the last group or block may be
  * smaller).  With amax the largest magnitude of a group, NaN left out,
- *   scale = max(amax / 448, 2^-126),   q = e4m3(x * (1 / scale)),
+ *   scale = max(amax / 448, 2^-126),   q = e4m3(x / scale),
  * rounded to nearest even; q * scale stands for x.  A NaN becomes e4m3's NaN;
  * a group that holds an infinity gets an infinite scale and stands for NaN.
  * Strides count elements of the tensor they belong to; columns are contiguous.

@@ -1,11 +1,16 @@
 // e4m3.cuh -- element conversions shared by the 8-bit layer kernels.
 //
 // Quantisation of a group with largest magnitude amax:
-//   scale = max(amax / 448, 2^-126),  q = e4m3(x * (1 / scale)),
+//   scale = max(amax / 448, 2^-126),  q = e4m3(x / scale),
 // so x ~ q * scale.  448 is e4m3's largest value.  The floor 2^-126 keeps
 // 1 / scale finite for a group of zeros (whose q are zeros).  A NaN does not
 // take part in amax and becomes e4m3's NaN; an infinity makes the scale
 // infinite, and the group then stands for NaN.
+// Inputs of 16 bits often have quotients half way between two e4m3 values, so what
+// is quantised as it is (EXACT) takes x * (1 / scale) with one correction by its
+// residual (Markstein, 1990), which rounds as a division would, for two more
+// operations an element (24000 x 4096: 54 -> 58 us).  A norm's values carry fp32
+// rounding errors of their own and do without.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -66,10 +71,28 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
-__device__ __forceinline__ uint2 e4m3x8(const float (&f)[8], float inv) {
+// A group's divisor.
+struct Divisor {
+    float scale, inv; // scale 0 stands for an infinite one: no correction
+    template <bool EXACT> __device__ __forceinline__ float quotient(float x) const {
+        const float q = x * inv;
+        return EXACT ? fmaf(fmaf(-q, scale, x), inv, q) : q;
+    }
+};
+__device__ __forceinline__ Divisor divisor_of(float scale) {
+    Divisor d;
+    d.scale = scale <= 3.402823466e38f ? scale : 0.f;
+    d.inv = __frcp_rn(scale);
+    return d;
+}
+template <bool EXACT> __device__ __forceinline__ uint2 e4m3x8(const float (&f)[8], const Divisor &d) {
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        q[i] = d.quotient<EXACT>(f[i]);
     uint2 r;
-    r.x = e4m3x2(f[0] * inv, f[1] * inv) | (e4m3x2(f[2] * inv, f[3] * inv) << 16);
-    r.y = e4m3x2(f[4] * inv, f[5] * inv) | (e4m3x2(f[6] * inv, f[7] * inv) << 16);
+    r.x = e4m3x2(q[0], q[1]) | (e4m3x2(q[2], q[3]) << 16);
+    r.y = e4m3x2(q[4], q[5]) | (e4m3x2(q[6], q[7]) << 16);
     return r;
 }
 __device__ __forceinline__ float amax8(const float (&f)[8]) {

@@ -601,12 +601,27 @@ template <int T> __global__ void __launch_bounds__(192, 1) linear_e4m3_few(const
     cluster_sync();
     if (writes) {
         const float b = bias_at(p, col);
-        for (int j = part; j < T && m0 + j < p.m; j += parts) {
-            const uint32_t at = smem_u32(sums + j * 128 + threadIdx.x);
-            float v = 0.f;
-            for (int r = 0; r < parts; ++r)
-                v += peer_load(at, r);
-            store_one(p, (m0 + j) * p.ldo + col, v + b);
+        // Eight rows at a time: their loads from a peer are in flight together.
+        for (int j0 = part; j0 < T && m0 + j0 < p.m; j0 += 8 * parts) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = b;
+            for (int r = 0; r < parts; ++r) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[i] = peer_load(smem_u32(sums + min(j0 + i * parts, T - 1) * 128 + threadIdx.x), r);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] += x[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int j = j0 + i * parts;
+                if (j < T && m0 + j < p.m)
+                    store_one(p, (m0 + j) * p.ldo + col, v[i]);
+            }
         }
     }
     cluster_sync(); // no CTA leaves while another reads its sums

@@ -44,7 +44,7 @@ __device__ __forceinline__ float half_warp_max(float v) {
 }
 
 // Thread t's elements of a row to `out`, as they are or in groups of e4m3.
-template <typename T, bool QUANT, int TPR, int VPT>
+template <typename T, bool NORM, bool QUANT, int TPR, int VPT>
 __device__ __forceinline__ void write_row(const RowsArgs &a, long long row, int groups, int t, float (&h)[VPT][8]) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -53,7 +53,7 @@ __device__ __forceinline__ void write_row(const RowsArgs &a, long long row, int 
             const float scale = group_scale(half_warp_max(amax8(h[i])));
             if (c < a.cols) {
                 uint8_t *q = static_cast<uint8_t *>(a.out) + row * a.out_stride + c;
-                *reinterpret_cast<uint2 *>(q) = e4m3x8(h[i], __frcp_rn(scale));
+                *reinterpret_cast<uint2 *>(q) = e4m3x8<!NORM>(h[i], divisor_of(scale));
                 if (t % 16 == 0)
                     a.scales[row * groups + c / kGroup] = scale;
             }
@@ -65,7 +65,7 @@ __device__ __forceinline__ void write_row(const RowsArgs &a, long long row, int 
 
 // Without a norm (no reduction to wait for) 64 registers, half the SM's threads,
 // keep most loads in flight: 24000 x 4096 bf16 54 us, with 80 registers 59, 48
-// registers 64.
+// registers 64 (before the exact quotients; with them 58).
 template <typename T, bool NORM, bool QUANT, int TPR, int VPT, int ROWS>
 __global__ void __launch_bounds__(TPR *ROWS, NORM ? 1 : 1024 / (TPR * ROWS)) rows_kernel(const RowsArgs a) {
     constexpr int WARPS = TPR / 32; // warps of a row
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(TPR *ROWS, NORM ? 1 : 1024 / (TPR * ROWS)) row
                 }
             }
         }
-        write_row<T, QUANT, TPR, VPT>(a, row, groups, t, h);
+        write_row<T, NORM, QUANT, TPR, VPT>(a, row, groups, t, h);
     }
 }
 
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kStreamThreads) rows_stream_kernel(const RowsA
                     h[i][e] = (i * TPR + t) * 8 < a.cols ? h[i][e] * rstd * wf[e] : 0.f;
             }
         }
-        write_row<T, QUANT, TPR, VPT>(a, row, groups, t, h);
+        write_row<T, NORM, QUANT, TPR, VPT>(a, row, groups, t, h);
     }
     // After a wait that gave up: every copy lands before the CTA's memory goes.
     if (threadIdx.x == 0) {
@@ -342,11 +342,10 @@ __global__ void __launch_bounds__(256) rows_scalar_kernel(const RowsArgs a) {
                 }
                 amax = fmaxf(amax, fabsf(y[e]));
             }
-            float scale = 1.f, inv = 1.f;
+            float scale = 1.f;
             if constexpr (QUANT) {
                 amax = half_warp_max(amax);
                 scale = group_scale(fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16)));
-                inv = __frcp_rn(scale);
                 if (lane == 0)
                     a.scales[row * groups + g] = scale;
             }
@@ -356,7 +355,8 @@ __global__ void __launch_bounds__(256) rows_scalar_kernel(const RowsArgs a) {
                 if (c >= a.cols)
                     continue;
                 if constexpr (QUANT)
-                    static_cast<uint8_t *>(a.out)[row * a.out_stride + c] = static_cast<uint8_t>(e4m3x2(y[e] * inv, 0.f));
+                    static_cast<uint8_t *>(a.out)[row * a.out_stride + c] =
+                        static_cast<uint8_t>(e4m3x2(divisor_of(scale).template quotient<!NORM>(y[e]), 0.f));
                 else
                     static_cast<T *>(a.out)[row * a.out_stride + c] = from_float<T>(y[e]);
             }
@@ -393,7 +393,8 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T *x, uint8_
 #pragma unroll
     for (int k = 0; k < 8; ++k)
         amax = fmaxf(amax, part[k]);
-    const float scale = group_scale(amax), inv = __frcp_rn(scale);
+    const float scale = group_scale(amax);
+    const Divisor divisor = divisor_of(scale);
     if (threadIdx.x == 0)
         scales[static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x] = scale;
 #pragma unroll
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T *x, uint8_
         if (r >= rows || c >= cols)
             continue;
         uint8_t *to = q + r * q_stride + c;
-        const uint2 v = e4m3x8(f[i], inv);
+        const uint2 v = e4m3x8<true>(f[i], divisor);
         if constexpr (VEC) {
             *reinterpret_cast<uint2 *>(to) = v;
         } else {
