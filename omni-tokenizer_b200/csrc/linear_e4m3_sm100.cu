@@ -691,15 +691,24 @@ int linear_e4m3_launch(const LinearArgs &a, cudaStream_t stream) {
     p.out_dtype = a.out_dtype;
     p.err = a.err;
     const int sms = fmha_sm_count();
-    const long long big = static_cast<long long>((a.m + kBigM - 1) / kBigM) * ((a.n + kBigN - 1) / kBigN);
-    if (a.m > 128 && 2 * big >= sms)
-        return launch_big(p, a, sms, stream);
-    // Split the groups over up to 8 CTAs while the tiles leave SMs idle.
+    // Few rows: the groups are split over up to 8 CTAs while the tiles leave SMs idle.
+    // Clusters of four and eight do not reach the last SMs of a GPC: 128 at once.
     const int t = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
     const long long tiles = static_cast<long long>((a.n + 127) / 128) * ((a.m + t - 1) / t);
     int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= sms && parts * 2 <= p.groups)
+    while (parts < 8 && tiles * parts * 2 <= (parts >= 2 ? std::min(sms, 128) : sms) && parts * 2 <= p.groups)
         parts *= 2;
+    // The cheaper kernel, in tenths of a microsecond as measured (launch, then groups
+    // one after another): 4096 x 4096, few rows / large tiles: m 1 6.1 / 17.1 us, m 64
+    // 9.8 / 17.6, m 128 13.7 / 18.2, m 256 20.3 / 18.1; 8192 x 1024: m 33 7.8 / 8.1, m
+    // 128 13.1 / 8.6; 1152 x 4304: m 384 13.9 / 24.9.
+    const long long big = static_cast<long long>((a.m + kBigM - 1) / kBigM) * ((a.n + kBigN - 1) / kBigN);
+    const long long at_once = parts >= 4 ? std::min(sms, 128) : sms;
+    const long long few_cost =
+        50 + t / 4 + (tiles * parts + at_once - 1) / at_once * ((p.groups + parts - 1) / parts) * (2 + t / 25);
+    const long long big_cost = 50 + (big + sms - 1) / sms * p.groups * 4;
+    if (big_cost < few_cost)
+        return launch_big(p, a, sms, stream);
     switch (t) {
     case 16:
         return launch_few<16>(p, a, parts, stream);
