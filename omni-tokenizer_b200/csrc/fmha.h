@@ -106,6 +106,7 @@ int attention_window(const WindowArgs &a, cudaStream_t stream);
 // Its kernels: few query rows for each key head (window_tokens.cu), and blocks of
 // 128 query rows (window_prompt_sm100.cu).
 int window_tokens_launch(const WindowArgs &a, cudaStream_t stream);
+int window_tokens_parts(const WindowArgs &a); // CTAs that it takes for one tile's keys
 int window_prompt_launch(const WindowArgs &a, cudaStream_t stream);
 
 // Returns 0 on success, a CUDA error code, or a negative/1000+ code for an

@@ -757,11 +757,23 @@ int window_prompt_launch(const WindowArgs &a, cudaStream_t stream) {
     return a.bf16 ? launch_typed<2, true>(p, sms, stream) : launch_typed<2, false>(p, sms, stream);
 }
 
-// Query rows that share a key head, up to which the kernel for few rows is taken.
-constexpr int kFewRows = 64;
-
+// The cheaper kernel, in tenths of a microsecond as measured.  Few rows: the keys
+// that every 16 rows read, and at least one warp's share of them; prompts: a block's
+// steps one after another, in rounds of what the chains of the SMs hold.  Measured,
+// prompts / few rows: 16 x 8/2 heads of 128, window 1024, 16 queries 21.1 / 21.3 us,
+// 32 queries 20.9 / 28.0; one sequence, 16384 keys, 8/1 heads, 64 queries 186 / 43;
+// 4 x 8 heads of 64, 4096 keys, 128 queries 58 / 52, 256 queries 58 / 101.
 int attention_window(const WindowArgs &a, cudaStream_t stream) {
-    if (static_cast<long long>(a.heads / a.kv_heads) * a.q_len <= kFewRows)
+    const double around = a.window > 0 ? static_cast<double>(a.window) + a.right + a.sinks : a.kv_len;
+    const double few_keys = std::min<double>(a.kv_len, around + a.q_len);
+    const long long tiles = (static_cast<long long>(a.heads / a.kv_heads) * a.q_len + 15) / 16;
+    const double read = few_keys * tiles * a.batch * a.kv_heads * a.hd / 155000.0;
+    const double share = few_keys / 64 / window_tokens_parts(a) * 7;
+    const double few_cost = 75 + std::max(read, share);
+    const double steps = std::min<double>(a.kv_len, around + 127) / kKeys + 1;
+    const double blocks = static_cast<double>(a.batch) * a.heads * ((a.q_len + 127) / 128);
+    const double prompt_cost = 70 + 7 * steps * std::max(1.0, blocks / (1.45 * fmha_sm_count()));
+    if (tiles <= 65535 && few_cost <= prompt_cost)
         return window_tokens_launch(a, stream);
     return window_prompt_launch(a, stream);
 }

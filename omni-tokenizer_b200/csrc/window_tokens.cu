@@ -397,6 +397,22 @@ template <bool BF16> int launch_type(const TokensParams &p, dim3 grid, cudaStrea
 
 } // namespace
 
+// CTAs that split the keys of one tile of rows: until two are on every SM, with two
+// chunks left for each warp.  Measured, 4101 keys x 128: 512 tiles 168 us with one
+// part, 180 with two; 128 tiles 36 and 28 us (four: 30); 32 tiles 38 us with two
+// parts, 23 with four, 20 with eight.
+int window_tokens_parts(const WindowArgs &a) {
+    const long long tiles = (static_cast<long long>(a.heads / a.kv_heads) * a.q_len + 15) / 16;
+    const long long ctas = tiles * a.batch * a.kv_heads, most = 2ll * fmha_sm_count();
+    long long keys = a.kv_len;
+    if (a.window > 0)
+        keys = std::min(keys, static_cast<long long>(a.window) + a.q_len + a.right + a.sinks);
+    int parts = 1;
+    while (parts < kMaxParts && ctas * parts * 2 <= most && keys >= 2ll * parts * 2 * kWarps * kChunk)
+        parts *= 2;
+    return parts;
+}
+
 int window_tokens_launch(const WindowArgs &a, cudaStream_t stream) {
     TokensParams p{};
     p.q = static_cast<const uint16_t *>(a.q);
@@ -422,19 +438,7 @@ int window_tokens_launch(const WindowArgs &a, cudaStream_t stream) {
     p.out_dtype = a.out_dtype;
     const double scale = a.scale > 0 ? a.scale : 1.0 / std::sqrt(static_cast<double>(a.hd));
     p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-    const int sms = fmha_sm_count();
-    // CTAs that split the keys of one tile: until two are on every SM, with two
-    // chunks left for each warp.  Measured, 4101 keys x 128: 512 tiles 168 us with
-    // one part, 180 with two; 128 tiles 36 and 28 us (four: 30); 32 tiles 38 us
-    // with two parts, 23 with four, 20 with eight.
-    const int tiles = (p.group * a.q_len + 15) / 16;
-    const long long ctas = static_cast<long long>(tiles) * a.batch * a.kv_heads;
-    long long keys = a.kv_len;
-    if (a.window > 0)
-        keys = std::min(keys, static_cast<long long>(a.window) + a.q_len + a.sinks);
-    int parts = 1;
-    while (parts < kMaxParts && ctas * parts * 2 <= 2ll * sms && keys >= 2ll * parts * 2 * kWarps * kChunk)
-        parts *= 2;
+    const int parts = window_tokens_parts(a), tiles = (p.group * a.q_len + 15) / 16;
     p.parts = parts;
     const dim3 grid(static_cast<unsigned>(parts) * a.batch * a.kv_heads, tiles);
     return a.bf16 ? launch_type<true>(p, grid, stream) : launch_type<false>(p, grid, stream);
