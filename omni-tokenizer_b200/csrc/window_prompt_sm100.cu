@@ -21,9 +21,9 @@
 // divisions and the reads of the lengths stay off the other warps' path.
 // Exponentials are taken to base 2 with the scale folded in, statistics are fp32; a
 // row keeps a stale maximum until it grows by more than 2^8, so that P <= 2^8 and O
-// is rarely rescaled.  Two barriers tell that O has the product of step g (g & 1): a
-// waiter may be a step behind the products, and one barrier's parity would mistake
-// the step before the last for the one awaited.
+// is rarely rescaled.  Steps take turns between two barriers where one side may
+// be a step ahead of the other (P written, products done): one barrier's parity would
+// mistake the step before the last for the one awaited.
 //
 // Tiles hold 64 columns (128 bytes, 128-byte swizzle) per row and chunk; columns
 // past head_dim and rows past the tensor are TMA's zero fill.  Rows of v past a
@@ -64,14 +64,14 @@ template <int NC> struct PromptShape {
     static constexpr int Q_BYTES = NC * 128 * 128, KV_BYTES = NC * kKeys * 128;
     static constexpr int CHAIN_BYTES = Q_BYTES + 2 * STAGES * KV_BYTES;
     static constexpr uint32_t COLS = NC == 1 ? 160 : 256, O_COL = NC == 1 ? 96 : 128;
-    // Barriers by their byte offsets.  k_*, v_*: one per stage; s_full, pv_done: by the
-    // step's parity; block_*: by the block's.  An arrive of each softmax warp: p_full,
+    // Barriers by their byte offsets.  k_*, v_*: one per stage; s_full, p_full, pv_done: by
+    // the step's parity; block_*: by the block's.  An arrive of each softmax warp: p_full,
     // o_free, s_free; of those and the issuer: block_empty.
     static constexpr uint32_t Q_FULL = 0, Q_EMPTY = 8, K_FULL = 2 * 8, K_EMPTY = 5 * 8, V_FULL = 8 * 8, V_EMPTY = 11 * 8,
-                              S_FULL = 14 * 8, PV_DONE = 16 * 8, DRAIN = 18 * 8, P_FULL = 19 * 8, O_FREE = 20 * 8,
-                              S_FREE = 21 * 8, BLOCK_FULL = 22 * 8, BLOCK_EMPTY = 24 * 8;
+                              S_FULL = 14 * 8, PV_DONE = 16 * 8, DRAIN = 18 * 8, P_FULL = 19 * 8, O_FREE = 21 * 8,
+                              S_FREE = 22 * 8, BLOCK_FULL = 23 * 8, BLOCK_EMPTY = 25 * 8;
     static_assert(STAGES <= 3, "barrier places");
-    static constexpr int BARS = 26, BLOCK_INTS = 12; // per chain; per published block (two of them)
+    static constexpr int BARS = 28, BLOCK_INTS = 12; // per chain; per published block (two of them)
     static constexpr int TABLE_BYTES = (4 * kMaxBatch + 1) * 4; // keys, rows, and (ragged) seq, pre
     static constexpr int BOXES_AT = CHAINS * CHAIN_BYTES, BARS_AT = BOXES_AT + SOFT_WARPS * kBoxBytes;
     static constexpr int TMEM_AT = BARS_AT + CHAINS * BARS * 8, BLOCKS_AT = TMEM_AT + 16;
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
         for (int c = 0; c < S::CHAINS; ++c) {
             uint64_t *bar = all_bars + c * S::BARS;
             for (int i = 0; i < S::BARS; ++i)
-                mbar_init(&bar[i], i >= 24 ? 5 : i >= 19 && i < 22 ? 4 : 1);
+                mbar_init(&bar[i], i >= 25 ? 5 : i >= 19 && i < 23 ? 4 : 1);
         }
         fence_mbarrier_init();
     }
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                         fence_proxy_async_smem();
                         __syncwarp();
                     }
-                    if (!(ok = warp_wait(bar + S::P_FULL, n & 1, err, kErrWaitP)))
+                    if (!(ok = warp_wait(bar + S::P_FULL + (n & 1) * 8, (n >> 1) & 1, err, kErrWaitP)))
                         break;
                     // The first product overwrites O: the last block's rows have been read.
                     if (j == 0 && items > 0 && !(ok = warp_wait(bar + S::O_FREE, (items - 1) & 1, err, kErrWaitO)))
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                 tmem_st32(NC == 2 ? ts : lanes + 64, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
                 tmem_wait_st();
                 tc_fence_before();
-                warp_arrive(bar + S::P_FULL);
+                warp_arrive(bar + S::P_FULL + (g & 1) * 8);
             }
             if (!ok)
                 break;

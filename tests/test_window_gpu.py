@@ -139,11 +139,26 @@ PROMPTS = [
     (1, 2, 1, 1200, 1200, 128, 0, 0, 0),
     (3, 40, 8, 600, 600, 64, 300, 10, 64),
 ]
+# Work enough for the kernel of 128-row blocks whatever its rule weighs.
+WIDE = [
+    (16, 8, 8, 128, 130, 64, 40, 0, 3),
+    (8, 32, 4, 129, 129, 128, 0, 0, 0),
+    (24, 8, 8, 257, 300, 72, 60, 59, 5),
+    (40, 8, 8, 130, 128, 32, 20, 0, 2),
+    (16, 24, 8, 200, 400, 80, 100, 0, 130),
+    (12, 16, 16, 300, 700, 96, 128, 0, 1),
+    (60, 20, 10, 256, 256, 8, 1, 0, 0),
+    (60, 16, 2, 250, 250, 16, 0, 50, 0),
+    (9, 24, 24, 390, 1500, 40, 64, 2000, 7),
+    (64, 8, 8, 100, 100, 24, 7, 300, 0),
+    (2, 64, 64, 1000, 1000, 128, 129, 0, 300),
+    (700, 2, 2, 65, 70, 64, 16, 0, 1),
+]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("layout", ["heads", "tokens", "rows"])
-@pytest.mark.parametrize("case", TOKENS + PROMPTS, ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("case", TOKENS + PROMPTS + WIDE, ids=lambda c: "-".join(map(str, c)))
 def test_window(ob, case, layout, dtype):
     B, H, Hkv, Lq, Lk, D, window, right, sinks = case
     q, k, v = _inputs(B, H, Hkv, Lq, Lk, D, dtype, layout, seed=sum(case))
@@ -158,32 +173,33 @@ def test_window(ob, case, layout, dtype):
 @pytest.mark.parametrize("case", [
     (6, 4, 2, 1, 300, 64, 100, 0, 4), (6, 6, 2, 5, 200, 72, 30, 4, 70), (6, 2, 1, 16, 90, 128, 0, 0, 0),
     (6, 2, 2, 300, 300, 64, 50, 0, 4), (6, 4, 1, 280, 900, 128, 200, 20, 150), (6, 2, 2, 520, 640, 96, 0, 0, 0),
-    (6, 3, 3, 333, 400, 32, 17, 5, 3),
+    (6, 3, 3, 333, 400, 32, 17, 5, 3), (6, 40, 8, 640, 640, 96, 0, 0, 0), (6, 40, 20, 300, 900, 128, 200, 20, 150),
+    (6, 48, 48, 520, 640, 72, 17, 5, 3), (6, 64, 64, 333, 400, 32, 0, 0, 0), (600, 4, 4, 130, 140, 64, 30, 0, 2),
 ], ids=lambda c: "-".join(map(str, c)))
 def test_window_lengths(ob, case, dtype):
     """Sequences of several lengths: empty, one key, queries that outnumber the keys
     (rows with no key give zeros), lengths inside and at the ends of tiles."""
     B, H, Hkv, Lq, Lk, D, window, right, sinks = case
     q, k, v = _inputs(B, H, Hkv, Lq, Lk, D, dtype, "heads", seed=sum(case) + 1)
-    lengths = [Lk, 0, 1, min(Lk, 129), Lk - 1, min(Lk, 128)]
+    lengths = [Lk, 0, 1, min(Lk, 129), Lk - 1, min(Lk, 128)] * (B // 6)
     mask = dict(window=window, right=right, sinks=sinks)
-    for q_lengths in (None, [Lq, Lq, Lq, max(1, Lq // 2), 0, min(Lq, 128)]):
+    for q_lengths in (None, [Lq, Lq, Lq, max(1, Lq // 2), 0, min(Lq, 128)] * (B // 6)):
         for out_dtype in (dtype, F32):
             got = _run(ob, q, k, v, lengths, q_lengths, out_dtype=out_dtype, **mask)
             _check(got, q, k, v, window, right, sinks, lengths, q_lengths)
     # Lengths beyond the tensors count as their sizes, negative ones as none.
-    far = _run(ob, q, k, v, [Lk] * 5 + [0], [Lq] * 6, **mask)
+    far = _run(ob, q, k, v, [Lk] * (B - 1) + [0], [Lq] * B, **mask)
     i32 = dict(dtype=torch.int32, device="cuda")
-    clamped = ob.attention_window(q, k, v, lengths=torch.tensor([Lk + 99] * 5 + [-3], **i32),
-                                  q_lengths=torch.tensor([2**31 - 1] * 6, **i32), **mask)
+    clamped = ob.attention_window(q, k, v, lengths=torch.tensor([Lk + 99] * (B - 1) + [-3], **i32),
+                                  q_lengths=torch.tensor([2**31 - 1] * B, **i32), **mask)
     ob.library().sync_check()
     assert torch.equal(far, clamped)
 
 
-@pytest.mark.parametrize("Lq", [1, 300])
-def test_window_scale_and_large_scores(ob, Lq):
+@pytest.mark.parametrize("B,H,Lq", [(1, 2, 1), (1, 2, 300), (8, 32, 300)])
+def test_window_scale_and_large_scores(ob, B, H, Lq):
     """Scores of a few hundred: the maximum is subtracted before the exponential."""
-    q, k, v = _inputs(1, 2, 2, Lq, 600, 64, BF16, "heads", seed=3)
+    q, k, v = _inputs(B, H, H, Lq, 600, 64, BF16, "heads", seed=3)
     for scale in (0.01, 2.0):
         got = _run(ob, q, k, v, window=100, sinks=3, scale=scale, out_dtype=F32)
         want, mean = _reference(q, k, v, 100, 0, 3, None, None, scale)
@@ -193,26 +209,29 @@ def test_window_scale_and_large_scores(ob, Lq):
         assert bool(((got.double() - want).abs() <= tol).all())
 
 
-@pytest.mark.parametrize("Lq", [1, 200])
-def test_window_writes_its_rows_only(ob, Lq):
+@pytest.mark.parametrize("B,H,Lq", [(2, 4, 1), (2, 4, 200), (20, 16, 200)])
+def test_window_writes_its_rows_only(ob, B, H, Lq):
     """An output inside a larger tensor: what lies around it stays."""
-    q, k, v = _inputs(2, 4, 2, Lq, 256, 64, BF16, "tokens", seed=5)
+    q, k, v = _inputs(B, H, 2, Lq, 256, 64, BF16, "tokens", seed=5)
     want = _run(ob, q, k, v, window=60, sinks=2)
-    wide = torch.full((2, Lq + 2, 4, 80), KEPT, dtype=BF16, device="cuda")
+    wide = torch.full((B, Lq + 2, H, 80), KEPT, dtype=BF16, device="cuda")
     inner = wide[:, 1:Lq + 1, :, 8:72].transpose(1, 2)
     _run(ob, q, k, v, window=60, sinks=2, out=inner)
     assert torch.equal(inner, want)
+    odd = torch.full((B, Lq, H, 65), KEPT, dtype=BF16, device="cuda")  # rows that no 16-byte store reaches
+    _run(ob, q, k, v, window=60, sinks=2, out=odd[..., 1:].transpose(1, 2))
+    assert torch.equal(odd[..., 1:].transpose(1, 2), want) and bool((odd[..., 0] == KEPT).all())
     inner.fill_(KEPT)
     assert bool((wide == KEPT).all())
 
 
-@pytest.mark.parametrize("Lq", [2, 300])
-def test_window_captured_on_two_streams(ob, Lq):
+@pytest.mark.parametrize("H,Lq", [(4, 2), (4, 300), (64, 300)])
+def test_window_captured_on_two_streams(ob, H, Lq):
     """Two captured calls with inputs of their own, replayed together and again with
     other lengths, give what plain calls give."""
     graphs = []
     for seed in (1, 2):
-        q, k, v = _inputs(3, 4, 2, Lq, 700, 64, BF16, "heads", seed=seed)
+        q, k, v = _inputs(3, H, 2, Lq, 700, 64, BF16, "heads", seed=seed)
         lengths = torch.tensor([700, 350, 301], dtype=torch.int32, device="cuda")
         out = torch.zeros_like(q)
         torch.cuda.synchronize()
@@ -247,3 +266,53 @@ def test_window_empty_calls(ob):
     assert ob.attention_window(q[:0], k[:0], v[:0]).shape == (0, 2, 4, 64)
     assert ob.attention_window(q[:, :, :0], k, v).shape == (2, 2, 0, 64)
     ob.library().sync_check()
+
+
+def test_layer_of_all_operators(ob):
+    """The operators together as a layer uses them: norm with the residual, product,
+    windowed attention over the joint projection's rows, quantisation, product.  Each
+    step is checked against its definition in 64 bits on the inputs it got."""
+    B, n, H, Hkv, D = 3, 400, 16, 4, 64
+    d, rows = H * D, 3 * 400
+    g = torch.Generator().manual_seed(11)
+    x, res = (torch.randn(rows, d, generator=g).to(BF16).cuda() for _ in range(2))
+    norm = (1 + 0.1 * torch.randn(d, generator=g)).to(BF16).cuda()
+    w_in, s_in = ob.quantize_e4m3(torch.randn((H + 2 * Hkv) * D, d, generator=g).cuda() * d**-0.5, block_rows=128)
+    w_out, s_out = ob.quantize_e4m3(torch.randn(d, d, generator=g).cuda() * d**-0.5, block_rows=128)
+    bias = torch.randn(d, generator=g).to(BF16).cuda()
+    lengths = [400, 133, 0]
+    held = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+
+    q, scales, h = ob.rms_norm_e4m3(x, norm, residual=res)
+    joint = ob.linear_e4m3(q, scales, w_in, s_in).view(B, n, H + 2 * Hkv, D).transpose(1, 2)
+    parts = joint[:, :H], joint[:, H:H + Hkv], joint[:, H + Hkv:]
+    mixed = torch.zeros(B, n, H, D, dtype=BF16, device="cuda")
+    ob.attention_window(*parts, window=64, sinks=4, lengths=held, q_lengths=held, out=mixed.transpose(1, 2))
+    a, a_scales = ob.quantize_e4m3(mixed.view(rows, d))
+    y = ob.linear_e4m3(a, a_scales, w_out, s_out, bias=bias)
+    ob.library().sync_check()
+
+    def wide(t, s, block):
+        return t.double() * s.double().repeat_interleave(block, 0)[:t.shape[0]].repeat_interleave(128, 1)[:, :t.shape[1]]
+
+    h64 = x.double() + res.double()
+    y64 = h64 / torch.sqrt(h64.square().mean(1, keepdim=True) + 1e-6) * norm.double()
+    # e4m3: half a step of 2^-4, at least 2^-10 of the group's scale.
+    s = scales.double().repeat_interleave(128, 1)
+    assert bool(((wide(q, scales, 1) - y64).abs() <= torch.maximum(y64.abs() * 2.0**-4, s * 2.0**-10) * 1.001).all())
+    assert bool(((h.double() - h64).abs() <= h64.abs() * 2.0**-8).all())
+
+    def product(t, ts, w, ws):
+        a64, w64 = wide(t, ts, 1), wide(w, ws, 128)
+        return a64 @ w64.t(), a64.abs() @ w64.abs().t()
+
+    want, mag = product(q, scales, w_in, s_in)
+    got = joint.transpose(1, 2).reshape(rows, -1).double()
+    assert bool(((got - want).abs() <= mag * 2.0**-11 + want.abs() * 2.0**-8).all())
+    ref, mean = _reference(*parts, 64, 0, 4, lengths, lengths)
+    err = (mixed.transpose(1, 2).double() - ref).abs()
+    assert bool((err <= mean * (2.0**-7 + 2.0**-12) + ref.abs() * 2.0**-8 + 1e-30).all())
+    want, mag = product(a, a_scales, w_out, s_out)
+    want = want + bias.double()
+    assert bool(((y.double() - want).abs() <= mag * 2.0**-11 + want.abs() * 2.0**-8 * 1.01).all())
+    assert bool((y.view(B, n, d)[2] == bias).all())  # a sequence without keys mixes to zeros
