@@ -431,10 +431,13 @@ def linear_e4m3(a, a_scales, w, w_scales, bias=None, out_dtype=None, out=None, s
         if bias.shape != (n,) or bias.dtype != dtype or (n > 1 and bias.stride(0) != 1):
             _refuse(f"linear_e4m3: bias must be contiguous [{n}] of the output's type")
         bias_ptr = bias.data_ptr()
-    device = _device_of("linear_e4m3", a, a_scales, w, w_scales, bias, out)
+    lda, ldw = _row_stride("linear_e4m3", a, shape), _row_stride("linear_e4m3", w, w_shape)
     # A single row counts as one padded to 16.
-    lda = _row_stride("linear_e4m3", a, shape) if m > 1 else (k + 15) // 16 * 16
-    ldw = _row_stride("linear_e4m3", w, w_shape) if n > 1 else (k + 15) // 16 * 16
+    if m == 1:
+        lda = (k + 15) // 16 * 16
+    if n == 1:
+        ldw = (k + 15) // 16 * 16
+    device = _device_of("linear_e4m3", a, a_scales, w, w_scales, bias, out)
     _call("omni_b200_linear_e4m3", device, stream, a.data_ptr(), a_scales.data_ptr(), w.data_ptr(),
           w_scales.data_ptr(), bias_ptr, out.data_ptr(), m, n, k, lda, ldw, stride, code)
     return out

@@ -105,6 +105,16 @@ def test_helpers_refuse():
         assert e.value.status == 1
 
 
+def test_linear_helper_refuses_strided_columns():
+    """Of a single row too, whose row stride does not matter."""
+    torch = pytest.importorskip("torch")
+    q, s = torch.zeros(4, 256).to(torch.float8_e4m3fn), torch.zeros(4, 2)
+    row = torch.zeros(256, 4).to(torch.float8_e4m3fn)[:, :1].t()  # [1, 256], every fourth element
+    for call in (lambda: ob.linear_e4m3(row, s[:1], q, s[:1]), lambda: ob.linear_e4m3(q, s, row, s[:1])):
+        with pytest.raises(ob.NativeError, match="columns must be contiguous"):
+            call()
+
+
 def _window(lib, strides=None, **k):
     a = dict(q=X, k=R, v=W, out=O, batch=2, heads=4, kv_heads=2, q_len=3, kv_len=40, hd=64, strides=None, lengths=None,
              q_lengths=None, window=8, right=0, sinks=1, scale=0.0, dtype=BF16, out_dtype=BF16)
