@@ -179,8 +179,8 @@ OMNI_B200_API int omni_b200_vq_argmin_noalloc(const void *x, const void *codeboo
  * omni_b200_rms_norm: per row of x [rows, cols],
  *   h = x + residual (or x),   out = h / sqrt(mean(h^2) + eps) * weight,
  * all in fp32.  residual != NULL also needs residual_out, which receives h
- * rounded to dtype; residual_out may be the same tensor as x or residual, and
- * out (of dtype) the same as any of them, with that tensor's stride; other
+ * rounded to dtype; residual_out and out (of dtype) may each be the same tensor
+ * as x or residual, with that tensor's stride, but not both the same one; other
  * overlaps are not allowed.  dtype F32, BF16 or F16 is the type of x, residual,
  * weight [cols] and residual_out.  out_dtype is dtype, with scales NULL, or
  * E4M3, with scales [rows, ceil(cols / 128)].  cols <= 2^24.
@@ -201,7 +201,9 @@ OMNI_B200_API int omni_b200_quantize_e4m3(const void *x, void *q, float *scales,
  *             (sum over the k of g of a[m, k] * w[n, k])   (+ bias[n])
  * a [m, k] and w [n, k] are e4m3 as above (a in groups of 128 columns, w in 128
  * x 128 blocks), 16-byte aligned with row strides lda and ldw >= k that are
- * multiples of 16.  The sums are fp32, rounded once to out_dtype (F32, BF16 or
+ * multiples of 16.  The product of two scales and the sums are fp32 (so such a
+ * product should be neither infinite nor below 2^-126 unless its columns are
+ * zeros on one side and finite), rounded once to out_dtype (F32, BF16 or
  * F16) [m, n] with row stride ldo; bias (NULL: none) is [n] of out_dtype.  k is
  * at most 2^24, n at most 2^22.  out overlaps no input.  No workspace; the
  * same call gives the same bits. */

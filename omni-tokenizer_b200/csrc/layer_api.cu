@@ -5,6 +5,7 @@
 #include "fmha.h"
 #include "layer.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cuda_runtime.h>
 
@@ -51,6 +52,13 @@ int omni_b200_rms_norm(const void *x, const void *residual, const void *weight, 
         (residual && (residual_stride < cols || residual_out_stride < cols || residual_stride > kMaxStride ||
                       residual_out_stride > kMaxStride)))
         return ctx_fail(1, "rms_norm: a row stride is smaller than cols, or above 2^40");
+    if (rows && (out == residual_out || (quantize && (out == x || out == residual))))
+        return ctx_fail(1, "rms_norm: out must not be residual_out, nor, in E4M3, an input");
+    if (rows > 1 && ((residual && ((residual_out == x && residual_out_stride != x_stride) ||
+                                   (residual_out == residual && residual_out_stride != residual_stride) ||
+                                   (out == residual && out_stride != residual_stride))) ||
+                     (out == x && out_stride != x_stride)))
+        return ctx_fail(1, "rms_norm: an output in an input's place must have its row stride");
     const size_t size = type_bytes(dtype);
     if (!aligned(x, size) || !aligned(residual, size) || !aligned(weight, size) || !aligned(residual_out, size) ||
         !aligned(out, quantize ? 1 : size) || !aligned(scales, 4))
@@ -217,7 +225,7 @@ int omni_b200_attention_window(const void *q, const void *k, const void *v, void
     a.lengths = lengths;
     a.q_lengths = q_lengths;
     a.window = window;
-    a.right = right;
+    a.right = std::min(right, kMost - 1); // as good as kMost, and a position + right + 1 fits in 32 bits
     a.sinks = sinks;
     a.bf16 = dtype == OMNI_B200_BF16;
     a.out_dtype = out_dtype;

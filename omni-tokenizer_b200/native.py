@@ -363,7 +363,8 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None, st
     """Root-mean-square norm of the rows of x [rows, cols] (+ residual).
 
     Returns (y, h): y = h / sqrt(mean(h^2) + eps) * weight in x's type, h = x + residual
-    (None without a residual).  residual_out may be x or residual, out any of them."""
+    (None without a residual).  residual_out and out may each be x or residual, not both
+    the same one."""
     shape, code = _matrix("rms_norm", x)
     if out is None:
         out, out_stride = _t.empty_like(x) if x.is_contiguous() else x.new_empty(shape), shape[1]

@@ -34,6 +34,8 @@ def _norm(lib, **k):
     dict(xs=255), dict(rs=255), dict(hs=0), dict(os=100), dict(xs=(1 << 40) + 8), dict(eps=-1.0),
     dict(eps=float("nan")), dict(eps=float("inf")), dict(x=X + 1), dict(out=O + 1), dict(weight=W + 1),
     dict(out_dtype=E4M3, scales=S + 2), dict(rows=(1 << 40) + 1),
+    dict(out=H), dict(out=X, residual_out=X), dict(residual_out=X, hs=264), dict(residual_out=R, hs=264),
+    dict(out=X, os=264), dict(out=R, os=264), dict(out=X, out_dtype=E4M3, scales=S),
 ])
 def test_rms_norm_refuses(lib, bad):
     assert _norm(lib, **bad) == 1
