@@ -445,6 +445,7 @@ def linear_e4m3(a, a_scales, w, w_scales, bias=None, out_dtype=None, out=None, s
 
 
 _STRIDES = C.c_int64 * 12
+_INT = 1 << 31
 
 
 def attention_window(q, k, v, window=0, sinks=0, right=0, lengths=None, q_lengths=None, scale=0.0, out=None,
@@ -463,6 +464,10 @@ def attention_window(q, k, v, window=0, sinks=0, right=0, lengths=None, q_length
     Bk, Hkv, Lk, Dk = k_shape
     if Bk != B or Dk != D:
         _refuse("attention_window: q, k and v must agree in batch and head dimension")
+    # The entry point takes 32-bit sizes and refuses the rest of what is out of range.
+    if not (-_INT < window < _INT and -_INT < right < _INT and -_INT < sinks < _INT
+            and max(B, H, Hkv, Lq, Lk, D) < _INT):
+        _refuse("attention_window: sizes, window, right and sinks must be below 2^31")
     dtype = q.dtype
     code = _t.codes.get(dtype, F32)
     if code == F32 or k.dtype != dtype or v.dtype != dtype:

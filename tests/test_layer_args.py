@@ -175,3 +175,13 @@ def test_window_helper_refuses():
         with pytest.raises(ob.NativeError) as e:
             call()
         assert e.value.status == 1
+
+
+@pytest.mark.parametrize("name", ["window", "right", "sinks"])
+@pytest.mark.parametrize("value", [1 << 31, (1 << 32) + 5, -(1 << 32) - 1])
+def test_window_helper_refuses_what_32_bits_do_not_hold(name, value):
+    """They would arrive as other numbers."""
+    torch = pytest.importorskip("torch")
+    q, k = torch.zeros(2, 4, 3, 64, dtype=torch.bfloat16), torch.zeros(2, 2, 40, 64, dtype=torch.bfloat16)
+    with pytest.raises(ob.NativeError, match="below 2\\^31"):
+        ob.attention_window(q, k, k, **{name: value})
