@@ -187,7 +187,7 @@ OMNI_B200_API int omni_b200_vq_argmin_noalloc(const void *x, const void *codeboo
  *
  * omni_b200_quantize_e4m3: x [rows, cols] to q and scales.  block_rows 1: scales
  * [rows, ceil(cols / 128)]; block_rows 128 (weights): scales
- * [ceil(rows / 128), ceil(cols / 128)], rows <= 8388480. */
+ * [ceil(rows / 128), ceil(cols / 128)], rows <= 8388480.  q overlaps no input. */
 OMNI_B200_API int omni_b200_rms_norm(const void *x, const void *residual, const void *weight,
                                      void *residual_out, void *out, float *scales, size_t rows,
                                      size_t cols, size_t x_stride, size_t residual_stride,

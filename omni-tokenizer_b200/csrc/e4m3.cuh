@@ -16,6 +16,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "sm100.cuh"
+
 namespace omni_b200 {
 
 constexpr int kGroup = 128; // columns (of weights: columns and rows) that share a scale
@@ -88,17 +90,24 @@ __device__ __forceinline__ Divisor divisor_of(float scale) {
 template <bool EXACT> __device__ __forceinline__ uint2 e4m3x8(const float (&f)[8], const Divisor &d) {
     float q[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        q[i] = d.quotient<EXACT>(f[i]);
+    for (int i = 0; i < 8; i += 2) { // two elements an instruction
+        if constexpr (EXACT) {
+            float e0, e1;
+            fmul2(q[i], q[i + 1], f[i], f[i + 1], d.inv, d.inv);
+            ffma2(e0, e1, q[i], q[i + 1], -d.scale, -d.scale, f[i], f[i + 1]);
+            ffma2(q[i], q[i + 1], e0, e1, d.inv, d.inv, q[i], q[i + 1]);
+        } else {
+            fmul2(q[i], q[i + 1], f[i], f[i + 1], d.inv, d.inv);
+        }
+    }
     uint2 r;
     r.x = e4m3x2(q[0], q[1]) | (e4m3x2(q[2], q[3]) << 16);
     r.y = e4m3x2(q[4], q[5]) | (e4m3x2(q[6], q[7]) << 16);
     return r;
 }
 __device__ __forceinline__ float amax8(const float (&f)[8]) {
-    const float a = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
-    const float b = fmaxf(fmaxf(fabsf(f[4]), fabsf(f[5])), fmaxf(fabsf(f[6]), fabsf(f[7])));
-    return fmaxf(a, b);
+    const float a = fmax3(fabsf(f[0]), fabsf(f[1]), fabsf(f[2])), b = fmax3(fabsf(f[3]), fabsf(f[4]), fabsf(f[5]));
+    return fmaxf(fmax3(a, b, fabsf(f[6])), fabsf(f[7]));
 }
 __device__ __forceinline__ float group_scale(float amax) {
     return fmaxf(__fdiv_rn(amax, kE4m3Max), kMinScale);

@@ -10,6 +10,7 @@
 // between the sum of squares and the scaling (vector kernel), so the bound is
 // the memory traffic of the inputs and outputs.
 //
+// quantize_rows_kernel: rows to e4m3 without a norm.
 // rows_kernel: TPR threads own a row, 8 consecutive elements each per step
 // (16-byte loads of 2-byte types), VPT steps.  A group of 128 columns is then
 // 16 neighbouring lanes, so its largest magnitude takes four shuffles and no
@@ -44,7 +45,7 @@ __device__ __forceinline__ float half_warp_max(float v) {
 }
 
 // Thread t's elements of a row to `out`, as they are or in groups of e4m3.
-template <typename T, bool NORM, bool QUANT, int TPR, int VPT>
+template <typename T, bool QUANT, int TPR, int VPT>
 __device__ __forceinline__ void write_row(const RowsArgs &a, long long row, int groups, int t, float (&h)[VPT][8]) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -53,7 +54,7 @@ __device__ __forceinline__ void write_row(const RowsArgs &a, long long row, int 
             const float scale = group_scale(half_warp_max(amax8(h[i])));
             if (c < a.cols) {
                 uint8_t *q = static_cast<uint8_t *>(a.out) + row * a.out_stride + c;
-                *reinterpret_cast<uint2 *>(q) = e4m3x8<!NORM>(h[i], divisor_of(scale));
+                *reinterpret_cast<uint2 *>(q) = e4m3x8<false>(h[i], divisor_of(scale));
                 if (t % 16 == 0)
                     a.scales[row * groups + c / kGroup] = scale;
             }
@@ -63,11 +64,8 @@ __device__ __forceinline__ void write_row(const RowsArgs &a, long long row, int 
     }
 }
 
-// Without a norm (no reduction to wait for) 64 registers, half the SM's threads,
-// keep most loads in flight: 24000 x 4096 bf16 54 us, with 80 registers 59, 48
-// registers 64 (before the exact quotients; with them 58).
-template <typename T, bool NORM, bool QUANT, int TPR, int VPT, int ROWS>
-__global__ void __launch_bounds__(TPR *ROWS, NORM ? 1 : 1024 / (TPR * ROWS)) rows_kernel(const RowsArgs a) {
+template <typename T, bool QUANT, int TPR, int VPT, int ROWS>
+__global__ void __launch_bounds__(TPR *ROWS) rows_kernel(const RowsArgs a) {
     constexpr int WARPS = TPR / 32; // warps of a row
     __shared__ float part[2][WARPS];
     static_assert(ROWS == 1 || TPR == 32, "a row of one warp, or a CTA for each row");
@@ -75,28 +73,26 @@ __global__ void __launch_bounds__(TPR *ROWS, NORM ? 1 : 1024 / (TPR * ROWS)) row
     const T *x = static_cast<const T *>(a.x), *res = static_cast<const T *>(a.residual);
     T *res_out = static_cast<T *>(a.residual_out);
     const int groups = (a.cols + kGroup - 1) / kGroup;
-    Vec8<T> w[NORM ? VPT : 1];
-    if constexpr (NORM) {
+    Vec8<T> w[VPT];
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int c = (i * TPR + t) * 8;
-            if (c < a.cols)
-                w[i] = load8(static_cast<const T *>(a.weight) + c);
-        }
+    for (int i = 0; i < VPT; ++i) {
+        const int c = (i * TPR + t) * 8;
+        if (c < a.cols)
+            w[i] = load8(static_cast<const T *>(a.weight) + c);
     }
     int turn = 0;
     const long long step = static_cast<long long>(gridDim.x) * ROWS;
     for (long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / TPR; row < a.rows; row += step) {
         float h[VPT][8];
         {
-            Vec8<T> xv[VPT], rv[NORM ? VPT : 1];
+            Vec8<T> xv[VPT], rv[VPT];
 #pragma unroll
             for (int i = 0; i < VPT; ++i) {
                 const int c = (i * TPR + t) * 8;
                 if (c < a.cols) {
                     xv[i] = load8(x + row * a.x_stride + c);
-                    if (NORM && res)
-                        rv[NORM ? i : 0] = load8(res + row * a.residual_stride + c);
+                    if (res)
+                        rv[i] = load8(res + row * a.residual_stride + c);
                 }
             }
 #pragma unroll
@@ -104,9 +100,9 @@ __global__ void __launch_bounds__(TPR *ROWS, NORM ? 1 : 1024 / (TPR * ROWS)) row
                 const int c = (i * TPR + t) * 8;
                 if (c < a.cols) {
                     unpack8(xv[i], h[i]);
-                    if (NORM && res) {
+                    if (res) {
                         float r[8];
-                        unpack8(rv[NORM ? i : 0], r);
+                        unpack8(rv[i], r);
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                             h[i][e] += r[e];
@@ -119,40 +115,38 @@ __global__ void __launch_bounds__(TPR *ROWS, NORM ? 1 : 1024 / (TPR * ROWS)) row
                 }
             }
         }
-        if constexpr (NORM) {
-            float sum = 0.f;
+        float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < VPT; ++i)
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                sum = fmaf(h[i][e], h[i][e], sum);
+        sum = warp_sum(sum);
+        if constexpr (WARPS > 1) {
+            // Two buffers: a warp may write the next row's part while
+            // another still reads this row's.
+            if (t % 32 == 0)
+                part[turn][t / 32] = sum;
+            __syncthreads();
+            sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < WARPS; ++k)
+                sum += part[turn][k];
+            turn ^= 1;
+        }
+        const float rstd = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * TPR + t) * 8;
+            if (c < a.cols) {
+                float wf[8];
+                unpack8(w[i], wf);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    sum = fmaf(h[i][e], h[i][e], sum);
-            sum = warp_sum(sum);
-            if constexpr (WARPS > 1) {
-                // Two buffers: a warp may write the next row's part while
-                // another still reads this row's.
-                if (t % 32 == 0)
-                    part[turn][t / 32] = sum;
-                __syncthreads();
-                sum = 0.f;
-#pragma unroll
-                for (int k = 0; k < WARPS; ++k)
-                    sum += part[turn][k];
-                turn ^= 1;
-            }
-            const float rstd = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                const int c = (i * TPR + t) * 8;
-                if (c < a.cols) {
-                    float wf[8];
-                    unpack8(w[i], wf);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        h[i][e] = h[i][e] * rstd * wf[e];
-                }
+                    h[i][e] = h[i][e] * rstd * wf[e];
             }
         }
-        write_row<T, NORM, QUANT, TPR, VPT>(a, row, groups, t, h);
+        write_row<T, QUANT, TPR, VPT>(a, row, groups, t, h);
     }
 }
 
@@ -167,14 +161,14 @@ __device__ __forceinline__ void bulk_load(uint32_t to, const void *from, uint32_
 // 256 / TPR rows at a time.  Stage: their x, then their residuals, `pitch` bytes
 // each.  Elements go to registers at once, so a stage is filled again while the
 // row is reduced, scaled and written.
-template <typename T, bool NORM, bool QUANT, int TPR, int VPT>
+template <typename T, bool QUANT, int TPR, int VPT>
 __global__ void __launch_bounds__(kStreamThreads) rows_stream_kernel(const RowsArgs a, int stages) {
     constexpr int ROWS = kStreamThreads / TPR, WARPS = TPR / 32;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ uint64_t full[kMaxStages];
     __shared__ float part[2][kStreamThreads / 32];
     const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-    const bool res = NORM && a.residual != nullptr;
+    const bool res = a.residual != nullptr;
     const uint32_t pitch = a.cols * sizeof(T), stage_bytes = ROWS * pitch * (res ? 2 : 1);
     const int groups = (a.cols + kGroup - 1) / kGroup;
     const long long turns = (a.rows + ROWS - 1) / ROWS;
@@ -202,14 +196,12 @@ __global__ void __launch_bounds__(kStreamThreads) rows_stream_kernel(const RowsA
     if (threadIdx.x == 0)
         for (int i = 0; i < stages && blockIdx.x + static_cast<long long>(i) * gridDim.x < turns; ++i)
             fill(blockIdx.x + static_cast<long long>(i) * gridDim.x, i);
-    Vec8<T> w[NORM ? VPT : 1];
-    if constexpr (NORM) {
+    Vec8<T> w[VPT];
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int c = (i * TPR + t) * 8;
-            if (c < a.cols)
-                w[i] = load8(static_cast<const T *>(a.weight) + c);
-        }
+    for (int i = 0; i < VPT; ++i) {
+        const int c = (i * TPR + t) * 8;
+        if (c < a.cols)
+            w[i] = load8(static_cast<const T *>(a.weight) + c);
     }
     int n = 0, stage = 0;
     for (long long turn = blockIdx.x; turn < turns; turn += gridDim.x, ++n) {
@@ -236,16 +228,14 @@ __global__ void __launch_bounds__(kStreamThreads) rows_stream_kernel(const RowsA
             }
         }
         float sum = 0.f;
-        if constexpr (NORM) {
 #pragma unroll
-            for (int i = 0; i < VPT; ++i)
+        for (int i = 0; i < VPT; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    sum = fmaf(h[i][e], h[i][e], sum);
-            sum = warp_sum(sum);
-            if (WARPS > 1 && threadIdx.x % 32 == 0)
-                part[n & 1][threadIdx.x / 32] = sum;
-        }
+            for (int e = 0; e < 8; ++e)
+                sum = fmaf(h[i][e], h[i][e], sum);
+        sum = warp_sum(sum);
+        if (WARPS > 1 && threadIdx.x % 32 == 0)
+            part[n & 1][threadIdx.x / 32] = sum;
         // Every thread has read the stage (and its row's parts are written).
         if (!__syncthreads_and(ok))
             break;
@@ -255,7 +245,7 @@ __global__ void __launch_bounds__(kStreamThreads) rows_stream_kernel(const RowsA
         stage = stage + 1 == stages ? 0 : stage + 1;
         if (row >= a.rows) // whole warps: the last turn's missing rows
             continue;
-        if (NORM && res) {
+        if (res) {
             T *to = static_cast<T *>(a.residual_out) + row * a.residual_out_stride;
 #pragma unroll
             for (int i = 0; i < VPT; ++i) {
@@ -264,24 +254,22 @@ __global__ void __launch_bounds__(kStreamThreads) rows_stream_kernel(const RowsA
                     store8(to + c, pack8<T>(h[i]));
             }
         }
-        if constexpr (NORM) {
-            if constexpr (WARPS > 1) {
-                sum = 0.f;
+        if constexpr (WARPS > 1) {
+            sum = 0.f;
 #pragma unroll
-                for (int k = 0; k < WARPS; ++k)
-                    sum += part[n & 1][slot * WARPS + k];
-            }
-            const float rstd = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                float wf[8];
-                unpack8(w[i], wf);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    h[i][e] = (i * TPR + t) * 8 < a.cols ? h[i][e] * rstd * wf[e] : 0.f;
-            }
+            for (int k = 0; k < WARPS; ++k)
+                sum += part[n & 1][slot * WARPS + k];
         }
-        write_row<T, NORM, QUANT, TPR, VPT>(a, row, groups, t, h);
+        const float rstd = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            float wf[8];
+            unpack8(w[i], wf);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                h[i][e] = (i * TPR + t) * 8 < a.cols ? h[i][e] * rstd * wf[e] : 0.f;
+        }
+        write_row<T, QUANT, TPR, VPT>(a, row, groups, t, h);
     }
     // After a wait that gave up: every copy lands before the CTA's memory goes.
     if (threadIdx.x == 0) {
@@ -364,6 +352,94 @@ __global__ void __launch_bounds__(256) rows_scalar_kernel(const RowsArgs a) {
     }
 }
 
+// The largest of four magnitudes over the 16 lanes of a half warp: while lanes halve, so
+// do the values that each still holds, and lane l ends with value l / 4 (5 shuffles, not
+// 16; 24000 x 4096 56 -> 50 us, with one lane's division for each).
+__device__ __forceinline__ float max_of_four(const float (&m)[4], int lane) {
+    const bool high = lane & 8, odd = lane & 4;
+    const float a = fmaxf(high ? m[2] : m[0], __shfl_xor_sync(0xffffffffu, high ? m[0] : m[2], 8));
+    const float b = fmaxf(high ? m[3] : m[1], __shfl_xor_sync(0xffffffffu, high ? m[1] : m[3], 8));
+    float v = fmaxf(odd ? b : a, __shfl_xor_sync(0xffffffffu, odd ? a : b, 4));
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+}
+
+// Groups of 128 columns need nothing from the rest of their row, so that all groups of
+// all rows are one list: a half warp takes a group, a warp runs of 8, in four steps.
+// 24000 x 4096 bf16 50 us (5.95 TB/s), 24000 x 1152 19 us; a row per CTA, as
+// rows_kernel takes them, 50 and 27 us: its threads past the row's end are idle.
+constexpr int kSteps = 4;
+// WHOLE: rows of whole groups, one behind the other in x and in out.
+template <typename T, bool WHOLE> __global__ void __launch_bounds__(256, 4) quantize_rows_kernel(const RowsArgs a) {
+    const int lane = threadIdx.x & 31, part = lane & 15, groups = (a.cols + kGroup - 1) / kGroup;
+    const long long total = a.rows * groups;
+    const long long begin = (blockIdx.x * 8ll + threadIdx.x / 32) * (2 * kSteps), stride = gridDim.x * 8ll * (2 * kSteps);
+    // This half warp's group `at`, its row and its place in the row.
+    long long at = begin + lane / 16, row = 0, rows_on = 0;
+    int g = 0, groups_on = 0;
+    if constexpr (!WHOLE) {
+        row = at / groups;
+        g = static_cast<int>(at - row * groups);
+        rows_on = stride / groups;
+        groups_on = static_cast<int>(stride - rows_on * groups);
+    }
+    const long long x_wrap = a.x_stride - static_cast<long long>(groups) * kGroup;
+    const long long q_wrap = a.out_stride - static_cast<long long>(groups) * kGroup;
+    for (long long first = begin; first < total; first += stride, at += stride) { // the whole warp
+        float h[kSteps][8], top[kSteps];
+        {
+            Vec8<T> v[kSteps];
+            const T *x = static_cast<const T *>(a.x) + (WHOLE ? at * kGroup : row * a.x_stride + g * kGroup) + part * 8;
+            int in = g;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                v[i] = Vec8<T>{};
+                if (at + 2 * i < total && (WHOLE || in * kGroup + part * 8 < a.cols))
+                    v[i] = load8(x);
+                x += 2 * kGroup;
+                if constexpr (!WHOLE)
+                    for (in += 2; in >= groups; in -= groups)
+                        x += x_wrap;
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+                unpack8(v[i], h[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+            top[i] = amax8(h[i]);
+        // A lane divides for one step and hands the result round.
+        constexpr int LANES = 16 / kSteps;
+        const float scale = group_scale(max_of_four(top, part));
+        const Divisor divisor = divisor_of(scale);
+        const long long own = at + 2 * (part / LANES);
+        if (part % LANES == 0 && own < total)
+            a.scales[own] = scale;
+        uint8_t *q = static_cast<uint8_t *>(a.out) + (WHOLE ? at * kGroup : row * a.out_stride + g * kGroup) + part * 8;
+        int in = g;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            Divisor d;
+            d.scale = __shfl_sync(0xffffffffu, divisor.scale, i * LANES, 16);
+            d.inv = __shfl_sync(0xffffffffu, divisor.inv, i * LANES, 16);
+            if (at + 2 * i < total && (WHOLE || in * kGroup + part * 8 < a.cols))
+                *reinterpret_cast<uint2 *>(q) = e4m3x8<true>(h[i], d);
+            q += 2 * kGroup;
+            if constexpr (!WHOLE)
+                for (in += 2; in >= groups; in -= groups)
+                    q += q_wrap;
+        }
+        if constexpr (!WHOLE) {
+            row += rows_on;
+            g += groups_on;
+            if (g >= groups) {
+                g -= groups;
+                ++row;
+            }
+        }
+    }
+}
+
 // One CTA per 128 x 128 block: thread = 8 columns of every 16th row, its 64
 // elements in registers between the largest magnitude and the conversion.
 template <typename T, bool VEC>
@@ -413,13 +489,13 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T *x, uint8_
     }
 }
 
-template <typename T, bool NORM, bool QUANT, int TPR, int VPT, int ROWS>
+template <typename T, bool QUANT, int TPR, int VPT, int ROWS>
 int launch_rows(const RowsArgs &a, cudaStream_t stream) {
     // As many CTAs as run at once: every one takes the same number of rows, +-1.
     static std::atomic<int> resident{0};
     int each = resident.load(std::memory_order_relaxed);
     if (!each) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, rows_kernel<T, NORM, QUANT, TPR, VPT, ROWS>,
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, rows_kernel<T, QUANT, TPR, VPT, ROWS>,
                                                           TPR * ROWS, 0) != cudaSuccess ||
             each < 1)
             each = 1;
@@ -427,26 +503,59 @@ int launch_rows(const RowsArgs &a, cudaStream_t stream) {
     }
     const long long ctas = (a.rows + ROWS - 1) / ROWS;
     const long long most = static_cast<long long>(fmha_sm_count()) * each;
-    rows_kernel<T, NORM, QUANT, TPR, VPT, ROWS>
+    rows_kernel<T, QUANT, TPR, VPT, ROWS>
         <<<static_cast<unsigned>(std::min(ctas, most)), TPR * ROWS, 0, stream>>>(a);
     return static_cast<int>(cudaGetLastError());
 }
 
-template <typename T, bool NORM, bool QUANT, int TPR, int VPT> int launch_stream(const RowsArgs &a, cudaStream_t stream) {
+template <typename T, bool QUANT, int TPR, int VPT> int launch_stream(const RowsArgs &a, cudaStream_t stream) {
     constexpr int ROWS = kStreamThreads / TPR;
     const int stage = ROWS * a.cols * static_cast<int>(sizeof(T)) * (a.residual ? 2 : 1);
     const int stages = std::max(2, std::min(kMaxStages, kStreamBytes / stage));
     static std::atomic<unsigned long long> done{0};
-    const cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(rows_stream_kernel<T, NORM, QUANT, TPR, VPT>),
+    const cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(rows_stream_kernel<T, QUANT, TPR, VPT>),
                                          std::max(kStreamBytes, 2 * 1024 * 8 * static_cast<int>(sizeof(T)) * 2), done);
     if (e != cudaSuccess)
         return static_cast<int>(e);
     const long long turns = (a.rows + ROWS - 1) / ROWS;
     const int each = 200 * 1024 / (stages * stage); // CTAs on an SM
     const long long most = static_cast<long long>(fmha_sm_count()) * std::max(1, std::min(each, 4));
-    rows_stream_kernel<T, NORM, QUANT, TPR, VPT>
+    rows_stream_kernel<T, QUANT, TPR, VPT>
         <<<static_cast<unsigned>(std::min(turns, most)), kStreamThreads, stages * stage, stream>>>(a, stages);
     return static_cast<int>(cudaGetLastError());
+}
+
+// Rows of `vecs` 8-element vectors.
+template <typename T, bool QUANT> int launch_norm(const RowsArgs &a, int vecs, cudaStream_t stream) {
+    // Rows enough for every SM to keep its ring busy.  Measured (bf16, residual,
+    // e4m3): 16384 x 8192 151 us against rows_kernel's 173, 16384 x 4096 85 and 101,
+    // 23328 x 1152 40 and 44.
+    if (vecs <= 1024 && a.rows * vecs >= 64ll * 1024 * 8) {
+        if (vecs <= 32)
+            return launch_stream<T, QUANT, 32, 1>(a, stream);
+        if (vecs <= 64)
+            return launch_stream<T, QUANT, 32, 2>(a, stream);
+        if (vecs <= 128)
+            return launch_stream<T, QUANT, 32, 4>(a, stream);
+        if (vecs <= 256)
+            return launch_stream<T, QUANT, 64, 4>(a, stream);
+        if (vecs <= 512)
+            return launch_stream<T, QUANT, 128, 4>(a, stream);
+        return launch_stream<T, QUANT, 256, 4>(a, stream);
+    }
+    if (vecs <= 32)
+        return launch_rows<T, QUANT, 32, 1, 4>(a, stream);
+    if (vecs <= 64)
+        return launch_rows<T, QUANT, 32, 2, 4>(a, stream);
+    if (vecs <= 128)
+        return launch_rows<T, QUANT, 32, 4, 4>(a, stream);
+    if (vecs <= 256)
+        return launch_rows<T, QUANT, 128, 2, 1>(a, stream);
+    if (vecs <= 512)
+        return launch_rows<T, QUANT, 128, 4, 1>(a, stream);
+    if (vecs <= 1024)
+        return launch_rows<T, QUANT, 256, 4, 1>(a, stream);
+    return launch_rows<T, QUANT, 512, 4, 1>(a, stream);
 }
 
 template <typename T, bool NORM, bool QUANT> int launch_typed(const RowsArgs &a, cudaStream_t stream) {
@@ -458,40 +567,21 @@ template <typename T, bool NORM, bool QUANT> int launch_typed(const RowsArgs &a,
                      (!a.residual || (a.residual_stride % kAlign == 0 && a.residual_out_stride % kAlign == 0)) &&
                      (QUANT ? out % 8 == 0 && a.out_stride % 8 == 0 : out % 16 == 0 && a.out_stride % kAlign == 0);
     const int vecs = a.cols / 8;
-    if (!vec || vecs > 2048) {
+    if (!vec || (NORM && vecs > 2048)) {
         const unsigned grid = static_cast<unsigned>(std::min<long long>(a.rows, 8ll * fmha_sm_count()));
         rows_scalar_kernel<T, NORM, QUANT><<<grid, 256, 0, stream>>>(a);
         return static_cast<int>(cudaGetLastError());
     }
-    // Rows enough for every SM to keep its ring busy.  Measured (bf16, residual,
-    // e4m3): 16384 x 8192 151 us against rows_kernel's 173, 16384 x 4096 85 and 101,
-    // 23328 x 1152 40 and 44.  Without a norm rows_kernel is the faster one.
-    if (NORM && vecs <= 1024 && a.rows * vecs >= 64ll * 1024 * 8) {
-        if (vecs <= 32)
-            return launch_stream<T, NORM, QUANT, 32, 1>(a, stream);
-        if (vecs <= 64)
-            return launch_stream<T, NORM, QUANT, 32, 2>(a, stream);
-        if (vecs <= 128)
-            return launch_stream<T, NORM, QUANT, 32, 4>(a, stream);
-        if (vecs <= 256)
-            return launch_stream<T, NORM, QUANT, 64, 4>(a, stream);
-        if (vecs <= 512)
-            return launch_stream<T, NORM, QUANT, 128, 4>(a, stream);
-        return launch_stream<T, NORM, QUANT, 256, 4>(a, stream);
-    }
-    if (vecs <= 32)
-        return launch_rows<T, NORM, QUANT, 32, 1, 4>(a, stream);
-    if (vecs <= 64)
-        return launch_rows<T, NORM, QUANT, 32, 2, 4>(a, stream);
-    if (vecs <= 128)
-        return launch_rows<T, NORM, QUANT, 32, 4, 4>(a, stream);
-    if (vecs <= 256)
-        return launch_rows<T, NORM, QUANT, 128, 2, 1>(a, stream);
-    if (vecs <= 512)
-        return launch_rows<T, NORM, QUANT, 128, 4, 1>(a, stream);
-    if (vecs <= 1024)
-        return launch_rows<T, NORM, QUANT, 256, 4, 1>(a, stream);
-    return launch_rows<T, NORM, QUANT, 512, 4, 1>(a, stream);
+    if constexpr (NORM)
+        return launch_norm<T, QUANT>(a, vecs, stream);
+    const long long runs = (a.rows * ((a.cols + kGroup - 1) / kGroup) + 2 * kSteps - 1) / (2 * kSteps);
+    const unsigned grid = static_cast<unsigned>(std::min((runs + 7) / 8, 4ll * fmha_sm_count()));
+    // 24000 x 1152 19 us either way, 24000 x 4096 49 and 52.
+    if (a.cols % kGroup == 0 && a.x_stride == a.cols && a.out_stride == a.cols)
+        quantize_rows_kernel<T, true><<<grid, 256, 0, stream>>>(a);
+    else
+        quantize_rows_kernel<T, false><<<grid, 256, 0, stream>>>(a);
+    return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T> int launch_dtype(const RowsArgs &a, cudaStream_t stream) {
