@@ -9,8 +9,8 @@
 // Inputs of 16 bits often have quotients half way between two e4m3 values, so what
 // is quantised as it is (EXACT) takes x * (1 / scale) with one correction by its
 // residual (Markstein, 1990), which rounds as a division would, for two more
-// operations an element (24000 x 4096: 54 -> 58 us).  A norm's values carry fp32
-// rounding errors of their own and do without.
+// operations on a pair of elements (24000 x 4304: 53 -> 56 us; 24000 x 4096: 49
+// either way).  A norm's values carry fp32 rounding errors of their own and do without.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

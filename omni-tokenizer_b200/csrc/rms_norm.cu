@@ -8,7 +8,8 @@
 // residual_out = h and out = y, each rounded once to the element type, or out =
 // the groups of e4m3.cuh.  A row is read once: its elements stay in registers
 // between the sum of squares and the scaling (vector kernel), so the bound is
-// the memory traffic of the inputs and outputs.
+// the memory traffic of the inputs and outputs: 16384 x 8192 bf16 with a residual to
+// e4m3 148 us, 6.37 TB/s; 24000 x 4096 bf16 to e4m3 49 us, 6.0 TB/s.
 //
 // quantize_rows_kernel: rows to e4m3 without a norm.
 // rows_kernel: TPR threads own a row, 8 consecutive elements each per step
@@ -17,7 +18,7 @@
 // shared memory.  The grid is persistent: the weight is read once per CTA.
 // rows_stream_kernel: many rows.  The same thread layout, rows through a ring of
 // shared memory that bulk copies fill several rows ahead, so that loads are in
-// flight at all times (rows_kernel's stop at every reduction).
+// flight at all times.
 // rows_scalar_kernel serves columns and pitches that 16-byte loads cannot, and
 // rows wider than the registers hold; it reads its row twice (the second time
 // from L2).
@@ -82,37 +83,51 @@ __global__ void __launch_bounds__(TPR *ROWS) rows_kernel(const RowsArgs a) {
     }
     int turn = 0;
     const long long step = static_cast<long long>(gridDim.x) * ROWS;
-    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / TPR; row < a.rows; row += step) {
-        float h[VPT][8];
-        {
-            Vec8<T> xv[VPT], rv[VPT];
+    // The next row's loads are under way while this one is reduced, scaled and written
+    // (23328 x 1152: 47 -> 38 us).
+    Vec8<T> xv[VPT], rv[VPT];
+    auto fetch = [&](long long row) {
 #pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                const int c = (i * TPR + t) * 8;
-                if (c < a.cols) {
-                    xv[i] = load8(x + row * a.x_stride + c);
-                    if (res)
-                        rv[i] = load8(res + row * a.residual_stride + c);
-                }
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * TPR + t) * 8;
+            if (c < a.cols) {
+                xv[i] = load8(x + row * a.x_stride + c);
+                if (res)
+                    rv[i] = load8(res + row * a.residual_stride + c);
             }
+        }
+    };
+    long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / TPR;
+    if (row < a.rows)
+        fetch(row);
+    for (; row < a.rows; row += step) {
+        float h[VPT][8];
 #pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                const int c = (i * TPR + t) * 8;
-                if (c < a.cols) {
-                    unpack8(xv[i], h[i]);
-                    if (res) {
-                        float r[8];
-                        unpack8(rv[i], r);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            h[i][e] += r[e];
-                        store8(res_out + row * a.residual_out_stride + c, pack8<T>(h[i]));
-                    }
-                } else {
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * TPR + t) * 8;
+            if (c < a.cols) {
+                unpack8(xv[i], h[i]);
+                if (res) {
+                    float r[8];
+                    unpack8(rv[i], r);
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        h[i][e] = 0.f;
+                        h[i][e] += r[e];
                 }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    h[i][e] = 0.f;
+            }
+        }
+        if (row + step < a.rows)
+            fetch(row + step);
+        if (res) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int c = (i * TPR + t) * 8;
+                if (c < a.cols)
+                    store8(res_out + row * a.residual_out_stride + c, pack8<T>(h[i]));
             }
         }
         float sum = 0.f;
@@ -366,8 +381,8 @@ __device__ __forceinline__ float max_of_four(const float (&m)[4], int lane) {
 
 // Groups of 128 columns need nothing from the rest of their row, so that all groups of
 // all rows are one list: a half warp takes a group, a warp runs of 8, in four steps.
-// 24000 x 4096 bf16 50 us (5.95 TB/s), 24000 x 1152 19 us; a row per CTA, as
-// rows_kernel takes them, 50 and 27 us: its threads past the row's end are idle.
+// 24000 x 4096 bf16 49 us, 24000 x 1152 16 us; a row per CTA took 50 and 27 us:
+// its threads past the row's end are idle.
 constexpr int kSteps = 4;
 // WHOLE: rows of whole groups, one behind the other in x and in out.
 template <typename T, bool WHOLE> __global__ void __launch_bounds__(256, 4) quantize_rows_kernel(const RowsArgs a) {
@@ -527,16 +542,11 @@ template <typename T, bool QUANT, int TPR, int VPT> int launch_stream(const Rows
 
 // Rows of `vecs` 8-element vectors.
 template <typename T, bool QUANT> int launch_norm(const RowsArgs &a, int vecs, cudaStream_t stream) {
-    // Rows enough for every SM to keep its ring busy.  Measured (bf16, residual,
-    // e4m3): 16384 x 8192 151 us against rows_kernel's 173, 16384 x 4096 85 and 101,
-    // 23328 x 1152 40 and 44.
-    if (vecs <= 1024 && a.rows * vecs >= 64ll * 1024 * 8) {
-        if (vecs <= 32)
-            return launch_stream<T, QUANT, 32, 1>(a, stream);
-        if (vecs <= 64)
-            return launch_stream<T, QUANT, 32, 2>(a, stream);
-        if (vecs <= 128)
-            return launch_stream<T, QUANT, 32, 4>(a, stream);
+    // Wide rows, and enough of them for every SM to keep its ring busy.  Measured (bf16,
+    // residual, e4m3): 16384 x 8192 148 us against rows_kernel's 176, 16384 x 4096 83 and
+    // 104, 23328 x 2048 65 and 79 (a warp for each row).  Narrower rows leave a ring less
+    // than a warp for each row gains: 23328 x 1024 38 and 30, 23328 x 512 26 and 20.
+    if (vecs > 192 && vecs <= 1024 && a.rows * vecs >= 64ll * 1024 * 8) {
         if (vecs <= 256)
             return launch_stream<T, QUANT, 64, 4>(a, stream);
         if (vecs <= 512)
@@ -549,6 +559,10 @@ template <typename T, bool QUANT> int launch_norm(const RowsArgs &a, int vecs, c
         return launch_rows<T, QUANT, 32, 2, 4>(a, stream);
     if (vecs <= 128)
         return launch_rows<T, QUANT, 32, 4, 4>(a, stream);
+    if (vecs <= 160) // 23328 x 1152 38 us; without the next row's loads 47, by 128 threads to a row 57
+        return launch_rows<T, QUANT, 32, 5, 4>(a, stream);
+    if (vecs <= 192)
+        return launch_rows<T, QUANT, 32, 6, 4>(a, stream);
     if (vecs <= 256)
         return launch_rows<T, QUANT, 128, 2, 1>(a, stream);
     if (vecs <= 512)
@@ -576,7 +590,7 @@ template <typename T, bool NORM, bool QUANT> int launch_typed(const RowsArgs &a,
         return launch_norm<T, QUANT>(a, vecs, stream);
     const long long runs = (a.rows * ((a.cols + kGroup - 1) / kGroup) + 2 * kSteps - 1) / (2 * kSteps);
     const unsigned grid = static_cast<unsigned>(std::min((runs + 7) / 8, 4ll * fmha_sm_count()));
-    // 24000 x 1152 19 us either way, 24000 x 4096 49 and 52.
+    // Without rows to keep track of: 24000 x 4096 49 us, with them 52.
     if (a.cols % kGroup == 0 && a.x_stride == a.cols && a.out_stride == a.cols)
         quantize_rows_kernel<T, true><<<grid, 256, 0, stream>>>(a);
     else
