@@ -179,6 +179,7 @@ __device__ __forceinline__ void bulk_load(uint32_t to, const void *from, uint32_
 template <typename T, bool QUANT, int TPR, int VPT>
 __global__ void __launch_bounds__(kStreamThreads) rows_stream_kernel(const RowsArgs a, int stages) {
     constexpr int ROWS = kStreamThreads / TPR, WARPS = TPR / 32;
+    static_assert(WARPS > 1, "narrow rows are rows_kernel's");
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ uint64_t full[kMaxStages];
     __shared__ float part[2][kStreamThreads / 32];
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(kStreamThreads) rows_stream_kernel(const RowsA
             for (int e = 0; e < 8; ++e)
                 sum = fmaf(h[i][e], h[i][e], sum);
         sum = warp_sum(sum);
-        if (WARPS > 1 && threadIdx.x % 32 == 0)
+        if (threadIdx.x % 32 == 0)
             part[n & 1][threadIdx.x / 32] = sum;
         // Every thread has read the stage (and its row's parts are written).
         if (!__syncthreads_and(ok))
@@ -269,12 +270,10 @@ __global__ void __launch_bounds__(kStreamThreads) rows_stream_kernel(const RowsA
                     store8(to + c, pack8<T>(h[i]));
             }
         }
-        if constexpr (WARPS > 1) {
-            sum = 0.f;
+        sum = 0.f;
 #pragma unroll
-            for (int k = 0; k < WARPS; ++k)
-                sum += part[n & 1][slot * WARPS + k];
-        }
+        for (int k = 0; k < WARPS; ++k)
+            sum += part[n & 1][slot * WARPS + k];
         const float rstd = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {

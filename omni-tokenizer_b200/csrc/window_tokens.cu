@@ -19,6 +19,7 @@
 //     of its four keys and pairs them up with byte permutes.
 // Rows are 128 or 256 bytes apart; the 16-byte pieces of a row are permuted by
 // the row number so that the eight lanes of a load phase meet all 32 banks.
+// 64 sequences of up to 16384 keys, 32/8 heads of 128, window 4096: 167 us, 6.19 TB/s.
 // A cluster of CTAs splits the keys of one tile of rows, so that few sequences
 // still load with many SMs; the parts meet in distributed shared memory, in rank
 // order (no atomics).
