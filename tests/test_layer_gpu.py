@@ -111,6 +111,29 @@ def test_rms_norm(ob, rows, cols, dtype):
     ob.library().sync_check()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,cols", [(2500, 33), (2500, 511), (1300, 513), (1300, 1013), (1300, 1025), (301, 2001),
+                                       (301, 3727), (301, 4097), (1300, 8191), (40, 9001)])
+def test_rms_norm_of_rows_that_vectors_cannot_read(ob, rows, cols, dtype):
+    """Odd columns, each kernel with more rows than run at once; and in place."""
+    test_rms_norm(ob, rows, cols, dtype)
+    x, res, w = (_randn(*n, seed=cols + i, dtype=dtype) for i, n in enumerate([(rows, cols), (rows, cols), (cols,)]))
+    want, hwant = ob.rms_norm(x, w, residual=res)
+    ob.rms_norm(x, w, residual=res, residual_out=res, out=x)
+    assert torch.equal(x, want) and torch.equal(res, hwant)
+
+
+@pytest.mark.parametrize("rows,cols", [(20000, 200), (9000, 512), (9000, 1152), (9000, 1280), (5000, 1536), (5000, 2048),
+                                       (3000, 8192)])
+def test_rms_norm_of_many_rows(ob, rows, cols):
+    """More rows than run at once, whose next ones are loaded ahead; and in place."""
+    test_rms_norm(ob, rows, cols, BF16)
+    x, res, w = (_randn(*n, seed=cols + i, dtype=BF16) for i, n in enumerate([(rows, cols), (rows, cols), (cols,)]))
+    want, hwant = ob.rms_norm(x, w, residual=res)
+    ob.rms_norm(x, w, residual=res, residual_out=res, out=x)
+    assert torch.equal(x, want) and torch.equal(res, hwant)
+
+
 @pytest.mark.parametrize("cols", [257, 512, 1152])
 def test_rms_norm_strides_and_places(ob, cols):
     """Pitched rows, a residual updated in place, and an output in x's place."""
@@ -157,6 +180,33 @@ def test_quantize(ob, rows, cols, block_rows, dtype):
     wide = _strided(x, 16 if cols % 16 == 0 else 3)
     q2, s2 = ob.quantize_e4m3(wide, block_rows=block_rows)
     assert torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2, s)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("rows,cols", [(9001, 128), (9001, 997), (30001, 64), (9001, 1152), (2001, 4097), (3001, 4304)])
+def test_quantize_many_rows(ob, rows, cols, block_rows, dtype):
+    """More groups than run at once, a row's last one short or single."""
+    x = _randn(rows, cols, seed=rows + cols, dtype=dtype, scale=0.3)
+    q, s = ob.quantize_e4m3(x, block_rows=block_rows)
+    _check_quantized(q, s, x.double(), block_rows)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("cols", [120, 125, 384])
+def test_quantize_to_any_address(ob, cols, block_rows):
+    """q at an odd address with an odd pitch; the bytes between its rows stay."""
+    x = _randn(150, cols, seed=cols, dtype=BF16)
+    want, s = ob.quantize_e4m3(x, block_rows=block_rows)
+    pitch = cols + 7
+    room = torch.full((150 * pitch + 3,), 0x55, dtype=torch.uint8, device="cuda")
+    s2 = torch.empty_like(s)
+    lib = ob.library()
+    lib.check(lib.lib.omni_b200_quantize_e4m3(x.data_ptr(), room.data_ptr() + 3, s2.data_ptr(), 150, cols, cols, pitch,
+                                              block_rows, 1, torch.cuda.current_stream().cuda_stream))
+    got = room[3:].view(150, pitch)
+    assert torch.equal(got[:, :cols], want.view(torch.uint8)) and torch.equal(s2, s)
+    assert bool((got[:, cols:] == 0x55).all()) and bool((room[:3] == 0x55).all())
 
 
 @pytest.mark.parametrize("block_rows", [1, 128])
