@@ -10,7 +10,9 @@
 // is quantised as it is (EXACT) takes x * (1 / scale) with one correction by its
 // residual (Markstein, 1990), which rounds as a division would, for two more
 // operations on a pair of elements (24000 x 4304: 53 -> 56 us; 24000 x 4096: 49
-// either way).  A norm's values carry fp32 rounding errors of their own and do without.
+// either way).  A norm's values carry fp32
+// rounding errors of their own and do without: of 27 million 17 round otherwise than in
+// 64 bits, 19 with fp32 divisions, and the correction costs 16384 x 8192 148 -> 165 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
