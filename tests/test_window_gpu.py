@@ -316,3 +316,35 @@ def test_layer_of_all_operators(ob):
     want = want + bias.double()
     assert bool(((y.double() - want).abs() <= mag * 2.0**-11 + want.abs() * 2.0**-8 * 1.01).all())
     assert bool((y.view(B, n, d)[2] == bias).all())  # a sequence without keys mixes to zeros
+
+
+def test_different_operators_at_once(ob):
+    """Kernels that share SMs, shared memory and tensor memory, on four streams: each
+    call's bits are those of the call alone."""
+    q, k, v = _inputs(2, 8, 2, 300, 900, 128, BF16, "heads", seed=1)
+    q1, k1, v1 = _inputs(4, 8, 8, 1, 2000, 64, BF16, "tokens", seed=2)
+    e, _, _ = _inputs(2, 4, 4, 500, 500, 72, BF16, "heads", seed=3)
+    x = torch.randn(700, 1152, generator=torch.Generator().manual_seed(4)).to(BF16).cuda()
+    w, sw = ob.quantize_e4m3(x[:640], block_rows=128)
+    a, sa = ob.quantize_e4m3(x)
+    calls = [
+        lambda s: ob.attention_window(q, k, v, window=200, sinks=4, stream=s),
+        lambda s: ob.linear_e4m3(a[:5].contiguous(), sa[:5], w, sw, stream=s),
+        lambda s: ob.attention_window(q1, k1, v1, window=700, stream=s),
+        lambda s: ob.attention_bhld(e, e, e, stream=s),
+        lambda s: ob.linear_e4m3(a, sa, w, sw, stream=s),
+        lambda s: ob.rms_norm(x, x[0].contiguous(), stream=s)[0],
+        lambda s: ob.quantize_e4m3(x, stream=s)[0].view(torch.uint8),
+    ]
+    want = [c(None) for c in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(4)], []
+    for turn in range(12):
+        for i, c in enumerate(calls):
+            s = streams[(i + turn) % 4]
+            with torch.cuda.stream(s):  # its own memory pool, and small copies in order
+                got.append((i, c(s)))
+    torch.cuda.synchronize()
+    for i, g in got:
+        assert torch.equal(g, want[i]), f"call {i}"
+    ob.library().sync_check()
