@@ -258,6 +258,11 @@ def attention_rows(q, k, v, heads, block=0, valid=None, fused=False, out_dtype=N
 # A call with one token is over in a few microseconds on the device, so these
 # helpers keep the host's part short: every tensor attribute is read once, and the
 # device's stream is looked up without building objects or importing per call.
+# They work on the current stream of the tensors' device.  stream=s (a torch.cuda.Stream)
+# is short for `with torch.cuda.stream(s):`.  As there, the inputs have to be ready on s
+# and kept (or recorded on s) until it is done with them, and the outputs are memory of
+# s: another stream waits for s before it reads them, and records them when it may
+# still read them after they are dropped.
 class _Torch:
     """torch's names that the helpers use, looked up at their first call."""
 
@@ -289,6 +294,17 @@ def _device_of(what, *tensors):
     return device
 
 
+def _on(what, stream, t):
+    """The context in which a helper that was given a stream works: a call with
+    stream=s is the call made inside torch.cuda.stream(s).  Outputs, those that the
+    caller drops at once among them, are memory of that stream, so that no kernel
+    pending on the current stream has it, and none there gets it before the call is over."""
+    device = t.get_device()
+    if 0 <= device != stream.device_index:
+        _refuse(f"{what}: stream must be on the tensors' device")
+    return _t.cuda.stream(stream)
+
+
 def _row_stride(what, t, shape):
     """Elements between the rows of a matrix with contiguous columns; a single row's
     stride does not matter."""
@@ -300,11 +316,11 @@ def _row_stride(what, t, shape):
     return rows if shape[0] > 1 else shape[1]
 
 
-def _call(name, device, stream, *args):
-    """Calls an entry point on `device` and on `stream`, or that device's current one."""
+def _call(name, device, *args):
+    """Calls an entry point on `device` and on its current stream."""
     lib = _LIB or library()
     fn = getattr(lib.lib, name)
-    s = _t.raw_stream(device) if stream is None else stream.cuda_stream
+    s = _t.raw_stream(device)
     if device == _t.current_device():
         status = fn(*args, s)
     else:
@@ -332,7 +348,7 @@ def _empty_e4m3(x, rows, cols):
     return x.new_empty((rows, pitch), dtype=_t.e4m3)[:, :cols], pitch
 
 
-def _norm(what, x, shape, code, weight, residual, residual_out, out, out_stride, scales, eps, out_code, stream):
+def _norm(what, x, shape, code, weight, residual, residual_out, out, out_stride, scales, eps, out_code):
     rows, cols = shape
     dtype = x.dtype
     if weight.shape != (cols,) or weight.dtype != dtype or (cols > 1 and weight.stride(0) != 1):
@@ -354,7 +370,7 @@ def _norm(what, x, shape, code, weight, residual, residual_out, out, out_stride,
         from_stride = _row_stride(what, residual, shape)
         from_ptr, to_ptr = residual.data_ptr(), residual_out.data_ptr()
     device = _device_of(what, x, weight, residual, residual_out, out)
-    _call("omni_b200_rms_norm", device, stream, x.data_ptr(), from_ptr, weight.data_ptr(), to_ptr, out.data_ptr(),
+    _call("omni_b200_rms_norm", device, x.data_ptr(), from_ptr, weight.data_ptr(), to_ptr, out.data_ptr(),
           scales, rows, cols, _row_stride(what, x, shape), from_stride, to_stride, out_stride, eps, code, out_code)
     return residual_out
 
@@ -365,6 +381,9 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None, st
     Returns (y, h): y = h / sqrt(mean(h^2) + eps) * weight in x's type, h = x + residual
     (None without a residual).  residual_out and out may each be x or residual, not both
     the same one."""
+    if stream is not None:
+        with _on("rms_norm", stream, x):
+            return rms_norm(x, weight, residual, eps, out, residual_out)
     shape, code = _matrix("rms_norm", x)
     if out is None:
         out, out_stride = _t.empty_like(x) if x.is_contiguous() else x.new_empty(shape), shape[1]
@@ -372,25 +391,30 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None, st
         _refuse("rms_norm: out must have x's shape and type")
     else:
         out_stride = _row_stride("rms_norm", out, shape)
-    return out, _norm("rms_norm", x, shape, code, weight, residual, residual_out, out, out_stride, None, eps, code,
-                      stream)
+    return out, _norm("rms_norm", x, shape, code, weight, residual, residual_out, out, out_stride, None, eps, code)
 
 
 def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, residual_out=None, stream=None):
     """rms_norm with its output in e4m3 and an fp32 scale for each 128 columns.
 
     Returns (q, scales, h); q and scales are what linear_e4m3 takes."""
+    if stream is not None:
+        with _on("rms_norm_e4m3", stream, x):
+            return rms_norm_e4m3(x, weight, residual, eps, residual_out)
     shape, code = _matrix("rms_norm_e4m3", x)
     rows, cols = shape
     q, pitch = _empty_e4m3(x, rows, cols)
     scales = x.new_empty((rows, (cols + 127) // 128), dtype=_t.f32)
     return q, scales, _norm("rms_norm_e4m3", x, shape, code, weight, residual, residual_out, q, pitch,
-                            scales.data_ptr(), eps, E4M3, stream)
+                            scales.data_ptr(), eps, E4M3)
 
 
 def quantize_e4m3(x, block_rows=1, stream=None):
     """x [rows, cols] in e4m3: (q, scales), a scale for each 128 columns of a row
     (block_rows=1) or each 128 x 128 block (block_rows=128, weights)."""
+    if stream is not None:
+        with _on("quantize_e4m3", stream, x):
+            return quantize_e4m3(x, block_rows)
     shape, code = _matrix("quantize_e4m3", x)
     if block_rows != 1 and block_rows != 128:
         _refuse("quantize_e4m3: block_rows must be 1 or 128")
@@ -399,14 +423,17 @@ def quantize_e4m3(x, block_rows=1, stream=None):
     stride = _row_stride("quantize_e4m3", x, shape)
     q, pitch = _empty_e4m3(x, rows, cols)
     scales = x.new_empty(((rows + block_rows - 1) // block_rows, (cols + 127) // 128), dtype=_t.f32)
-    _call("omni_b200_quantize_e4m3", device, stream, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols, stride,
-          pitch, block_rows, code)
+    _call("omni_b200_quantize_e4m3", device, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols, stride, pitch,
+          block_rows, code)
     return q, scales
 
 
 def linear_e4m3(a, a_scales, w, w_scales, bias=None, out_dtype=None, out=None, stream=None):
     """a [m, k] times w [n, k] transposed, both e4m3 with scales (quantize_e4m3 with
     block_rows 1 and 128), plus bias [n]: [m, n] of out_dtype (bfloat16)."""
+    if stream is not None:
+        with _on("linear_e4m3", stream, a):
+            return linear_e4m3(a, a_scales, w, w_scales, bias, out_dtype, out)
     shape, w_shape = a.shape, w.shape
     if len(shape) != 2 or len(w_shape) != 2 or a.dtype != _t.e4m3 or w.dtype != _t.e4m3 or w_shape[1] != shape[1]:
         _refuse("linear_e4m3: a [m, k] and w [n, k] must be float8_e4m3fn matrices")
@@ -439,8 +466,8 @@ def linear_e4m3(a, a_scales, w, w_scales, bias=None, out_dtype=None, out=None, s
     if n == 1:
         ldw = (k + 15) // 16 * 16
     device = _device_of("linear_e4m3", a, a_scales, w, w_scales, bias, out)
-    _call("omni_b200_linear_e4m3", device, stream, a.data_ptr(), a_scales.data_ptr(), w.data_ptr(),
-          w_scales.data_ptr(), bias_ptr, out.data_ptr(), m, n, k, lda, ldw, stride, code)
+    _call("omni_b200_linear_e4m3", device, a.data_ptr(), a_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), bias_ptr,
+          out.data_ptr(), m, n, k, lda, ldw, stride, code)
     return out
 
 
@@ -457,6 +484,9 @@ def attention_window(q, k, v, window=0, sinks=0, right=0, lengths=None, q_length
     last ones (CUDA int32 tensors).  The query at position p sees `window` keys up to its
     own (window <= 0: all), the first `sinks` keys, and `right` keys past it.  Rows past a
     sequence's queries are left as they are in `out`, undefined in a new one."""
+    if stream is not None:
+        with _on("attention_window", stream, q):
+            return attention_window(q, k, v, window, sinks, right, lengths, q_lengths, scale, out, out_dtype)
     q_shape, k_shape = q.shape, k.shape
     if len(q_shape) != 4 or len(k_shape) != 4 or v.shape != k_shape:
         _refuse("attention_window: q must be [B, H, Lq, D], k and v [B, Hkv, Lk, D]")
@@ -494,7 +524,7 @@ def attention_window(q, k, v, window=0, sinks=0, right=0, lengths=None, q_length
     ob, oh, ot, od = out.stride()
     if qd != 1 or kd != 1 or vd != 1 or od != 1:
         _refuse("attention_window: columns must be contiguous")
-    _call("omni_b200_attention_window", device, stream, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B, H,
-          Hkv, Lq, Lk, D, _STRIDES(qb, qh, qt, kb, kh, kt, vb, vh, vt, ob, oh, ot), *pointers, window, right, sinks,
-          scale, code, out_code)
+    _call("omni_b200_attention_window", device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B, H, Hkv, Lq,
+          Lk, D, _STRIDES(qb, qh, qt, kb, kh, kt, vb, vh, vt, ob, oh, ot), *pointers, window, right, sinks, scale, code,
+          out_code)
     return out
