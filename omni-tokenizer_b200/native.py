@@ -146,11 +146,27 @@ def _stream_ptr(stream):
     return C.c_void_p(s.cuda_stream)
 
 
+def _on(what, stream, t):
+    """The context in which a helper that was given a stream works: a call with
+    stream=s is the call made inside torch.cuda.stream(s).  Outputs and workspaces, those
+    that are dropped at once among them, are memory of that stream, so that no kernel
+    pending on the current stream has it, and none there gets it before the call is over."""
+    device = t.get_device()
+    if not hasattr(stream, "device_index"):  # another library's, known by its cuda_stream
+        stream = _t.cuda.ExternalStream(stream.cuda_stream, device=device)
+    if 0 <= device != stream.device_index:
+        _refuse(f"{what}: stream must be on the tensors' device")
+    return _t.cuda.stream(stream)
+
+
 def attention_bhld(q, k, v, out=None, lengths=None, block=0, skip_padded_queries=False, scale=0.0,
                    out_dtype=None, stream=None):
     """Head-major batched attention: q, k, v are CUDA tensors [B, H, L, D]."""
     import torch
 
+    if stream is not None:
+        with _on("attention_bhld", stream, q):
+            return attention_bhld(q, k, v, out, lengths, block, skip_padded_queries, scale, out_dtype)
     B, H, L, D = q.shape
     if out is None:
         out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
@@ -224,6 +240,9 @@ def attention_rows(q, k, v, heads, block=0, valid=None, fused=False, out_dtype=N
     workspace=False passes only the repacking bytes (no key split scratch)."""
     import torch
 
+    if stream is not None:
+        with _on("attention_rows", stream, q):
+            return attention_rows(q, k, v, heads, block, valid, fused, out_dtype, None, batch, lengths, workspace)
     rows = q.shape[0]
     n = rows // batch
     d = q.shape[1] // 3 if fused else q.shape[1]
@@ -292,17 +311,6 @@ def _device_of(what, *tensors):
         if t is not None and (device < 0 or t.get_device() != device):
             _refuse(f"{what}: every tensor must be on the same CUDA device")
     return device
-
-
-def _on(what, stream, t):
-    """The context in which a helper that was given a stream works: a call with
-    stream=s is the call made inside torch.cuda.stream(s).  Outputs, those that the
-    caller drops at once among them, are memory of that stream, so that no kernel
-    pending on the current stream has it, and none there gets it before the call is over."""
-    device = t.get_device()
-    if 0 <= device != stream.device_index:
-        _refuse(f"{what}: stream must be on the tensors' device")
-    return _t.cuda.stream(stream)
 
 
 def _row_stride(what, t, shape):

@@ -128,3 +128,79 @@ def test_outputs_are_no_memory_of_the_current_stream(gpu, name):
     del got, g
     assert _apart(_blocks([torch.empty(s, dtype=d, device="cuda") for s, d in shapes]), dropped)
     ob.library().sync_check()
+
+
+def _older_calls(device):
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(2, 4, 70, 64, generator=g).to(BF16).to(device)
+    rows = torch.randn(2 * 70, 4 * 72, generator=g).to(device)
+    held = torch.full((2,), 70, dtype=torch.int32, device=device)
+    return {
+        "attention_bhld": lambda s: ob.attention_bhld(x, x, x, stream=s),
+        "attention_rows": lambda s: ob.attention_rows(rows, rows, rows, 4, stream=s),
+        "attention_rows of a batch": lambda s: ob.attention_rows(rows, rows, rows, 4, batch=2, lengths=held, stream=s),
+    }
+
+
+OLDER = ["attention_bhld", "attention_rows", "attention_rows of a batch"]
+
+
+@pytest.mark.parametrize("named", [True, False])
+@pytest.mark.parametrize("name", OLDER)
+def test_attention_outputs_and_workspaces_are_the_streams(monkeypatch, name, named):
+    """The bidirectional attention's helpers, with a torch stream and with an object that
+    only has its cuda_stream."""
+    native, entered, made, launched = ob.native, [], [], []
+    stream = types.SimpleNamespace(cuda_stream=0x77, **({"device_index": 0} if named else {}))
+    torch_stream = stream if named else types.SimpleNamespace(cuda_stream=0x77, device_index=-1)
+
+    @contextlib.contextmanager
+    def enter(s):
+        entered.append(s)
+        yield
+        entered.pop()
+
+    real_empty = torch.empty
+
+    def empty(*args, **kwargs):
+        made.append(bool(entered) and entered[-1] is torch_stream)
+        return real_empty(*args, **kwargs)
+
+    class Entry:
+        def __getattr__(self, name):
+            return lambda *args: (1 << 10 if name.endswith("workspace") else
+                                  launched.append(entered[-1].cuda_stream if entered else 0))
+
+    call = _older_calls("cpu")[name]
+    native._t.codes
+    monkeypatch.setattr(native._t, "cuda", types.SimpleNamespace(
+        stream=enter, ExternalStream=lambda ptr, device: torch_stream if ptr == 0x77 else None))
+    monkeypatch.setattr(torch, "empty", empty)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: entered[-1] if entered else stream)
+    monkeypatch.setattr(native, "library", lambda: types.SimpleNamespace(lib=Entry(), check=lambda status: None))
+    call(stream)
+    assert made and all(made) and launched == [0x77] and not entered
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", OLDER)
+def test_attention_outputs_are_no_memory_of_the_current_stream(gpu, name):
+    call = _older_calls("cuda")[name]
+    want = call(None)
+    kept, freed = want.clone(), _blocks([want])
+    del want
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    busy = torch.empty_like(kept)
+    torch.cuda._sleep(20_000_000)
+    busy.fill_(3)
+    freed += _blocks([busy])
+    del busy
+    got = call(stream)
+    assert _apart(_blocks([got]), freed)
+    torch.cuda.synchronize()
+    assert torch.equal(got, kept)
+    dropped = _blocks([got])
+    del got
+    assert _apart(_blocks([torch.empty_like(kept)]), dropped)
+    ob.library().sync_check()
