@@ -134,7 +134,9 @@ int omni_b200_linear_e4m3(const void *a, const float *a_scales, const void *w, c
         return ctx_fail(1, "linear_e4m3: out_dtype must be F32, BF16 or F16");
     if (n == 0 || k == 0 || n > (1u << 22) || k > kMaxCols || m > (1u << 30))
         return ctx_fail(1, "linear_e4m3: n must be in [1, 2^22], k in [1, 2^24], m at most 2^30");
-    if (m && (!a || !a_scales || !w || !w_scales || !out))
+    if (m == 0)
+        return 0;
+    if (!a || !a_scales || !w || !w_scales || !out)
         return ctx_fail(1, "linear_e4m3: null pointer");
     if (lda < k || ldw < k || ldo < n || lda > kMaxStride / 2 || ldw > kMaxStride / 2 || ldo > kMaxStride / 8)
         return ctx_fail(1, "linear_e4m3: a row stride is smaller than its row, or above 2^37");
@@ -145,8 +147,6 @@ int omni_b200_linear_e4m3(const void *a, const float *a_scales, const void *w, c
         return ctx_fail(1, "linear_e4m3: a pointer is not aligned to its element type");
     if (((m + 127) / 128) * ((n + 255) / 256) > (1u << 30))
         return ctx_fail(4, "linear_e4m3: out has more than 2^30 tiles");
-    if (m == 0)
-        return 0;
     LinearArgs l;
     l.a = a;
     l.w = w;

@@ -185,3 +185,24 @@ def test_window_helper_refuses_what_32_bits_do_not_hold(name, value):
     q, k = torch.zeros(2, 4, 3, 64, dtype=torch.bfloat16), torch.zeros(2, 2, 40, 64, dtype=torch.bfloat16)
     with pytest.raises(ob.NativeError, match="below 2\\^31"):
         ob.attention_window(q, k, k, **{name: value})
+
+
+@pytest.mark.parametrize("lda,ldw", [(997, 1008), (1008, 997), (0, 0)])
+def test_linear_without_rows_looks_at_no_stride(lib, lda, ldw):
+    """An empty tensor's pitch is whatever its maker says: torch calls a [0, 997] slice
+    of padded rows contiguous, with 997 columns between its rows."""
+    assert lib.omni_b200_linear_e4m3(X, S, W, H, None, O, 0, 300, 997, lda, ldw, 300, BF16, None) == 0
+
+
+def test_linear_helper_of_an_empty_batch_with_odd_columns(lib, monkeypatch):
+    torch = pytest.importorskip("torch")
+    native = ob.native
+    native._t.codes
+    monkeypatch.setattr(native, "_device_of", lambda *_: 0)
+    monkeypatch.setattr(native, "_call", lambda name, device, *args: ob.library().check(getattr(lib, name)(*args, None)))
+    for cols in (997, 1000):
+        x = torch.zeros(5, cols, dtype=torch.bfloat16)[:0]
+        w = torch.zeros(300, (cols + 15) // 16 * 16).to(torch.float8_e4m3fn)[:, :cols]
+        scales = torch.ones(3, 8)
+        for q, s in (ob.quantize_e4m3(x), ob.rms_norm_e4m3(x, torch.zeros(cols, dtype=torch.bfloat16))[:2]):
+            assert ob.linear_e4m3(q, s, w, scales).shape == (0, 300)

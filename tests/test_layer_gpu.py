@@ -404,3 +404,14 @@ def test_rms_norm_many_rows(ob, rows, cols, dtype):
     q, scales = ob.quantize_e4m3(x)
     _check_quantized(q, scales, x.double())
     ob.library().sync_check()
+
+
+@pytest.mark.parametrize("cols", [1, 997, 1000])
+def test_empty_calls_with_odd_columns(ob, cols):
+    """No rows, of a width that the producers pad: a layer with nothing to do."""
+    x, w = torch.empty(0, cols, dtype=BF16, device="cuda"), _randn(cols, seed=1, dtype=BF16)
+    wq, ws = ob.quantize_e4m3(_randn(300, cols, seed=2), block_rows=128)
+    bias = _randn(300, seed=3, dtype=BF16)
+    for q, s in (ob.quantize_e4m3(x), ob.rms_norm_e4m3(x, w)[:2], ob.rms_norm_e4m3(x, w, residual=x)[:2]):
+        assert ob.linear_e4m3(q, s, wq, ws, bias=bias).shape == (0, 300)
+    ob.library().sync_check()
