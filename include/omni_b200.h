@@ -226,6 +226,7 @@ OMNI_B200_API int omni_b200_linear_e4m3(const void *a, const float *a_scales, co
  * they are.  lengths and q_lengths are DEVICE int32[batch], clamped to
  * [0, kv_len] and [0, q_len].  Keys and values at s >= n are not used, whatever
  * they hold; those below n must be finite, also where a mask hides them.
+ * A query with scores that are not finite over these keys gives NaN.
  * strides: HOST int64[12], the (batch, head, token) strides of q, k, v and out in
  * elements, columns contiguous; NULL: contiguous tensors of the shapes above.
  * dtype BF16 or F16, out_dtype F32 or dtype.  head_dim is a multiple of 8 in

@@ -624,7 +624,9 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
             }
             if (!ok)
                 break;
-            const float inv = l > 0.f ? 1.f / l : 0.f;
+            // Zeros for a row that sees no key, which `limit` tells; a sum that is no positive
+            // number otherwise stands for scores that are not finite, and gives NaN.
+            const float inv = limit > 0 ? 1.f / l : 0.f;
             if (steps > 0) {
                 if (!(ok = warp_wait(bar + S::PV_DONE + ((g - 1) & 1) * 8, ((g - 1) >> 1) & 1, err, kErrWaitO)))
                     break;

@@ -343,8 +343,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) window_tokens_kernel(const __g
             l = cta_l[r];
             v = part_o[0][r][col];
         }
-        v = l > 0.f ? v / l : 0.f; // a row that sees no key
         const int row = row0 + r;
+        // Zeros for a row that sees no key, which its position tells: a sum that is no
+        // positive number otherwise stands for scores that are not finite, and gives NaN.
+        v = min(n, pos0 + row / p.group + p.right + 1) > 0 ? v / l : 0.f;
         const long long at = b * p.os[0] + (kvh * p.group + row % p.group) * p.os[1] + (row / p.group) * p.os[2] + col;
         if (p.out_dtype == kOutF32)
             static_cast<float *>(p.out)[at] = v;

@@ -348,3 +348,30 @@ def test_different_operators_at_once(ob):
     for i, g in got:
         assert torch.equal(g, want[i]), f"call {i}"
     ob.library().sync_check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("case", [
+    (1, 4, 2, 1, 300, 64, 100, 0, 4), (3, 16, 2, 2, 2048, 128, 512, 0, 4), (2, 3, 3, 16, 10, 32, 7, 3, 2),
+    (1, 1, 1, 60, 40, 24, 10, 2, 5), (2, 4, 2, 300, 700, 128, 128, 0, 1), (24, 8, 8, 257, 250, 72, 60, 59, 5),
+    (16, 24, 8, 200, 150, 80, 0, 0, 0), (64, 8, 8, 100, 100, 24, 7, 300, 0),
+], ids=lambda c: "-".join(map(str, c)))
+def test_window_queries_that_are_not_finite(ob, case, dtype):
+    """A query whose scores hold a NaN or an infinity gives what the softmax gives, NaN, not
+    numbers; one that sees no key gives zeros all the same; other rows do not change."""
+    B, H, Hkv, Lq, Lk, D, window, right, sinks = case
+    q, k, v = _inputs(B, H, Hkv, Lq, Lk, D, dtype, "heads", seed=sum(case) + 2)
+    k[..., 1] = k[..., 1].abs() + 0.5  # with a query's -inf there every score is -inf
+    mask = dict(window=window, right=right, sinks=sinks)
+    plain = _run(ob, q, k, v, out_dtype=F32, **mask)
+    sees = torch.arange(Lq, device="cuda") + Lk - Lq + right >= 0  # any key at all
+    for value, column in ((float("nan"), 5), (float("inf"), 1), (-float("inf"), 1)):
+        for head, rows in ((0, slice(0, None, 3)), (H - 1, slice(1, None, 2)), (0, slice(Lq - 1, Lq))):
+            bad = q.clone()
+            bad[:, head, rows, column] = value
+            got = _run(ob, bad, k, v, out_dtype=F32, **mask)
+            spoilt = torch.zeros(B, H, Lq, dtype=torch.bool, device="cuda")
+            spoilt[:, head, rows] = True
+            assert bool(torch.isnan(got[spoilt & sees]).all()), f"query {value}: numbers in its row"
+            assert torch.equal(got[~(spoilt & sees)], plain[~(spoilt & sees)])
+            assert bool((got[..., ~sees, :] == 0).all())
