@@ -1,0 +1,87 @@
+"""The layer operators where a kernel goes round: stages of a ring that are filled again,
+rows past those that run at once.  Each test says which kernel its shapes reach, and fails
+when a change of the rules that choose a kernel takes them elsewhere.  Tolerances as in
+test_layer_gpu.py."""
+
+import re
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from tests.launches import launched  # noqa: E402
+from tests.test_layer_gpu import BF16, F16, F32, _half_step, _product64  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def ob():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from tests.conftest import load_package
+
+    return load_package()
+
+
+# ----------------------------------------------------- products of few rows
+def _few_rows(call, tmp_path):
+    """(rows of a tile, CTAs of a cluster, stages of a CTA's ring) of a product of few rows."""
+    (name, grid, _), = launched(call, tmp_path)
+    found = re.search(r"linear_e4m3_fewILi(\d+)E", name)
+    assert found, name
+    tile = int(found.group(1))
+    return tile, grid[0], 180 * 1024 // (128 * 128 + tile * 128)  # FewShape<tile>::STAGES
+
+
+# m, n, k, rows of the tile, CTAs of a cluster.  With one CTA the sums go out without a
+# cluster (tiles of 64 and 128 rows never run so: the other kernel is cheaper there).
+FEW = [(1, 16385, 4100, 16, 1), (13, 9600, 2000, 16, 1), (7, 8192, 8192, 16, 2), (1, 1024, 14336, 16, 8),
+       (32, 14336, 4096, 32, 1), (20, 16385, 2000, 32, 1), (17, 1000, 14340, 32, 8), (64, 8200, 4096, 64, 2),
+       (61, 1101, 14336, 64, 8), (128, 4096, 8192, 128, 4), (100, 641, 8200, 128, 8), (120, 300, 14336, 128, 8)]
+
+
+def _e4m3(values):
+    """e4m3 [rows, k] with a row pitch of 16 bytes and NaN between the rows."""
+    rows, k = values.shape
+    wide = torch.full((rows, (k + 15) // 16 * 16 + 16), 0x7F, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    wide[:, :k] = values.to(torch.float8_e4m3fn)
+    return wide[:, :k]
+
+
+@pytest.mark.parametrize("m,n,k,tile,parts", FEW)
+def test_linear_of_few_rows_refills_its_ring(ob, tmp_path, m, n, k, tile, parts):
+    """More groups of k to a CTA than its ring has stages."""
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    groups = -(-k // 128)
+    a, w = (_e4m3((torch.randn(rows, k, generator=g, device="cuda") * 40).clamp(-448, 448)) for rows in (m, n))
+    sa, sw = (torch.exp(torch.randn(rows, groups, generator=g, device="cuda")) * 2.0**-8 for rows in (m, -(-n // 128)))
+    got_tile, got_parts, stages = _few_rows(lambda: ob.linear_e4m3(a, sa, w, sw), tmp_path)
+    assert (got_tile, got_parts) == (tile, parts) and groups // parts > stages
+    ref, mag = _product64(a, sa, w, sw)
+    for dtype, with_bias in ((F32, False), (BF16, True), (F16, False)):
+        bias = torch.randn(n, generator=g, device="cuda").to(dtype) if with_bias else None
+        got = ob.linear_e4m3(a, sa, w, sw, bias=bias, out_dtype=dtype)
+        want = ref + bias.double() if with_bias else ref
+        err = (got.double() - want).abs()
+        tol = mag * 2.0**-11 + (mag + want.abs()) * (groups + 3) * 2.0**-24 + _half_step(want, dtype) * (1 + 2.0**-8)
+        assert bool((err <= tol).all()), f"{dtype}: worst {float((err / tol).max()):.3f} of the tolerance"
+        assert torch.equal(got, ob.linear_e4m3(a, sa, w, sw, bias=bias, out_dtype=dtype))
+    ob.library().sync_check()
+
+
+@pytest.mark.parametrize("m,n,k,tile,parts", FEW)
+def test_linear_of_few_rows_is_exact_on_whole_numbers(ob, tmp_path, m, n, k, tile, parts):
+    """Values in {-2..2}, scales in {1/2, 1, 2}: a group's sum is a whole number of at most
+    2^9, a factor one of 2^-2..2^2, so the sums of up to 113 groups are multiples of 2^-2
+    below 2^18: 20 bits, exact in any order.  A stage read a turn early or late shows."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    groups = -(-k // 128)
+    a, w = (_e4m3(torch.randint(-2, 3, (rows, k), generator=g, device="cuda").float()) for rows in (m, n))
+    sa, sw = (torch.exp2(torch.randint(-1, 2, (rows, groups), generator=g, device="cuda").float())
+              for rows in (m, -(-n // 128)))
+    got_tile, got_parts, stages = _few_rows(lambda: ob.linear_e4m3(a, sa, w, sw, out_dtype=F32), tmp_path)
+    assert (got_tile, got_parts) == (tile, parts) and groups // parts > stages
+    ref, _ = _product64(a, sa, w, sw)
+    for _ in range(3):
+        assert torch.equal(ob.linear_e4m3(a, sa, w, sw, out_dtype=F32).double(), ref)
+    ob.library().sync_check()
