@@ -85,3 +85,27 @@ def test_linear_of_few_rows_is_exact_on_whole_numbers(ob, tmp_path, m, n, k, til
     for _ in range(3):
         assert torch.equal(ob.linear_e4m3(a, sa, w, sw, out_dtype=F32).double(), ref)
     ob.library().sync_check()
+
+
+# ------------------------------------------------------- quantised quotients
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("rows,cols,pad", [(20000, 1024, 0), (20000, 1152, 0), (20000, 1000, 24), (20000, 997, 0),
+                                           (20000, 1024, 3)])
+def test_quantize_rounds_as_a_division(ob, rows, cols, pad, block_rows, dtype):
+    """Every byte is that of x / scale in fp32, rounded to nearest even.  Quotients half way
+    between two e4m3 values are what tells: of 8.4 million such inputs a product with the
+    scale's reciprocal rounds 4158 otherwise in bf16, 460 in fp16 and 4 in fp32."""
+    g = torch.Generator(device="cuda").manual_seed(rows + cols + pad)
+    wide = torch.exp(torch.randn(cols + pad, generator=g, device="cuda"))
+    x = (torch.randn(rows, cols + pad, generator=g, device="cuda") * wide).to(dtype)[:, :cols]
+    q, s = ob.quantize_e4m3(x, block_rows=block_rows)
+    scales = s.repeat_interleave(block_rows, 0)[:rows].repeat_interleave(128, 1)[:, :cols]
+    # A 53-bit quotient rounded to 24 bits is the 24-bit quotient (53 >= 2 * 24 + 2).
+    want = (x.double() / scales.double()).float().to(torch.float8_e4m3fn)
+    assert torch.equal(q.view(torch.uint8), want.view(torch.uint8))
+    top = torch.zeros(-(-rows // block_rows) * block_rows, -(-cols // 128) * 128, device="cuda")
+    top[:rows, :cols] = x.abs()
+    top = top.view(-1, block_rows, s.shape[1], 128).amax(dim=(1, 3))
+    assert torch.equal(s, (top.double() / 448).float())
+    ob.library().sync_check()
