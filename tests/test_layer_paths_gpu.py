@@ -10,6 +10,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
+import tests.test_layer_gpu as base  # noqa: E402
 from tests.launches import launched  # noqa: E402
 from tests.test_layer_gpu import BF16, F16, F32, _half_step, _product64  # noqa: E402
 
@@ -108,4 +109,56 @@ def test_quantize_rounds_as_a_division(ob, rows, cols, pad, block_rows, dtype):
     top[:rows, :cols] = x.abs()
     top = top.view(-1, block_rows, s.shape[1], 128).amax(dim=(1, 3))
     assert torch.equal(s, (top.double() / 448).float())
+    ob.library().sync_check()
+
+
+# -------------------------------------------------------- norms of many rows
+def _goes_round(call, rows, kernel, tmp_path):
+    """That the call's kernel is `kernel`, with fewer CTAs than its rows would take."""
+    (name, (grid,), _), = launched(call, tmp_path)
+    found = re.search(r"(rows(?:_\w+)?_kernel)I(?:f|6__half|13__nv_bfloat16)((?:L[bi]\d+E)+)E", name)
+    assert found, name
+    numbers = [int(n) for n in re.findall(r"L[bi](\d+)E", found.group(2))][1:]
+    assert (found.group(1), *numbers) == kernel
+    each = {"rows_kernel": lambda tpr, vpt, r: r, "rows_odd_kernel": lambda warps, groups: 8 // warps,
+            "rows_stream_kernel": lambda tpr, vpt: 256 // tpr, "rows_scalar_kernel": lambda: 1}[kernel[0]](*numbers)
+    assert rows > grid * each
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,cols,kernel", [
+    # Widths that 16-byte loads cannot read.
+    (20000, 33, ("rows_odd_kernel", 1, 4)), (20000, 1013, ("rows_odd_kernel", 1, 8)),
+    (2500, 2001, ("rows_odd_kernel", 8, 2)), (2500, 3727, ("rows_odd_kernel", 8, 4)),
+    (2500, 8191, ("rows_odd_kernel", 8, 8)), (2500, 9001, ("rows_scalar_kernel",)),
+    (1500, 16400, ("rows_scalar_kernel",)),  # more than registers hold
+    # A warp, or a CTA, for each row.
+    (20000, 200, ("rows_kernel", 32, 1, 4)), (9000, 512, ("rows_kernel", 32, 2, 4)), (9000, 1024, ("rows_kernel", 32, 4, 4)),
+    (9000, 1152, ("rows_kernel", 32, 5, 4)), (9000, 1536, ("rows_kernel", 32, 6, 4)),
+    (2700, 1544, ("rows_kernel", 128, 2, 1)), (2040, 2048, ("rows_kernel", 128, 2, 1)),
+    (1020, 4096, ("rows_kernel", 128, 4, 1)), (500, 8192, ("rows_kernel", 256, 4, 1)),
+    (1100, 8200, ("rows_kernel", 512, 4, 1)), (1100, 12000, ("rows_kernel", 512, 4, 1)),
+    (1100, 16384, ("rows_kernel", 512, 4, 1)),
+    # The ring.
+    (2501, 2048, ("rows_stream_kernel", 64, 4)), (1501, 4096, ("rows_stream_kernel", 128, 4)),
+    (1031, 8192, ("rows_stream_kernel", 256, 4)),
+], ids=lambda v: "-".join(map(str, v)) if isinstance(v, tuple) else str(v))
+def test_rms_norm_of_more_rows_than_run_at_once(ob, tmp_path, rows, cols, kernel, dtype):
+    """With and without a residual, in both output types, and in place."""
+    g = torch.Generator(device="cuda").manual_seed(rows + cols)
+    x, res, w = (torch.randn(*n, generator=g, device="cuda").to(dtype) for n in ((rows, cols), (rows, cols), (cols,)))
+    for r in (None, res):
+        _goes_round(lambda: ob.rms_norm(x, w, residual=r), rows, kernel, tmp_path)
+        _goes_round(lambda: ob.rms_norm_e4m3(x, w, residual=r), rows, kernel, tmp_path)
+        h, y = base._norm64(x, w, r, 1e-6)
+        got, hout = ob.rms_norm(x, w, residual=r)
+        base._check_rounded(got, y, dtype, 48 * 2.0**-24)
+        q, scales, hq = ob.rms_norm_e4m3(x, w, residual=r)
+        base._check_quantized(q, scales, y)
+        if r is not None:
+            base._check_rounded(hout, h, dtype, 2.0**-24)
+            assert torch.equal(hout, hq)
+        del h, y
+    ob.rms_norm(x, w, residual=res, residual_out=res, out=x)
+    assert torch.equal(x, got) and torch.equal(res, hout)
     ob.library().sync_check()
