@@ -375,3 +375,76 @@ def test_window_queries_that_are_not_finite(ob, case, dtype):
             assert bool(torch.isnan(got[spoilt & sees]).all()), f"query {value}: numbers in its row"
             assert torch.equal(got[~(spoilt & sees)], plain[~(spoilt & sees)])
             assert bool((got[..., ~sees, :] == 0).all())
+
+
+def _kernels(ob, cases, tmp_path):
+    """The kernels that the cases run: {name: template instances}, and "clusters": sizes."""
+    import re
+
+    from tests.launches import launched
+
+    found = {}
+    for B, H, Hkv, Lq, Lk, D, window, right, sinks in cases:
+        q, k, v = _inputs(B, H, Hkv, Lq, Lk, D, BF16, "heads", seed=1)
+        (name, grid, _), = launched(lambda: ob.attention_window(q, k, v, window=window, right=right, sinks=sinks), tmp_path)
+        kind, instance = re.search(r"(window_[a-z]+_kernel)ILi(\d)E", name).groups()
+        found.setdefault(kind, set()).add(int(instance))
+        if kind == "window_tokens_kernel":
+            found.setdefault("clusters", set()).add(grid[0] // (B * Hkv))
+    return found
+
+
+def test_window_cases_reach_both_kernels(ob, tmp_path):
+    """The lists above are meant for one kernel each, in every template instance of it: a
+    change of the rule that chooses would show here."""
+    tokens = _kernels(ob, TOKENS, tmp_path)
+    assert tokens == {"window_tokens_kernel": {1, 2, 3, 4}, "clusters": {1, 4, 16}}
+    assert _kernels(ob, WIDE, tmp_path) == {"window_prompt_kernel": {1, 2}}
+    assert set(_kernels(ob, PROMPTS, tmp_path)) == {"window_prompt_kernel", "window_tokens_kernel", "clusters"}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("clusters,case", [
+    (2, (2, 4, 2, 1, 300, 64, 0, 0, 4)), (2, (3, 6, 3, 5, 450, 128, 0, 3, 0)), (4, (3, 4, 2, 1, 1000, 72, 0, 0, 0)),
+    (8, (3, 8, 2, 1, 1800, 32, 1200, 5, 70)), (8, (2, 4, 1, 2, 1500, 96, 0, 0, 0)), (16, (2, 4, 2, 1, 2500, 128, 0, 0, 0)),
+], ids=lambda c: str(c) if isinstance(c, int) else "-".join(map(str, c)))
+def test_window_of_every_cluster_size(ob, tmp_path, clusters, case, dtype):
+    """Keys split over CTAs, with sequences so short that some of them get none."""
+    B, H, Hkv, Lq, Lk, D, window, right, sinks = case
+    assert _kernels(ob, [case], tmp_path)["clusters"] == {clusters}
+    q, k, v = _inputs(B, H, Hkv, Lq, Lk, D, dtype, "tokens", seed=sum(case) + 3)
+    mask = dict(window=window, right=right, sinks=sinks)
+    for lengths in (None, [Lk, 17, 0][:B], [Lk - 1, Lk // 2, 65][:B]):
+        for out_dtype in (dtype, F32):
+            got = _run(ob, q, k, v, lengths, out_dtype=out_dtype, **mask)
+            _check(got, q, k, v, window, right, sinks, lengths, None)
+
+
+@pytest.mark.parametrize("B,H,Hkv,Lq,Lk,D,kernel", [(1, 4, 2, 1, 260, 64, "tokens"), (1, 8, 1, 3, 300, 128, "tokens"),
+                                                    (2, 64, 64, 140, 150, 64, "prompt"), (2, 64, 64, 129, 130, 128, "prompt")])
+def test_window_offsets_past_32_bits(ob, tmp_path, B, H, Hkv, Lq, Lk, D, kernel):
+    """Tokens so far apart that the last ones lie more than 2^32 elements into their tensors."""
+    from tests.launches import launched
+
+    q, k, v = _inputs(B, H, Hkv, Lq, Lk, D, BF16, "heads", seed=4)
+    lengths = [Lk, Lk - 2][:B]
+    mask = dict(window=100, sinks=3)
+    want = _run(ob, q, k, v, lengths, **mask)
+
+    def apart(t, heads, n):
+        """[B, heads, n, D] with more than 2^32 elements between its first and last token."""
+        stride = -(-(2**32 + 2**20) // (n - 1) // 8) * 8 if n > 1 else heads * B * D
+        room = torch.empty((n - 1) * stride + heads * B * D, dtype=BF16, device="cuda")
+        wide = room.as_strided((B, heads, n, D), (heads * D, D, stride, 1))
+        wide.copy_(t)
+        return wide
+
+    out = apart(torch.full_like(q, KEPT), H, Lq)
+    ins = apart(q, H, Lq), apart(k, Hkv, Lk), apart(v, Hkv, Lk)
+    held = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    (name, _, _), = launched(lambda: ob.attention_window(*ins, lengths=held, out=out, **mask), tmp_path)
+    assert f"window_{kernel}_kernel" in name
+    out.fill_(KEPT)
+    ob.attention_window(*ins, lengths=held, out=out, **mask)
+    ob.library().sync_check()
+    assert torch.equal(out, want)
