@@ -162,3 +162,42 @@ def test_rms_norm_of_more_rows_than_run_at_once(ob, tmp_path, rows, cols, kernel
     ob.rms_norm(x, w, residual=res, residual_out=res, out=x)
     assert torch.equal(x, got) and torch.equal(res, hout)
     ob.library().sync_check()
+
+
+# ------------------------------------------------------------- far-off rows
+def _far(t, total=2**32 + 2**20):
+    """The same rows, so far apart that the last one lies past 2^32 elements."""
+    rows, cols = t.shape
+    stride = -(-total // (rows - 1) // 16) * 16
+    wide = torch.empty((rows - 1) * stride + cols, dtype=t.dtype, device="cuda").as_strided((rows, cols), (stride, 1))
+    wide.view(torch.uint8 if t.element_size() == 1 else t.dtype).copy_(t.view(torch.uint8) if t.element_size() == 1 else t)
+    return wide
+
+
+@pytest.mark.parametrize("rows,cols", [(9, 1024), (9, 999), (130, 4096), (3, 20001), (600, 8192)])
+def test_rows_past_32_bits(ob, rows, cols):
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x, res, w = (torch.randn(*n, generator=g, device="cuda").to(BF16) for n in ((rows, cols), (rows, cols), (cols,)))
+    want, hwant = ob.rms_norm(x, w, residual=res)
+    xf, rf, out = _far(x), _far(res), _far(torch.zeros_like(x))
+    got, h = ob.rms_norm(xf, w, residual=rf, residual_out=rf, out=out)
+    assert torch.equal(got, want) and torch.equal(h, hwant)
+    for block_rows in (1, 128):
+        q, s = ob.quantize_e4m3(x, block_rows=block_rows)
+        qf, sf = ob.quantize_e4m3(xf, block_rows=block_rows)
+        assert torch.equal(qf.view(torch.uint8), q.view(torch.uint8)) and torch.equal(sf, s)
+    ob.library().sync_check()
+
+
+@pytest.mark.parametrize("m,n,k,kernel", [(5, 700, 1024, "few"), (33, 257, 1100, "few"), (300, 600, 512, "big")])
+def test_product_of_rows_past_32_bits(ob, tmp_path, m, n, k, kernel):
+    g = torch.Generator(device="cuda").manual_seed(m)
+    a, sa = ob.quantize_e4m3(torch.randn(m, k, generator=g, device="cuda"))
+    w, sw = ob.quantize_e4m3(torch.randn(n, k, generator=g, device="cuda"), block_rows=128)
+    want = ob.linear_e4m3(a, sa, w, sw)
+    af, wf, out = _far(a), _far(w), _far(torch.zeros_like(want))
+    (name, _, _), = launched(lambda: ob.linear_e4m3(af, sa, wf, sw, out=out), tmp_path)
+    assert f"linear_e4m3_{kernel}" in name
+    out.zero_()
+    assert torch.equal(ob.linear_e4m3(af, sa, wf, sw, out=out), want)
+    ob.library().sync_check()
