@@ -9,6 +9,7 @@ accept torch tensors only as holders of device pointers.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from pathlib import Path
@@ -147,15 +148,19 @@ def _stream_ptr(stream):
 
 
 def _on(what, stream, t):
-    """The context in which a helper that was given a stream works: a call with
+    """The context in which a helper that was given a stream makes tensors: a call with
     stream=s is the call made inside torch.cuda.stream(s).  Outputs and workspaces, those
     that are dropped at once among them, are memory of that stream, so that no kernel
-    pending on the current stream has it, and none there gets it before the call is over."""
+    pending on the current stream has it, and none there gets it before the call is over.
+    (Entering the stream takes the host 8 us; calls that make no tensor are launched on it
+    without.)"""
     device = t.get_device()
     if not hasattr(stream, "device_index"):  # another library's, known by its cuda_stream
         stream = _t.cuda.ExternalStream(stream.cuda_stream, device=device)
     if 0 <= device != stream.device_index:
         _refuse(f"{what}: stream must be on the tensors' device")
+    if device >= 0 and device == _t.current_device() and stream.cuda_stream == _t.raw_stream(device):
+        return contextlib.nullcontext()
     return _t.cuda.stream(stream)
 
 
@@ -164,7 +169,7 @@ def attention_bhld(q, k, v, out=None, lengths=None, block=0, skip_padded_queries
     """Head-major batched attention: q, k, v are CUDA tensors [B, H, L, D]."""
     import torch
 
-    if stream is not None:
+    if stream is not None and out is None:
         with _on("attention_bhld", stream, q):
             return attention_bhld(q, k, v, out, lengths, block, skip_padded_queries, scale, out_dtype)
     B, H, L, D = q.shape
@@ -278,7 +283,8 @@ def attention_rows(q, k, v, heads, block=0, valid=None, fused=False, out_dtype=N
 # helpers keep the host's part short: every tensor attribute is read once, and the
 # device's stream is looked up without building objects or importing per call.
 # They work on the current stream of the tensors' device.  stream=s (a torch.cuda.Stream)
-# is short for `with torch.cuda.stream(s):`.  As there, the inputs have to be ready on s
+# is short for `with torch.cuda.stream(s):` (which a loop of small calls enters once, 8 us of
+# the host's time less for each).  As there, the inputs have to be ready on s
 # and kept (or recorded on s) until it is done with them, and the outputs are memory of
 # s: another stream waits for s before it reads them, and records them when it may
 # still read them after they are dropped.
@@ -324,11 +330,11 @@ def _row_stride(what, t, shape):
     return rows if shape[0] > 1 else shape[1]
 
 
-def _call(name, device, *args):
-    """Calls an entry point on `device` and on its current stream."""
+def _call(name, device, stream, *args):
+    """Calls an entry point on `device` and on `stream`, or that device's current one."""
     lib = _LIB or library()
     fn = getattr(lib.lib, name)
-    s = _t.raw_stream(device)
+    s = _t.raw_stream(device) if stream is None else stream.cuda_stream
     if device == _t.current_device():
         status = fn(*args, s)
     else:
@@ -356,7 +362,8 @@ def _empty_e4m3(x, rows, cols):
     return x.new_empty((rows, pitch), dtype=_t.e4m3)[:, :cols], pitch
 
 
-def _norm(what, x, shape, code, weight, residual, residual_out, out, out_stride, scales, eps, out_code):
+def _norm(what, x, shape, code, weight, residual, residual_out, out, out_stride, scales, eps, out_code,
+          stream=None):
     rows, cols = shape
     dtype = x.dtype
     if weight.shape != (cols,) or weight.dtype != dtype or (cols > 1 and weight.stride(0) != 1):
@@ -378,7 +385,7 @@ def _norm(what, x, shape, code, weight, residual, residual_out, out, out_stride,
         from_stride = _row_stride(what, residual, shape)
         from_ptr, to_ptr = residual.data_ptr(), residual_out.data_ptr()
     device = _device_of(what, x, weight, residual, residual_out, out)
-    _call("omni_b200_rms_norm", device, x.data_ptr(), from_ptr, weight.data_ptr(), to_ptr, out.data_ptr(),
+    _call("omni_b200_rms_norm", device, stream, x.data_ptr(), from_ptr, weight.data_ptr(), to_ptr, out.data_ptr(),
           scales, rows, cols, _row_stride(what, x, shape), from_stride, to_stride, out_stride, eps, code, out_code)
     return residual_out
 
@@ -389,7 +396,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None, st
     Returns (y, h): y = h / sqrt(mean(h^2) + eps) * weight in x's type, h = x + residual
     (None without a residual).  residual_out and out may each be x or residual, not both
     the same one."""
-    if stream is not None:
+    if stream is not None and (out is None or (residual is not None and residual_out is None)):
         with _on("rms_norm", stream, x):
             return rms_norm(x, weight, residual, eps, out, residual_out)
     shape, code = _matrix("rms_norm", x)
@@ -399,7 +406,8 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None, st
         _refuse("rms_norm: out must have x's shape and type")
     else:
         out_stride = _row_stride("rms_norm", out, shape)
-    return out, _norm("rms_norm", x, shape, code, weight, residual, residual_out, out, out_stride, None, eps, code)
+    return out, _norm("rms_norm", x, shape, code, weight, residual, residual_out, out, out_stride, None, eps, code,
+                      stream)
 
 
 def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, residual_out=None, stream=None):
@@ -431,15 +439,15 @@ def quantize_e4m3(x, block_rows=1, stream=None):
     stride = _row_stride("quantize_e4m3", x, shape)
     q, pitch = _empty_e4m3(x, rows, cols)
     scales = x.new_empty(((rows + block_rows - 1) // block_rows, (cols + 127) // 128), dtype=_t.f32)
-    _call("omni_b200_quantize_e4m3", device, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols, stride, pitch,
-          block_rows, code)
+    _call("omni_b200_quantize_e4m3", device, None, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols, stride,
+          pitch, block_rows, code)
     return q, scales
 
 
 def linear_e4m3(a, a_scales, w, w_scales, bias=None, out_dtype=None, out=None, stream=None):
     """a [m, k] times w [n, k] transposed, both e4m3 with scales (quantize_e4m3 with
     block_rows 1 and 128), plus bias [n]: [m, n] of out_dtype (bfloat16)."""
-    if stream is not None:
+    if stream is not None and out is None:
         with _on("linear_e4m3", stream, a):
             return linear_e4m3(a, a_scales, w, w_scales, bias, out_dtype, out)
     shape, w_shape = a.shape, w.shape
@@ -474,8 +482,8 @@ def linear_e4m3(a, a_scales, w, w_scales, bias=None, out_dtype=None, out=None, s
     if n == 1:
         ldw = (k + 15) // 16 * 16
     device = _device_of("linear_e4m3", a, a_scales, w, w_scales, bias, out)
-    _call("omni_b200_linear_e4m3", device, a.data_ptr(), a_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), bias_ptr,
-          out.data_ptr(), m, n, k, lda, ldw, stride, code)
+    _call("omni_b200_linear_e4m3", device, stream, a.data_ptr(), a_scales.data_ptr(), w.data_ptr(),
+          w_scales.data_ptr(), bias_ptr, out.data_ptr(), m, n, k, lda, ldw, stride, code)
     return out
 
 
@@ -492,7 +500,7 @@ def attention_window(q, k, v, window=0, sinks=0, right=0, lengths=None, q_length
     last ones (CUDA int32 tensors).  The query at position p sees `window` keys up to its
     own (window <= 0: all), the first `sinks` keys, and `right` keys past it.  Rows past a
     sequence's queries are left as they are in `out`, undefined in a new one."""
-    if stream is not None:
+    if stream is not None and out is None:
         with _on("attention_window", stream, q):
             return attention_window(q, k, v, window, sinks, right, lengths, q_lengths, scale, out, out_dtype)
     q_shape, k_shape = q.shape, k.shape
@@ -532,7 +540,7 @@ def attention_window(q, k, v, window=0, sinks=0, right=0, lengths=None, q_length
     ob, oh, ot, od = out.stride()
     if qd != 1 or kd != 1 or vd != 1 or od != 1:
         _refuse("attention_window: columns must be contiguous")
-    _call("omni_b200_attention_window", device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B, H, Hkv, Lq,
-          Lk, D, _STRIDES(qb, qh, qt, kb, kh, kt, vb, vh, vt, ob, oh, ot), *pointers, window, right, sinks, scale, code,
-          out_code)
+    _call("omni_b200_attention_window", device, stream, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B, H,
+          Hkv, Lq, Lk, D, _STRIDES(qb, qh, qt, kb, kh, kt, vb, vh, vt, ob, oh, ot), *pointers, window, right, sinks,
+          scale, code, out_code)
     return out

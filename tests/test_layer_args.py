@@ -199,7 +199,7 @@ def test_linear_helper_of_an_empty_batch_with_odd_columns(lib, monkeypatch):
     native = ob.native
     native._t.codes
     monkeypatch.setattr(native, "_device_of", lambda *_: 0)
-    monkeypatch.setattr(native, "_call", lambda name, device, *args: ob.library().check(getattr(lib, name)(*args, None)))
+    monkeypatch.setattr(native, "_call", lambda name, device, stream, *args: ob.library().check(getattr(lib, name)(*args, None)))
     for cols in (997, 1000):
         x = torch.zeros(5, cols, dtype=torch.bfloat16)[:0]
         w = torch.zeros(300, (cols + 15) // 16 * 16).to(torch.float8_e4m3fn)[:, :cols]

@@ -72,6 +72,26 @@ def test_allocations_and_launch_are_the_streams(monkeypatch, name):
     assert made and not any(made) and launched == [False]
 
 
+def test_calls_that_make_no_tensor_stay_on_the_current_stream(monkeypatch):
+    """They are launched on the stream that was given, and it is not entered."""
+    native, launched = ob.native, []
+    stream = types.SimpleNamespace(cuda_stream=0x77, device_index=0)
+    x = torch.zeros(4, 256, dtype=BF16)
+    a, b, s = x.to(E4M3), torch.zeros(256, 256).to(E4M3), torch.ones(4, 2)
+    q = torch.zeros(2, 2, 40, 64, dtype=BF16)
+    native._t.codes
+    monkeypatch.setattr(native._t, "cuda", None)
+    monkeypatch.setattr(native._t, "empty_like", None)
+    monkeypatch.setattr(torch.Tensor, "new_empty", None)
+    monkeypatch.setattr(native, "_device_of", lambda *_: 0)
+    monkeypatch.setattr(native, "_call", lambda name, device, on, *_: launched.append(on))
+    ob.rms_norm(x, x[0], out=x, stream=stream)
+    ob.rms_norm(x, x[0], residual=x, out=x.clone(), residual_out=x, stream=stream)
+    ob.linear_e4m3(a, s, b, s[:2], out=x, stream=stream)
+    ob.attention_window(q, q, q, out=q.clone(), stream=stream)
+    assert launched == [stream] * 4
+
+
 def test_a_stream_of_another_device_is_refused():
     stream = types.SimpleNamespace(cuda_stream=0x77, device_index=1)
     tensor = types.SimpleNamespace(get_device=lambda: 0)
