@@ -171,19 +171,23 @@ OMNI_B200_API int omni_b200_vq_argmin_noalloc(const void *x, const void *codeboo
  * weight: each block of 128 rows x 128 columns; the last group or block may be
  * smaller).  With amax the largest magnitude of a group, NaN left out,
  *   scale = max(amax / 448, 2^-126),   q = e4m3(x / scale),
- * rounded to nearest even; q * scale stands for x.  A NaN becomes e4m3's NaN;
+ * rounded to nearest even; q * scale stands for x.  (quantize_e4m3 rounds the fp32
+ * quotient.  rms_norm, whose values carry fp32 rounding errors of their own, rounds x
+ * times the scale's reciprocal: next to the middle of two e4m3 values it may take the
+ * other one.)  A NaN becomes e4m3's NaN;
  * a group that holds an infinity gets an infinite scale and stands for NaN.
  * Strides count elements of the tensor they belong to; columns are contiguous.
  * rows == 0 (m == 0) does nothing.
  *
  * omni_b200_rms_norm: per row of x [rows, cols],
  *   h = x + residual (or x),   out = h / sqrt(mean(h^2) + eps) * weight,
- * all in fp32.  residual != NULL also needs residual_out, which receives h
- * rounded to dtype; residual_out and out (of dtype) may each be the same tensor
+ * all in fp32 (a row's sum of squares must stay within its range).  residual !=
+ * NULL also needs residual_out, which receives h rounded to dtype; residual_out and out (of dtype) may each be the same tensor
  * as x or residual, with that tensor's stride, but not both the same one; other
  * overlaps are not allowed.  dtype F32, BF16 or F16 is the type of x, residual,
  * weight [cols] and residual_out.  out_dtype is dtype, with scales NULL, or
- * E4M3, with scales [rows, ceil(cols / 128)].  cols <= 2^24.
+ * E4M3, with scales [rows, ceil(cols / 128)].  cols is in [1, 2^24]; row strides are at
+ * least cols.
  *
  * omni_b200_quantize_e4m3: x [rows, cols] to q and scales.  block_rows 1: scales
  * [rows, ceil(cols / 128)]; block_rows 128 (weights): scales
@@ -205,7 +209,7 @@ OMNI_B200_API int omni_b200_quantize_e4m3(const void *x, void *q, float *scales,
  * product should be neither infinite nor below 2^-126 unless its columns are
  * zeros on one side and finite), rounded once to out_dtype (F32, BF16 or
  * F16) [m, n] with row stride ldo; bias (NULL: none) is [n] of out_dtype.  k is
- * at most 2^24, n at most 2^22.  out overlaps no input.  No workspace; the
+ * in [1, 2^24], n in [1, 2^22]; m may be 0.  out overlaps no input.  No workspace; the
  * same call gives the same bits. */
 OMNI_B200_API int omni_b200_linear_e4m3(const void *a, const float *a_scales, const void *w,
                                         const float *w_scales, const void *bias, void *out,
@@ -227,10 +231,15 @@ OMNI_B200_API int omni_b200_linear_e4m3(const void *a, const float *a_scales, co
  * [0, kv_len] and [0, q_len].  Keys and values at s >= n are not used, whatever
  * they hold; those below n must be finite, also where a mask hides them.
  * A query with scores that are not finite over these keys gives NaN.
+ * Scores, maxima and sums are fp32; the softmax's numerators are rounded to dtype
+ * for the product with v (half a step of each, whatever out_dtype is), whose sums are fp32.
  * strides: HOST int64[12], the (batch, head, token) strides of q, k, v and out in
- * elements, columns contiguous; NULL: contiguous tensors of the shapes above.
+ * elements, columns contiguous, each at least head_dim (so no key head is expanded by a
+ * stride of 0: kv_heads says it); NULL: contiguous tensors of the shapes above.
  * dtype BF16 or F16, out_dtype F32 or dtype.  head_dim is a multiple of 8 in
- * [8, 128]; q, k, v are 16-byte aligned and their strides multiples of 8.  out
+ * [8, 128]; q, k, v are 16-byte aligned and their strides multiples of 8.  kv_len is at
+ * least 1 (a cache that holds nothing yet is one with lengths of 0); without queries
+ * (batch or q_len 0) the call does nothing.  out
  * overlaps no input.  No workspace; the same call gives the same bits. */
 OMNI_B200_API int omni_b200_attention_window(const void *q, const void *k, const void *v, void *out,
                                              int batch, int heads, int kv_heads, int q_len,

@@ -594,6 +594,9 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                     x3 = ex2_approx(x3);
                     fadd2(a0, a1, a0, a1, x0, x1);
                     fadd2(b0, b1, b0, b1, x2, x3);
+                    // To the type of v, as the tensor cores take them: up to half a step of each
+                    // (8192 tokens in bf16: off by 0.0022, relative, where fp32 weights give
+                    // 0.0016; fp16 2.7e-5 and 1.9e-5).  l is the sum of the unrounded values.
                     raw[c] = pack_pair<BF16>(x0, x1);
                     raw[c + 1] = pack_pair<BF16>(x2, x3);
                 }

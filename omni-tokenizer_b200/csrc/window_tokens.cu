@@ -255,6 +255,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) window_tokens_kernel(const __g
                 o[j][3] *= grown[1];
             }
         }
+        // The tensor cores multiply 16-bit operands: P loses up to half a step of its type
+        // here (the sums above are of the unrounded values).  One sequence's next token in
+        // bf16 is off by 0.0019 (root mean square, relative) where fp32 weights give 0.0016,
+        // the rounding of the output alone; products in fp32 would leave the tensor cores.
         const uint32_t pa[4] = {pack_pair<BF16>(s[0][0], s[0][1]), pack_pair<BF16>(s[0][2], s[0][3]),
                                 pack_pair<BF16>(s[1][0], s[1][1]), pack_pair<BF16>(s[1][2], s[1][3])};
 #pragma unroll

@@ -395,7 +395,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None, st
 
     Returns (y, h): y = h / sqrt(mean(h^2) + eps) * weight in x's type, h = x + residual
     (None without a residual).  residual_out and out may each be x or residual, not both
-    the same one."""
+    the same one.  stream=s is, here and below, the call inside torch.cuda.stream(s)."""
     if stream is not None and (out is None or (residual is not None and residual_out is None)):
         with _on("rms_norm", stream, x):
             return rms_norm(x, weight, residual, eps, out, residual_out)
@@ -499,7 +499,8 @@ def attention_window(q, k, v, window=0, sinks=0, right=0, lengths=None, q_length
     Sequence b holds lengths[b] keys (None: Lk) and q_lengths[b] queries (None: Lq), its
     last ones (CUDA int32 tensors).  The query at position p sees `window` keys up to its
     own (window <= 0: all), the first `sinks` keys, and `right` keys past it.  Rows past a
-    sequence's queries are left as they are in `out`, undefined in a new one."""
+    sequence's queries are left as they are in `out`, undefined in a new one.  `out` must not
+    overlap q, k or v; Lk is at least 1 (an empty cache: lengths of 0)."""
     if stream is not None and out is None:
         with _on("attention_window", stream, q):
             return attention_window(q, k, v, window, sinks, right, lengths, q_lengths, scale, out, out_dtype)
