@@ -248,6 +248,100 @@ OMNI_B200_API int omni_b200_attention_window(const void *q, const void *k, const
                                              int window, int right, int sinks, float scale,
                                              int dtype, int out_dtype, void *stream);
 
+/* ---- Rotary positions and the 4-bit key/value cache ----------------------
+ * No counterpart in the reference.
+ *
+ * omni_b200_rotary: q [batch, heads, tokens, head_dim] and, where k != NULL, k [batch,
+ * kv_heads, tokens, head_dim] of one type (F32, BF16 or F16) with their pairs of columns
+ * turned: pair i < pairs is columns (i, i + pairs), or (2i, 2i + 1) where adjacent != 0, and
+ *   angle = positions[axes[i], batch, token] * frequencies[i],
+ *   (y0, y1) = (x0 cos - x1 sin, x1 cos + x0 sin);
+ * inverse != 0 turns back (-sin), which is the gradient's way.  Columns from 2 * pairs on
+ * are copied.  The angle and its whole turns are fp64, the rest fp32, rounded once; an angle
+ * that is not finite gives NaN.
+ * positions: DEVICE [n_axes, batch, tokens] of position_type; frequencies: DEVICE float[pairs]
+ * (double where frequency_f64 != 0); axes: HOST uint8[pairs], each below n_axes, or NULL:
+ * axis 0.  pairs is in [1, 256], 2 * pairs at most head_dim (at most 65536).
+ * strides: HOST int64[12], (batch, head, token) of q, q_out, k and k_out in elements, columns
+ * contiguous, at least head_dim; NULL: contiguous.  position_strides: HOST int64[3] (axis,
+ * batch, token), 0 allowed; NULL: contiguous.  q_out may be q and k_out k, with its strides;
+ * other overlaps are not allowed. */
+enum omni_b200_position_type { OMNI_B200_POSITION_I32 = 0, OMNI_B200_POSITION_I64 = 1, OMNI_B200_POSITION_F32 = 2 };
+OMNI_B200_API int omni_b200_rotary(const void *q, void *q_out, const void *k, void *k_out,
+                                   const void *positions, const void *frequencies,
+                                   const uint8_t *axes, int batch, int heads, int kv_heads,
+                                   int tokens, int head_dim, int pairs, int n_axes,
+                                   const int64_t *strides, const int64_t *position_strides,
+                                   int adjacent, int inverse, int position_type, int frequency_f64,
+                                   int dtype, void *stream);
+
+/* A cache of keys and values in 4 bits: bytes [pages, kv_heads, page], a page holding
+ * page_tokens tokens (a multiple of 16) of one key head; omni_b200_cache_e2m1_bytes says how
+ * many bytes a page of a head has (18 * D for 16 tokens, D = head_dim rounded up to a multiple
+ * of 32; 0 for sizes that are refused).  Strides count bytes, multiples of 16; data is 16-byte
+ * aligned.  table: DEVICE int32[batch, table_width], the pages of each sequence in their
+ * order; NULL: page b is all that sequence b has.  Entries are read as far as a call needs
+ * them.  An entry that is none of [0, pages) is not followed: nothing is written there, rows
+ * read as NaN and queries that see a key there give NaN (for prompts, see below, other
+ * queries of that sequence may, too).
+ *
+ * Columns share a scale in groups of 32 (the last may be smaller).  With amax the largest
+ * magnitude of a group of a token,
+ *   scale = amax / 6 to six significant bits, within [2^-14, 10752],  value = e2m1(x / scale),
+ * both to nearest even, values up to 6: what is beyond 64512 stands for that.  value * scale
+ * has eight significant bits, so it is the same in F32, BF16 and F16.  A group that holds a
+ * NaN or an infinity stands for NaN.
+ *
+ * A sequence holds n = lengths[b] tokens, and a call is about its last m = q_lengths[b] (NULL:
+ * q_len; clamped to [0, q_len]): row i stands at position n - m + i.  Rows i >= m, and those
+ * whose position is not within [0, what the pages hold), are neither read nor written.
+ * lengths and q_lengths are DEVICE int32[batch].
+ *
+ * omni_b200_cache_write_e2m1 quantises k and v [batch, kv_heads, q_len, head_dim] (BF16 or F16)
+ * into the cache; omni_b200_cache_read_e2m1 writes what the cache stands for to k and v (F32,
+ * BF16 or F16).  strides: HOST int64[6], (batch, head, token) of k and v in elements, columns
+ * contiguous, at least head_dim and multiples of 16 bytes; NULL: contiguous.  k and v are
+ * 16-byte aligned.  head_dim is a multiple of 8 in [8, 128].  Two sequences of a call must not
+ * write to the same page. */
+typedef struct omni_b200_cache_e2m1 {
+    void *data;
+    const int32_t *table;
+    int32_t pages, page_tokens, table_width;
+    int64_t page_stride, head_stride;
+} omni_b200_cache_e2m1;
+OMNI_B200_API size_t omni_b200_cache_e2m1_bytes(size_t tokens, int head_dim);
+OMNI_B200_API int omni_b200_cache_write_e2m1(const void *k, const void *v,
+                                             const omni_b200_cache_e2m1 *cache,
+                                             const int32_t *lengths, const int32_t *q_lengths,
+                                             int batch, int kv_heads, int q_len, int head_dim,
+                                             const int64_t *strides, int dtype, void *stream);
+OMNI_B200_API int omni_b200_cache_read_e2m1(const omni_b200_cache_e2m1 *cache, void *k, void *v,
+                                            const int32_t *lengths, const int32_t *q_lengths,
+                                            int batch, int kv_heads, int q_len, int head_dim,
+                                            const int64_t *strides, int dtype, void *stream);
+
+/* omni_b200_attention_window over such a cache: the same mask, rows, scale, types and
+ * results, k and v being what the cache stands for.  kv_len is the most tokens that a
+ * sequence holds, at most what its pages hold; lengths are clamped to [0, kv_len].  strides:
+ * HOST int64[6], (batch, head, token) of q (multiples of 8) and out in elements; NULL:
+ * contiguous.  Tokens from lengths[b] on are not used, whatever the cache holds there.
+ * Sums, maxima and scores are fp32; the softmax's numerators are rounded to F16 (for prompts
+ * to dtype) for the product with v.  workspace: 16-byte aligned, of at least
+ * omni_b200_attention_window_e2m1_workspace bytes (0 for few queries: they read the cache
+ * as it is; prompts put keys and values back to 16 bits there first).  Its contents do not
+ * matter; calls that may overlap on the GPU must not share it. */
+OMNI_B200_API size_t omni_b200_attention_window_e2m1_workspace(int batch, int heads, int kv_heads,
+                                                               int q_len, int kv_len, int head_dim,
+                                                               int window, int right, int sinks);
+OMNI_B200_API int omni_b200_attention_window_e2m1(const void *q, const omni_b200_cache_e2m1 *cache,
+                                                  void *out, const int32_t *lengths,
+                                                  const int32_t *q_lengths, int batch, int heads,
+                                                  int kv_heads, int q_len, int kv_len, int head_dim,
+                                                  const int64_t *strides, int window, int right,
+                                                  int sinks, float scale, int dtype, int out_dtype,
+                                                  void *workspace, size_t workspace_bytes,
+                                                  void *stream);
+
 /* ---- Diagnostics (failure detection without a GPU fault) ----------------
  * Every pipeline wait in this library's kernels is bounded: a wait that has
  * not completed after 2 s records a bit in the current device's kernel error

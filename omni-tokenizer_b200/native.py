@@ -70,6 +70,15 @@ SIGNATURES = {
         [_P, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, _P, C.c_int, C.c_int, C.c_int,
          C.c_float, C.c_int, C.c_int, _P],
     ),
+    "omni_b200_rotary": (C.c_int, [_P] * 7 + [C.c_int] * 7 + [_P, _P] + [C.c_int] * 5 + [_P]),
+    "omni_b200_cache_e2m1_bytes": (C.c_size_t, [C.c_size_t, C.c_int]),
+    "omni_b200_cache_write_e2m1": (C.c_int, [_P] * 5 + [C.c_int] * 4 + [_P, C.c_int, _P]),
+    "omni_b200_cache_read_e2m1": (C.c_int, [_P] * 5 + [C.c_int] * 4 + [_P, C.c_int, _P]),
+    "omni_b200_attention_window_e2m1_workspace": (C.c_size_t, [C.c_int] * 9),
+    "omni_b200_attention_window_e2m1": (
+        C.c_int,
+        [_P] * 5 + [C.c_int] * 6 + [_P, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, C.c_int, _P, C.c_size_t, _P],
+    ),
     "omni_b200_squares": (C.c_int, [_P, _P, C.c_size_t, C.c_size_t, C.c_int, C.c_int, _P]),
     "omni_b200_vq_argmin": (
         C.c_int,
@@ -296,6 +305,8 @@ class _Torch:
 
         self.codes = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
         self.e4m3, self.f32, self.bf16, self.i32 = torch.float8_e4m3fn, torch.float32, torch.bfloat16, torch.int32
+        self.u8, self.f64, self.zeros = torch.uint8, torch.float64, torch.zeros
+        self.position_codes = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
         self.empty_like, self.cuda, self.current_device = torch.empty_like, torch.cuda, torch.cuda.current_device
         self.raw_stream = torch._C._cuda_getCurrentRawStream
         if name not in self.__dict__:
@@ -544,4 +555,247 @@ def attention_window(q, k, v, window=0, sinks=0, right=0, lengths=None, q_length
     _call("omni_b200_attention_window", device, stream, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B, H,
           Hkv, Lq, Lk, D, _STRIDES(qb, qh, qt, kb, kh, kt, vb, vh, vt, ob, oh, ot), *pointers, window, right, sinks,
           scale, code, out_code)
+    return out
+
+
+# ------------------------------------- rotary positions and the 4-bit key/value cache
+def rotary_axes(sections, interleaved=False):
+    """The axis of each pair for rotary(): sections[a] pairs of axis a, one run after the
+    other, or dealt out in turn (0, 1, 2, 0, 1, 2, ...) until an axis has none left."""
+    left = [int(n) for n in sections]
+    if not left or len(left) > 256 or min(left) < 0 or sum(left) == 0:
+        _refuse("rotary_axes: need the pairs of each axis")
+    if not interleaved:
+        return bytes(a for a, n in enumerate(left) for _ in range(n))
+    axes = []
+    while any(left):
+        for a, n in enumerate(left):
+            if n:
+                axes.append(a)
+                left[a] -= 1
+    return bytes(axes)
+
+
+def rotary(q, k, positions, frequencies, axes=None, adjacent=False, inverse=False, q_out=None, k_out=None,
+           stream=None):
+    """q [B, H, T, D] and k [B, Hkv, T, D] (or None) with rotary positions: (q_out, k_out).
+
+    positions is [axes, B, T], or [B, T] for one axis, int32, int64 or float32 (any strides, 0
+    among them); frequencies [pairs], float32 or float64, 2 * pairs <= D.  Pair i is columns
+    (i, i + pairs), or (2i, 2i + 1) with adjacent, and turns by positions[axes[i]] *
+    frequencies[i]; axes is bytes or a list of numbers (rotary_axes), None: axis 0.  The other
+    columns are copied.  inverse turns back: the gradients of q and k are those of q_out
+    and k_out with inverse.  q_out and k_out may be q and k."""
+    if stream is not None and (q_out is None or (k is not None and k_out is None)):
+        with _on("rotary", stream, q):
+            return rotary(q, k, positions, frequencies, axes, adjacent, inverse, q_out, k_out)
+    shape, dtype = q.shape, q.dtype
+    code = _t.codes.get(dtype)
+    if code is None or len(shape) != 4:
+        _refuse("rotary: q must be [B, H, T, D] of float32, bfloat16 or float16")
+    B, H, T, D = shape
+    Hkv, k_ptr, k_to = 0, None, None
+    if q_out is None:
+        q_out = q.new_empty(shape)
+    elif q_out.shape != shape or q_out.dtype != dtype:
+        _refuse("rotary: q_out must have q's shape and type")
+    qb, qh, qt, qd = q.stride()
+    ob, oh, ot, od = q_out.stride()
+    ends = qd != 1 or od != 1
+    if k is not None:
+        Hkv = k.shape[1] if len(k.shape) == 4 else 0
+        if k.shape != (B, Hkv, T, D) or Hkv == 0 or k.dtype != dtype:
+            _refuse("rotary: k must be [B, Hkv, T, D] of q's type")
+        if k_out is None:
+            k_out = k.new_empty(k.shape)
+        elif k_out.shape != k.shape or k_out.dtype != dtype:
+            _refuse("rotary: k_out must have k's shape and type")
+        kb, kh, kt, kd = k.stride()
+        lb, lh, lt, ld = k_out.stride()
+        ends = ends or kd != 1 or ld != 1
+        strides = _STRIDES(qb, qh, qt, ob, oh, ot, kb, kh, kt, lb, lh, lt)
+        k_ptr, k_to = k.data_ptr(), k_out.data_ptr()
+    else:
+        if k_out is not None:
+            _refuse("rotary: k_out needs a k")
+        strides = _STRIDES(qb, qh, qt, ob, oh, ot)
+    if ends and D > 1:
+        _refuse("rotary: columns must be contiguous")
+    p_shape, p_code = positions.shape, _t.position_codes.get(positions.dtype)
+    if p_code is None or (p_shape[1:] if len(p_shape) == 3 else p_shape) != (B, T):
+        _refuse("rotary: positions must be [axes, B, T] or [B, T] of int32, int64 or float32")
+    A = p_shape[0] if len(p_shape) == 3 else 1
+    if len(frequencies.shape) != 1 or frequencies.dtype not in (_t.f32, _t.f64) or not frequencies.is_contiguous():
+        _refuse("rotary: frequencies must be contiguous [pairs], float32 or float64")
+    pairs = frequencies.shape[0]
+    if axes is not None:
+        axes = bytes(axes)
+        if len(axes) != pairs:
+            _refuse("rotary: axes must name an axis for each pair")
+    if max(B, H, Hkv, T, D, pairs, A) >= _INT:
+        _refuse("rotary: sizes must be below 2^31")
+    device = _device_of("rotary", q, k, positions, frequencies, q_out, k_out)
+    p_strides = positions.stride()
+    _call("omni_b200_rotary", device, stream, q.data_ptr(), q_out.data_ptr(), k_ptr, k_to, positions.data_ptr(),
+          frequencies.data_ptr(), axes, B, H, Hkv, T, D, pairs, A, strides,
+          _THREE(*p_strides) if len(p_strides) == 3 else _THREE(0, *p_strides), int(adjacent), int(inverse), p_code,
+          int(frequencies.dtype == _t.f64), code)
+    return q_out, k_out
+
+
+_THREE, _SIX = C.c_int64 * 3, C.c_int64 * 6
+
+
+class _CacheE2m1(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("table", C.c_void_p), ("pages", C.c_int32), ("page_tokens", C.c_int32),
+                ("table_width", C.c_int32), ("page_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+def empty_cache_e2m1(pages, kv_heads, page_tokens, head_dim, device="cuda", stream=None):
+    """A cache of keys and values in 4 bits, uint8 [pages, kv_heads, bytes of a page], all
+    zeros.  A page holds page_tokens tokens (a multiple of 16) of one key head; head_dim is a
+    multiple of 8 up to 128."""
+    if stream is not None:
+        with _t.cuda.stream(stream):
+            return empty_cache_e2m1(pages, kv_heads, page_tokens, head_dim, device)
+    in_range = 0 <= page_tokens < _INT and 0 <= head_dim < _INT
+    size = library().lib.omni_b200_cache_e2m1_bytes(page_tokens, head_dim) if in_range else 0
+    if size == 0 or pages <= 0 or kv_heads <= 0:
+        _refuse("empty_cache_e2m1: page_tokens must be a multiple of 16 up to 2^30, head_dim a multiple of 8 up to 128")
+    return _t.zeros((pages, kv_heads, size), dtype=_t.u8, device=device)
+
+
+def _cache(what, cache, head_dim, batch, table, lengths, q_lengths):
+    """(the entry points' description of a cache, kv_heads, what a sequence's pages hold,
+    pointers of lengths and q_lengths)."""
+    shape = cache.shape
+    if len(shape) != 3 or cache.dtype != _t.u8:
+        _refuse(f"{what}: the cache must be uint8 [pages, kv_heads, bytes]")
+    pages, kv_heads, size = shape
+    block = (head_dim + 31) // 32 * 576
+    if head_dim <= 0 or head_dim > 128 or head_dim % 8 or size == 0 or size % block:
+        _refuse(f"{what}: a page of {size} bytes is none of head_dim {head_dim} (a multiple of 8 up to 128)")
+    page_stride, head_stride, last = cache.stride()
+    if last != 1:
+        _refuse(f"{what}: the bytes of a page must be contiguous")
+    tokens, width, table_ptr = size // block * 16, 1, None
+    if table is not None:
+        if len(table.shape) != 2 or table.shape[0] != batch or table.dtype != _t.i32 or not table.is_contiguous():
+            _refuse(f"{what}: table must be contiguous int32 [B, pages of a sequence]")
+        width, table_ptr = table.shape[1], table.data_ptr()
+    if max(pages, kv_heads, tokens, width) >= _INT:
+        _refuse(f"{what}: sizes must be below 2^31")
+    pointers = [None, None]
+    for i, n in enumerate((lengths, q_lengths)):
+        if n is not None:
+            if n.shape != (batch,) or n.dtype != _t.i32 or not n.is_contiguous():
+                _refuse(f"{what}: lengths and q_lengths must be contiguous int32 [B]")
+            pointers[i] = n.data_ptr()
+    return (_CacheE2m1(cache.data_ptr(), table_ptr, pages, tokens, width, page_stride, head_stride), kv_heads,
+            tokens * width, pointers)
+
+
+def _pair_strides(what, a, b):
+    ab, ah, at, ad = a.stride()
+    bb, bh, bt, bd = b.stride()
+    if (ad != 1 or bd != 1) and a.shape[3] > 1:
+        _refuse(f"{what}: columns must be contiguous")
+    return _SIX(ab, ah, at, bb, bh, bt)
+
+
+def cache_write_e2m1(k, v, cache, lengths, q_lengths=None, table=None, stream=None):
+    """Quantises k and v [B, Hkv, T, D] (bfloat16 or float16, any strides that are multiples of
+    8 with contiguous columns) into the cache (empty_cache_e2m1), which it returns.
+
+    Sequence b holds lengths[b] tokens when the call is over; k and v are its last
+    q_lengths[b] of them (None: T), from row 0 on.  table [B, pages of a sequence] names the
+    pages (None: page b is sequence b).  lengths, q_lengths and table are CUDA int32
+    tensors."""
+    shape, dtype = k.shape, k.dtype
+    code = _t.codes.get(dtype, F32)
+    if code == F32 or len(shape) != 4 or v.shape != shape or v.dtype != dtype:
+        _refuse("cache_write_e2m1: k and v must be [B, Hkv, T, D], both bfloat16 or both float16")
+    B, Hkv, T, D = shape
+    what, heads, _, pointers = _cache("cache_write_e2m1", cache, D, B, table, lengths, q_lengths)
+    if heads != Hkv or max(B, T) >= _INT:
+        _refuse("cache_write_e2m1: k, v and the cache must have the same key heads")
+    device = _device_of("cache_write_e2m1", k, v, cache, lengths, q_lengths, table)
+    _call("omni_b200_cache_write_e2m1", device, stream, k.data_ptr(), v.data_ptr(), C.byref(what), *pointers, B, Hkv,
+          T, D, _pair_strides("cache_write_e2m1", k, v), code)
+    return cache
+
+
+def cache_read_e2m1(cache, head_dim, lengths, rows=None, q_lengths=None, table=None, dtype=None, out=None,
+                    stream=None):
+    """What the cache stands for: (k, v), the last q_lengths[b] tokens of each sequence (None:
+    all rows) from row 0 on.
+
+    out is a pair of tensors [B, Hkv, rows, D] of float32, bfloat16 or float16; without it they
+    are made, of dtype (bfloat16) and with `rows` rows (None: as many tokens as a sequence's
+    pages hold).  Rows past q_lengths[b] or before a sequence's start stay as they are,
+    undefined in new tensors."""
+    if stream is not None and out is None:
+        with _on("cache_read_e2m1", stream, cache):
+            return cache_read_e2m1(cache, head_dim, lengths, rows, q_lengths, table, dtype)
+    B = lengths.shape[0] if len(lengths.shape) == 1 else -1
+    what, Hkv, capacity, pointers = _cache("cache_read_e2m1", cache, head_dim, B, table, lengths, q_lengths)
+    if out is None:
+        shape = (B, Hkv, capacity if rows is None else rows, head_dim)
+        k, v = (cache.new_empty(shape, dtype=_t.bf16 if dtype is None else dtype) for _ in range(2))
+    else:
+        k, v = out
+        shape = k.shape
+        if len(shape) != 4 or shape[0] != B or shape[1] != Hkv or shape[3] != head_dim or v.shape != shape or (
+                rows is not None and rows != shape[2]):
+            _refuse("cache_read_e2m1: out must be two tensors [B, Hkv, rows, D]")
+    code = _t.codes.get(k.dtype)
+    if code is None or v.dtype != k.dtype or (dtype is not None and k.dtype != dtype):
+        _refuse("cache_read_e2m1: k and v must both be float32, bfloat16 or float16, of dtype")
+    if max(B, shape[2]) >= _INT:
+        _refuse("cache_read_e2m1: sizes must be below 2^31")
+    device = _device_of("cache_read_e2m1", cache, lengths, q_lengths, table, k, v)
+    _call("omni_b200_cache_read_e2m1", device, stream, C.byref(what), k.data_ptr(), v.data_ptr(), *pointers, B, Hkv,
+          shape[2], head_dim, _pair_strides("cache_read_e2m1", k, v), code)
+    return k, v
+
+
+def attention_window_e2m1(q, cache, lengths, q_lengths=None, table=None, window=0, sinks=0, right=0, scale=0.0,
+                          kv_len=None, out=None, out_dtype=None, stream=None):
+    """attention_window over a cache in 4 bits: q [B, H, T, D] (bfloat16 or float16, strides
+    that are multiples of 8), the last q_lengths[b] tokens (None: T) of the lengths[b] that
+    sequence b holds, the cache as cache_write_e2m1 left it.
+
+    kv_len is the most tokens that a sequence holds (None: as many as its pages do): what
+    work is planned for, and for prompts how large a workspace is (bytes 4 B Hkv kv_len D).
+    Rows past a sequence's queries are left as they are in `out`, undefined in a new one."""
+    shape, dtype = q.shape, q.dtype
+    code = _t.codes.get(dtype, F32)
+    if code == F32 or len(shape) != 4:
+        _refuse("attention_window_e2m1: q must be [B, H, T, D], bfloat16 or float16")
+    B, H, T, D = shape
+    what, Hkv, capacity, pointers = _cache("attention_window_e2m1", cache, D, B, table, lengths, q_lengths)
+    if kv_len is None:
+        kv_len = capacity
+    if not (-_INT < window < _INT and -_INT < right < _INT and -_INT < sinks < _INT and 0 <= kv_len < _INT
+            and max(B, H, T) < _INT):
+        _refuse("attention_window_e2m1: sizes, window, right and sinks must be below 2^31")
+    size = library().lib.omni_b200_attention_window_e2m1_workspace(B, H, Hkv, T, kv_len, D, window, right, sinks)
+    if stream is not None and (out is None or size):
+        with _on("attention_window_e2m1", stream, q):
+            return attention_window_e2m1(q, cache, lengths, q_lengths, table, window, sinks, right, scale, kv_len, out,
+                                         out_dtype)
+    out_code = code
+    if out is None:
+        out = q.new_empty(shape, dtype=dtype if out_dtype is None else out_dtype)
+    elif out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
+        _refuse("attention_window_e2m1: out must have q's shape and out_dtype")
+    if out.dtype != dtype:
+        if out.dtype != _t.f32:
+            _refuse("attention_window_e2m1: the output's type must be q's, or float32")
+        out_code = F32
+    device = _device_of("attention_window_e2m1", q, cache, lengths, q_lengths, table, out)
+    workspace = q.new_empty(size, dtype=_t.u8) if size else None
+    _call("omni_b200_attention_window_e2m1", device, stream, q.data_ptr(), C.byref(what), out.data_ptr(), *pointers, B,
+          H, Hkv, T, kv_len, D, _pair_strides("attention_window_e2m1", q, out), window, right, sinks, scale, code,
+          out_code, workspace.data_ptr() if size else None, size)
     return out
