@@ -101,6 +101,5 @@ size_t window_e2m1_workspace(const WindowE2m1Args &a);
 int window_e2m1_launch(const WindowE2m1Args &a, cudaStream_t stream);
 // Its kernel for few rows (window_e2m1_tokens.cu).
 int window_e2m1_tokens_launch(const WindowE2m1Args &a, cudaStream_t stream);
-int window_e2m1_tokens_parts(const WindowE2m1Args &a);
 
 } // namespace omni_b200

@@ -16,11 +16,18 @@
 // down to 2^-28 of it keep all their bits, what is below loses less than 2^-39 of it.
 //
 // The bound is the cache's bytes.  A block of 16 tokens of a head (2304 bytes at 128 columns)
-// is one contiguous piece; each warp copies its own blocks to a ring in shared memory
-// (cp.async, no barrier between warps) and keeps its own softmax state.  The running maximum
-// is lazy: a warp looks at the other lanes' maxima only when some score is more than 2^8
-// above the reference.  A cluster of CTAs splits the keys of one tile of rows; the parts meet
-// in distributed shared memory, in rank order (no atomics).
+// is one contiguous piece; each warp copies its own blocks, two at a time, to a ring in shared
+// memory (cp.async, no barrier between warps) and keeps its own softmax state.  Converting
+// takes a conversion and a product for two elements, 128 instructions of a block's ~200; the
+// rest is kept short: a lane looks up the pages of 32 blocks at once, and the running maximum
+// is lazy (other lanes are asked only when some score is more than 2^8 above the reference).
+//
+// Two ways to split the keys over CTAs:
+//   * few tiles of rows: a cluster takes each; its parts meet in distributed shared memory, in
+//     rank order (no atomics, no workspace, one launch);
+//   * else the blocks of all tiles, one list, go to CTAs that are all on the GPU at once, the
+//     same number to each whatever the sequences' lengths are.  A tile that is one CTA's is
+//     finished there; parts of others go to the workspace, and a second kernel joins them.
 #include "cache_e2m1.cuh"
 #include "fmha.h"
 #include "layer.h"
@@ -31,16 +38,18 @@
 namespace omni_b200 {
 namespace {
 
-constexpr int kWarps = 4, kMaxParts = 16;
+constexpr int kMaxParts = 16;
 constexpr float kLazy = 8.f; // log2 units a score may be above the reference
 
 struct TokensParams {
     CacheView cache;
     const uint16_t *q;
     void *out;
+    float *parts_at; // of the list's parts: [CTA][first or last tile][m, l of the rows, then rows x D]
     long long qs[3], os[3];
     const int *lengths, *q_lengths;
-    int parts, kv_heads, group, q_len, kv_len, hd;
+    int parts; // CTAs of a cluster, or 0: the list
+    int batch, kv_heads, group, q_len, kv_len, hd, tiles; // tiles of rows that a sequence may have
     int window, right, sinks;
     int out_dtype;
     float scale_log2;
@@ -48,12 +57,14 @@ struct TokensParams {
 
 template <int D, int NT> struct TokensShape {
     static constexpr int BLOCK = CacheBlock<D>::BYTES;
-    static constexpr int STAGES = 6;
-    static constexpr int RING = kWarps * STAGES * BLOCK;
+    static constexpr int WARPS = 8, CTAS = NT == 1 ? 2 : 1; // of an SM
+    static constexpr int STAGES = 3, STAGE = 2 * BLOCK;
+    static constexpr int RING = WARPS * STAGES * STAGE;
     static constexpr int ROWS = 8 * NT;
     // The parts' place at the end, over the ring: m, l of the warps and the CTA, outputs.
-    static constexpr int PARTS = (2 * kWarps + 2) * ROWS * 4 + kWarps * ROWS * (D + 4) * 4;
+    static constexpr int PARTS = (2 * WARPS + 2) * ROWS * 4 + WARPS * ROWS * (D + 4) * 4;
     static constexpr int SMEM = RING > PARTS ? RING : PARTS;
+    static constexpr int SLOT = ROWS * (D + 2); // floats of a part in the workspace
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -105,42 +116,138 @@ template <int D> struct Columns {
     __device__ static constexpr int first(int word, int c) { return TOGETHER ? c * (D / 4) + word * 8 : word * 32 + c * 8; }
 };
 
+// A tile of rows of a sequence and key head, and the blocks of the cache that it sees: [0,
+// sink_blocks) and from `begin` on, in that order `blocks` of them.
+struct Tile {
+    int n, m, row0, rows, pos0;
+    int first, last, low, high, sink, sink_blocks, begin, blocks;
+};
+__device__ __forceinline__ void lengths_of(const TokensParams &p, int b, int &n, int &m) {
+    n = max(0, min(p.lengths[b], p.kv_len));
+    m = p.q_lengths ? max(0, min(p.q_lengths[b], p.q_len)) : p.q_len;
+}
+template <int ROWS> __device__ __forceinline__ Tile tile_of(const TokensParams &p, int n, int m, int tile) {
+    Tile t;
+    t.n = n;
+    t.m = m;
+    // Rows r of the tile: query (row0 + r) / group, head kvh * group + (row0 + r) % group.
+    t.row0 = tile * ROWS;
+    t.rows = min(ROWS, p.group * m - t.row0);
+    t.pos0 = n - m;
+    // Keys that some row of the tile sees: [0, sink) and [low, high).
+    t.first = t.pos0 + t.row0 / p.group;
+    t.last = t.pos0 + (t.row0 + max(t.rows, 1) - 1) / p.group;
+    t.high = t.rows > 0 ? max(0, min(n, t.last + p.right + 1)) : 0;
+    t.low = p.window > 0 ? max(0, min(t.first - p.window + 1, t.high)) : 0;
+    t.sink = min(p.sinks, t.low);
+    t.sink_blocks = (t.sink + kCacheBlock - 1) / kCacheBlock;
+    t.begin = max(t.low / kCacheBlock, t.sink_blocks);
+    t.blocks = t.sink_blocks + max(0, (t.high + kCacheBlock - 1) / kCacheBlock - t.begin);
+    return t;
+}
+// Its length in the list: a tile that sees nothing still has rows to write.
+__device__ __forceinline__ int listed(const Tile &t) { return t.rows > 0 ? max(t.blocks, 1) : 0; }
+// Blocks of all tiles of a sequence's key head.
+template <int ROWS> __device__ __forceinline__ int listed_of(const TokensParams &p, int b) {
+    int n, m, sum = 0;
+    lengths_of(p, b, n, m);
+    for (int i = 0; i < p.tiles; ++i)
+        sum += listed(tile_of<ROWS>(p, n, m, i));
+    return sum;
+}
+
+__device__ __forceinline__ void store_out(const TokensParams &p, const Tile &t, int b, int kvh, int r, int col, float v, float l) {
+    const int row = t.row0 + r, query = row / p.group;
+    // Zeros for a row that sees no key, which its position tells: a sum that is no positive
+    // number otherwise stands for scores that are not finite, and gives NaN.
+    v = min(t.n, t.pos0 + query + p.right + 1) > 0 ? v / l : 0.f;
+    const long long to = b * p.os[0] + (kvh * p.group + row % p.group) * p.os[1] + query * p.os[2] + col;
+    if (p.out_dtype == kOutF32)
+        static_cast<float *>(p.out)[to] = v;
+    else if (p.out_dtype == kOutBF16)
+        static_cast<__nv_bfloat16 *>(p.out)[to] = __float2bfloat16_rn(v);
+    else
+        static_cast<__half *>(p.out)[to] = __float2half_rn(v);
+}
+
+// The CTA's softmax over blocks j0, j0 + step, ... pairs of them, below j1 of a tile: leaves
+// m, l of the rows in cta_m and cta_l and the outputs in part_o[0].
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) window_e2m1_tokens_kernel(const __grid_constant__ TokensParams p) {
+__device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, int b, int kvh, int j0, int j1, int step,
+                                       uint8_t *smem, float *&cta_m, float *&cta_l, float (*&part_o)[8 * NT][D + 4]) {
     using S = TokensShape<D, NT>;
     using B = CacheBlock<D>;
     using C = Columns<D>;
-    constexpr int ROWS = S::ROWS, ST = S::STAGES;
-    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int ROWS = S::ROWS, ST = S::STAGES, W = S::WARPS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int parts = p.parts, pair = blockIdx.x / parts, part = blockIdx.x - pair * parts;
-    const int b = pair / p.kv_heads, kvh = pair - b * p.kv_heads;
-    const int n = max(0, min(p.lengths[b], p.kv_len));
-    const int m = p.q_lengths ? max(0, min(p.q_lengths[b], p.q_len)) : p.q_len;
-    const int row0 = blockIdx.y * ROWS, rows = min(ROWS, p.group * m - row0);
-    // Rows r of the tile: query (row0 + r) / group, head kvh * group + (row0 + r) % group.
-    const int pos0 = n - m;
 
-    // Keys that some row of the tile sees: [0, sink) and [low, high); blocks [0, sink_blocks)
-    // and from `begin` on.
-    const int first = pos0 + row0 / p.group, last = pos0 + (row0 + max(rows, 1) - 1) / p.group;
-    const int high = rows > 0 ? max(0, min(n, last + p.right + 1)) : 0;
-    const int low = p.window > 0 ? max(0, min(first - p.window + 1, high)) : 0;
-    const int sink = min(p.sinks, low);
-    const int sink_blocks = (sink + kCacheBlock - 1) / kCacheBlock;
-    const int begin = max(low / kCacheBlock, sink_blocks);
-    const int blocks = sink_blocks + max(0, (high + kCacheBlock - 1) / kCacheBlock - begin);
-    const int stride = parts * kWarps;
-    const int limit_all = min(n, first + p.right + 1), floor_all = p.window > 0 ? last - p.window + 1 : 0;
+    // Blocks of pairs: this warp's pair k is blocks j0 + (warp + k W) step and the next one.
+    const uint32_t ring = smem_u32(smem) + warp * ST * S::STAGE;
+    const uint8_t *head = p.cache.data + kvh * p.cache.head_stride;
+    auto block_of = [&](int i) { return i < tile.sink_blocks ? i : tile.begin + i - tile.sink_blocks; };
+    // Lane l knows block l % 2 of pair k + l / 2, k a multiple of 16: its address, 0 where there
+    // is none, and bits of those whose page is none of the cache's; pages of the next 16 pairs.
+    unsigned long long place = 0;
+    uint32_t unpaged = 0;
+    int page_next = 0;
+    auto look_up = [&](int k, int &within, bool &real) {
+        const int i = j0 + (warp + (k + (lane >> 1)) * W) * step + (lane & 1);
+        real = i < j1;
+        return real ? p.cache.page_of(b, block_of(i), within) : 0;
+    };
+    auto places = [&](int k) {
+        int within = 0;
+        bool real;
+        int page = page_next;
+        const int i = j0 + (warp + (k + (lane >> 1)) * W) * step + (lane & 1);
+        real = i < j1;
+        within = real ? block_of(i) % p.cache.page_blocks : 0;
+        unpaged = __ballot_sync(0xffffffffu, real && page < 0);
+        place = real && page >= 0 ? reinterpret_cast<unsigned long long>(head + page * p.cache.page_stride +
+                                                                         static_cast<long long>(within) * S::BLOCK)
+                                  : 0ull;
+        page_next = look_up(k + 16, within, real);
+    };
+    uint32_t bad_bits = 0; // two for each stage
+    auto fetch = [&](int k, int stage) {
+        if ((k & 15) == 0)
+            places(k);
+        bad_bits = (bad_bits & ~(3u << (2 * stage))) | (unpaged >> (2 * (k & 15)) & 3u) << (2 * stage);
+        const uint32_t to = ring + stage * S::STAGE + lane * 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const unsigned long long at = __shfl_sync(0xffffffffu, place, 2 * (k & 15) + h);
+            if (at) {
+                const uint8_t *from = reinterpret_cast<const uint8_t *>(at) + lane * 16;
+#pragma unroll
+                for (int x = 0; x < S::BLOCK; x += 512)
+                    if (x + 512 <= S::BLOCK || lane * 16 < S::BLOCK - x)
+                        copy_async_16(to + h * S::BLOCK + x, from + x);
+            }
+        }
+    };
+    const int pairs = j1 - j0 > warp * step ? (j1 - j0 - warp * step + W * step - 1) / (W * step) : 0;
+    {
+        int within;
+        bool real;
+        page_next = look_up(0, within, real);
+    }
+#pragma unroll
+    for (int k = 0; k < ST - 1; ++k) {
+        if (k < pairs)
+            fetch(k, k);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
 
     // The queries as B operands, and the masks of columns 2c and 2c + 1.
+    const int limit_all = min(tile.n, tile.first + p.right + 1), floor_all = p.window > 0 ? tile.last - p.window + 1 : 0;
     uint32_t qb[NT][D / 16][2];
     float factor[NT][2]; // from S to log2 units
     int limit[NT][2], floor_[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int r = row0 + 8 * t + g;
-        const bool real = 8 * t + g < rows;
+        const int r = tile.row0 + 8 * t + g;
+        const bool real = 8 * t + g < tile.rows;
         const uint16_t *q = p.q + b * p.qs[0] + (kvh * p.group + r % p.group) * p.qs[1] + (r / p.group) * p.qs[2];
         uint4 w[C::WORDS];
         uint32_t top2 = 0;
@@ -179,122 +286,118 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) window_e2m1_toke
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int col = 8 * t + 2 * c + h, pos = pos0 + (row0 + col) / p.group;
+            const int col = 8 * t + 2 * c + h, pos = tile.pos0 + (tile.row0 + col) / p.group;
             const int of_col = __shfl_sync(0xffffffffu, exponent, 4 * (2 * c + h));
-            factor[t][h] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - of_col) << 23);
-            limit[t][h] = col < rows ? min(n, pos + p.right + 1) : n; // a row that is none: anything finite
-            floor_[t][h] = col < rows && p.window > 0 ? pos - p.window + 1 : 0;
+            // Not 0, so that a hidden key's -inf stays -inf.
+            factor[t][h] = fmaxf(p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - of_col) << 23), 1.4e-45f);
+            limit[t][h] = col < tile.rows ? min(tile.n, pos + p.right + 1) : tile.n; // a row that is none: anything finite
+            floor_[t][h] = col < tile.rows && p.window > 0 ? pos - p.window + 1 : 0;
         }
     }
 
     float o[NT][D / 16][4];
-    float ref[NT][2], sum[NT][2];
+    float ref[NT][2], sum[NT][2], bar[NT][2]; // bar: what a score of S must not be above
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int x = 0; x < D / 16; ++x)
             o[t][x][0] = o[t][x][1] = o[t][x][2] = o[t][x][3] = 0.f;
-        ref[t][0] = ref[t][1] = -INFINITY;
+        ref[t][0] = ref[t][1] = 0.f;
+        bar[t][0] = bar[t][1] = -INFINITY;
         sum[t][0] = sum[t][1] = 0.f;
     }
+    bool none[NT][2]; // no score yet
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+        none[t][0] = none[t][1] = true;
 
-    auto block_of = [&](int i) { return i < sink_blocks ? i : begin + i - sink_blocks; };
-    const uint32_t ring = smem_u32(smem) + warp * ST * S::BLOCK;
-    uint32_t missing = 0; // bit per stage: its page is none of the cache's
-    auto fetch = [&](int i, int stage) {
-        int within;
-        const int page = p.cache.page_of(b, block_of(i), within);
-        missing = page < 0 ? missing | 1u << stage : missing & ~(1u << stage);
-        if (page < 0)
-            return;
-        const uint8_t *from = p.cache.block_at(page, kvh, within, S::BLOCK);
-        const uint32_t to = ring + stage * S::BLOCK;
-#pragma unroll
-        for (int x = lane * 16; x < S::BLOCK; x += 512)
-            copy_async_16(to + x, from + x);
-    };
-    int i = part * kWarps + warp;
-#pragma unroll
-    for (int k = 0; k < ST - 1; ++k) {
-        if (i + k * stride < blocks)
-            fetch(i + k * stride, k);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    for (int stage = 0; i < blocks; i += stride, stage = stage + 1 == ST ? 0 : stage + 1) {
+    for (int k = 0, stage = 0; k < pairs; ++k, stage = stage + 1 == ST ? 0 : stage + 1) {
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
-        __syncwarp(); // this block has landed for every lane, and every lane is done with the last one
-        const bool bad = missing >> stage & 1u;
-        if (i + (ST - 1) * stride < blocks)
-            fetch(i + (ST - 1) * stride, stage == 0 ? ST - 1 : stage - 1);
+        __syncwarp(); // this pair has landed for every lane, and every lane is done with the last one
+        const uint32_t bad = bad_bits >> (2 * stage) & 3u;
+        if (k + ST - 1 < pairs)
+            fetch(k + ST - 1, stage == 0 ? ST - 1 : stage - 1);
         asm volatile("cp.async.commit_group;" ::: "memory");
-        const uint32_t at = ring + stage * S::BLOCK;
+        const uint32_t at = ring + stage * S::STAGE;
 
-        // S^T: tokens g (rows 0 to 7) and g + 8.
-        uint32_t kw[2][C::WORDS], scales[C::TOGETHER ? 1 : C::WORDS];
+        // S^T: tokens g (rows 0 to 7) and g + 8 of each block.
+        float s[2][NT][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t row = at + B::KEYS + (g + 8 * h) * (D / 2);
-            if constexpr (C::TOGETHER)
-                shared_words<C::WORDS>(row + c * 4 * C::WORDS, kw[h]);
-            else
+        for (int u = 0; u < 2; ++u) {
+            uint32_t kw[2][C::WORDS], scales[C::TOGETHER ? 1 : C::WORDS];
 #pragma unroll
-                for (int j = 0; j < C::WORDS; ++j)
-                    shared_words<1>(row + j * 16 + c * 4, &kw[h][j]);
-        }
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t row = at + u * S::BLOCK + B::KEYS + (g + 8 * h) * (D / 2);
+                if constexpr (C::TOGETHER)
+                    shared_words<C::WORDS>(row + c * 4 * C::WORDS, kw[h]);
+                else
 #pragma unroll
-        for (int j = 0; j < (C::TOGETHER ? 1 : C::WORDS); ++j) // both tokens' scales of the lane's group
-            shared_words<1>(at + B::KEY_SCALES + 2 * B::key_scale(g, C::first(j, c) / 32), &scales[j]);
-        float s[NT][4], s2[NT][4]; // two chains of dependent products
+                    for (int j = 0; j < C::WORDS; ++j)
+                        shared_words<1>(row + j * 16 + c * 4, &kw[h][j]);
+            }
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+            for (int j = 0; j < (C::TOGETHER ? 1 : C::WORDS); ++j) // both tokens' scales of the lane's group
+                shared_words<1>(at + u * S::BLOCK + B::KEY_SCALES + 2 * B::key_scale(g, C::first(j, c) / 32), &scales[j]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                s[t][e] = s2[t][e] = 0.f;
+            for (int t = 0; t < NT; ++t)
+                s[u][t][0] = s[u][t][1] = s[u][t][2] = s[u][t][3] = 0.f;
 #pragma unroll
-        for (int j = 0; j < C::WORDS; ++j) {
-            const uint32_t both = scales[C::TOGETHER ? 0 : j];
-            const uint32_t s_g = __byte_perm(both, 0, 0x1010), s_g8 = __byte_perm(both, 0, 0x3232);
-            uint32_t x[4], y[4];
-            f16x8(kw[0][j], x);
-            f16x8(kw[1][j], y);
-            const uint32_t a0[4] = {hmul2(x[0], s_g), hmul2(y[0], s_g8), hmul2(x[1], s_g), hmul2(y[1], s_g8)};
-            const uint32_t a1[4] = {hmul2(x[2], s_g), hmul2(y[2], s_g8), hmul2(x[3], s_g), hmul2(y[3], s_g8)};
+            for (int j = 0; j < C::WORDS; ++j) {
+                const uint32_t both = scales[C::TOGETHER ? 0 : j];
+                const uint32_t s_g = __byte_perm(both, 0, 0x1010), s_g8 = __byte_perm(both, 0, 0x3232);
+                uint32_t x[4], y[4];
+                f16x8(kw[0][j], x);
+                f16x8(kw[1][j], y);
+                const uint32_t a0[4] = {hmul2(x[0], s_g), hmul2(y[0], s_g8), hmul2(x[1], s_g), hmul2(y[1], s_g8)};
+                const uint32_t a1[4] = {hmul2(x[2], s_g), hmul2(y[2], s_g8), hmul2(x[3], s_g), hmul2(y[3], s_g8)};
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                mma16816(s[t], a0, qb[t][2 * j][0], qb[t][2 * j][1]);
-                mma16816(s2[t], a1, qb[t][2 * j + 1][0], qb[t][2 * j + 1][1]);
+                for (int t = 0; t < NT; ++t) {
+                    mma16816(s[u][t], a0, qb[t][2 * j][0], qb[t][2 * j][1]);
+                    mma16816(s[u][t], a1, qb[t][2 * j + 1][0], qb[t][2 * j + 1][1]);
+                }
             }
         }
-        const int key = block_of(i) * kCacheBlock;
-        // A block that every row sees whole needs no mask.
-        const bool whole = !bad && key + kCacheBlock <= limit_all && (key >= floor_all || key + kCacheBlock <= p.sinks);
+        // A pair that every row sees whole needs no mask.
+        const int i0 = j0 + (warp + k * W) * step, key0 = block_of(i0) * kCacheBlock;
+        const int key1 = i0 + 1 < j1 ? block_of(i0 + 1) * kCacheBlock : tile.n; // no token is there
+        const bool whole = !bad && max(key0, key1) + kCacheBlock <= limit_all &&
+                           (min(key0, key1) >= floor_all || max(key0, key1) + kCacheBlock <= p.sinks);
+        if (!whole) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { // token g + 8 (e / 2), query 2c + e % 2
+                        const int token = (u ? key1 : key0) + g + 8 * (e >> 1);
+                        const bool seen = token < limit[t][e & 1] && (token >= floor_[t][e & 1] || token < p.sinks);
+                        s[u][t][e] = seen ? (bad >> u & 1u ? NAN : s[u][t][e]) : -INFINITY;
+                    }
+        }
         bool above = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { // token g + 8 (e / 2), query 2c + e % 2
-                float x = (s[t][e] + s2[t][e]) * factor[t][e & 1];
-                if (!whole) {
-                    const int token = key + g + 8 * (e >> 1);
-                    const bool seen = token < limit[t][e & 1] && (token >= floor_[t][e & 1] || token < p.sinks);
-                    x = seen ? (bad ? NAN : x) : -INFINITY;
-                }
-                s[t][e] = x;
-                above |= x > ref[t][e & 1] + kLazy;
-            }
+            for (int h = 0; h < 2; ++h)
+                above |= fmaxf(fmax3(s[0][t][h], s[0][t][h + 2], s[1][t][h]), s[1][t][h + 2]) > bar[t][h];
         if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 float times[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float top = fmaxf(s[t][h], s[t][h + 2]);
+                    float top = fmaxf(fmax3(s[0][t][h], s[0][t][h + 2], s[1][t][h]), s[1][t][h + 2]);
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    top = fmaxf(top, ref[t][h]);
-                    times[h] = top > ref[t][h] ? ex2_approx(ref[t][h] - top) : 1.f;
-                    ref[t][h] = top;
+                    times[h] = 1.f;
+                    if (top > bar[t][h] || (!none[t][h] && top * factor[t][h] > ref[t][h])) {
+                        const float next = top * factor[t][h];
+                        times[h] = none[t][h] ? 0.f : ex2_approx(ref[t][h] - next);
+                        none[t][h] = false;
+                        ref[t][h] = next;
+                        bar[t][h] = (next + kLazy) / factor[t][h];
+                    }
                     sum[t][h] *= times[h];
                 }
 #pragma unroll
@@ -306,62 +409,69 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) window_e2m1_toke
                 }
             }
         }
-        uint32_t pb[NT][2];
+        uint32_t pb[2][NT][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float r = ref[t][e & 1];
-                s[t][e] = ex2_approx(s[t][e] - (r == -INFINITY ? 0.f : r));
-                sum[t][e & 1] += s[t][e];
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[u][t][e] = ex2_approx(fmaf(s[u][t][e], factor[t][e & 1], -ref[t][e & 1]));
+                    sum[t][e & 1] += s[u][t][e];
+                }
+                pb[u][t][0] = turn(pack_f16(s[u][t][0], s[u][t][1]));
+                pb[u][t][1] = turn(pack_f16(s[u][t][2], s[u][t][3]));
             }
-            pb[t][0] = turn(pack_f16(s[t][0], s[t][1]));
-            pb[t][1] = turn(pack_f16(s[t][2], s[t][3]));
-        }
 
         // O^T: a lane's scales are those of tokens 2c, 2c + 1 and 2c + 8, 2c + 9.
-        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-        if (!whole) { // values that no row sees may be anything: their scale is zero
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                keep[h] = 0;
+        for (int u = 0; u < 2; ++u) {
+            uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+            if (!whole) { // values that no row sees may be anything: their scale is zero
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int token = key + 2 * c + 8 * h + e;
-                    if (!bad && token < high && (token >= low || token < sink))
-                        keep[h] |= 0xffffu << (16 * e);
+                for (int h = 0; h < 2; ++h) {
+                    keep[h] = 0;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int token = (u ? key1 : key0) + 2 * c + 8 * h + e;
+                        if (!(bad >> u & 1u) && token < tile.high && (token >= tile.low || token < tile.sink))
+                            keep[h] |= 0xffffu << (16 * e);
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (int v = 0; v < D / 16 / B::W; ++v) {
-            uint32_t vw[B::W];
-            shared_words<B::W>(at + B::VALUES + B::value_word(v * B::W, lane), vw);
+            for (int v = 0; v < D / 16 / B::W; ++v) {
+                uint32_t vw[B::W];
+                shared_words<B::W>(at + u * S::BLOCK + B::VALUES + B::value_word(v * B::W, lane), vw);
 #pragma unroll
-            for (int j = 0; j < B::W; j += 2) {
-                uint32_t vs[2]; // one group of 32 columns
-                shared_words<2>(at + B::VALUE_SCALES + 2 * B::value_scale(2 * c, (v * B::W + j) / 2), vs);
-                vs[0] &= keep[0];
-                vs[1] &= keep[1];
+                for (int j = 0; j < B::W; j += 2) {
+                    uint32_t vs[2]; // one group of 32 columns
+                    shared_words<2>(at + u * S::BLOCK + B::VALUE_SCALES + 2 * B::value_scale(2 * c, (v * B::W + j) / 2), vs);
+                    if (!whole) {
+                        vs[0] &= keep[0];
+                        vs[1] &= keep[1];
+                    }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    uint32_t x[4];
-                    f16x8(vw[j + e], x);
-                    const uint32_t a[4] = {hmul2(x[0], vs[0]), hmul2(x[1], vs[0]), hmul2(x[2], vs[1]), hmul2(x[3], vs[1])};
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t x[4];
+                        f16x8(vw[j + e], x);
+                        const uint32_t a[4] = {hmul2(x[0], vs[0]), hmul2(x[1], vs[0]), hmul2(x[2], vs[1]), hmul2(x[3], vs[1])};
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
-                        mma16816(o[t][v * B::W + j + e], a, pb[t][0], pb[t][1]);
+                        for (int t = 0; t < NT; ++t)
+                            mma16816(o[t][v * B::W + j + e], a, pb[u][t][0], pb[u][t][1]);
+                    }
                 }
             }
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads(); // the ring becomes the parts' place
-    float(*part_m)[ROWS] = reinterpret_cast<float(*)[ROWS]>(smem), (*part_l)[ROWS] = part_m + kWarps;
-    float *cta_m = part_l[kWarps], *cta_l = cta_m + ROWS;
-    float(*part_o)[ROWS][D + 4] = reinterpret_cast<float(*)[ROWS][D + 4]>(cta_l + ROWS);
+    float(*part_m)[ROWS] = reinterpret_cast<float(*)[ROWS]>(smem), (*part_l)[ROWS] = part_m + W;
+    cta_m = part_l[W];
+    cta_l = cta_m + ROWS;
+    part_o = reinterpret_cast<float(*)[ROWS][D + 4]>(cta_l + ROWS);
 
-    // The warps' parts, then the CTAs': out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
+    // The warps' parts: out = sum_i 2^(m_i - m) o_i, l = sum_i 2^(m_i - m) l_i.
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -371,7 +481,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) window_e2m1_toke
             sum[t][h] += __shfl_xor_sync(0xffffffffu, sum[t][h], 16);
             const int r = 8 * t + 2 * c + h;
             if (g == 0) {
-                part_m[warp][r] = ref[t][h];
+                part_m[warp][r] = none[t][h] ? -INFINITY : ref[t][h];
                 part_l[warp][r] = sum[t][h];
             }
 #pragma unroll
@@ -381,16 +491,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) window_e2m1_toke
             }
         }
     __syncthreads();
-    for (int x = threadIdx.x; x < ROWS * D; x += kWarps * 32) {
+    for (int x = threadIdx.x; x < ROWS * D; x += W * 32) {
         const int r = x / D, col = x - r * D;
         float mx = part_m[0][r];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w)
+        for (int w = 1; w < W; ++w)
             mx = fmaxf(mx, part_m[w][r]);
         const float base = mx == -INFINITY ? 0.f : mx;
         float l = 0.f, v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float f = exp2f(part_m[w][r] - base);
             l += f * part_l[w][r];
             v += f * part_o[w][r][col];
@@ -401,13 +511,28 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) window_e2m1_toke
             cta_l[r] = l;
         }
     }
+}
+
+// A cluster for each tile.
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D, NT>::CTAS)
+    window_e2m1_cluster_kernel(const __grid_constant__ TokensParams p) {
+    using S = TokensShape<D, NT>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int parts = p.parts, pair = blockIdx.x / parts, part = blockIdx.x - pair * parts;
+    const int b = pair / p.kv_heads, kvh = pair - b * p.kv_heads;
+    int n, m;
+    lengths_of(p, b, n, m);
+    const Tile tile = tile_of<S::ROWS>(p, n, m, blockIdx.y);
+    float *cta_m, *cta_l, (*part_o)[S::ROWS][D + 4];
+    attend<D, NT, BF16>(p, tile, b, kvh, 2 * part, tile.blocks, 2 * parts, smem, cta_m, cta_l, part_o);
     if (parts > 1)
         cluster_sync();
     else
         __syncthreads();
-    for (int x = part * kWarps * 32 + threadIdx.x; x < ROWS * D; x += parts * kWarps * 32) {
+    for (int x = part * S::WARPS * 32 + threadIdx.x; x < S::ROWS * D; x += parts * S::WARPS * 32) {
         const int r = x / D, col = x - r * D;
-        if (r >= rows || col >= p.hd)
+        if (r >= tile.rows || col >= p.hd)
             continue;
         float l, v;
         if (parts > 1) {
@@ -425,70 +550,249 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) window_e2m1_toke
             l = cta_l[r];
             v = part_o[0][r][col];
         }
-        const int row = row0 + r;
-        // Zeros for a row that sees no key, which its position tells: a sum that is no
-        // positive number otherwise stands for scores that are not finite, and gives NaN.
-        v = min(n, pos0 + row / p.group + p.right + 1) > 0 ? v / l : 0.f;
-        const long long to = b * p.os[0] + (kvh * p.group + row % p.group) * p.os[1] + (row / p.group) * p.os[2] + col;
-        if (p.out_dtype == kOutF32)
-            static_cast<float *>(p.out)[to] = v;
-        else if (p.out_dtype == kOutBF16)
-            static_cast<__nv_bfloat16 *>(p.out)[to] = __float2bfloat16_rn(v);
-        else
-            static_cast<__half *>(p.out)[to] = __float2half_rn(v);
+        store_out(p, tile, b, kvh, r, col, v, l);
     }
     if (parts > 1)
         cluster_sync(); // no CTA leaves while another reads its part
 }
 
-template <int D, int NT, bool BF16> int launch_rows(const TokensParams &p, int batch, cudaStream_t stream) {
+// Sums over the CTA's threads; every thread gets the result.
+template <int WARPS> __device__ __forceinline__ long long cta_sum(long long v, long long *place) {
+#pragma unroll
+    for (int x = 16; x; x >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, x);
+    if ((threadIdx.x & 31) == 0)
+        place[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w)
+        v += place[w];
+    __syncthreads();
+    return v;
+}
+
+// The list: blocks of the tiles, sequence after sequence, key head after key head, tile after
+// tile.  CTA i takes blocks [i per, (i + 1) per).
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D, NT>::CTAS)
+    window_e2m1_list_kernel(const __grid_constant__ TokensParams p) {
     using S = TokensShape<D, NT>;
-    static std::atomic<unsigned long long> done{0};
-    const void *kernel = reinterpret_cast<const void *>(window_e2m1_tokens_kernel<D, NT, BF16>);
-    const cudaError_t e = set_smem_limit(kernel, S::SMEM, done);
-    if (e != cudaSuccess)
-        return static_cast<int>(e);
-    if (p.parts > 8) { // clusters above 8 CTAs need the kernel's consent
-        const cudaError_t w = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (w != cudaSuccess)
-            return static_cast<int>(w);
+    constexpr int THREADS = S::WARPS * 32;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ long long place[S::WARPS], start_at;
+    __shared__ int start_b;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // Each thread has a run of sequences; the thread in whose run this CTA's first block is finds the sequence.
+    const int run = (p.batch + THREADS - 1) / THREADS, b0 = threadIdx.x * run, b1 = min(p.batch, b0 + run);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b)
+        mine += listed_of<S::ROWS>(p, b);
+    mine *= p.kv_heads;
+    long long before = mine;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, before, x);
+        before += lane >= x ? y : 0;
     }
-    const int tiles = (p.group * p.q_len + S::ROWS - 1) / S::ROWS;
+    if (lane == 31)
+        place[warp] = before;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < S::WARPS; ++w) {
+        before += w < warp ? place[w] : 0;
+        total += place[w];
+    }
+    before -= mine;
+    const long long per = (total + gridDim.x - 1) / gridDim.x;
+    const long long from = blockIdx.x * per, to = min(total, from + per);
+    if (from >= to)
+        return;
+    if (from >= before && from < before + mine) {
+        long long at = before;
+        int b = b0;
+        for (; b < b1 - 1; ++b) {
+            const long long next = at + static_cast<long long>(listed_of<S::ROWS>(p, b)) * p.kv_heads;
+            if (from < next)
+                break;
+            at = next;
+        }
+        start_at = at;
+        start_b = b;
+    }
+    __syncthreads();
+    long long at = start_at; // where the next tile begins
+    int b = start_b;
+    for (int parts = 0; at < to; ++b) {
+        int n, m;
+        lengths_of(p, b, n, m);
+        for (int kvh = 0; kvh < p.kv_heads && at < to; ++kvh)
+            for (int i = 0; i < p.tiles && at < to; ++i) {
+                const Tile tile = tile_of<S::ROWS>(p, n, m, i);
+                const int size = listed(tile);
+                const long long begin = at;
+                at += size;
+                if (at <= from || size == 0)
+                    continue;
+                const int j0 = static_cast<int>(max(from - begin, 0ll)), j1 = static_cast<int>(min(to - begin, static_cast<long long>(size)));
+                float *cta_m, *cta_l, (*part_o)[S::ROWS][D + 4];
+                attend<D, NT, BF16>(p, tile, b, kvh, j0, min(j1, tile.blocks), 2, smem, cta_m, cta_l, part_o);
+                __syncthreads();
+                if (j0 == 0 && j1 == size) {
+                    for (int x = threadIdx.x; x < S::ROWS * D; x += THREADS) {
+                        const int r = x / D, col = x - r * D;
+                        if (r < tile.rows && col < p.hd)
+                            store_out(p, tile, b, kvh, r, col, part_o[0][r][col], cta_l[r]);
+                    }
+                } else {
+                    float *slot = p.parts_at + (2ll * blockIdx.x + (begin > from)) * S::SLOT;
+                    for (int r = threadIdx.x; r < tile.rows; r += THREADS) {
+                        slot[2 * r] = cta_m[r];
+                        slot[2 * r + 1] = cta_l[r];
+                    }
+                    for (int x = threadIdx.x * 4; x < tile.rows * D; x += THREADS * 4)
+                        *reinterpret_cast<float4 *>(slot + 2 * S::ROWS + x) =
+                            *reinterpret_cast<const float4 *>(&part_o[0][x / D][x % D]);
+                }
+                __syncthreads(); // the parts' place becomes the ring again
+            }
+    }
+}
+
+// Joins the parts of the tiles that several CTAs share: a CTA for each tile.
+template <int D, int NT> __global__ void __launch_bounds__(256) window_e2m1_join_kernel(const __grid_constant__ TokensParams p, int ctas) {
+    using S = TokensShape<D, NT>;
+    __shared__ long long place[8];
+    const int i = blockIdx.x % p.tiles, pair = blockIdx.x / p.tiles, b = pair / p.kv_heads, kvh = pair - b * p.kv_heads;
+    long long before = 0, total = 0;
+    for (int x = threadIdx.x; x < p.batch; x += 256) {
+        const long long size = static_cast<long long>(listed_of<S::ROWS>(p, x)) * p.kv_heads;
+        total += size;
+        before += x < b ? size : 0;
+    }
+    total = cta_sum<8>(total, place);
+    before = cta_sum<8>(before, place);
+    int n, m;
+    lengths_of(p, b, n, m);
+    const long long per = max(1ll, (total + ctas - 1) / ctas);
+    before += static_cast<long long>(listed_of<S::ROWS>(p, b)) * kvh;
+    for (int x = 0; x < i; ++x)
+        before += listed(tile_of<S::ROWS>(p, n, m, x));
+    const Tile tile = tile_of<S::ROWS>(p, n, m, i);
+    const int size = listed(tile);
+    const int first = static_cast<int>(before / per), last = static_cast<int>((before + size - 1) / per);
+    asm volatile("griddepcontrol.wait;" ::: "memory"); // every CTA: this grid's end stands for the list's as well
+    if (size == 0 || first == last)
+        return;
+    // The tile is the last one of its first CTA, unless it begins with it, and the first one of the others.
+    const float *slot0 = p.parts_at + (2ll * first + (before > first * per)) * S::SLOT;
+    auto slot = [&](int c) { return c == first ? slot0 : p.parts_at + 2ll * c * S::SLOT; };
+    for (int x = threadIdx.x * 4; x < tile.rows * D; x += 1024) {
+        const int r = x / D, col = x - r * D;
+        float mx = -INFINITY;
+#pragma unroll 8
+        for (int c = first; c <= last; ++c)
+            mx = fmaxf(mx, slot(c)[2 * r]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int c = first; c <= last; ++c) {
+            const float2 ml = *reinterpret_cast<const float2 *>(slot(c) + 2 * r);
+            const float4 o = *reinterpret_cast<const float4 *>(slot(c) + 2 * S::ROWS + x);
+            const float f = exp2f(ml.x - base);
+            l += f * ml.y;
+            v[0] += f * o.x;
+            v[1] += f * o.y;
+            v[2] += f * o.z;
+            v[3] += f * o.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < p.hd)
+                store_out(p, tile, b, kvh, r, col + e, v[e], l);
+    }
+}
+
+template <int D, int NT, bool BF16> int launch_rows(const TokensParams &p, int ctas, cudaStream_t stream) {
+    using S = TokensShape<D, NT>;
     cudaLaunchConfig_t cfg{};
-    cfg.dynamicSmemBytes = S::SMEM;
-    cfg.gridDim = dim3(static_cast<unsigned>(p.parts) * batch * p.kv_heads, tiles);
-    cfg.blockDim = dim3(kWarps * 32);
-    cfg.stream = stream;
     cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = p.parts;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.blockDim = dim3(S::WARPS * 32);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return static_cast<int>(cudaLaunchKernelEx(&cfg, window_e2m1_tokens_kernel<D, NT, BF16>, p));
+    if (p.parts) {
+        static std::atomic<unsigned long long> done{0};
+        const void *kernel = reinterpret_cast<const void *>(window_e2m1_cluster_kernel<D, NT, BF16>);
+        cudaError_t e = set_smem_limit(kernel, S::SMEM, done);
+        if (e == cudaSuccess && p.parts > 8) // clusters above 8 CTAs need the kernel's consent
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess)
+            return static_cast<int>(e);
+        cfg.gridDim = dim3(static_cast<unsigned>(p.parts) * p.batch * p.kv_heads, p.tiles);
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = p.parts;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        return static_cast<int>(cudaLaunchKernelEx(&cfg, window_e2m1_cluster_kernel<D, NT, BF16>, p));
+    }
+    static std::atomic<unsigned long long> done{0};
+    cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(window_e2m1_list_kernel<D, NT, BF16>), S::SMEM, done);
+    if (e != cudaSuccess)
+        return static_cast<int>(e);
+    cfg.gridDim = dim3(ctas);
+    cfg.numAttrs = 0;
+    e = cudaLaunchKernelEx(&cfg, window_e2m1_list_kernel<D, NT, BF16>, p);
+    if (e != cudaSuccess)
+        return static_cast<int>(e);
+    // The join is set up while the list's kernel runs, and waits for its end before it reads the parts.
+    cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.kv_heads * p.tiles);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, window_e2m1_join_kernel<D, NT>, p, ctas));
 }
-template <int D> int launch_d(const TokensParams &p, int batch, bool bf16, cudaStream_t stream) {
+template <int D> int launch_d(const TokensParams &p, int ctas, bool bf16, cudaStream_t stream) {
     if (p.group * p.q_len <= 8)
-        return bf16 ? launch_rows<D, 1, true>(p, batch, stream) : launch_rows<D, 1, false>(p, batch, stream);
-    return bf16 ? launch_rows<D, 2, true>(p, batch, stream) : launch_rows<D, 2, false>(p, batch, stream);
+        return bf16 ? launch_rows<D, 1, true>(p, ctas, stream) : launch_rows<D, 1, false>(p, ctas, stream);
+    return bf16 ? launch_rows<D, 2, true>(p, ctas, stream) : launch_rows<D, 2, false>(p, ctas, stream);
+}
+
+// How a call is split: CTAs of a cluster, or (parts 0) of the list.
+struct Split {
+    int rows, tiles, parts, ctas;
+    size_t workspace;
+};
+Split split_of(const WindowE2m1Args &a) {
+    const CacheArgs &c = a.cache;
+    const long long rows = static_cast<long long>(a.heads / c.kv_heads) * c.q_len;
+    Split s;
+    s.rows = rows <= 8 ? 8 : 16;
+    s.tiles = static_cast<int>((rows + s.rows - 1) / s.rows);
+    long long keys = a.kv_len;
+    if (a.window > 0)
+        keys = std::min(keys, static_cast<long long>(a.window) + c.q_len + a.right + a.sinks);
+    const long long of_tile = (keys + kCacheBlock - 1) / kCacheBlock + 1;
+    const long long tiles = static_cast<long long>(s.tiles) * c.batch * c.kv_heads;
+    const long long most = (s.rows == 8 ? 2ll : 1ll) * fmha_sm_count();
+    s.parts = 1;
+    while (s.parts < kMaxParts && tiles * s.parts * 2 <= most && of_tile >= 2ll * s.parts * 16)
+        s.parts *= 2;
+    s.ctas = 0;
+    s.workspace = 0;
+    if (tiles * of_tile > 64 * most) {
+        s.parts = 0;
+        s.ctas = static_cast<int>(most);
+        s.workspace = 2ull * most * s.rows * (cache_width(c.hd) + 2) * 4;
+    }
+    return s;
 }
 
 } // namespace
-
-// CTAs that split the keys of one tile of rows: until four (two of 16 rows) are on every SM,
-// with two blocks left for each warp.
-int window_e2m1_tokens_parts(const WindowE2m1Args &a) {
-    const long long rows = static_cast<long long>(a.heads / a.cache.kv_heads) * a.cache.q_len;
-    const long long tile = rows <= 8 ? 8 : 16, tiles = (rows + tile - 1) / tile;
-    const long long ctas = tiles * a.cache.batch * a.cache.kv_heads, most = (rows <= 8 ? 4ll : 2ll) * fmha_sm_count();
-    long long keys = a.kv_len;
-    if (a.window > 0)
-        keys = std::min(keys, static_cast<long long>(a.window) + a.cache.q_len + a.right + a.sinks);
-    int parts = 1;
-    while (parts < kMaxParts && ctas * parts * 2 <= most && keys >= 2ll * parts * 2 * kWarps * kCacheBlock)
-        parts *= 2;
-    return parts;
-}
 
 int window_e2m1_tokens_launch(const WindowE2m1Args &a, cudaStream_t stream) {
     TokensParams p{};
@@ -519,34 +823,40 @@ int window_e2m1_tokens_launch(const WindowE2m1Args &a, cudaStream_t stream) {
     p.out_dtype = a.out_dtype;
     const double scale = a.scale > 0 ? a.scale : 1.0 / std::sqrt(static_cast<double>(c.hd));
     p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-    p.parts = window_e2m1_tokens_parts(a);
+    const Split split = split_of(a);
+    p.parts = split.parts;
+    p.tiles = split.tiles;
+    p.batch = c.batch;
+    p.parts_at = static_cast<float *>(a.workspace);
     const bool bf16 = a.dtype == kBF16;
     switch (cache_width(c.hd)) {
     case 32:
-        return launch_d<32>(p, c.batch, bf16, stream);
+        return launch_d<32>(p, split.ctas, bf16, stream);
     case 64:
-        return launch_d<64>(p, c.batch, bf16, stream);
+        return launch_d<64>(p, split.ctas, bf16, stream);
     case 96:
-        return launch_d<96>(p, c.batch, bf16, stream);
+        return launch_d<96>(p, split.ctas, bf16, stream);
     default:
-        return launch_d<128>(p, c.batch, bf16, stream);
+        return launch_d<128>(p, split.ctas, bf16, stream);
     }
 }
 
-// A workspace means: the keys and values go back to 16 bits there (exactly), and the
-// prompts' kernel reads them.
+// Few rows read the cache as it is; for others the keys and values go back to 16 bits in the
+// workspace (exactly), and the prompts' kernel reads them.
+static bool few_rows(const WindowE2m1Args &a) {
+    return (static_cast<long long>(a.heads / a.cache.kv_heads) * a.cache.q_len + 15) / 16 <= 4;
+}
+
 size_t window_e2m1_workspace(const WindowE2m1Args &a) {
-    const CacheArgs &c = a.cache;
-    const long long rows = static_cast<long long>(a.heads / c.kv_heads) * c.q_len, tiles = (rows + 15) / 16;
-    if (tiles <= 4)
-        return 0;
-    return 4ull * c.batch * c.kv_heads * a.kv_len * c.hd;
+    if (few_rows(a))
+        return split_of(a).workspace;
+    return 4ull * a.cache.batch * a.cache.kv_heads * a.kv_len * a.cache.hd;
 }
 
 int window_e2m1_launch(const WindowE2m1Args &a, cudaStream_t stream) {
-    const size_t bytes = window_e2m1_workspace(a);
-    if (bytes == 0)
+    if (few_rows(a))
         return window_e2m1_tokens_launch(a, stream);
+    const size_t bytes = window_e2m1_workspace(a);
     const CacheArgs &c = a.cache;
     WindowArgs w;
     w.q = a.q;
