@@ -17,7 +17,7 @@
 //
 // The bound is the cache's bytes.  A block of 16 tokens of a head (2304 bytes at 128 columns)
 // is one contiguous piece; each warp copies its own blocks, two at a time, to a ring in shared
-// memory (cp.async, no barrier between warps) and keeps its own softmax state.  Converting
+// memory (a bulk copy for a block, no barrier between warps) and keeps its own softmax state.  Converting
 // takes a conversion and a product for two elements, 128 instructions of a block's ~200; the
 // rest is kept short: a lane looks up the pages of 32 blocks at once, and the running maximum
 // is lazy (other lanes are asked only when some score is more than 2^8 above the reference).
@@ -39,6 +39,7 @@ namespace omni_b200 {
 namespace {
 
 constexpr int kMaxParts = 16;
+constexpr int kMostRows = 64; // of a key head, group * q_len
 constexpr float kLazy = 8.f; // log2 units a score may be above the reference
 
 struct TokensParams {
@@ -49,10 +50,12 @@ struct TokensParams {
     long long qs[3], os[3];
     const int *lengths, *q_lengths;
     int parts; // CTAs of a cluster, or 0: the list
+    uint32_t group_inv; // ceil(2^16 / group): rows of a call are few (kMostRows), their quotients by it exact
     int batch, kv_heads, group, q_len, kv_len, hd, tiles; // tiles of rows that a sequence may have
     int window, right, sinks;
     int out_dtype;
     float scale_log2;
+    int *err;
 };
 
 template <int D, int NT> struct TokensShape {
@@ -73,6 +76,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The same with zeros to add to.
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t turn(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -90,8 +100,11 @@ template <int N> __device__ __forceinline__ void shared_words(uint32_t at, uint3
     else
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
 }
-__device__ __forceinline__ void copy_async_16(uint32_t to, const uint8_t *from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+// One contiguous piece (16-byte addresses and size) to shared memory, counted by `bar`.
+__device__ __forceinline__ void copy_piece(uint32_t to, unsigned long long from, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -122,6 +135,7 @@ struct Tile {
     int n, m, row0, rows, pos0;
     int first, last, low, high, sink, sink_blocks, begin, blocks;
 };
+__device__ __forceinline__ int query_of(const TokensParams &p, int row) { return static_cast<int>(row * p.group_inv >> 16); }
 __device__ __forceinline__ void lengths_of(const TokensParams &p, int b, int &n, int &m) {
     n = max(0, min(p.lengths[b], p.kv_len));
     m = p.q_lengths ? max(0, min(p.q_lengths[b], p.q_len)) : p.q_len;
@@ -135,8 +149,8 @@ template <int ROWS> __device__ __forceinline__ Tile tile_of(const TokensParams &
     t.rows = min(ROWS, p.group * m - t.row0);
     t.pos0 = n - m;
     // Keys that some row of the tile sees: [0, sink) and [low, high).
-    t.first = t.pos0 + t.row0 / p.group;
-    t.last = t.pos0 + (t.row0 + max(t.rows, 1) - 1) / p.group;
+    t.first = t.pos0 + query_of(p, t.row0);
+    t.last = t.pos0 + query_of(p, t.row0 + max(t.rows, 1) - 1);
     t.high = t.rows > 0 ? max(0, min(n, t.last + p.right + 1)) : 0;
     t.low = p.window > 0 ? max(0, min(t.first - p.window + 1, t.high)) : 0;
     t.sink = min(p.sinks, t.low);
@@ -145,8 +159,10 @@ template <int ROWS> __device__ __forceinline__ Tile tile_of(const TokensParams &
     t.blocks = t.sink_blocks + max(0, (t.high + kCacheBlock - 1) / kCacheBlock - t.begin);
     return t;
 }
-// Its length in the list: a tile that sees nothing still has rows to write.
-__device__ __forceinline__ int listed(const Tile &t) { return t.rows > 0 ? max(t.blocks, 1) : 0; }
+// Its length in the list: beginning and ending a tile takes a CTA as long as some blocks do
+// (1.2 us against 0.13 us for one: 64 x up to 16384 keys TILECOST), so it counts for those as well.
+constexpr int kTileCost = 8;
+__device__ __forceinline__ int listed(const Tile &t) { return t.rows > 0 ? kTileCost + t.blocks : 0; }
 // Blocks of all tiles of a sequence's key head.
 template <int ROWS> __device__ __forceinline__ int listed_of(const TokensParams &p, int b) {
     int n, m, sum = 0;
@@ -157,11 +173,11 @@ template <int ROWS> __device__ __forceinline__ int listed_of(const TokensParams 
 }
 
 __device__ __forceinline__ void store_out(const TokensParams &p, const Tile &t, int b, int kvh, int r, int col, float v, float l) {
-    const int row = t.row0 + r, query = row / p.group;
+    const int row = t.row0 + r, query = query_of(p, row);
     // Zeros for a row that sees no key, which its position tells: a sum that is no positive
     // number otherwise stands for scores that are not finite, and gives NaN.
     v = min(t.n, t.pos0 + query + p.right + 1) > 0 ? v / l : 0.f;
-    const long long to = b * p.os[0] + (kvh * p.group + row % p.group) * p.os[1] + query * p.os[2] + col;
+    const long long to = b * p.os[0] + (kvh * p.group + row - query * p.group) * p.os[1] + query * p.os[2] + col;
     if (p.out_dtype == kOutF32)
         static_cast<float *>(p.out)[to] = v;
     else if (p.out_dtype == kOutBF16)
@@ -174,7 +190,7 @@ __device__ __forceinline__ void store_out(const TokensParams &p, const Tile &t, 
 // m, l of the rows in cta_m and cta_l and the outputs in part_o[0].
 template <int D, int NT, bool BF16>
 __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, int b, int kvh, int j0, int j1, int step,
-                                       uint8_t *smem, float *&cta_m, float *&cta_l, float (*&part_o)[8 * NT][D + 4]) {
+                                       uint8_t *smem, uint64_t *bars, uint32_t &phases, float *&cta_m, float *&cta_l, float (*&part_o)[8 * NT][D + 4]) {
     using S = TokensShape<D, NT>;
     using B = CacheBlock<D>;
     using C = Columns<D>;
@@ -183,61 +199,41 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
 
     // Blocks of pairs: this warp's pair k is blocks j0 + (warp + k W) step and the next one.
     const uint32_t ring = smem_u32(smem) + warp * ST * S::STAGE;
-    const uint8_t *head = p.cache.data + kvh * p.cache.head_stride;
+    uint64_t *full = bars + warp * ST; // a stage's two copies have landed
     auto block_of = [&](int i) { return i < tile.sink_blocks ? i : tile.begin + i - tile.sink_blocks; };
-    // Lane l knows block l % 2 of pair k + l / 2, k a multiple of 16: its address, 0 where there
-    // is none, and bits of those whose page is none of the cache's; pages of the next 16 pairs.
+    // Lane l knows where block l % 2 of pair k + l / 2 is, k a multiple of 16 (0: nowhere), and
+    // copies it; whether a block's page is none of the cache's; the pages of the next 16 pairs.
     unsigned long long place = 0;
     uint32_t unpaged = 0;
-    int page_next = 0;
-    auto look_up = [&](int k, int &within, bool &real) {
+    int page_next = 0, within_next = 0;
+    auto look_up = [&](int k) {
         const int i = j0 + (warp + (k + (lane >> 1)) * W) * step + (lane & 1);
-        real = i < j1;
-        return real ? p.cache.page_of(b, block_of(i), within) : 0;
-    };
-    auto places = [&](int k) {
-        int within = 0;
-        bool real;
-        int page = page_next;
-        const int i = j0 + (warp + (k + (lane >> 1)) * W) * step + (lane & 1);
-        real = i < j1;
-        within = real ? block_of(i) % p.cache.page_blocks : 0;
-        unpaged = __ballot_sync(0xffffffffu, real && page < 0);
-        place = real && page >= 0 ? reinterpret_cast<unsigned long long>(head + page * p.cache.page_stride +
-                                                                         static_cast<long long>(within) * S::BLOCK)
-                                  : 0ull;
-        page_next = look_up(k + 16, within, real);
+        page_next = i < j1 ? p.cache.page_of(b, block_of(i), within_next) : -2;
     };
     uint32_t bad_bits = 0; // two for each stage
     auto fetch = [&](int k, int stage) {
-        if ((k & 15) == 0)
-            places(k);
-        bad_bits = (bad_bits & ~(3u << (2 * stage))) | (unpaged >> (2 * (k & 15)) & 3u) << (2 * stage);
-        const uint32_t to = ring + stage * S::STAGE + lane * 16;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const unsigned long long at = __shfl_sync(0xffffffffu, place, 2 * (k & 15) + h);
-            if (at) {
-                const uint8_t *from = reinterpret_cast<const uint8_t *>(at) + lane * 16;
-#pragma unroll
-                for (int x = 0; x < S::BLOCK; x += 512)
-                    if (x + 512 <= S::BLOCK || lane * 16 < S::BLOCK - x)
-                        copy_async_16(to + h * S::BLOCK + x, from + x);
-            }
+        if ((k & 15) == 0) {
+            unpaged = __ballot_sync(0xffffffffu, page_next == -1);
+            place = page_next >= 0 ? reinterpret_cast<unsigned long long>(p.cache.block_at(page_next, kvh, within_next, S::BLOCK)) : 0ull;
+            look_up(k + 16);
+        }
+        if (unpaged) // rare: no such page
+            bad_bits = (bad_bits & ~(3u << (2 * stage))) | (unpaged >> (2 * (k & 15)) & 3u) << (2 * stage);
+        else
+            bad_bits &= ~(3u << (2 * stage));
+        if ((lane >> 1) == (k & 15)) {
+            const uint32_t bytes = place ? S::BLOCK : 0;
+            mbar_arrive_expect_tx(full + stage, bytes);
+            if (place)
+                copy_piece(ring + stage * S::STAGE + (lane & 1) * S::BLOCK, place, S::BLOCK, smem_u32(full + stage));
         }
     };
     const int pairs = j1 - j0 > warp * step ? (j1 - j0 - warp * step + W * step - 1) / (W * step) : 0;
-    {
-        int within;
-        bool real;
-        page_next = look_up(0, within, real);
-    }
+    look_up(0);
 #pragma unroll
-    for (int k = 0; k < ST - 1; ++k) {
+    for (int k = 0; k < ST - 1; ++k)
         if (k < pairs)
             fetch(k, k);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
 
     // The queries as B operands, and the masks of columns 2c and 2c + 1.
     const int limit_all = min(tile.n, tile.first + p.right + 1), floor_all = p.window > 0 ? tile.last - p.window + 1 : 0;
@@ -248,7 +244,8 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
     for (int t = 0; t < NT; ++t) {
         const int r = tile.row0 + 8 * t + g;
         const bool real = 8 * t + g < tile.rows;
-        const uint16_t *q = p.q + b * p.qs[0] + (kvh * p.group + r % p.group) * p.qs[1] + (r / p.group) * p.qs[2];
+        const int query = query_of(p, r);
+        const uint16_t *q = p.q + b * p.qs[0] + (kvh * p.group + r - query * p.group) * p.qs[1] + query * p.qs[2];
         uint4 w[C::WORDS];
         uint32_t top2 = 0;
 #pragma unroll
@@ -286,7 +283,7 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int col = 8 * t + 2 * c + h, pos = tile.pos0 + (tile.row0 + col) / p.group;
+            const int col = 8 * t + 2 * c + h, pos = tile.pos0 + query_of(p, tile.row0 + col);
             const int of_col = __shfl_sync(0xffffffffu, exponent, 4 * (2 * c + h));
             // Not 0, so that a hidden key's -inf stays -inf.
             factor[t][h] = fmaxf(p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - of_col) << 23), 1.4e-45f);
@@ -311,58 +308,91 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
     for (int t = 0; t < NT; ++t)
         none[t][0] = none[t][1] = true;
 
-    for (int k = 0, stage = 0; k < pairs; ++k, stage = stage + 1 == ST ? 0 : stage + 1) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
-        __syncwarp(); // this pair has landed for every lane, and every lane is done with the last one
+    // Pairs that every row sees whole need no mask: blocks [whole0, whole1) (sinks are left to it).
+    const int ahead = tile.sink_blocks - tile.begin;
+    const int whole0 = max(tile.sink_blocks, (max(floor_all, 0) + kCacheBlock - 1) / kCacheBlock + ahead);
+    const int whole1 = min(j1, max(limit_all, 0) / kCacheBlock + ahead);
+    int i0 = j0 + warp * step, left = ST;
+    for (int k = 0, stage = 0; k < pairs; ++k, i0 += W * step, stage = stage + 1 == ST ? 0 : stage + 1) {
+        __syncwarp(); // every lane is done with the last pair, whose place is the next copy's
         const uint32_t bad = bad_bits >> (2 * stage) & 3u;
         if (k + ST - 1 < pairs)
             fetch(k + ST - 1, stage == 0 ? ST - 1 : stage - 1);
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (!mbar_wait(full + stage, phases >> stage & 1u, p.err, kErrWaitK)) {
+            // Gives up, but not before its copies under way are over, or had their time.
+            for (; k < pairs && left > 0; ++k, --left, stage = stage + 1 == ST ? 0 : stage + 1) {
+                const uint64_t start = globaltimer_ns();
+                while (!mbar_try_wait(smem_u32(full + stage), phases >> stage & 1u) && globaltimer_ns() - start < kWaitLimitNs) {
+                }
+                phases ^= 1u << stage;
+            }
+            break;
+        }
+        phases ^= 1u << stage;
         const uint32_t at = ring + stage * S::STAGE;
 
-        // S^T: tokens g (rows 0 to 7) and g + 8 of each block.
+        // S^T: tokens g (rows 0 to 7) and g + 8 of each block; the blocks' products take turns,
+        // so that none waits for the one before it.
         float s[2][NT][4];
+        uint32_t kw[2][2][C::WORDS], scales[2][C::TOGETHER ? 1 : C::WORDS];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            uint32_t kw[2][C::WORDS], scales[C::TOGETHER ? 1 : C::WORDS];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint32_t row = at + u * S::BLOCK + B::KEYS + (g + 8 * h) * (D / 2);
                 if constexpr (C::TOGETHER)
-                    shared_words<C::WORDS>(row + c * 4 * C::WORDS, kw[h]);
+                    shared_words<C::WORDS>(row + c * 4 * C::WORDS, kw[u][h]);
                 else
 #pragma unroll
                     for (int j = 0; j < C::WORDS; ++j)
-                        shared_words<1>(row + j * 16 + c * 4, &kw[h][j]);
+                        shared_words<1>(row + j * 16 + c * 4, &kw[u][h][j]);
             }
 #pragma unroll
             for (int j = 0; j < (C::TOGETHER ? 1 : C::WORDS); ++j) // both tokens' scales of the lane's group
-                shared_words<1>(at + u * S::BLOCK + B::KEY_SCALES + 2 * B::key_scale(g, C::first(j, c) / 32), &scales[j]);
+                shared_words<1>(at + u * S::BLOCK + B::KEY_SCALES + 2 * B::key_scale(g, C::first(j, c) / 32), &scales[u][j]);
+        }
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-                s[u][t][0] = s[u][t][1] = s[u][t][2] = s[u][t][3] = 0.f;
+        for (int j = 0; j < C::WORDS; ++j) {
+            uint32_t a[2][2][4];
 #pragma unroll
-            for (int j = 0; j < C::WORDS; ++j) {
-                const uint32_t both = scales[C::TOGETHER ? 0 : j];
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t both = scales[u][C::TOGETHER ? 0 : j];
                 const uint32_t s_g = __byte_perm(both, 0, 0x1010), s_g8 = __byte_perm(both, 0, 0x3232);
                 uint32_t x[4], y[4];
-                f16x8(kw[0][j], x);
-                f16x8(kw[1][j], y);
-                const uint32_t a0[4] = {hmul2(x[0], s_g), hmul2(y[0], s_g8), hmul2(x[1], s_g), hmul2(y[1], s_g8)};
-                const uint32_t a1[4] = {hmul2(x[2], s_g), hmul2(y[2], s_g8), hmul2(x[3], s_g), hmul2(y[3], s_g8)};
+                f16x8(kw[u][0][j], x);
+                f16x8(kw[u][1][j], y);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    mma16816(s[u][t], a0, qb[t][2 * j][0], qb[t][2 * j][1]);
-                    mma16816(s[u][t], a1, qb[t][2 * j + 1][0], qb[t][2 * j + 1][1]);
+                for (int e = 0; e < 2; ++e) {
+                    a[u][e][0] = hmul2(x[2 * e], s_g);
+                    a[u][e][1] = hmul2(y[2 * e], s_g8);
+                    a[u][e][2] = hmul2(x[2 * e + 1], s_g);
+                    a[u][e][3] = hmul2(y[2 * e + 1], s_g8);
                 }
             }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        if (j == 0 && e == 0)
+                            mma16816_first(s[u][t], a[u][e], qb[t][2 * j + e][0], qb[t][2 * j + e][1]);
+                        else
+                            mma16816(s[u][t], a[u][e], qb[t][2 * j + e][0], qb[t][2 * j + e][1]);
         }
-        // A pair that every row sees whole needs no mask.
-        const int i0 = j0 + (warp + k * W) * step, key0 = block_of(i0) * kCacheBlock;
-        const int key1 = i0 + 1 < j1 ? block_of(i0 + 1) * kCacheBlock : tile.n; // no token is there
-        const bool whole = !bad && max(key0, key1) + kCacheBlock <= limit_all &&
-                           (min(key0, key1) >= floor_all || max(key0, key1) + kCacheBlock <= p.sinks);
-        if (!whole) {
+        if (bad || i0 < whole0 || i0 + 1 >= whole1) {
+            const int key0 = block_of(i0) * kCacheBlock;
+            const int key1 = i0 + 1 < j1 ? block_of(i0 + 1) * kCacheBlock : tile.n; // no token is there
+            // Values that no row sees may be anything: their scales become zeros.
+            for (int x = lane; x < 2 * kCacheBlock * B::G; x += 32) {
+                const int u = x / (kCacheBlock * B::G), r = x / B::G % kCacheBlock, token = (u ? key1 : key0) + r;
+                if ((bad >> u & 1u) || token >= tile.high || (token < tile.low && token >= tile.sink))
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + u * S::BLOCK + B::VALUE_SCALES + 2 * B::value_scale(r, x % B::G)),
+                                 "h"(static_cast<uint16_t>(0))
+                                 : "memory");
+            }
+            fence_proxy_async_smem(); // the next copy's writes come after these
+            __syncwarp();
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -426,19 +456,6 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
         // O^T: a lane's scales are those of tokens 2c, 2c + 1 and 2c + 8, 2c + 9.
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-            if (!whole) { // values that no row sees may be anything: their scale is zero
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    keep[h] = 0;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int token = (u ? key1 : key0) + 2 * c + 8 * h + e;
-                        if (!(bad >> u & 1u) && token < tile.high && (token >= tile.low || token < tile.sink))
-                            keep[h] |= 0xffffu << (16 * e);
-                    }
-                }
-            }
 #pragma unroll
             for (int v = 0; v < D / 16 / B::W; ++v) {
                 uint32_t vw[B::W];
@@ -447,10 +464,6 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
                 for (int j = 0; j < B::W; j += 2) {
                     uint32_t vs[2]; // one group of 32 columns
                     shared_words<2>(at + u * S::BLOCK + B::VALUE_SCALES + 2 * B::value_scale(2 * c, (v * B::W + j) / 2), vs);
-                    if (!whole) {
-                        vs[0] &= keep[0];
-                        vs[1] &= keep[1];
-                    }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         uint32_t x[4];
@@ -464,7 +477,6 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
             }
         }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads(); // the ring becomes the parts' place
     float(*part_m)[ROWS] = reinterpret_cast<float(*)[ROWS]>(smem), (*part_l)[ROWS] = part_m + W;
     cta_m = part_l[W];
@@ -491,26 +503,46 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
             }
         }
     __syncthreads();
-    for (int x = threadIdx.x; x < ROWS * D; x += W * 32) {
-        const int r = x / D, col = x - r * D;
-        float mx = part_m[0][r];
+    if (threadIdx.x < ROWS) {
+        const int r = threadIdx.x;
+        float mx = part_m[0][r], l = 0.f;
 #pragma unroll
         for (int w = 1; w < W; ++w)
             mx = fmaxf(mx, part_m[w][r]);
         const float base = mx == -INFINITY ? 0.f : mx;
-        float l = 0.f, v = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            const float f = exp2f(part_m[w][r] - base);
+            const float f = ex2_approx(part_m[w][r] - base);
             l += f * part_l[w][r];
-            v += f * part_o[w][r][col];
+            part_m[w][r] = f; // the warp's weight from here on
         }
-        part_o[0][r][col] = v;
-        if (col == 0) {
-            cta_m[r] = mx;
-            cta_l[r] = l;
-        }
+        cta_m[r] = mx;
+        cta_l[r] = l;
     }
+    __syncthreads();
+    for (int x = threadIdx.x * 4; x < ROWS * D; x += W * 32 * 4) {
+        const int r = x / D, col = x - r * D;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float f = part_m[w][r];
+            const float4 o4 = *reinterpret_cast<const float4 *>(&part_o[w][r][col]);
+            v.x += f * o4.x;
+            v.y += f * o4.y;
+            v.z += f * o4.z;
+            v.w += f * o4.w;
+        }
+        *reinterpret_cast<float4 *>(&part_o[0][r][col]) = v;
+    }
+}
+
+// Barriers of the stages: each waits for the two lanes that copy a pair's blocks.
+template <int N> __device__ __forceinline__ void make_bars(uint64_t *bars) {
+    if (threadIdx.x < N)
+        mbar_init(bars + threadIdx.x, 2);
+    fence_mbarrier_init();
+    fence_proxy_async_smem();
+    __syncthreads();
 }
 
 // A cluster for each tile.
@@ -519,13 +551,16 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
     window_e2m1_cluster_kernel(const __grid_constant__ TokensParams p) {
     using S = TokensShape<D, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t bars[S::WARPS * S::STAGES];
     const int parts = p.parts, pair = blockIdx.x / parts, part = blockIdx.x - pair * parts;
     const int b = pair / p.kv_heads, kvh = pair - b * p.kv_heads;
     int n, m;
     lengths_of(p, b, n, m);
     const Tile tile = tile_of<S::ROWS>(p, n, m, blockIdx.y);
     float *cta_m, *cta_l, (*part_o)[S::ROWS][D + 4];
-    attend<D, NT, BF16>(p, tile, b, kvh, 2 * part, tile.blocks, 2 * parts, smem, cta_m, cta_l, part_o);
+    uint32_t phases = 0;
+    make_bars<S::WARPS * S::STAGES>(bars);
+    attend<D, NT, BF16>(p, tile, b, kvh, 2 * part, tile.blocks, 2 * parts, smem, bars, phases, cta_m, cta_l, part_o);
     if (parts > 1)
         cluster_sync();
     else
@@ -556,6 +591,16 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
         cluster_sync(); // no CTA leaves while another reads its part
 }
 
+// Quotients that mostly need 32 bits only.
+__device__ __forceinline__ int quotient(long long a, long long b) {
+    return (a | b) >> 32 ? static_cast<int>(a / b) : static_cast<int>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+}
+// Blocks of a CTA where `ctas` share `total`.
+__device__ __forceinline__ long long share_of(long long total, int ctas) {
+    const long long up = total + ctas - 1;
+    return up >> 32 ? up / ctas : static_cast<long long>(static_cast<uint32_t>(up) / static_cast<uint32_t>(ctas));
+}
+
 // Sums over the CTA's threads; every thread gets the result.
 template <int WARPS> __device__ __forceinline__ long long cta_sum(long long v, long long *place) {
 #pragma unroll
@@ -580,8 +625,11 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
     using S = TokensShape<D, NT>;
     constexpr int THREADS = S::WARPS * 32;
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t bars[S::WARPS * S::STAGES];
     __shared__ long long place[S::WARPS], start_at;
     __shared__ int start_b;
+    uint32_t phases = 0;
+    make_bars<S::WARPS * S::STAGES>(bars);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // Each thread has a run of sequences; the thread in whose run this CTA's first block is finds the sequence.
     const int run = (p.batch + THREADS - 1) / THREADS, b0 = threadIdx.x * run, b1 = min(p.batch, b0 + run);
@@ -606,7 +654,7 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
         total += place[w];
     }
     before -= mine;
-    const long long per = (total + gridDim.x - 1) / gridDim.x;
+    const long long per = share_of(total, gridDim.x);
     const long long from = blockIdx.x * per, to = min(total, from + per);
     if (from >= to)
         return;
@@ -638,7 +686,7 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
                     continue;
                 const int j0 = static_cast<int>(max(from - begin, 0ll)), j1 = static_cast<int>(min(to - begin, static_cast<long long>(size)));
                 float *cta_m, *cta_l, (*part_o)[S::ROWS][D + 4];
-                attend<D, NT, BF16>(p, tile, b, kvh, j0, min(j1, tile.blocks), 2, smem, cta_m, cta_l, part_o);
+                attend<D, NT, BF16>(p, tile, b, kvh, max(j0 - kTileCost, 0), j1 - kTileCost, 2, smem, bars, phases, cta_m, cta_l, part_o);
                 __syncthreads();
                 if (j0 == 0 && j1 == size) {
                     for (int x = threadIdx.x; x < S::ROWS * D; x += THREADS) {
@@ -656,62 +704,98 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
                         *reinterpret_cast<float4 *>(slot + 2 * S::ROWS + x) =
                             *reinterpret_cast<const float4 *>(&part_o[0][x / D][x % D]);
                 }
+                fence_proxy_async_smem();
                 __syncthreads(); // the parts' place becomes the ring again
             }
     }
 }
 
-// Joins the parts of the tiles that several CTAs share: a CTA for each tile.
-template <int D, int NT> __global__ void __launch_bounds__(256) window_e2m1_join_kernel(const __grid_constant__ TokensParams p, int ctas) {
+// Joins the parts of the tiles that several CTAs share: a CTA for each tile and two of its rows
+// (with eight, few tiles of many parts met in few SMs: 131072 keys x 8 heads 45 -> JOIN us).  A
+// part's weight is worked out once for a row; SHARES threads share a column's parts.
+constexpr int kJoinThreads = 256, kJoinParts = 512, kJoinRows = 2;
+template <int D, int NT>
+__global__ void __launch_bounds__(kJoinThreads) window_e2m1_join_kernel(const __grid_constant__ TokensParams p, int ctas) {
     using S = TokensShape<D, NT>;
-    __shared__ long long place[8];
+    constexpr int WARPS = kJoinThreads / 32, FOURS = kJoinRows * D / 4, SHARES = kJoinThreads / FOURS;
+    __shared__ long long place[WARPS];
+    __shared__ float weight[kJoinRows][kJoinParts], sums[kJoinRows][kJoinParts], total_l[kJoinRows];
+    __shared__ __align__(16) float share[SHARES - 1][kJoinRows * D];
     const int i = blockIdx.x % p.tiles, pair = blockIdx.x / p.tiles, b = pair / p.kv_heads, kvh = pair - b * p.kv_heads;
     long long before = 0, total = 0;
-    for (int x = threadIdx.x; x < p.batch; x += 256) {
+    for (int x = threadIdx.x; x < p.batch; x += kJoinThreads) {
         const long long size = static_cast<long long>(listed_of<S::ROWS>(p, x)) * p.kv_heads;
         total += size;
         before += x < b ? size : 0;
     }
-    total = cta_sum<8>(total, place);
-    before = cta_sum<8>(before, place);
+    total = cta_sum<WARPS>(total, place);
+    before = cta_sum<WARPS>(before, place);
     int n, m;
     lengths_of(p, b, n, m);
-    const long long per = max(1ll, (total + ctas - 1) / ctas);
+    const long long per = max(1ll, share_of(total, ctas));
     before += static_cast<long long>(listed_of<S::ROWS>(p, b)) * kvh;
     for (int x = 0; x < i; ++x)
         before += listed(tile_of<S::ROWS>(p, n, m, x));
     const Tile tile = tile_of<S::ROWS>(p, n, m, i);
-    const int size = listed(tile);
-    const int first = static_cast<int>(before / per), last = static_cast<int>((before + size - 1) / per);
+    const int size = listed(tile), row0 = blockIdx.y * kJoinRows, rows = min(kJoinRows, tile.rows - row0);
+    const int first = quotient(before, per), parts = quotient(before + max(size, 1) - 1, per) - first + 1;
     asm volatile("griddepcontrol.wait;" ::: "memory"); // every CTA: this grid's end stands for the list's as well
-    if (size == 0 || first == last)
+    if (size == 0 || parts == 1 || rows <= 0)
         return;
     // The tile is the last one of its first CTA, unless it begins with it, and the first one of the others.
-    const float *slot0 = p.parts_at + (2ll * first + (before > first * per)) * S::SLOT;
-    auto slot = [&](int c) { return c == first ? slot0 : p.parts_at + 2ll * c * S::SLOT; };
-    for (int x = threadIdx.x * 4; x < tile.rows * D; x += 1024) {
-        const int r = x / D, col = x - r * D;
-        float mx = -INFINITY;
-#pragma unroll 8
-        for (int c = first; c <= last; ++c)
-            mx = fmaxf(mx, slot(c)[2 * r]);
+    const float *from = p.parts_at + 2ll * first * S::SLOT;
+    const int skip = before > first * per ? S::SLOT : 0;
+    auto slot = [&](int c) { return from + 2ll * c * S::SLOT + (c == 0 ? skip : 0); };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp < rows) {
+        float mx = -INFINITY, l = 0.f;
+        for (int c = lane; c < parts; c += 32) {
+            const float2 ml = *reinterpret_cast<const float2 *>(slot(c) + 2 * (row0 + warp));
+            weight[warp][c] = ml.x;
+            sums[warp][c] = ml.y;
+            mx = fmaxf(mx, ml.x);
+        }
+#pragma unroll
+        for (int x = 16; x; x >>= 1)
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
         const float base = mx == -INFINITY ? 0.f : mx;
-        float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c = lane; c < parts; c += 32) {
+            const float f = ex2_approx(weight[warp][c] - base);
+            weight[warp][c] = f;
+            l += f * sums[warp][c];
+        }
+#pragma unroll
+        for (int x = 16; x; x >>= 1)
+            l += __shfl_xor_sync(0xffffffffu, l, x);
+        if (lane == 0)
+            total_l[warp] = l;
+    }
+    __syncthreads();
+    const int of = threadIdx.x / FOURS, x = threadIdx.x % FOURS * 4, r = x / D, col = x % D;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (of < SHARES && r < rows) {
 #pragma unroll 8
-        for (int c = first; c <= last; ++c) {
-            const float2 ml = *reinterpret_cast<const float2 *>(slot(c) + 2 * r);
-            const float4 o = *reinterpret_cast<const float4 *>(slot(c) + 2 * S::ROWS + x);
-            const float f = exp2f(ml.x - base);
-            l += f * ml.y;
+        for (int c = of; c < parts; c += SHARES) {
+            const float4 o = *reinterpret_cast<const float4 *>(slot(c) + 2 * S::ROWS + row0 * D + x);
+            const float f = weight[r][c];
             v[0] += f * o.x;
             v[1] += f * o.y;
             v[2] += f * o.z;
             v[3] += f * o.w;
         }
+        if (of)
+            *reinterpret_cast<float4 *>(&share[of - 1][x]) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+    __syncthreads();
+    if (of == 0 && r < rows) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int k = 0; k < SHARES - 1; ++k)
+                v[e] += share[k][x + e];
             if (col + e < p.hd)
-                store_out(p, tile, b, kvh, r, col + e, v[e], l);
+                store_out(p, tile, b, kvh, row0 + r, col + e, v[e], total_l[r]);
+        }
     }
 }
 
@@ -748,8 +832,8 @@ template <int D, int NT, bool BF16> int launch_rows(const TokensParams &p, int c
     if (e != cudaSuccess)
         return static_cast<int>(e);
     // The join is set up while the list's kernel runs, and waits for its end before it reads the parts.
-    cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.kv_heads * p.tiles);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.kv_heads * p.tiles, S::ROWS / kJoinRows);
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -814,6 +898,7 @@ int window_e2m1_tokens_launch(const WindowE2m1Args &a, cudaStream_t stream) {
     p.q_lengths = c.q_lengths;
     p.kv_heads = c.kv_heads;
     p.group = a.heads / c.kv_heads;
+    p.group_inv = (65536u + p.group - 1) / p.group;
     p.q_len = c.q_len;
     p.kv_len = a.kv_len;
     p.hd = c.hd;
@@ -828,6 +913,7 @@ int window_e2m1_tokens_launch(const WindowE2m1Args &a, cudaStream_t stream) {
     p.tiles = split.tiles;
     p.batch = c.batch;
     p.parts_at = static_cast<float *>(a.workspace);
+    p.err = a.err;
     const bool bf16 = a.dtype == kBF16;
     switch (cache_width(c.hd)) {
     case 32:
@@ -844,7 +930,7 @@ int window_e2m1_tokens_launch(const WindowE2m1Args &a, cudaStream_t stream) {
 // Few rows read the cache as it is; for others the keys and values go back to 16 bits in the
 // workspace (exactly), and the prompts' kernel reads them.
 static bool few_rows(const WindowE2m1Args &a) {
-    return (static_cast<long long>(a.heads / a.cache.kv_heads) * a.cache.q_len + 15) / 16 <= 4;
+    return static_cast<long long>(a.heads / a.cache.kv_heads) * a.cache.q_len <= kMostRows;
 }
 
 size_t window_e2m1_workspace(const WindowE2m1Args &a) {
