@@ -34,6 +34,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace omni_b200 {
 namespace {
@@ -186,11 +187,23 @@ __device__ __forceinline__ void store_out(const TokensParams &p, const Tile &t, 
         static_cast<__half *>(p.out)[to] = __float2half_rn(v);
 }
 
+// Where a warp is in its ring: the stage of the next pair, and the parity of its barrier.
+template <int ST> struct Turn {
+    int stage = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++stage == ST) {
+            stage = 0;
+            parity ^= 1u;
+        }
+    }
+};
+
 // The CTA's softmax over blocks j0, j0 + step, ... pairs of them, below j1 of a tile: leaves
 // m, l of the rows in cta_m and cta_l and the outputs in part_o[0].
 template <int D, int NT, bool BF16>
 __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, int b, int kvh, int j0, int j1, int step,
-                                       uint8_t *smem, uint64_t *bars, uint32_t &phases, float *&cta_m, float *&cta_l, float (*&part_o)[8 * NT][D + 4]) {
+                                       uint8_t *smem, uint64_t *bars, Turn<TokensShape<D, NT>::STAGES> &at_turn, float *&cta_m, float *&cta_l, float (*&part_o)[8 * NT][D + 4]) {
     using S = TokensShape<D, NT>;
     using B = CacheBlock<D>;
     using C = Columns<D>;
@@ -201,42 +214,43 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
     const uint32_t ring = smem_u32(smem) + warp * ST * S::STAGE;
     uint64_t *full = bars + warp * ST; // a stage's two copies have landed
     auto block_of = [&](int i) { return i < tile.sink_blocks ? i : tile.begin + i - tile.sink_blocks; };
+    // Pairs that every row sees whole need no mask: blocks [whole0, whole1) (sinks are left to
+    // it, and so is everything once a page is none of the cache's).
+    const int limit_all = min(tile.n, tile.first + p.right + 1), floor_all = p.window > 0 ? tile.last - p.window + 1 : 0;
+    const int ahead = tile.sink_blocks - tile.begin;
+    const int whole0 = max(tile.sink_blocks, (max(floor_all, 0) + kCacheBlock - 1) / kCacheBlock + ahead);
+    int whole1 = min(j1, max(limit_all, 0) / kCacheBlock + ahead) - 1;
+
     // Lane l knows where block l % 2 of pair k + l / 2 is, k a multiple of 16 (0: nowhere), and
-    // copies it; whether a block's page is none of the cache's; the pages of the next 16 pairs.
+    // copies it; and the pages of the next 16 pairs.
     unsigned long long place = 0;
-    uint32_t unpaged = 0;
     int page_next = 0, within_next = 0;
     auto look_up = [&](int k) {
         const int i = j0 + (warp + (k + (lane >> 1)) * W) * step + (lane & 1);
         page_next = i < j1 ? p.cache.page_of(b, block_of(i), within_next) : -2;
     };
-    uint32_t bad_bits = 0; // two for each stage
     auto fetch = [&](int k, int stage) {
         if ((k & 15) == 0) {
-            unpaged = __ballot_sync(0xffffffffu, page_next == -1);
+            if (__any_sync(0xffffffffu, page_next == -1))
+                whole1 = -1;
             place = page_next >= 0 ? reinterpret_cast<unsigned long long>(p.cache.block_at(page_next, kvh, within_next, S::BLOCK)) : 0ull;
             look_up(k + 16);
         }
-        if (unpaged) // rare: no such page
-            bad_bits = (bad_bits & ~(3u << (2 * stage))) | (unpaged >> (2 * (k & 15)) & 3u) << (2 * stage);
-        else
-            bad_bits &= ~(3u << (2 * stage));
         if ((lane >> 1) == (k & 15)) {
-            const uint32_t bytes = place ? S::BLOCK : 0;
-            mbar_arrive_expect_tx(full + stage, bytes);
+            mbar_arrive_expect_tx(full + stage, place ? S::BLOCK : 0);
             if (place)
                 copy_piece(ring + stage * S::STAGE + (lane & 1) * S::BLOCK, place, S::BLOCK, smem_u32(full + stage));
         }
     };
+    auto after = [](int stage, int n) { return stage + n >= ST ? stage + n - ST : stage + n; };
     const int pairs = j1 - j0 > warp * step ? (j1 - j0 - warp * step + W * step - 1) / (W * step) : 0;
     look_up(0);
 #pragma unroll
     for (int k = 0; k < ST - 1; ++k)
         if (k < pairs)
-            fetch(k, k);
+            fetch(k, after(at_turn.stage, k));
 
     // The queries as B operands, and the masks of columns 2c and 2c + 1.
-    const int limit_all = min(tile.n, tile.first + p.right + 1), floor_all = p.window > 0 ? tile.last - p.window + 1 : 0;
     uint32_t qb[NT][D / 16][2];
     float factor[NT][2]; // from S to log2 units
     int limit[NT][2], floor_[NT][2];
@@ -308,29 +322,9 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
     for (int t = 0; t < NT; ++t)
         none[t][0] = none[t][1] = true;
 
-    // Pairs that every row sees whole need no mask: blocks [whole0, whole1) (sinks are left to it).
-    const int ahead = tile.sink_blocks - tile.begin;
-    const int whole0 = max(tile.sink_blocks, (max(floor_all, 0) + kCacheBlock - 1) / kCacheBlock + ahead);
-    const int whole1 = min(j1, max(limit_all, 0) / kCacheBlock + ahead);
-    int i0 = j0 + warp * step, left = ST;
-    for (int k = 0, stage = 0; k < pairs; ++k, i0 += W * step, stage = stage + 1 == ST ? 0 : stage + 1) {
-        __syncwarp(); // every lane is done with the last pair, whose place is the next copy's
-        const uint32_t bad = bad_bits >> (2 * stage) & 3u;
-        if (k + ST - 1 < pairs)
-            fetch(k + ST - 1, stage == 0 ? ST - 1 : stage - 1);
-        if (!mbar_wait(full + stage, phases >> stage & 1u, p.err, kErrWaitK)) {
-            // Gives up, but not before its copies under way are over, or had their time.
-            for (; k < pairs && left > 0; ++k, --left, stage = stage + 1 == ST ? 0 : stage + 1) {
-                const uint64_t start = globaltimer_ns();
-                while (!mbar_try_wait(smem_u32(full + stage), phases >> stage & 1u) && globaltimer_ns() - start < kWaitLimitNs) {
-                }
-                phases ^= 1u << stage;
-            }
-            break;
-        }
-        phases ^= 1u << stage;
-        const uint32_t at = ring + stage * S::STAGE;
-
+    // One pair, at `at` in the ring.  (Two instances, so that pairs without a mask carry none of its instructions.)
+    auto attend_pair = [&](auto masked, uint32_t at, int i0) {
+        constexpr bool MASKED = decltype(masked)::value;
         // S^T: tokens g (rows 0 to 7) and g + 8 of each block; the blocks' products take turns,
         // so that none waits for the one before it.
         float s[2][NT][4];
@@ -380,7 +374,10 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
                         else
                             mma16816(s[u][t], a[u][e], qb[t][2 * j + e][0], qb[t][2 * j + e][1]);
         }
-        if (bad || i0 < whole0 || i0 + 1 >= whole1) {
+        if constexpr (MASKED) {
+            int within;
+            const uint32_t bad = (p.cache.page_of(b, block_of(i0), within) < 0 ? 1u : 0u) |
+                                 (i0 + 1 < j1 && p.cache.page_of(b, block_of(i0 + 1), within) < 0 ? 2u : 0u);
             const int key0 = block_of(i0) * kCacheBlock;
             const int key1 = i0 + 1 < j1 ? block_of(i0 + 1) * kCacheBlock : tile.n; // no token is there
             // Values that no row sees may be anything: their scales become zeros.
@@ -476,6 +473,30 @@ __device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, 
                 }
             }
         }
+    };
+
+    int i0 = j0 + warp * step;
+    for (int k = 0; k < pairs; ++k, i0 += W * step) {
+        __syncwarp(); // every lane is done with the last pair, whose place is the next copy's
+        if (k + ST - 1 < pairs)
+            fetch(k + ST - 1, after(at_turn.stage, ST - 1));
+        const int stage = at_turn.stage;
+        if (!mbar_wait(full + stage, at_turn.parity, p.err, kErrWaitK)) {
+            // Gives up, but not before its copies under way are over, or had their time.
+            for (const int end = min(pairs, k + ST); k < end; ++k) {
+                const uint64_t start = globaltimer_ns();
+                while (!mbar_try_wait(smem_u32(full + at_turn.stage), at_turn.parity) && globaltimer_ns() - start < kWaitLimitNs) {
+                }
+                at_turn.next();
+            }
+            break;
+        }
+        at_turn.next();
+        const uint32_t at = ring + stage * S::STAGE;
+        if (i0 < whole0 || i0 >= whole1)
+            attend_pair(std::true_type(), at, i0);
+        else
+            attend_pair(std::false_type(), at, i0);
     }
     __syncthreads(); // the ring becomes the parts' place
     float(*part_m)[ROWS] = reinterpret_cast<float(*)[ROWS]>(smem), (*part_l)[ROWS] = part_m + W;
@@ -558,9 +579,9 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
     lengths_of(p, b, n, m);
     const Tile tile = tile_of<S::ROWS>(p, n, m, blockIdx.y);
     float *cta_m, *cta_l, (*part_o)[S::ROWS][D + 4];
-    uint32_t phases = 0;
+    Turn<S::STAGES> at_turn;
     make_bars<S::WARPS * S::STAGES>(bars);
-    attend<D, NT, BF16>(p, tile, b, kvh, 2 * part, tile.blocks, 2 * parts, smem, bars, phases, cta_m, cta_l, part_o);
+    attend<D, NT, BF16>(p, tile, b, kvh, 2 * part, tile.blocks, 2 * parts, smem, bars, at_turn, cta_m, cta_l, part_o);
     if (parts > 1)
         cluster_sync();
     else
@@ -628,7 +649,7 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
     __shared__ uint64_t bars[S::WARPS * S::STAGES];
     __shared__ long long place[S::WARPS], start_at;
     __shared__ int start_b;
-    uint32_t phases = 0;
+    Turn<S::STAGES> at_turn;
     make_bars<S::WARPS * S::STAGES>(bars);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // Each thread has a run of sequences; the thread in whose run this CTA's first block is finds the sequence.
@@ -686,7 +707,7 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
                     continue;
                 const int j0 = static_cast<int>(max(from - begin, 0ll)), j1 = static_cast<int>(min(to - begin, static_cast<long long>(size)));
                 float *cta_m, *cta_l, (*part_o)[S::ROWS][D + 4];
-                attend<D, NT, BF16>(p, tile, b, kvh, max(j0 - kTileCost, 0), j1 - kTileCost, 2, smem, bars, phases, cta_m, cta_l, part_o);
+                attend<D, NT, BF16>(p, tile, b, kvh, max(j0 - kTileCost, 0), j1 - kTileCost, 2, smem, bars, at_turn, cta_m, cta_l, part_o);
                 __syncthreads();
                 if (j0 == 0 && j1 == size) {
                     for (int x = threadIdx.x; x < S::ROWS * D; x += THREADS) {
