@@ -62,12 +62,12 @@ struct TokensParams {
 template <int D, int NT> struct TokensShape {
     static constexpr int BLOCK = CacheBlock<D>::BYTES;
     static constexpr int WARPS = 8, CTAS = NT == 1 ? 2 : 1; // of an SM
-    static constexpr int STAGES = 3, STAGE = 2 * BLOCK;
+    static constexpr int STAGES = 2, STAGE = 2 * BLOCK;
     static constexpr int RING = WARPS * STAGES * STAGE;
     static constexpr int ROWS = 8 * NT;
-    // The parts' place at the end, over the ring: m, l of the warps and the CTA, outputs.
+    // The warps' results: m, l of each and of the CTA, outputs.
     static constexpr int PARTS = (2 * WARPS + 2) * ROWS * 4 + WARPS * ROWS * (D + 4) * 4;
-    static constexpr int SMEM = RING > PARTS ? RING : PARTS;
+    static constexpr int SMEM = RING + PARTS;
     static constexpr int SLOT = ROWS * (D + 2); // floats of a part in the workspace
 };
 
@@ -187,375 +187,402 @@ __device__ __forceinline__ void store_out(const TokensParams &p, const Tile &t, 
         static_cast<__half *>(p.out)[to] = __float2half_rn(v);
 }
 
-// Where a warp is in its ring: the stage of the next pair, and the parity of its barrier.
-template <int ST> struct Turn {
-    int stage = 0;
-    uint32_t parity = 0;
-    __device__ __forceinline__ void next() {
-        if (++stage == ST) {
-            stage = 0;
-            parity ^= 1u;
-        }
-    }
+// What a CTA does at a time: pairs of blocks j0, j0 + step, ... below j1 of a tile.  slot: where
+// its part goes in the workspace, or -1: it is the whole tile.  b < 0: there is nothing.
+struct Segment {
+    Tile tile;
+    int b, kvh, j0, j1, slot;
+    __device__ __forceinline__ int block_of(int i) const { return i < tile.sink_blocks ? i : tile.begin + i - tile.sink_blocks; }
 };
 
-// The CTA's softmax over blocks j0, j0 + step, ... pairs of them, below j1 of a tile: leaves
-// m, l of the rows in cta_m and cta_l and the outputs in part_o[0].
-template <int D, int NT, bool BF16>
-__device__ __forceinline__ void attend(const TokensParams &p, const Tile &tile, int b, int kvh, int j0, int j1, int step,
-                                       uint8_t *smem, uint64_t *bars, Turn<TokensShape<D, NT>::STAGES> &at_turn, float *&cta_m, float *&cta_l, float (*&part_o)[8 * NT][D + 4]) {
+// The warps' results in shared memory.
+template <int D, int NT> struct Parts {
+    using S = TokensShape<D, NT>;
+    float m[S::WARPS][S::ROWS]; // then the warps' weights
+    float l[S::WARPS][S::ROWS];
+    float cta_m[S::ROWS], cta_l[S::ROWS];
+    float o[S::WARPS][S::ROWS][D + 4];
+};
+
+template <int D, int NT, bool BF16> struct Worker {
     using S = TokensShape<D, NT>;
     using B = CacheBlock<D>;
     using C = Columns<D>;
-    constexpr int ROWS = S::ROWS, ST = S::STAGES, W = S::WARPS;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    static constexpr int ROWS = S::ROWS, ST = S::STAGES, W = S::WARPS;
+    static_assert(sizeof(Parts<D, NT>) == S::PARTS, "the parts' place");
 
-    // Blocks of pairs: this warp's pair k is blocks j0 + (warp + k W) step and the next one.
-    const uint32_t ring = smem_u32(smem) + warp * ST * S::STAGE;
-    uint64_t *full = bars + warp * ST; // a stage's two copies have landed
-    auto block_of = [&](int i) { return i < tile.sink_blocks ? i : tile.begin + i - tile.sink_blocks; };
-    // Pairs that every row sees whole need no mask: blocks [whole0, whole1) (sinks are left to
-    // it, and so is everything once a page is none of the cache's).
-    const int limit_all = min(tile.n, tile.first + p.right + 1), floor_all = p.window > 0 ? tile.last - p.window + 1 : 0;
-    const int ahead = tile.sink_blocks - tile.begin;
-    const int whole0 = max(tile.sink_blocks, (max(floor_all, 0) + kCacheBlock - 1) / kCacheBlock + ahead);
-    int whole1 = min(j1, max(limit_all, 0) / kCacheBlock + ahead) - 1;
-
+    const TokensParams &p;
+    const int step, warp, lane;
+    const uint32_t ring;
+    uint64_t *const full; // a stage's two copies have landed
+    // Where the warp is in its ring: the stage of the next pair, and the parity of its barrier.
+    int stage_at = 0;
+    uint32_t parity = 0;
+    // Of the segment that is read: pairs [whole0, whole1) every row sees whole, so they need no
+    // mask (sinks are left to it, and so is everything once a page is none of the cache's).
+    int whole0 = 0, whole1 = 0, pairs = 0;
     // Lane l knows where block l % 2 of pair k + l / 2 is, k a multiple of 16 (0: nowhere), and
     // copies it; and the pages of the next 16 pairs.
     unsigned long long place = 0;
     int page_next = 0, within_next = 0;
-    auto look_up = [&](int k) {
-        const int i = j0 + (warp + (k + (lane >> 1)) * W) * step + (lane & 1);
-        page_next = i < j1 ? p.cache.page_of(b, block_of(i), within_next) : -2;
-    };
-    auto fetch = [&](int k, int stage) {
+
+    __device__ __forceinline__ Worker(const TokensParams &p_, int step_, uint8_t *smem, uint64_t *bars)
+        : p(p_), step(step_), warp(threadIdx.x >> 5), lane(threadIdx.x & 31),
+          ring(smem_u32(smem) + (threadIdx.x >> 5) * ST * S::STAGE), full(bars + (threadIdx.x >> 5) * ST) {}
+
+    __device__ __forceinline__ void next_stage() {
+        if (++stage_at == ST) {
+            stage_at = 0;
+            parity ^= 1u;
+        }
+    }
+    __device__ __forceinline__ void look_up(const Segment &s, int k) {
+        const int i = s.j0 + (warp + (k + (lane >> 1)) * W) * step + (lane & 1);
+        page_next = i < s.j1 ? p.cache.page_of(s.b, s.block_of(i), within_next) : -2;
+    }
+    __device__ __forceinline__ void copy(const Segment &s, int k, int stage) {
         if ((k & 15) == 0) {
             if (__any_sync(0xffffffffu, page_next == -1))
                 whole1 = -1;
-            place = page_next >= 0 ? reinterpret_cast<unsigned long long>(p.cache.block_at(page_next, kvh, within_next, S::BLOCK)) : 0ull;
-            look_up(k + 16);
+            place = page_next >= 0 ? reinterpret_cast<unsigned long long>(p.cache.block_at(page_next, s.kvh, within_next, S::BLOCK)) : 0ull;
+            look_up(s, k + 16);
         }
         if ((lane >> 1) == (k & 15)) {
             mbar_arrive_expect_tx(full + stage, place ? S::BLOCK : 0);
             if (place)
                 copy_piece(ring + stage * S::STAGE + (lane & 1) * S::BLOCK, place, S::BLOCK, smem_u32(full + stage));
         }
-    };
-    auto after = [](int stage, int n) { return stage + n >= ST ? stage + n - ST : stage + n; };
-    const int pairs = j1 - j0 > warp * step ? (j1 - j0 - warp * step + W * step - 1) / (W * step) : 0;
-    look_up(0);
+    }
+    // Begins a segment: asks for its first pages, and then for its first blocks.
+    __device__ __forceinline__ void first_pages(const Segment &s) {
+        const Tile &tile = s.tile;
+        const int limit_all = min(tile.n, tile.first + p.right + 1), floor_all = p.window > 0 ? tile.last - p.window + 1 : 0;
+        const int ahead = tile.sink_blocks - tile.begin;
+        whole0 = max(tile.sink_blocks, (max(floor_all, 0) + kCacheBlock - 1) / kCacheBlock + ahead);
+        whole1 = min(s.j1, max(limit_all, 0) / kCacheBlock + ahead) - 1;
+        const int mine = s.j1 - s.j0 - warp * step;
+        pairs = mine > 0 ? (mine + W * step - 1) / (W * step) : 0;
+        look_up(s, 0);
+    }
+    __device__ __forceinline__ void first_copies(const Segment &s) {
 #pragma unroll
-    for (int k = 0; k < ST - 1; ++k)
-        if (k < pairs)
-            fetch(k, after(at_turn.stage, k));
+        for (int k = 0; k < ST - 1; ++k)
+            if (k < pairs)
+                copy(s, k, (stage_at + k) % ST);
+    }
 
-    // The queries as B operands, and the masks of columns 2c and 2c + 1.
-    uint32_t qb[NT][D / 16][2];
-    float factor[NT][2]; // from S to log2 units
-    int limit[NT][2], floor_[NT][2];
+    // The segment's softmax, the warp's share of it, to `parts`.  `ahead()` is called when its
+    // last block has been read.
+    template <typename F> __device__ __forceinline__ void attend(const Segment &seg, Parts<D, NT> &parts, F &&ahead) {
+        const Tile &tile = seg.tile;
+        const int g = lane >> 2, c = lane & 3, j1 = seg.j1;
+        // The queries as B operands, and the masks of columns 2c and 2c + 1.
+        uint32_t qb[NT][D / 16][2];
+        float factor[NT][2]; // from S to log2 units
+        int limit[NT][2], floor_[NT][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int r = tile.row0 + 8 * t + g;
-        const bool real = 8 * t + g < tile.rows;
-        const int query = query_of(p, r);
-        const uint16_t *q = p.q + b * p.qs[0] + (kvh * p.group + r - query * p.group) * p.qs[1] + query * p.qs[2];
-        uint4 w[C::WORDS];
-        uint32_t top2 = 0;
-#pragma unroll
-        for (int j = 0; j < C::WORDS; ++j) {
-            const int col = C::first(j, c);
-            w[j] = real && col < p.hd ? *reinterpret_cast<const uint4 *>(q + col) : make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t *x = &w[j].x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                top2 = __vmaxu2(top2, x[e] & 0x7fff7fffu);
-        }
-        int exponent = 0; // q is multiplied by 2^exponent
-        if constexpr (BF16) {
-            uint32_t top = max(top2 & 0xffffu, top2 >> 16);
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // The largest element is in [2^(e - 127), 2^(e - 126)); a row that is not finite stays as it is.
-            const int e = static_cast<int>(top >> 7);
-            exponent = e == 255 ? 0 : min(141 - e, 120);
-            const float times = __uint_as_float(static_cast<uint32_t>(exponent + 127) << 23);
+        for (int t = 0; t < NT; ++t) {
+            const int r = tile.row0 + 8 * t + g;
+            const bool real = 8 * t + g < tile.rows;
+            const int query = query_of(p, r);
+            const uint16_t *q = p.q + seg.b * p.qs[0] + (seg.kvh * p.group + r - query * p.group) * p.qs[1] + query * p.qs[2];
+            uint4 w[C::WORDS];
+            uint32_t top2 = 0;
 #pragma unroll
             for (int j = 0; j < C::WORDS; ++j) {
-                uint32_t *x = &w[j].x;
+                const int col = C::first(j, c);
+                w[j] = real && col < p.hd ? *reinterpret_cast<const uint4 *>(q + col) : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t *x = &w[j].x;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    x[i] = pack_f16(__uint_as_float(x[i] << 16) * times, __uint_as_float(x[i] & 0xffff0000u) * times);
+                for (int e = 0; e < 4; ++e)
+                    top2 = __vmaxu2(top2, x[e] & 0x7fff7fffu);
             }
-        }
+            int exponent = 0; // q is multiplied by 2^exponent
+            if constexpr (BF16) {
+                uint32_t top = max(top2 & 0xffffu, top2 >> 16);
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // The largest element is in [2^(e - 127), 2^(e - 126)); a row that is not finite stays as it is.
+                const int e = static_cast<int>(top >> 7);
+                exponent = e == 255 ? 0 : min(141 - e, 120);
+                const float times = __uint_as_float(static_cast<uint32_t>(exponent + 127) << 23);
 #pragma unroll
-        for (int j = 0; j < C::WORDS; ++j) {
-            qb[t][2 * j][0] = w[j].x;
-            qb[t][2 * j][1] = w[j].y;
-            qb[t][2 * j + 1][0] = w[j].z;
-            qb[t][2 * j + 1][1] = w[j].w;
-        }
+                for (int j = 0; j < C::WORDS; ++j) {
+                    uint32_t *x = &w[j].x;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int col = 8 * t + 2 * c + h, pos = tile.pos0 + query_of(p, tile.row0 + col);
-            const int of_col = __shfl_sync(0xffffffffu, exponent, 4 * (2 * c + h));
-            // Not 0, so that a hidden key's -inf stays -inf.
-            factor[t][h] = fmaxf(p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - of_col) << 23), 1.4e-45f);
-            limit[t][h] = col < tile.rows ? min(tile.n, pos + p.right + 1) : tile.n; // a row that is none: anything finite
-            floor_[t][h] = col < tile.rows && p.window > 0 ? pos - p.window + 1 : 0;
-        }
-    }
-
-    float o[NT][D / 16][4];
-    float ref[NT][2], sum[NT][2], bar[NT][2]; // bar: what a score of S must not be above
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int x = 0; x < D / 16; ++x)
-            o[t][x][0] = o[t][x][1] = o[t][x][2] = o[t][x][3] = 0.f;
-        ref[t][0] = ref[t][1] = 0.f;
-        bar[t][0] = bar[t][1] = -INFINITY;
-        sum[t][0] = sum[t][1] = 0.f;
-    }
-    bool none[NT][2]; // no score yet
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-        none[t][0] = none[t][1] = true;
-
-    // One pair, at `at` in the ring.  (Two instances, so that pairs without a mask carry none of its instructions.)
-    auto attend_pair = [&](auto masked, uint32_t at, int i0) {
-        constexpr bool MASKED = decltype(masked)::value;
-        // S^T: tokens g (rows 0 to 7) and g + 8 of each block; the blocks' products take turns,
-        // so that none waits for the one before it.
-        float s[2][NT][4];
-        uint32_t kw[2][2][C::WORDS], scales[2][C::TOGETHER ? 1 : C::WORDS];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t row = at + u * S::BLOCK + B::KEYS + (g + 8 * h) * (D / 2);
-                if constexpr (C::TOGETHER)
-                    shared_words<C::WORDS>(row + c * 4 * C::WORDS, kw[u][h]);
-                else
-#pragma unroll
-                    for (int j = 0; j < C::WORDS; ++j)
-                        shared_words<1>(row + j * 16 + c * 4, &kw[u][h][j]);
-            }
-#pragma unroll
-            for (int j = 0; j < (C::TOGETHER ? 1 : C::WORDS); ++j) // both tokens' scales of the lane's group
-                shared_words<1>(at + u * S::BLOCK + B::KEY_SCALES + 2 * B::key_scale(g, C::first(j, c) / 32), &scales[u][j]);
-        }
-#pragma unroll
-        for (int j = 0; j < C::WORDS; ++j) {
-            uint32_t a[2][2][4];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint32_t both = scales[u][C::TOGETHER ? 0 : j];
-                const uint32_t s_g = __byte_perm(both, 0, 0x1010), s_g8 = __byte_perm(both, 0, 0x3232);
-                uint32_t x[4], y[4];
-                f16x8(kw[u][0][j], x);
-                f16x8(kw[u][1][j], y);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    a[u][e][0] = hmul2(x[2 * e], s_g);
-                    a[u][e][1] = hmul2(y[2 * e], s_g8);
-                    a[u][e][2] = hmul2(x[2 * e + 1], s_g);
-                    a[u][e][3] = hmul2(y[2 * e + 1], s_g8);
+                    for (int i = 0; i < 4; ++i)
+                        x[i] = pack_f16(__uint_as_float(x[i] << 16) * times, __uint_as_float(x[i] & 0xffff0000u) * times);
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        if (j == 0 && e == 0)
-                            mma16816_first(s[u][t], a[u][e], qb[t][2 * j + e][0], qb[t][2 * j + e][1]);
-                        else
-                            mma16816(s[u][t], a[u][e], qb[t][2 * j + e][0], qb[t][2 * j + e][1]);
-        }
-        if constexpr (MASKED) {
-            int within;
-            const uint32_t bad = (p.cache.page_of(b, block_of(i0), within) < 0 ? 1u : 0u) |
-                                 (i0 + 1 < j1 && p.cache.page_of(b, block_of(i0 + 1), within) < 0 ? 2u : 0u);
-            const int key0 = block_of(i0) * kCacheBlock;
-            const int key1 = i0 + 1 < j1 ? block_of(i0 + 1) * kCacheBlock : tile.n; // no token is there
-            // Values that no row sees may be anything: their scales become zeros.
-            for (int x = lane; x < 2 * kCacheBlock * B::G; x += 32) {
-                const int u = x / (kCacheBlock * B::G), r = x / B::G % kCacheBlock, token = (u ? key1 : key0) + r;
-                if ((bad >> u & 1u) || token >= tile.high || (token < tile.low && token >= tile.sink))
-                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + u * S::BLOCK + B::VALUE_SCALES + 2 * B::value_scale(r, x % B::G)),
-                                 "h"(static_cast<uint16_t>(0))
-                                 : "memory");
+            for (int j = 0; j < C::WORDS; ++j) {
+                qb[t][2 * j][0] = w[j].x;
+                qb[t][2 * j][1] = w[j].y;
+                qb[t][2 * j + 1][0] = w[j].z;
+                qb[t][2 * j + 1][1] = w[j].w;
             }
-            fence_proxy_async_smem(); // the next copy's writes come after these
-            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int col = 8 * t + 2 * c + h, pos = tile.pos0 + query_of(p, tile.row0 + col);
+                const int of_col = __shfl_sync(0xffffffffu, exponent, 4 * (2 * c + h));
+                // Not 0, so that a hidden key's -inf stays -inf.
+                factor[t][h] = fmaxf(p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - of_col) << 23), 1.4e-45f);
+                limit[t][h] = col < tile.rows ? min(tile.n, pos + p.right + 1) : tile.n; // a row that is none: anything finite
+                floor_[t][h] = col < tile.rows && p.window > 0 ? pos - p.window + 1 : 0;
+            }
+        }
+
+        float o[NT][D / 16][4];
+        float ref[NT][2], sum[NT][2], bar[NT][2]; // bar: what a score of S must not be above
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x)
+                o[t][x][0] = o[t][x][1] = o[t][x][2] = o[t][x][3] = 0.f;
+            ref[t][0] = ref[t][1] = 0.f;
+            bar[t][0] = bar[t][1] = -INFINITY;
+            sum[t][0] = sum[t][1] = 0.f;
+        }
+        bool none[NT][2]; // no score yet
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            none[t][0] = none[t][1] = true;
+
+        // One pair, at `at` in the ring.  (Two instances, so that pairs without a mask carry none of its instructions.)
+        auto attend_pair = [&](auto masked, uint32_t at, int i0) {
+            constexpr bool MASKED = decltype(masked)::value;
+            // S^T: tokens g (rows 0 to 7) and g + 8 of each block; the blocks' products take turns,
+            // so that none waits for the one before it.
+            float s[2][NT][4];
+            uint32_t kw[2][2][C::WORDS], scales[2][C::TOGETHER ? 1 : C::WORDS];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t row = at + u * S::BLOCK + B::KEYS + (g + 8 * h) * (D / 2);
+                    if constexpr (C::TOGETHER)
+                        shared_words<C::WORDS>(row + c * 4 * C::WORDS, kw[u][h]);
+                    else
+#pragma unroll
+                        for (int j = 0; j < C::WORDS; ++j)
+                            shared_words<1>(row + j * 16 + c * 4, &kw[u][h][j]);
+                }
+#pragma unroll
+                for (int j = 0; j < (C::TOGETHER ? 1 : C::WORDS); ++j) // both tokens' scales of the lane's group
+                    shared_words<1>(at + u * S::BLOCK + B::KEY_SCALES + 2 * B::key_scale(g, C::first(j, c) / 32), &scales[u][j]);
+            }
+#pragma unroll
+            for (int j = 0; j < C::WORDS; ++j) {
+                uint32_t a[2][2][4];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t both = scales[u][C::TOGETHER ? 0 : j];
+                    const uint32_t s_g = __byte_perm(both, 0, 0x1010), s_g8 = __byte_perm(both, 0, 0x3232);
+                    uint32_t x[4], y[4];
+                    f16x8(kw[u][0][j], x);
+                    f16x8(kw[u][1][j], y);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        a[u][e][0] = hmul2(x[2 * e], s_g);
+                        a[u][e][1] = hmul2(y[2 * e], s_g8);
+                        a[u][e][2] = hmul2(x[2 * e + 1], s_g);
+                        a[u][e][3] = hmul2(y[2 * e + 1], s_g8);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            if (j == 0 && e == 0)
+                                mma16816_first(s[u][t], a[u][e], qb[t][2 * j + e][0], qb[t][2 * j + e][1]);
+                            else
+                                mma16816(s[u][t], a[u][e], qb[t][2 * j + e][0], qb[t][2 * j + e][1]);
+            }
+            if constexpr (MASKED) {
+                int within;
+                const uint32_t bad = (p.cache.page_of(seg.b, seg.block_of(i0), within) < 0 ? 1u : 0u) |
+                                     (i0 + 1 < j1 && p.cache.page_of(seg.b, seg.block_of(i0 + 1), within) < 0 ? 2u : 0u);
+                const int key0 = seg.block_of(i0) * kCacheBlock;
+                const int key1 = i0 + 1 < j1 ? seg.block_of(i0 + 1) * kCacheBlock : tile.n; // no token is there
+                // Values that no row sees may be anything: their scales become zeros.
+                for (int x = lane; x < 2 * kCacheBlock * B::G; x += 32) {
+                    const int u = x / (kCacheBlock * B::G), r = x / B::G % kCacheBlock, token = (u ? key1 : key0) + r;
+                    if ((bad >> u & 1u) || token >= tile.high || (token < tile.low && token >= tile.sink))
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + u * S::BLOCK + B::VALUE_SCALES + 2 * B::value_scale(r, x % B::G)),
+                                     "h"(static_cast<uint16_t>(0))
+                                     : "memory");
+                }
+                fence_proxy_async_smem(); // the next copy's writes come after these
+                __syncwarp();
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) { // token g + 8 (e / 2), query 2c + e % 2
+                            const int token = (u ? key1 : key0) + g + 8 * (e >> 1);
+                            const bool seen = token < limit[t][e & 1] && (token >= floor_[t][e & 1] || token < p.sinks);
+                            s[u][t][e] = seen ? (bad >> u & 1u ? NAN : s[u][t][e]) : -INFINITY;
+                        }
+            }
+            bool above = false;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    above |= fmaxf(fmax3(s[0][t][h], s[0][t][h + 2], s[1][t][h]), s[1][t][h + 2]) > bar[t][h];
+            if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    float times[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float top = fmaxf(fmax3(s[0][t][h], s[0][t][h + 2], s[1][t][h]), s[1][t][h + 2]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        times[h] = 1.f;
+                        if (top > bar[t][h] || (!none[t][h] && top * factor[t][h] > ref[t][h])) {
+                            const float next = top * factor[t][h];
+                            times[h] = none[t][h] ? 0.f : ex2_approx(ref[t][h] - next);
+                            none[t][h] = false;
+                            ref[t][h] = next;
+                            bar[t][h] = (next + kLazy) / factor[t][h];
+                        }
+                        sum[t][h] *= times[h];
+                    }
+#pragma unroll
+                    for (int x = 0; x < D / 16; ++x) {
+                        o[t][x][0] *= times[0];
+                        o[t][x][1] *= times[1];
+                        o[t][x][2] *= times[0];
+                        o[t][x][3] *= times[1];
+                    }
+                }
+            }
+            uint32_t pb[2][NT][2];
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { // token g + 8 (e / 2), query 2c + e % 2
-                        const int token = (u ? key1 : key0) + g + 8 * (e >> 1);
-                        const bool seen = token < limit[t][e & 1] && (token >= floor_[t][e & 1] || token < p.sinks);
-                        s[u][t][e] = seen ? (bad >> u & 1u ? NAN : s[u][t][e]) : -INFINITY;
+                    for (int e = 0; e < 4; ++e) {
+                        s[u][t][e] = ex2_approx(fmaf(s[u][t][e], factor[t][e & 1], -ref[t][e & 1]));
+                        sum[t][e & 1] += s[u][t][e];
                     }
+                    pb[u][t][0] = turn(pack_f16(s[u][t][0], s[u][t][1]));
+                    pb[u][t][1] = turn(pack_f16(s[u][t][2], s[u][t][3]));
+                }
+
+            // O^T: a lane's scales are those of tokens 2c, 2c + 1 and 2c + 8, 2c + 9.
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int v = 0; v < D / 16 / B::W; ++v) {
+                    uint32_t vw[B::W];
+                    shared_words<B::W>(at + u * S::BLOCK + B::VALUES + B::value_word(v * B::W, lane), vw);
+#pragma unroll
+                    for (int j = 0; j < B::W; j += 2) {
+                        uint32_t vs[2]; // one group of 32 columns
+                        shared_words<2>(at + u * S::BLOCK + B::VALUE_SCALES + 2 * B::value_scale(2 * c, (v * B::W + j) / 2), vs);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint32_t x[4];
+                            f16x8(vw[j + e], x);
+                            const uint32_t a[4] = {hmul2(x[0], vs[0]), hmul2(x[1], vs[0]), hmul2(x[2], vs[1]), hmul2(x[3], vs[1])};
+#pragma unroll
+                            for (int t = 0; t < NT; ++t)
+                                mma16816(o[t][v * B::W + j + e], a, pb[u][t][0], pb[u][t][1]);
+                        }
+                    }
+                }
+            }
+        };
+
+        int i0 = seg.j0 + warp * step;
+        for (int k = 0; k < pairs; ++k, i0 += W * step) {
+            __syncwarp(); // every lane is done with the last pair, whose place is the next copy's
+            if (k + ST - 1 < pairs)
+                copy(seg, k + ST - 1, (stage_at + ST - 1) % ST);
+            const uint32_t at = ring + stage_at * S::STAGE;
+            if (!mbar_wait(full + stage_at, parity, p.err, kErrWaitK)) {
+                // Gives up, but not before its copies under way are over, or had their time.
+                for (const int end = min(pairs, k + ST); k < end; ++k) {
+                    const uint64_t start = globaltimer_ns();
+                    while (!mbar_try_wait(smem_u32(full + stage_at), parity) && globaltimer_ns() - start < kWaitLimitNs) {
+                    }
+                    next_stage();
+                }
+                break;
+            }
+            next_stage();
+            if (i0 < whole0 || i0 >= whole1)
+                attend_pair(std::true_type(), at, i0);
+            else
+                attend_pair(std::false_type(), at, i0);
         }
-        bool above = false;
+        __syncwarp();
+        ahead();
+
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                above |= fmaxf(fmax3(s[0][t][h], s[0][t][h + 2], s[1][t][h]), s[1][t][h + 2]) > bar[t][h];
-        if (__any_sync(0xffffffffu, above)) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float times[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float top = fmaxf(fmax3(s[0][t][h], s[0][t][h + 2], s[1][t][h]), s[1][t][h + 2]);
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    times[h] = 1.f;
-                    if (top > bar[t][h] || (!none[t][h] && top * factor[t][h] > ref[t][h])) {
-                        const float next = top * factor[t][h];
-                        times[h] = none[t][h] ? 0.f : ex2_approx(ref[t][h] - next);
-                        none[t][h] = false;
-                        ref[t][h] = next;
-                        bar[t][h] = (next + kLazy) / factor[t][h];
-                    }
-                    sum[t][h] *= times[h];
+            for (int h = 0; h < 2; ++h) {
+                sum[t][h] += __shfl_xor_sync(0xffffffffu, sum[t][h], 4);
+                sum[t][h] += __shfl_xor_sync(0xffffffffu, sum[t][h], 8);
+                sum[t][h] += __shfl_xor_sync(0xffffffffu, sum[t][h], 16);
+                const int r = 8 * t + 2 * c + h;
+                if (g == 0) {
+                    parts.m[warp][r] = none[t][h] ? -INFINITY : ref[t][h];
+                    parts.l[warp][r] = sum[t][h];
                 }
 #pragma unroll
                 for (int x = 0; x < D / 16; ++x) {
-                    o[t][x][0] *= times[0];
-                    o[t][x][1] *= times[1];
-                    o[t][x][2] *= times[0];
-                    o[t][x][3] *= times[1];
+                    parts.o[warp][r][16 * x + g] = o[t][x][h];
+                    parts.o[warp][r][16 * x + 8 + g] = o[t][x][2 + h];
                 }
             }
-        }
-        uint32_t pb[2][NT][2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[u][t][e] = ex2_approx(fmaf(s[u][t][e], factor[t][e & 1], -ref[t][e & 1]));
-                    sum[t][e & 1] += s[u][t][e];
-                }
-                pb[u][t][0] = turn(pack_f16(s[u][t][0], s[u][t][1]));
-                pb[u][t][1] = turn(pack_f16(s[u][t][2], s[u][t][3]));
-            }
-
-        // O^T: a lane's scales are those of tokens 2c, 2c + 1 and 2c + 8, 2c + 9.
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int v = 0; v < D / 16 / B::W; ++v) {
-                uint32_t vw[B::W];
-                shared_words<B::W>(at + u * S::BLOCK + B::VALUES + B::value_word(v * B::W, lane), vw);
-#pragma unroll
-                for (int j = 0; j < B::W; j += 2) {
-                    uint32_t vs[2]; // one group of 32 columns
-                    shared_words<2>(at + u * S::BLOCK + B::VALUE_SCALES + 2 * B::value_scale(2 * c, (v * B::W + j) / 2), vs);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        uint32_t x[4];
-                        f16x8(vw[j + e], x);
-                        const uint32_t a[4] = {hmul2(x[0], vs[0]), hmul2(x[1], vs[0]), hmul2(x[2], vs[1]), hmul2(x[3], vs[1])};
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-                            mma16816(o[t][v * B::W + j + e], a, pb[u][t][0], pb[u][t][1]);
-                    }
-                }
-            }
-        }
-    };
-
-    int i0 = j0 + warp * step;
-    for (int k = 0; k < pairs; ++k, i0 += W * step) {
-        __syncwarp(); // every lane is done with the last pair, whose place is the next copy's
-        if (k + ST - 1 < pairs)
-            fetch(k + ST - 1, after(at_turn.stage, ST - 1));
-        const int stage = at_turn.stage;
-        if (!mbar_wait(full + stage, at_turn.parity, p.err, kErrWaitK)) {
-            // Gives up, but not before its copies under way are over, or had their time.
-            for (const int end = min(pairs, k + ST); k < end; ++k) {
-                const uint64_t start = globaltimer_ns();
-                while (!mbar_try_wait(smem_u32(full + at_turn.stage), at_turn.parity) && globaltimer_ns() - start < kWaitLimitNs) {
-                }
-                at_turn.next();
-            }
-            break;
-        }
-        at_turn.next();
-        const uint32_t at = ring + stage * S::STAGE;
-        if (i0 < whole0 || i0 >= whole1)
-            attend_pair(std::true_type(), at, i0);
-        else
-            attend_pair(std::false_type(), at, i0);
     }
-    __syncthreads(); // the ring becomes the parts' place
-    float(*part_m)[ROWS] = reinterpret_cast<float(*)[ROWS]>(smem), (*part_l)[ROWS] = part_m + W;
-    cta_m = part_l[W];
-    cta_l = cta_m + ROWS;
-    part_o = reinterpret_cast<float(*)[ROWS][D + 4]>(cta_l + ROWS);
 
-    // The warps' parts: out = sum_i 2^(m_i - m) o_i, l = sum_i 2^(m_i - m) l_i.
+    // The warps' parts as one, out = sum_i 2^(m_i - m) o_i, l = sum_i 2^(m_i - m) l_i: m and l to
+    // cta_m and cta_l, four columns at a time of out to take(row, column, values).  All threads
+    // are past a barrier when this begins.
+    template <typename F> __device__ __forceinline__ static void join(Parts<D, NT> &parts, F &&take) {
+        if (threadIdx.x < ROWS) {
+            const int r = threadIdx.x;
+            float mx = parts.m[0][r], l = 0.f;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+            for (int w = 1; w < W; ++w)
+                mx = fmaxf(mx, parts.m[w][r]);
+            const float base = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            sum[t][h] += __shfl_xor_sync(0xffffffffu, sum[t][h], 4);
-            sum[t][h] += __shfl_xor_sync(0xffffffffu, sum[t][h], 8);
-            sum[t][h] += __shfl_xor_sync(0xffffffffu, sum[t][h], 16);
-            const int r = 8 * t + 2 * c + h;
-            if (g == 0) {
-                part_m[warp][r] = none[t][h] ? -INFINITY : ref[t][h];
-                part_l[warp][r] = sum[t][h];
+            for (int w = 0; w < W; ++w) {
+                const float f = ex2_approx(parts.m[w][r] - base);
+                l += f * parts.l[w][r];
+                parts.m[w][r] = f;
             }
+            parts.cta_m[r] = mx;
+            parts.cta_l[r] = l;
+        }
+        __syncthreads();
+        for (int x = threadIdx.x * 4; x < ROWS * D; x += W * 32 * 4) {
+            const int r = x / D, col = x - r * D;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int x = 0; x < D / 16; ++x) {
-                part_o[warp][r][16 * x + g] = o[t][x][h];
-                part_o[warp][r][16 * x + 8 + g] = o[t][x][2 + h];
+            for (int w = 0; w < W; ++w) {
+                const float f = parts.m[w][r];
+                const float4 o4 = *reinterpret_cast<const float4 *>(&parts.o[w][r][col]);
+                v.x += f * o4.x;
+                v.y += f * o4.y;
+                v.z += f * o4.z;
+                v.w += f * o4.w;
             }
+            take(r, col, v);
         }
-    __syncthreads();
-    if (threadIdx.x < ROWS) {
-        const int r = threadIdx.x;
-        float mx = part_m[0][r], l = 0.f;
-#pragma unroll
-        for (int w = 1; w < W; ++w)
-            mx = fmaxf(mx, part_m[w][r]);
-        const float base = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float f = ex2_approx(part_m[w][r] - base);
-            l += f * part_l[w][r];
-            part_m[w][r] = f; // the warp's weight from here on
-        }
-        cta_m[r] = mx;
-        cta_l[r] = l;
     }
-    __syncthreads();
-    for (int x = threadIdx.x * 4; x < ROWS * D; x += W * 32 * 4) {
-        const int r = x / D, col = x - r * D;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float f = part_m[w][r];
-            const float4 o4 = *reinterpret_cast<const float4 *>(&part_o[w][r][col]);
-            v.x += f * o4.x;
-            v.y += f * o4.y;
-            v.z += f * o4.z;
-            v.w += f * o4.w;
-        }
-        *reinterpret_cast<float4 *>(&part_o[0][r][col]) = v;
-    }
-}
+};
 
 // Barriers of the stages: each waits for the two lanes that copy a pair's blocks.
 template <int N> __device__ __forceinline__ void make_bars(uint64_t *bars) {
@@ -573,40 +600,48 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
     using S = TokensShape<D, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[S::WARPS * S::STAGES];
+    Parts<D, NT> &mine = *reinterpret_cast<Parts<D, NT> *>(smem + S::RING);
     const int parts = p.parts, pair = blockIdx.x / parts, part = blockIdx.x - pair * parts;
-    const int b = pair / p.kv_heads, kvh = pair - b * p.kv_heads;
+    Segment seg;
+    seg.b = pair / p.kv_heads;
+    seg.kvh = pair - seg.b * p.kv_heads;
     int n, m;
-    lengths_of(p, b, n, m);
-    const Tile tile = tile_of<S::ROWS>(p, n, m, blockIdx.y);
-    float *cta_m, *cta_l, (*part_o)[S::ROWS][D + 4];
-    Turn<S::STAGES> at_turn;
+    lengths_of(p, seg.b, n, m);
+    seg.tile = tile_of<S::ROWS>(p, n, m, blockIdx.y);
+    seg.j0 = 2 * part;
+    seg.j1 = seg.tile.blocks;
     make_bars<S::WARPS * S::STAGES>(bars);
-    attend<D, NT, BF16>(p, tile, b, kvh, 2 * part, tile.blocks, 2 * parts, smem, bars, at_turn, cta_m, cta_l, part_o);
+    Worker<D, NT, BF16> worker(p, 2 * parts, smem, bars);
+    worker.first_pages(seg);
+    worker.first_copies(seg);
+    worker.attend(seg, mine, [] {});
+    __syncthreads();
+    worker.join(mine, [&](int r, int col, const float4 &v) { *reinterpret_cast<float4 *>(&mine.o[0][r][col]) = v; });
     if (parts > 1)
         cluster_sync();
     else
         __syncthreads();
     for (int x = part * S::WARPS * 32 + threadIdx.x; x < S::ROWS * D; x += parts * S::WARPS * 32) {
         const int r = x / D, col = x - r * D;
-        if (r >= tile.rows || col >= p.hd)
+        if (r >= seg.tile.rows || col >= p.hd)
             continue;
         float l, v;
         if (parts > 1) {
             float mx = -INFINITY;
             for (int k = 0; k < parts; ++k)
-                mx = fmaxf(mx, peer_load(peer(&cta_m[r], k)));
+                mx = fmaxf(mx, peer_load(peer(&mine.cta_m[r], k)));
             const float base = mx == -INFINITY ? 0.f : mx;
             l = v = 0.f;
             for (int k = 0; k < parts; ++k) {
-                const float f = exp2f(peer_load(peer(&cta_m[r], k)) - base);
-                l += f * peer_load(peer(&cta_l[r], k));
-                v += f * peer_load(peer(&part_o[0][r][col], k));
+                const float f = exp2f(peer_load(peer(&mine.cta_m[r], k)) - base);
+                l += f * peer_load(peer(&mine.cta_l[r], k));
+                v += f * peer_load(peer(&mine.o[0][r][col], k));
             }
         } else {
-            l = cta_l[r];
-            v = part_o[0][r][col];
+            l = mine.cta_l[r];
+            v = mine.o[0][r][col];
         }
-        store_out(p, tile, b, kvh, r, col, v, l);
+        store_out(p, seg.tile, seg.b, seg.kvh, r, col, v, l);
     }
     if (parts > 1)
         cluster_sync(); // no CTA leaves while another reads its part
@@ -639,7 +674,8 @@ template <int WARPS> __device__ __forceinline__ long long cta_sum(long long v, l
 }
 
 // The list: blocks of the tiles, sequence after sequence, key head after key head, tile after
-// tile.  CTA i takes blocks [i per, (i + 1) per).
+// tile.  CTA i takes blocks [i per, (i + 1) per).  While it reads a segment the next one is
+// known, and its first blocks are on their way before the segment's parts are joined.
 template <int D, int NT, bool BF16>
 __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D, NT>::CTAS)
     window_e2m1_list_kernel(const __grid_constant__ TokensParams p) {
@@ -647,12 +683,17 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
     constexpr int THREADS = S::WARPS * 32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[S::WARPS * S::STAGES];
-    __shared__ long long place[S::WARPS], start_at;
-    __shared__ int start_b;
-    Turn<S::STAGES> at_turn;
-    make_bars<S::WARPS * S::STAGES>(bars);
+    __shared__ long long place[S::WARPS];
+    __shared__ Segment segments[3];
+    __shared__ struct {
+        long long at; // where the tile begins in the list
+        int b, kvh, tile;
+    } walk;
+    Parts<D, NT> &parts = *reinterpret_cast<Parts<D, NT> *>(smem + S::RING);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    // Each thread has a run of sequences; the thread in whose run this CTA's first block is finds the sequence.
+    make_bars<S::WARPS * S::STAGES>(bars);
+    // Each thread has a run of sequences; the thread in whose run this CTA's first block is finds
+    // the sequence and key head.
     const int run = (p.batch + THREADS - 1) / THREADS, b0 = threadIdx.x * run, b1 = min(p.batch, b0 + run);
     long long mine = 0;
     for (int b = b0; b < b1; ++b)
@@ -680,54 +721,93 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
     if (from >= to)
         return;
     if (from >= before && from < before + mine) {
-        long long at = before;
-        int b = b0;
-        for (; b < b1 - 1; ++b) {
-            const long long next = at + static_cast<long long>(listed_of<S::ROWS>(p, b)) * p.kv_heads;
-            if (from < next)
-                break;
-            at = next;
-        }
-        start_at = at;
-        start_b = b;
+        int b = b0, of_head = listed_of<S::ROWS>(p, b);
+        for (; b < b1 - 1 && from >= before + static_cast<long long>(of_head) * p.kv_heads; of_head = listed_of<S::ROWS>(p, b))
+            before += static_cast<long long>(of_head) * p.kv_heads, ++b;
+        walk.b = b;
+        walk.kvh = quotient(from - before, of_head);
+        walk.tile = 0;
+        walk.at = before + static_cast<long long>(walk.kvh) * of_head;
     }
     __syncthreads();
-    long long at = start_at; // where the next tile begins
-    int b = start_b;
-    for (int parts = 0; at < to; ++b) {
-        int n, m;
-        lengths_of(p, b, n, m);
-        for (int kvh = 0; kvh < p.kv_heads && at < to; ++kvh)
-            for (int i = 0; i < p.tiles && at < to; ++i) {
-                const Tile tile = tile_of<S::ROWS>(p, n, m, i);
-                const int size = listed(tile);
-                const long long begin = at;
-                at += size;
-                if (at <= from || size == 0)
-                    continue;
-                const int j0 = static_cast<int>(max(from - begin, 0ll)), j1 = static_cast<int>(min(to - begin, static_cast<long long>(size)));
-                float *cta_m, *cta_l, (*part_o)[S::ROWS][D + 4];
-                attend<D, NT, BF16>(p, tile, b, kvh, max(j0 - kTileCost, 0), j1 - kTileCost, 2, smem, bars, at_turn, cta_m, cta_l, part_o);
-                __syncthreads();
-                if (j0 == 0 && j1 == size) {
-                    for (int x = threadIdx.x; x < S::ROWS * D; x += THREADS) {
-                        const int r = x / D, col = x - r * D;
-                        if (r < tile.rows && col < p.hd)
-                            store_out(p, tile, b, kvh, r, col, part_o[0][r][col], cta_l[r]);
-                    }
-                } else {
-                    float *slot = p.parts_at + (2ll * blockIdx.x + (begin > from)) * S::SLOT;
-                    for (int r = threadIdx.x; r < tile.rows; r += THREADS) {
-                        slot[2 * r] = cta_m[r];
-                        slot[2 * r + 1] = cta_l[r];
-                    }
-                    for (int x = threadIdx.x * 4; x < tile.rows * D; x += THREADS * 4)
-                        *reinterpret_cast<float4 *>(slot + 2 * S::ROWS + x) =
-                            *reinterpret_cast<const float4 *>(&part_o[0][x / D][x % D]);
-                }
-                fence_proxy_async_smem();
-                __syncthreads(); // the parts' place becomes the ring again
+    // One thread walks the list, two segments ahead.
+    const bool walker = threadIdx.x == THREADS - 32;
+    auto advance = [&](Segment &s) {
+        int b = walk.b, kvh = walk.kvh, i = walk.tile, n, m;
+        long long at = walk.at;
+        s.b = -1;
+        while (at < to) {
+            lengths_of(p, b, n, m);
+            const Tile tile = tile_of<S::ROWS>(p, n, m, i);
+            const int size = listed(tile);
+            const long long begin = at;
+            if (size && begin + size > from) {
+                const int j0 = static_cast<int>(max(from - begin, 0ll));
+                const int j1 = static_cast<int>(min(to - begin, static_cast<long long>(size)));
+                s.tile = tile;
+                s.b = b;
+                s.kvh = kvh;
+                s.j0 = max(j0 - kTileCost, 0);
+                s.j1 = j1 - kTileCost;
+                s.slot = j0 == 0 && j1 == size ? -1 : 2 * blockIdx.x + (begin > from);
             }
+            at += size;
+            if (++i == p.tiles) {
+                i = 0;
+                if (++kvh == p.kv_heads) {
+                    kvh = 0;
+                    ++b;
+                }
+            }
+            if (s.b >= 0)
+                break;
+        }
+        walk.b = b;
+        walk.kvh = kvh;
+        walk.tile = i;
+        walk.at = at;
+    };
+    if (walker) {
+        advance(segments[0]);
+        advance(segments[1]);
+    }
+    __syncthreads();
+    Worker<D, NT, BF16> worker(p, 2, smem, bars);
+    worker.first_pages(segments[0]);
+    worker.first_copies(segments[0]);
+    for (int cur = 0; segments[cur].b >= 0;) {
+        const int next = cur == 2 ? 0 : cur + 1;
+        const Segment &seg = segments[cur];
+        if (walker)
+            advance(segments[next == 2 ? 0 : next + 1]);
+        __syncwarp();
+        const bool more = segments[next].b >= 0;
+        worker.attend(seg, parts, [&] {
+            if (more)
+                worker.first_pages(segments[next]);
+        });
+        if (more)
+            worker.first_copies(segments[next]);
+        __syncthreads();
+        if (seg.slot < 0) {
+            worker.join(parts, [&](int r, int col, const float4 &v) {
+                const float *e = &v.x;
+                if (r < seg.tile.rows)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        if (col + x < p.hd)
+                            store_out(p, seg.tile, seg.b, seg.kvh, r, col + x, e[x], parts.cta_l[r]);
+            });
+        } else {
+            float *slot = p.parts_at + static_cast<long long>(seg.slot) * S::SLOT;
+            worker.join(parts, [&](int r, int col, const float4 &v) {
+                if (col == 0)
+                    *reinterpret_cast<float2 *>(slot + 2 * r) = make_float2(parts.cta_m[r], parts.cta_l[r]);
+                *reinterpret_cast<float4 *>(slot + 2 * S::ROWS + r * D + col) = v;
+            });
+        }
+        __syncthreads(); // the parts' place is free, and the segment after the next one known
+        cur = next;
     }
 }
 
@@ -862,9 +942,12 @@ template <int D, int NT, bool BF16> int launch_rows(const TokensParams &p, int c
     return static_cast<int>(cudaLaunchKernelEx(&cfg, window_e2m1_join_kernel<D, NT>, p, ctas));
 }
 template <int D> int launch_d(const TokensParams &p, int ctas, bool bf16, cudaStream_t stream) {
-    if (p.group * p.q_len <= 8)
+    const int rows = p.group * p.q_len;
+    if (rows <= 8)
         return bf16 ? launch_rows<D, 1, true>(p, ctas, stream) : launch_rows<D, 1, false>(p, ctas, stream);
-    return bf16 ? launch_rows<D, 2, true>(p, ctas, stream) : launch_rows<D, 2, false>(p, ctas, stream);
+    if (rows <= 16)
+        return bf16 ? launch_rows<D, 2, true>(p, ctas, stream) : launch_rows<D, 2, false>(p, ctas, stream);
+    return bf16 ? launch_rows<D, 3, true>(p, ctas, stream) : launch_rows<D, 3, false>(p, ctas, stream);
 }
 
 // How a call is split: CTAs of a cluster, or (parts 0) of the list.
@@ -876,7 +959,7 @@ Split split_of(const WindowE2m1Args &a) {
     const CacheArgs &c = a.cache;
     const long long rows = static_cast<long long>(a.heads / c.kv_heads) * c.q_len;
     Split s;
-    s.rows = rows <= 8 ? 8 : 16;
+    s.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 24;
     s.tiles = static_cast<int>((rows + s.rows - 1) / s.rows);
     long long keys = a.kv_len;
     if (a.window > 0)
