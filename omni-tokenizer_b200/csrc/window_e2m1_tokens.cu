@@ -51,6 +51,7 @@ struct TokensParams {
     long long qs[3], os[3];
     const int *lengths, *q_lengths;
     int parts; // CTAs of a cluster, or 0: the list
+    int ctas;  // of the list
     uint32_t group_inv; // ceil(2^16 / group): rows of a call are few (kMostRows), their quotients by it exact
     int batch, kv_heads, group, q_len, kv_len, hd, tiles; // tiles of rows that a sequence may have
     int window, right, sinks;
@@ -59,10 +60,13 @@ struct TokensParams {
     int *err;
 };
 
+// CTAs on an SM: as many as their registers allow.
+template <int NT> constexpr int kCtas = NT == 1 ? 4 : 2;
+
 template <int D, int NT> struct TokensShape {
     static constexpr int BLOCK = CacheBlock<D>::BYTES;
-    static constexpr int WARPS = 8, CTAS = NT == 1 ? 2 : 1; // of an SM
-    static constexpr int STAGES = 2, STAGE = 2 * BLOCK;
+    static constexpr int WARPS = 4, CTAS = kCtas<NT>;
+    static constexpr int STAGES = 2, STAGE = 2 * BLOCK; // a pair that is read, one on its way
     static constexpr int RING = WARPS * STAGES * STAGE;
     static constexpr int ROWS = 8 * NT;
     // The warps' results: m, l of each and of the CTA, outputs.
@@ -162,7 +166,7 @@ template <int ROWS> __device__ __forceinline__ Tile tile_of(const TokensParams &
 }
 // Its length in the list: beginning and ending a tile takes a CTA as long as some blocks do
 // (1.2 us against 0.13 us for one: 64 x up to 16384 keys TILECOST), so it counts for those as well.
-constexpr int kTileCost = 8;
+constexpr int kTileCost = 16;
 __device__ __forceinline__ int listed(const Tile &t) { return t.rows > 0 ? kTileCost + t.blocks : 0; }
 // Blocks of all tiles of a sequence's key head.
 template <int ROWS> __device__ __forceinline__ int listed_of(const TokensParams &p, int b) {
@@ -198,7 +202,7 @@ struct Segment {
 // The warps' results in shared memory.
 template <int D, int NT> struct Parts {
     using S = TokensShape<D, NT>;
-    float m[S::WARPS][S::ROWS]; // then the warps' weights
+    float m[S::WARPS][S::ROWS];
     float l[S::WARPS][S::ROWS];
     float cta_m[S::ROWS], cta_l[S::ROWS];
     float o[S::WARPS][S::ROWS][D + 4];
@@ -218,34 +222,32 @@ template <int D, int NT, bool BF16> struct Worker {
     // Where the warp is in its ring: the stage of the next pair, and the parity of its barrier.
     int stage_at = 0;
     uint32_t parity = 0;
-    // Of the segment that is read: pairs [whole0, whole1) every row sees whole, so they need no
+    // Of the segment that is fetched: pairs [whole0, whole1) every row sees whole, so they need no
     // mask (sinks are left to it, and so is everything once a page is none of the cache's).
     int whole0 = 0, whole1 = 0, pairs = 0;
     // Lane l knows where block l % 2 of pair k + l / 2 is, k a multiple of 16 (0: nowhere), and
-    // copies it; and the pages of the next 16 pairs.
+    // copies it; and the pages of the next 16 pairs, or of the next segment's first.
     unsigned long long place = 0;
-    int page_next = 0, within_next = 0;
+    int page_next = 0, within_next = 0, page_then = 0, within_then = 0;
 
     __device__ __forceinline__ Worker(const TokensParams &p_, int step_, uint8_t *smem, uint64_t *bars)
         : p(p_), step(step_), warp(threadIdx.x >> 5), lane(threadIdx.x & 31),
           ring(smem_u32(smem) + (threadIdx.x >> 5) * ST * S::STAGE), full(bars + (threadIdx.x >> 5) * ST) {}
 
     __device__ __forceinline__ void next_stage() {
-        if (++stage_at == ST) {
-            stage_at = 0;
-            parity ^= 1u;
-        }
+        stage_at ^= 1;
+        parity ^= stage_at ^ 1;
     }
-    __device__ __forceinline__ void look_up(const Segment &s, int k) {
+    __device__ __forceinline__ int page_at(const Segment &s, int k, int &within) const {
         const int i = s.j0 + (warp + (k + (lane >> 1)) * W) * step + (lane & 1);
-        page_next = i < s.j1 ? p.cache.page_of(s.b, s.block_of(i), within_next) : -2;
+        return i < s.j1 ? p.cache.page_of(s.b, s.block_of(i), within) : -2;
     }
-    __device__ __forceinline__ void copy(const Segment &s, int k, int stage) {
+    __device__ __forceinline__ void copy(const Segment &s, int k, int stage, int &whole1) {
         if ((k & 15) == 0) {
             if (__any_sync(0xffffffffu, page_next == -1))
                 whole1 = -1;
             place = page_next >= 0 ? reinterpret_cast<unsigned long long>(p.cache.block_at(page_next, s.kvh, within_next, S::BLOCK)) : 0ull;
-            look_up(s, k + 16);
+            page_next = page_at(s, k + 16, within_next);
         }
         if ((lane >> 1) == (k & 15)) {
             mbar_arrive_expect_tx(full + stage, place ? S::BLOCK : 0);
@@ -253,8 +255,9 @@ template <int D, int NT, bool BF16> struct Worker {
                 copy_piece(ring + stage * S::STAGE + (lane & 1) * S::BLOCK, place, S::BLOCK, smem_u32(full + stage));
         }
     }
-    // Begins a segment: asks for its first pages, and then for its first blocks.
-    __device__ __forceinline__ void first_pages(const Segment &s) {
+    // Asks for the pages of a segment's first pairs, and begins it: its first pair to `stage`.
+    __device__ __forceinline__ void ask(const Segment &s) { page_then = page_at(s, 0, within_then); }
+    __device__ __forceinline__ void begin(const Segment &s, int stage) {
         const Tile &tile = s.tile;
         const int limit_all = min(tile.n, tile.first + p.right + 1), floor_all = p.window > 0 ? tile.last - p.window + 1 : 0;
         const int ahead = tile.sink_blocks - tile.begin;
@@ -262,18 +265,36 @@ template <int D, int NT, bool BF16> struct Worker {
         whole1 = min(s.j1, max(limit_all, 0) / kCacheBlock + ahead) - 1;
         const int mine = s.j1 - s.j0 - warp * step;
         pairs = mine > 0 ? (mine + W * step - 1) / (W * step) : 0;
-        look_up(s, 0);
-    }
-    __device__ __forceinline__ void first_copies(const Segment &s) {
-#pragma unroll
-        for (int k = 0; k < ST - 1; ++k)
-            if (k < pairs)
-                copy(s, k, (stage_at + k) % ST);
+        page_next = page_then;
+        within_next = within_then;
+        if (pairs)
+            copy(s, 0, stage, whole1);
     }
 
-    // The segment's softmax, the warp's share of it, to `parts`.  `ahead()` is called when its
-    // last block has been read.
-    template <typename F> __device__ __forceinline__ void attend(const Segment &seg, Parts<D, NT> &parts, F &&ahead) {
+    // Its rows of q, as they are: this lane's columns of rows g.
+    uint4 queries[NT][C::WORDS];
+    __device__ __forceinline__ void load_queries(const Segment &s) {
+        const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int r = s.tile.row0 + 8 * t + g, query = query_of(p, r);
+            const bool real = 8 * t + g < s.tile.rows;
+            const uint16_t *q = p.q + s.b * p.qs[0] + (s.kvh * p.group + r - query * p.group) * p.qs[1] + query * p.qs[2];
+#pragma unroll
+            for (int j = 0; j < C::WORDS; ++j) {
+                const int col = C::first(j, c);
+                queries[t][j] = real && col < p.hd ? *reinterpret_cast<const uint4 *>(q + col) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+    }
+
+    // The softmax of the segment that has begun, the warp's share of it, to `parts`; begins the
+    // next one (NULL: there is none) before the last pair's turn.
+    __device__ __forceinline__ void attend(const Segment &seg, const Segment *next, Parts<D, NT> &parts) {
+        const int whole0 = this->whole0, pairs = this->pairs;
+        int whole1 = this->whole1;
+        if (next)
+            ask(*next);
         const Tile &tile = seg.tile;
         const int g = lane >> 2, c = lane & 3, j1 = seg.j1;
         // The queries as B operands, and the masks of columns 2c and 2c + 1.
@@ -282,16 +303,10 @@ template <int D, int NT, bool BF16> struct Worker {
         int limit[NT][2], floor_[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const int r = tile.row0 + 8 * t + g;
-            const bool real = 8 * t + g < tile.rows;
-            const int query = query_of(p, r);
-            const uint16_t *q = p.q + seg.b * p.qs[0] + (seg.kvh * p.group + r - query * p.group) * p.qs[1] + query * p.qs[2];
-            uint4 w[C::WORDS];
+            uint4 (&w)[C::WORDS] = queries[t];
             uint32_t top2 = 0;
 #pragma unroll
             for (int j = 0; j < C::WORDS; ++j) {
-                const int col = C::first(j, c);
-                w[j] = real && col < p.hd ? *reinterpret_cast<const uint4 *>(q + col) : make_uint4(0u, 0u, 0u, 0u);
                 const uint32_t *x = &w[j].x;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -502,19 +517,31 @@ template <int D, int NT, bool BF16> struct Worker {
         };
 
         int i0 = seg.j0 + warp * step;
+        if (pairs == 0 && next)
+            begin(*next, stage_at);
         for (int k = 0; k < pairs; ++k, i0 += W * step) {
             __syncwarp(); // every lane is done with the last pair, whose place is the next copy's
-            if (k + ST - 1 < pairs)
-                copy(seg, k + ST - 1, (stage_at + ST - 1) % ST);
+            const bool more = k + 1 < pairs;
+            if (more)
+                copy(seg, k + 1, stage_at ^ 1, whole1);
+            else if (next)
+                begin(*next, stage_at ^ 1);
             const uint32_t at = ring + stage_at * S::STAGE;
             if (!mbar_wait(full + stage_at, parity, p.err, kErrWaitK)) {
-                // Gives up, but not before its copies under way are over, or had their time.
-                for (const int end = min(pairs, k + ST); k < end; ++k) {
+                // Gives up (the host learns of it), but not before its copies under way are over,
+                // or had their time.
+                for (int wait = 0; wait < 2; ++wait) {
                     const uint64_t start = globaltimer_ns();
                     while (!mbar_try_wait(smem_u32(full + stage_at), parity) && globaltimer_ns() - start < kWaitLimitNs) {
                     }
+                    if (!more)
+                        break; // what the next segment has under way is waited for there
                     next_stage();
                 }
+                if (!more)
+                    next_stage();
+                else if (next)
+                    begin(*next, stage_at);
                 break;
             }
             next_stage();
@@ -524,7 +551,6 @@ template <int D, int NT, bool BF16> struct Worker {
                 attend_pair(std::false_type(), at, i0);
         }
         __syncwarp();
-        ahead();
 
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -546,40 +572,28 @@ template <int D, int NT, bool BF16> struct Worker {
             }
     }
 
-    // The warps' parts as one, out = sum_i 2^(m_i - m) o_i, l = sum_i 2^(m_i - m) l_i: m and l to
-    // cta_m and cta_l, four columns at a time of out to take(row, column, values).  All threads
-    // are past a barrier when this begins.
-    template <typename F> __device__ __forceinline__ static void join(Parts<D, NT> &parts, F &&take) {
-        if (threadIdx.x < ROWS) {
-            const int r = threadIdx.x;
-            float mx = parts.m[0][r], l = 0.f;
-#pragma unroll
-            for (int w = 1; w < W; ++w)
-                mx = fmaxf(mx, parts.m[w][r]);
-            const float base = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float f = ex2_approx(parts.m[w][r] - base);
-                l += f * parts.l[w][r];
-                parts.m[w][r] = f;
-            }
-            parts.cta_m[r] = mx;
-            parts.cta_l[r] = l;
-        }
-        __syncthreads();
+    // The warps' parts as one, m, l and four columns at a time of sum_i 2^(m_i - m) o_i, to
+    // take(row, column, m, l, values).  All threads are past a barrier when this begins.
+    template <typename F> __device__ __forceinline__ static void join(const Parts<D, NT> &parts, F &&take) {
         for (int x = threadIdx.x * 4; x < ROWS * D; x += W * 32 * 4) {
             const int r = x / D, col = x - r * D;
+            float weight[W], mx = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                mx = fmaxf(mx, weight[w] = parts.m[w][r]);
+            const float base = mx == -INFINITY ? 0.f : mx;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const float f = parts.m[w][r];
+                const float f = ex2_approx(weight[w] - base);
                 const float4 o4 = *reinterpret_cast<const float4 *>(&parts.o[w][r][col]);
+                l += f * parts.l[w][r];
                 v.x += f * o4.x;
                 v.y += f * o4.y;
                 v.z += f * o4.z;
                 v.w += f * o4.w;
             }
-            take(r, col, v);
+            take(r, col, mx, l, v);
         }
     }
 };
@@ -612,11 +626,18 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
     seg.j1 = seg.tile.blocks;
     make_bars<S::WARPS * S::STAGES>(bars);
     Worker<D, NT, BF16> worker(p, 2 * parts, smem, bars);
-    worker.first_pages(seg);
-    worker.first_copies(seg);
-    worker.attend(seg, mine, [] {});
+    worker.ask(seg);
+    worker.load_queries(seg);
+    worker.begin(seg, 0);
+    worker.attend(seg, nullptr, mine);
     __syncthreads();
-    worker.join(mine, [&](int r, int col, const float4 &v) { *reinterpret_cast<float4 *>(&mine.o[0][r][col]) = v; });
+    worker.join(mine, [&](int r, int col, float m, float l, const float4 &v) {
+        if (col == 0) {
+            mine.cta_m[r] = m;
+            mine.cta_l[r] = l;
+        }
+        *reinterpret_cast<float4 *>(&mine.o[0][r][col]) = v;
+    });
     if (parts > 1)
         cluster_sync();
     else
@@ -657,25 +678,18 @@ __device__ __forceinline__ long long share_of(long long total, int ctas) {
     return up >> 32 ? up / ctas : static_cast<long long>(static_cast<uint32_t>(up) / static_cast<uint32_t>(ctas));
 }
 
-// Sums over the CTA's threads; every thread gets the result.
-template <int WARPS> __device__ __forceinline__ long long cta_sum(long long v, long long *place) {
-#pragma unroll
-    for (int x = 16; x; x >>= 1)
-        v += __shfl_xor_sync(0xffffffffu, v, x);
-    if ((threadIdx.x & 31) == 0)
-        place[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w)
-        v += place[w];
-    __syncthreads();
-    return v;
+// A tile that begins in a CTA's share of the list and ends in another's: for each CTA, behind
+// the parts' slots.  parts 0: there is none.
+struct alignas(16) SharedTile {
+    int b = 0, kvh = 0, tile = 0, slot = 0, parts = 0, unused[3] = {};
+};
+template <int D, int NT> __device__ __forceinline__ SharedTile *shared_tile(const TokensParams &p, int cta) {
+    return reinterpret_cast<SharedTile *>(p.parts_at + 2ll * p.ctas * TokensShape<D, NT>::SLOT) + cta;
 }
 
 // The list: blocks of the tiles, sequence after sequence, key head after key head, tile after
-// tile.  CTA i takes blocks [i per, (i + 1) per).  While it reads a segment the next one is
-// known, and its first blocks are on their way before the segment's parts are joined.
+// tile.  CTA i takes blocks [i per, (i + 1) per).  The next segment's first blocks are on their
+// way before the last ones of a segment are read.
 template <int D, int NT, bool BF16>
 __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D, NT>::CTAS)
     window_e2m1_list_kernel(const __grid_constant__ TokensParams p) {
@@ -684,10 +698,10 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[S::WARPS * S::STAGES];
     __shared__ long long place[S::WARPS];
-    __shared__ Segment segments[3];
+    __shared__ Segment segments[32];
     __shared__ struct {
-        long long at; // where the tile begins in the list
-        int b, kvh, tile;
+        long long at, tile; // where the next tile begins in the list, and its number
+        int count;          // of the segments
     } walk;
     Parts<D, NT> &parts = *reinterpret_cast<Parts<D, NT> *>(smem + S::RING);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -718,135 +732,130 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
     before -= mine;
     const long long per = share_of(total, gridDim.x);
     const long long from = blockIdx.x * per, to = min(total, from + per);
+    if (threadIdx.x == 0)
+        *shared_tile<D, NT>(p, blockIdx.x) = SharedTile{};
     if (from >= to)
         return;
     if (from >= before && from < before + mine) {
         int b = b0, of_head = listed_of<S::ROWS>(p, b);
         for (; b < b1 - 1 && from >= before + static_cast<long long>(of_head) * p.kv_heads; of_head = listed_of<S::ROWS>(p, b))
             before += static_cast<long long>(of_head) * p.kv_heads, ++b;
-        walk.b = b;
-        walk.kvh = quotient(from - before, of_head);
-        walk.tile = 0;
-        walk.at = before + static_cast<long long>(walk.kvh) * of_head;
+        const int kvh = quotient(from - before, of_head);
+        walk.tile = (static_cast<long long>(b) * p.kv_heads + kvh) * p.tiles;
+        walk.at = before + static_cast<long long>(kvh) * of_head;
     }
-    __syncthreads();
-    // One thread walks the list, two segments ahead.
-    const bool walker = threadIdx.x == THREADS - 32;
-    auto advance = [&](Segment &s) {
-        int b = walk.b, kvh = walk.kvh, i = walk.tile, n, m;
-        long long at = walk.at;
-        s.b = -1;
-        while (at < to) {
+    // A warp works out 32 tiles at once, those of them that this CTA has a share in.
+    const int of_sequence = p.kv_heads * p.tiles;
+    auto refill = [&] {
+        const long long at = walk.at, number = walk.tile + lane;
+        const int b = quotient(number, of_sequence), in_b = static_cast<int>(number - static_cast<long long>(b) * of_sequence);
+        Segment s;
+        s.b = b;
+        s.kvh = in_b / p.tiles;
+        int size = 0, n, m;
+        if (b < p.batch) {
             lengths_of(p, b, n, m);
-            const Tile tile = tile_of<S::ROWS>(p, n, m, i);
-            const int size = listed(tile);
-            const long long begin = at;
-            if (size && begin + size > from) {
-                const int j0 = static_cast<int>(max(from - begin, 0ll));
-                const int j1 = static_cast<int>(min(to - begin, static_cast<long long>(size)));
-                s.tile = tile;
-                s.b = b;
-                s.kvh = kvh;
-                s.j0 = max(j0 - kTileCost, 0);
-                s.j1 = j1 - kTileCost;
-                s.slot = j0 == 0 && j1 == size ? -1 : 2 * blockIdx.x + (begin > from);
-            }
-            at += size;
-            if (++i == p.tiles) {
-                i = 0;
-                if (++kvh == p.kv_heads) {
-                    kvh = 0;
-                    ++b;
-                }
-            }
-            if (s.b >= 0)
-                break;
+            s.tile = tile_of<S::ROWS>(p, n, m, in_b - s.kvh * p.tiles);
+            size = listed(s.tile);
         }
-        walk.b = b;
-        walk.kvh = kvh;
-        walk.tile = i;
-        walk.at = at;
-    };
-    if (walker) {
-        advance(segments[0]);
-        advance(segments[1]);
-    }
-    __syncthreads();
-    Worker<D, NT, BF16> worker(p, 2, smem, bars);
-    worker.first_pages(segments[0]);
-    worker.first_copies(segments[0]);
-    for (int cur = 0; segments[cur].b >= 0;) {
-        const int next = cur == 2 ? 0 : cur + 1;
-        const Segment &seg = segments[cur];
-        if (walker)
-            advance(segments[next == 2 ? 0 : next + 1]);
-        __syncwarp();
-        const bool more = segments[next].b >= 0;
-        worker.attend(seg, parts, [&] {
-            if (more)
-                worker.first_pages(segments[next]);
-        });
-        if (more)
-            worker.first_copies(segments[next]);
-        __syncthreads();
-        if (seg.slot < 0) {
-            worker.join(parts, [&](int r, int col, const float4 &v) {
-                const float *e = &v.x;
-                if (r < seg.tile.rows)
+        uint32_t sum = size; // 32 tiles of at most 2^26 blocks
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        if (col + x < p.hd)
-                            store_out(p, seg.tile, seg.b, seg.kvh, r, col + x, e[x], parts.cta_l[r]);
-            });
-        } else {
-            float *slot = p.parts_at + static_cast<long long>(seg.slot) * S::SLOT;
-            worker.join(parts, [&](int r, int col, const float4 &v) {
-                if (col == 0)
-                    *reinterpret_cast<float2 *>(slot + 2 * r) = make_float2(parts.cta_m[r], parts.cta_l[r]);
-                *reinterpret_cast<float4 *>(slot + 2 * S::ROWS + r * D + col) = v;
-            });
+        for (int x = 1; x < 32; x <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, sum, x);
+            sum += lane >= x ? y : 0;
         }
-        __syncthreads(); // the parts' place is free, and the segment after the next one known
-        cur = next;
-    }
+        const long long begin = at + (sum - size);
+        const bool has = size && begin + size > from && begin < to;
+        const uint32_t those = __ballot_sync(0xffffffffu, has);
+        if (has) {
+            const int j0 = static_cast<int>(max(from - begin, 0ll)), j1 = static_cast<int>(min(to - begin, static_cast<long long>(size)));
+            s.j0 = max(j0 - kTileCost, 0);
+            s.j1 = j1 - kTileCost;
+            s.slot = j0 == 0 && j1 == size ? -1 : 2 * static_cast<int>(blockIdx.x) + (begin > from);
+            segments[__popc(those & ((1u << lane) - 1))] = s;
+            if (j0 == 0 && j1 < size) { // begins here, ends elsewhere: what the join needs to know
+                SharedTile t;
+                t.b = b;
+                t.kvh = s.kvh;
+                t.tile = in_b - s.kvh * p.tiles;
+                t.slot = s.slot;
+                t.parts = quotient(begin + size - 1, per) - static_cast<int>(blockIdx.x) + 1;
+                *shared_tile<D, NT>(p, blockIdx.x) = t;
+            }
+        }
+        __syncwarp();
+        if (lane == 31) {
+            walk.at = at + sum;
+            walk.tile = number + 1;
+            walk.count = __popc(those);
+        }
+    };
+    Worker<D, NT, BF16> worker(p, 2, smem, bars);
+    do {
+        __syncthreads(); // walk and the segments are as they were left
+        if (warp == 0)
+            refill();
+        __syncthreads();
+        const int count = walk.count;
+        if (count) {
+            worker.ask(segments[0]);
+            worker.load_queries(segments[0]);
+            worker.begin(segments[0], worker.stage_at);
+        }
+        for (int i = 0; i < count; ++i) {
+            const Segment &seg = segments[i], *next = i + 1 < count ? &segments[i + 1] : nullptr;
+            worker.attend(seg, next, parts);
+            if (next)
+                worker.load_queries(*next);
+            __syncthreads();
+            if (seg.slot < 0) {
+                worker.join(parts, [&](int r, int col, float, float l, const float4 &v) {
+                    const float *e = &v.x;
+                    if (r < seg.tile.rows)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            if (col + x < p.hd)
+                                store_out(p, seg.tile, seg.b, seg.kvh, r, col + x, e[x], l);
+                });
+            } else {
+                float *slot = p.parts_at + static_cast<long long>(seg.slot) * S::SLOT;
+                worker.join(parts, [&](int r, int col, float m, float l, const float4 &v) {
+                    if (col == 0)
+                        *reinterpret_cast<float2 *>(slot + 2 * r) = make_float2(m, l);
+                    *reinterpret_cast<float4 *>(slot + 2 * S::ROWS + r * D + col) = v;
+                });
+            }
+            __syncthreads(); // the parts' place is free
+        }
+    } while (walk.at < to);
 }
 
-// Joins the parts of the tiles that several CTAs share: a CTA for each tile and two of its rows
-// (with eight, few tiles of many parts met in few SMs: 131072 keys x 8 heads 45 -> JOIN us).  A
-// part's weight is worked out once for a row; SHARES threads share a column's parts.
-constexpr int kJoinThreads = 256, kJoinParts = 512, kJoinRows = 2;
+// Joins the parts of the tiles that several CTAs share: a CTA for each of the list's, and two
+// rows of the tile that begins there (with eight, few tiles of many parts met in few SMs: 131072
+// keys x 8 heads 45 -> 41 us).  A part's weight is worked out once for a row; SHARES threads
+// share a column's parts.
+constexpr int kJoinThreads = 256, kJoinParts = 1024, kJoinRows = 2;
 template <int D, int NT>
-__global__ void __launch_bounds__(kJoinThreads) window_e2m1_join_kernel(const __grid_constant__ TokensParams p, int ctas) {
+__global__ void __launch_bounds__(kJoinThreads) window_e2m1_join_kernel(const __grid_constant__ TokensParams p) {
     using S = TokensShape<D, NT>;
-    constexpr int WARPS = kJoinThreads / 32, FOURS = kJoinRows * D / 4, SHARES = kJoinThreads / FOURS;
-    __shared__ long long place[WARPS];
+    constexpr int FOURS = kJoinRows * D / 4, SHARES = kJoinThreads / FOURS;
     __shared__ float weight[kJoinRows][kJoinParts], sums[kJoinRows][kJoinParts], total_l[kJoinRows];
     __shared__ __align__(16) float share[SHARES - 1][kJoinRows * D];
-    const int i = blockIdx.x % p.tiles, pair = blockIdx.x / p.tiles, b = pair / p.kv_heads, kvh = pair - b * p.kv_heads;
-    long long before = 0, total = 0;
-    for (int x = threadIdx.x; x < p.batch; x += kJoinThreads) {
-        const long long size = static_cast<long long>(listed_of<S::ROWS>(p, x)) * p.kv_heads;
-        total += size;
-        before += x < b ? size : 0;
-    }
-    total = cta_sum<WARPS>(total, place);
-    before = cta_sum<WARPS>(before, place);
-    int n, m;
-    lengths_of(p, b, n, m);
-    const long long per = max(1ll, share_of(total, ctas));
-    before += static_cast<long long>(listed_of<S::ROWS>(p, b)) * kvh;
-    for (int x = 0; x < i; ++x)
-        before += listed(tile_of<S::ROWS>(p, n, m, x));
-    const Tile tile = tile_of<S::ROWS>(p, n, m, i);
-    const int size = listed(tile), row0 = blockIdx.y * kJoinRows, rows = min(kJoinRows, tile.rows - row0);
-    const int first = quotient(before, per), parts = quotient(before + max(size, 1) - 1, per) - first + 1;
     asm volatile("griddepcontrol.wait;" ::: "memory"); // every CTA: this grid's end stands for the list's as well
-    if (size == 0 || parts == 1 || rows <= 0)
+    const SharedTile what = *shared_tile<D, NT>(p, blockIdx.x);
+    const int parts = what.parts, row0 = blockIdx.y * kJoinRows;
+    if (parts == 0)
         return;
-    // The tile is the last one of its first CTA, unless it begins with it, and the first one of the others.
-    const float *from = p.parts_at + 2ll * first * S::SLOT;
-    const int skip = before > first * per ? S::SLOT : 0;
-    auto slot = [&](int c) { return from + 2ll * c * S::SLOT + (c == 0 ? skip : 0); };
+    int n, m;
+    lengths_of(p, what.b, n, m);
+    const Tile tile = tile_of<S::ROWS>(p, n, m, what.tile);
+    const int rows = min(kJoinRows, tile.rows - row0), b = what.b, kvh = what.kvh;
+    if (rows <= 0)
+        return;
+    // Its first part is where the tile began, the others are first parts of their CTAs.
+    const float *from = p.parts_at + static_cast<long long>(what.slot) * S::SLOT;
+    const float *others = p.parts_at + 2ll * blockIdx.x * S::SLOT;
+    auto slot = [&](int c) { return c ? others + 2ll * c * S::SLOT : from; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp < rows) {
         float mx = -INFINITY, l = 0.f;
@@ -900,7 +909,7 @@ __global__ void __launch_bounds__(kJoinThreads) window_e2m1_join_kernel(const __
     }
 }
 
-template <int D, int NT, bool BF16> int launch_rows(const TokensParams &p, int ctas, cudaStream_t stream) {
+template <int D, int NT, bool BF16> int launch_rows(const TokensParams &p, cudaStream_t stream) {
     using S = TokensShape<D, NT>;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
@@ -927,27 +936,27 @@ template <int D, int NT, bool BF16> int launch_rows(const TokensParams &p, int c
     cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(window_e2m1_list_kernel<D, NT, BF16>), S::SMEM, done);
     if (e != cudaSuccess)
         return static_cast<int>(e);
-    cfg.gridDim = dim3(ctas);
+    cfg.gridDim = dim3(p.ctas);
     cfg.numAttrs = 0;
     e = cudaLaunchKernelEx(&cfg, window_e2m1_list_kernel<D, NT, BF16>, p);
     if (e != cudaSuccess)
         return static_cast<int>(e);
     // The join is set up while the list's kernel runs, and waits for its end before it reads the parts.
-    cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.kv_heads * p.tiles, S::ROWS / kJoinRows);
+    cfg.gridDim = dim3(p.ctas, S::ROWS / kJoinRows);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
-    return static_cast<int>(cudaLaunchKernelEx(&cfg, window_e2m1_join_kernel<D, NT>, p, ctas));
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, window_e2m1_join_kernel<D, NT>, p));
 }
-template <int D> int launch_d(const TokensParams &p, int ctas, bool bf16, cudaStream_t stream) {
+template <int D> int launch_d(const TokensParams &p, bool bf16, cudaStream_t stream) {
     const int rows = p.group * p.q_len;
     if (rows <= 8)
-        return bf16 ? launch_rows<D, 1, true>(p, ctas, stream) : launch_rows<D, 1, false>(p, ctas, stream);
+        return bf16 ? launch_rows<D, 1, true>(p, stream) : launch_rows<D, 1, false>(p, stream);
     if (rows <= 16)
-        return bf16 ? launch_rows<D, 2, true>(p, ctas, stream) : launch_rows<D, 2, false>(p, ctas, stream);
-    return bf16 ? launch_rows<D, 3, true>(p, ctas, stream) : launch_rows<D, 3, false>(p, ctas, stream);
+        return bf16 ? launch_rows<D, 2, true>(p, stream) : launch_rows<D, 2, false>(p, stream);
+    return bf16 ? launch_rows<D, 3, true>(p, stream) : launch_rows<D, 3, false>(p, stream);
 }
 
 // How a call is split: CTAs of a cluster, or (parts 0) of the list.
@@ -966,16 +975,16 @@ Split split_of(const WindowE2m1Args &a) {
         keys = std::min(keys, static_cast<long long>(a.window) + c.q_len + a.right + a.sinks);
     const long long of_tile = (keys + kCacheBlock - 1) / kCacheBlock + 1;
     const long long tiles = static_cast<long long>(s.tiles) * c.batch * c.kv_heads;
-    const long long most = (s.rows == 8 ? 2ll : 1ll) * fmha_sm_count();
+    const long long most = std::min<long long>(kJoinParts, (s.rows == 8 ? kCtas<1> : kCtas<2>) * fmha_sm_count()); // CTAs at once
     s.parts = 1;
-    while (s.parts < kMaxParts && tiles * s.parts * 2 <= most && of_tile >= 2ll * s.parts * 16)
+    while (s.parts < kMaxParts && tiles * s.parts * 2 <= most && of_tile >= 2ll * s.parts * 8)
         s.parts *= 2;
     s.ctas = 0;
     s.workspace = 0;
-    if (tiles * of_tile > 64 * most) {
+    if (tiles * of_tile > 32 * most) {
         s.parts = 0;
         s.ctas = static_cast<int>(most);
-        s.workspace = 2ull * most * s.rows * (cache_width(c.hd) + 2) * 4;
+        s.workspace = most * (2ull * s.rows * (cache_width(c.hd) + 2) * 4 + sizeof(SharedTile));
     }
     return s;
 }
@@ -1014,6 +1023,7 @@ int window_e2m1_tokens_launch(const WindowE2m1Args &a, cudaStream_t stream) {
     p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
     const Split split = split_of(a);
     p.parts = split.parts;
+    p.ctas = split.ctas;
     p.tiles = split.tiles;
     p.batch = c.batch;
     p.parts_at = static_cast<float *>(a.workspace);
@@ -1021,13 +1031,13 @@ int window_e2m1_tokens_launch(const WindowE2m1Args &a, cudaStream_t stream) {
     const bool bf16 = a.dtype == kBF16;
     switch (cache_width(c.hd)) {
     case 32:
-        return launch_d<32>(p, split.ctas, bf16, stream);
+        return launch_d<32>(p, bf16, stream);
     case 64:
-        return launch_d<64>(p, split.ctas, bf16, stream);
+        return launch_d<64>(p, bf16, stream);
     case 96:
-        return launch_d<96>(p, split.ctas, bf16, stream);
+        return launch_d<96>(p, bf16, stream);
     default:
-        return launch_d<128>(p, split.ctas, bf16, stream);
+        return launch_d<128>(p, bf16, stream);
     }
 }
 
