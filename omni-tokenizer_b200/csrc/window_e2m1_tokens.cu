@@ -40,7 +40,7 @@ namespace omni_b200 {
 namespace {
 
 constexpr int kMaxParts = 16;
-constexpr int kMostRows = 64; // of a key head, group * q_len
+constexpr int kMostRows = 512; // of a key head, group * q_len
 constexpr float kLazy = 8.f; // log2 units a score may be above the reference
 
 struct TokensParams {
@@ -51,8 +51,8 @@ struct TokensParams {
     long long qs[3], os[3];
     const int *lengths, *q_lengths;
     int parts; // CTAs of a cluster, or 0: the list
-    int ctas;  // of the list
-    uint32_t group_inv; // ceil(2^16 / group): rows of a call are few (kMostRows), their quotients by it exact
+    int ctas;       // of the list
+    uint32_t group_inv; // ceil(2^20 / group): exact for quotients of numbers up to kMostRows by group up to it
     int batch, kv_heads, group, q_len, kv_len, hd, tiles; // tiles of rows that a sequence may have
     int window, right, sinks;
     int out_dtype;
@@ -140,7 +140,7 @@ struct Tile {
     int n, m, row0, rows, pos0;
     int first, last, low, high, sink, sink_blocks, begin, blocks;
 };
-__device__ __forceinline__ int query_of(const TokensParams &p, int row) { return static_cast<int>(row * p.group_inv >> 16); }
+__device__ __forceinline__ int query_of(const TokensParams &p, int row) { return static_cast<int>(row * p.group_inv >> 20); }
 __device__ __forceinline__ void lengths_of(const TokensParams &p, int b, int &n, int &m) {
     n = max(0, min(p.lengths[b], p.kv_len));
     m = p.q_lengths ? max(0, min(p.q_lengths[b], p.q_len)) : p.q_len;
@@ -165,7 +165,7 @@ template <int ROWS> __device__ __forceinline__ Tile tile_of(const TokensParams &
     return t;
 }
 // Its length in the list: beginning and ending a tile takes a CTA as long as some blocks do
-// (1.2 us against 0.13 us for one: 64 x up to 16384 keys TILECOST), so it counts for those as well.
+// (3 us against 0.22 us for one; 64 x up to 16384 keys 124 us with 8 here, 122 with 16), so it counts for those as well.
 constexpr int kTileCost = 16;
 __device__ __forceinline__ int listed(const Tile &t) { return t.rows > 0 ? kTileCost + t.blocks : 0; }
 // Blocks of all tiles of a sequence's key head.
@@ -638,34 +638,50 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
         }
         *reinterpret_cast<float4 *>(&mine.o[0][r][col]) = v;
     });
-    if (parts > 1)
-        cluster_sync();
-    else
+    if (parts == 1) {
         __syncthreads();
+        for (int x = threadIdx.x; x < S::ROWS * D; x += S::WARPS * 32) {
+            const int r = x / D, col = x - r * D;
+            if (r < seg.tile.rows && col < p.hd)
+                store_out(p, seg.tile, seg.b, seg.kvh, r, col, mine.o[0][r][col], mine.cta_l[r]);
+        }
+        return;
+    }
+    // The CTAs' parts: their weights once for each row (over the ring, which is read), then each
+    // CTA its share of the columns.
+    float(*weight)[S::ROWS] = reinterpret_cast<float(*)[S::ROWS]>(smem), (*sums)[S::ROWS] = weight + kMaxParts;
+    cluster_sync();
+    for (int x = threadIdx.x; x < parts * S::ROWS; x += S::WARPS * 32) {
+        const int k = x / S::ROWS, r = x - k * S::ROWS;
+        weight[k][r] = peer_load(peer(&mine.cta_m[r], k));
+        sums[k][r] = peer_load(peer(&mine.cta_l[r], k));
+    }
+    __syncthreads();
+    if (threadIdx.x < S::ROWS) {
+        const int r = threadIdx.x;
+        float mx = -INFINITY, l = 0.f;
+        for (int k = 0; k < parts; ++k)
+            mx = fmaxf(mx, weight[k][r]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        for (int k = 0; k < parts; ++k) {
+            const float f = ex2_approx(weight[k][r] - base);
+            weight[k][r] = f;
+            l += f * sums[k][r];
+        }
+        sums[0][r] = l;
+    }
+    __syncthreads();
     for (int x = part * S::WARPS * 32 + threadIdx.x; x < S::ROWS * D; x += parts * S::WARPS * 32) {
         const int r = x / D, col = x - r * D;
         if (r >= seg.tile.rows || col >= p.hd)
             continue;
-        float l, v;
-        if (parts > 1) {
-            float mx = -INFINITY;
-            for (int k = 0; k < parts; ++k)
-                mx = fmaxf(mx, peer_load(peer(&mine.cta_m[r], k)));
-            const float base = mx == -INFINITY ? 0.f : mx;
-            l = v = 0.f;
-            for (int k = 0; k < parts; ++k) {
-                const float f = exp2f(peer_load(peer(&mine.cta_m[r], k)) - base);
-                l += f * peer_load(peer(&mine.cta_l[r], k));
-                v += f * peer_load(peer(&mine.o[0][r][col], k));
-            }
-        } else {
-            l = mine.cta_l[r];
-            v = mine.o[0][r][col];
-        }
-        store_out(p, seg.tile, seg.b, seg.kvh, r, col, v, l);
+        float v = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < parts; ++k)
+            v += weight[k][r] * peer_load(peer(&mine.o[0][r][col], k));
+        store_out(p, seg.tile, seg.b, seg.kvh, r, col, v, sums[0][r]);
     }
-    if (parts > 1)
-        cluster_sync(); // no CTA leaves while another reads its part
+    cluster_sync(); // no CTA leaves while another reads its part
 }
 
 // Quotients that mostly need 32 bits only.
@@ -831,9 +847,10 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
 }
 
 // Joins the parts of the tiles that several CTAs share: a CTA for each of the list's, and two
-// rows of the tile that begins there (with eight, few tiles of many parts met in few SMs: 131072
-// keys x 8 heads 45 -> 41 us).  A part's weight is worked out once for a row; SHARES threads
-// share a column's parts.
+// rows of the tile that begins there (few tiles of many parts would meet in few SMs otherwise:
+// 131072 keys x 8 heads, 75 parts each, 40 us so and 59 with eight rows, 64 x up to 16384 keys
+// 122 either way).  A part's weight is worked out once for a row; SHARES threads share a
+// column's parts.
 constexpr int kJoinThreads = 256, kJoinParts = 1024, kJoinRows = 2;
 template <int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads) window_e2m1_join_kernel(const __grid_constant__ TokensParams p) {
@@ -882,8 +899,9 @@ __global__ void __launch_bounds__(kJoinThreads) window_e2m1_join_kernel(const __
     }
     __syncthreads();
     const int of = threadIdx.x / FOURS, x = threadIdx.x % FOURS * 4, r = x / D, col = x % D;
+    const bool mine = of < SHARES && r < rows;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (of < SHARES && r < rows) {
+    if (mine) {
 #pragma unroll 8
         for (int c = of; c < parts; c += SHARES) {
             const float4 o = *reinterpret_cast<const float4 *>(slot(c) + 2 * S::ROWS + row0 * D + x);
@@ -897,15 +915,15 @@ __global__ void __launch_bounds__(kJoinThreads) window_e2m1_join_kernel(const __
             *reinterpret_cast<float4 *>(&share[of - 1][x]) = make_float4(v[0], v[1], v[2], v[3]);
     }
     __syncthreads();
-    if (of == 0 && r < rows) {
+    if (of || !mine)
+        return;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 4; ++e) {
 #pragma unroll
-            for (int k = 0; k < SHARES - 1; ++k)
-                v[e] += share[k][x + e];
-            if (col + e < p.hd)
-                store_out(p, tile, b, kvh, row0 + r, col + e, v[e], total_l[r]);
-        }
+        for (int k = 0; k < SHARES - 1; ++k)
+            v[e] += share[k][x + e];
+        if (col + e < p.hd)
+            store_out(p, tile, b, kvh, row0 + r, col + e, v[e], total_l[r]);
     }
 }
 
@@ -963,6 +981,7 @@ template <int D> int launch_d(const TokensParams &p, bool bf16, cudaStream_t str
 struct Split {
     int rows, tiles, parts, ctas;
     size_t workspace;
+    double us; // about what it takes
 };
 Split split_of(const WindowE2m1Args &a) {
     const CacheArgs &c = a.cache;
@@ -977,14 +996,27 @@ Split split_of(const WindowE2m1Args &a) {
     const long long tiles = static_cast<long long>(s.tiles) * c.batch * c.kv_heads;
     const long long most = std::min<long long>(kJoinParts, (s.rows == 8 ? kCtas<1> : kCtas<2>) * fmha_sm_count()); // CTAs at once
     s.parts = 1;
-    while (s.parts < kMaxParts && tiles * s.parts * 2 <= most && of_tile >= 2ll * s.parts * 8)
+    // (Clusters of 16 with 24 rows do not all fit at once: 2 x 2048 keys, 20 rows, 23 us with 16, 12 with 8.)
+    const int most_parts = s.rows == 24 ? 8 : kMaxParts;
+    while (s.parts < most_parts && tiles * s.parts * 2 <= most && of_tile >= 2ll * s.parts * 8)
         s.parts *= 2;
-    s.ctas = 0;
+    // In microseconds, as measured: a CTA's blocks one after another, slower the more CTAs share
+    // its SM; the list has its second kernel on top, but also evens out sequences that are
+    // shorter than kv_len, which is not known here, and gets a tenth for that.  Measured, cluster
+    // / list, 8 key heads of 128: 1 x 8192 10.5 / 13.5, 1 x
+    // 32768 22.7 / 19.9, 1 x 65536 39.6 / 25.7, 16 x 4096 15.9 / 22.1, 64 x 2048 26.0 / 32.0, 64
+    // x up to 4096 46.9 / 45.3, 64 x up to 16384 208 / 122.
+    const double sms = fmha_sm_count(), ctas = static_cast<double>(tiles) * s.parts, slow = (s.rows == 8 ? 1.0 : 1.6) * (0.1 + 0.9 * cache_width(c.hd) / 128);
+    const double rounds = std::max(1.0, ctas / most);
+    const double cluster = 1 + 4 * rounds + slow * of_tile / s.parts * rounds * (0.11 + 0.028 * std::min(ctas, static_cast<double>(most)) / sms);
+    const double total = static_cast<double>(tiles) * (of_tile + kTileCost);
+    s.ctas = static_cast<int>(std::min<double>(most, std::ceil(total / 32)));
+    const double list = 13 + slow * total / s.ctas * (0.11 + 0.028 * s.ctas / sms);
     s.workspace = 0;
-    if (tiles * of_tile > 32 * most) {
+    s.us = std::min(list, cluster);
+    if (list < 1.1 * cluster) {
         s.parts = 0;
-        s.ctas = static_cast<int>(most);
-        s.workspace = most * (2ull * s.rows * (cache_width(c.hd) + 2) * 4 + sizeof(SharedTile));
+        s.workspace = s.ctas * (2ull * s.rows * (cache_width(c.hd) + 2) * 4 + sizeof(SharedTile));
     }
     return s;
 }
@@ -1011,7 +1043,7 @@ int window_e2m1_tokens_launch(const WindowE2m1Args &a, cudaStream_t stream) {
     p.q_lengths = c.q_lengths;
     p.kv_heads = c.kv_heads;
     p.group = a.heads / c.kv_heads;
-    p.group_inv = (65536u + p.group - 1) / p.group;
+    p.group_inv = ((1u << 20) + p.group - 1) / p.group;
     p.q_len = c.q_len;
     p.kv_len = a.kv_len;
     p.hd = c.hd;
@@ -1042,9 +1074,24 @@ int window_e2m1_tokens_launch(const WindowE2m1Args &a, cudaStream_t stream) {
 }
 
 // Few rows read the cache as it is; for others the keys and values go back to 16 bits in the
-// workspace (exactly), and the prompts' kernel reads them.
+// workspace (exactly), and the prompts' kernel reads them.  What each takes, in microseconds as
+// measured: the prompts' kernel has blocks of 128 rows, whose steps of 64 keys come one after
+// another, in rounds of what the SMs hold.  Measured, few rows / prompts, 32/8 heads of 128: one
+// sequence of 8192 keys, 16 queries 23 / 109; 32
+// queries 36 / 109, 128 queries 81 / 109; 16 of up to 4096 keys, 32 queries 103 / 128, 64 queries
+// 155 / 129; one of 1024 keys, 100 queries 20 / 22.
 static bool few_rows(const WindowE2m1Args &a) {
-    return static_cast<long long>(a.heads / a.cache.kv_heads) * a.cache.q_len <= kMostRows;
+    const CacheArgs &c = a.cache;
+    if (static_cast<long long>(a.heads / c.kv_heads) * c.q_len > kMostRows)
+        return false;
+    double keys = a.kv_len;
+    if (a.window > 0)
+        keys = std::min<double>(keys, static_cast<double>(a.window) + c.q_len + a.right + a.sinks);
+    const double steps = std::min<double>(a.kv_len, keys + 127) / 64 + 1;
+    const double blocks = static_cast<double>(c.batch) * a.heads * ((c.q_len + 127) / 128);
+    const double read = 2.0 * c.batch * c.kv_heads * keys * c.hd * 2.6 / 4e6;
+    const double prompt = 10 + read + 0.7 * steps * std::max(1.0, blocks / (1.45 * fmha_sm_count()));
+    return split_of(a).us <= prompt;
 }
 
 size_t window_e2m1_workspace(const WindowE2m1Args &a) {
