@@ -1,12 +1,13 @@
 // cache_e2m1.cu -- keys and values into the 4-bit cache, and back out of it (layout and
 // formulas in cache_e2m1.cuh).
 //
-// Both move every element once and are bound by the memory's traffic.  A warp takes one
-// block (16 tokens) of one head, so that no two warps share a byte: the values of tokens 2c
-// and 2c + 1 lie in one, and a call may bring only one of the two.  A lane takes groups of
-// 32 columns of a token, whole: its largest magnitude needs no other lane, and its 64 bytes
-// are two memory sectors.  Keys lie in the cache as they come; values change places
-// through shared memory.
+// Both move every element once and are bound by the memory's traffic.  A warp takes the keys
+// or the values of one block (16 tokens) of one head, so that no two warps share a byte: the values of tokens 2c
+// and 2c + 1 lie in one, and a call may bring only one of the two.  A lane takes eight columns
+// of a token at a time, 16 bytes, and four lanes a group, so that rows are read and written
+// whole by each instruction (with 32 columns a lane, 8191 tokens x 8 heads of 128 written and
+// read back: WRITEFIG).  Keys lie in the cache as they come; values change places through
+// shared memory.
 #include "cache_e2m1.cuh"
 #include "layer.h"
 
@@ -34,13 +35,13 @@ struct Piece {
     long long zero;
 };
 __device__ __forceinline__ bool piece_of(const RowsParams &p, Piece &w) {
-    const long long at = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    const uint32_t at = blockIdx.x * kWarps + (threadIdx.x >> 5); // below 2^32: the entry points see to it
     if (at >= p.warps)
         return false;
-    const long long of_head = at / p.kv_heads;
+    const uint32_t of_head = at / static_cast<uint32_t>(p.kv_heads);
     w.head = static_cast<int>(at - of_head * p.kv_heads);
-    w.b = static_cast<int>(of_head / p.blocks);
-    const int j = static_cast<int>(of_head - static_cast<long long>(w.b) * p.blocks);
+    w.b = static_cast<int>(of_head / static_cast<uint32_t>(p.blocks));
+    const int j = static_cast<int>(of_head - static_cast<uint32_t>(w.b) * p.blocks);
     const long long n = max(p.lengths[w.b], 0);
     const long long m = p.q_lengths ? max(0, min(p.q_lengths[w.b], p.q_len)) : p.q_len;
     const long long first = p.whole ? 0 : max(n - m, 0ll);
@@ -55,46 +56,37 @@ __device__ __forceinline__ bool piece_of(const RowsParams &p, Piece &w) {
     return true;
 }
 
-__device__ __forceinline__ uint32_t abs_bits(uint32_t pair) { return pair & 0x7fff7fffu; }
-
-// Quantises 32 columns (those behind `cols` are zeros): scale's f16 bits, and values in q.
-template <typename T> __device__ __forceinline__ uint16_t quantize_group(const T *x, int cols, uint4 &q) {
-    Vec8<T> in[4];
-    uint32_t top2 = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        in[i].w[0] = make_uint4(0u, 0u, 0u, 0u);
-        if (i * 8 < cols)
-            in[i] = load8(x + i * 8);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t m = __vmaxu2(__vmaxu2(abs_bits(in[i].w[0].x), abs_bits(in[i].w[0].y)),
-                                    __vmaxu2(abs_bits(in[i].w[0].z), abs_bits(in[i].w[0].w)));
-        top2 = __vmaxu2(top2, m);
-    }
-    // Magnitudes' bits order as the magnitudes do, infinities and NaN above them.
-    const uint16_t top = static_cast<uint16_t>(max(top2 & 0xffffu, top2 >> 16));
-    T amax;
-    *reinterpret_cast<uint16_t *>(&amax) = top;
-    const float a = to_float(amax);
+// Quantises eight columns, four neighbouring lanes a group: scale's f16 bits, and the word.
+// Quotients in the middle of two values have to be exact, which a product with the scale's
+// reciprocal is not.  It is within 2^-22 of the quotient; another quotient is at least 2^-11 of
+// it away from a middle (an input has 11 significant bits, a middle times a scale 9), 2^-13 for
+// the smallest middle, 1/4.  So rounding the product to multiples of 2^-14 makes middles exact
+// and moves nothing else to one or across it: one addition, and its subtraction.
+template <typename T> __device__ __forceinline__ uint16_t quantize_words(const Vec8<T> &in, uint32_t &word) {
+    constexpr uint32_t kAbs = 0x7fff7fffu;
+    uint32_t top = __vmaxu2(__vmaxu2(in.w[0].x & kAbs, in.w[0].y & kAbs), __vmaxu2(in.w[0].z & kAbs, in.w[0].w & kAbs));
+    top = max(top & 0xffffu, top >> 16); // magnitudes' bits order as they do, infinities and NaN above them
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint16_t bits = static_cast<uint16_t>(top);
+    const float a = to_float(*reinterpret_cast<const T *>(&bits));
     const bool finite = a <= 3.402823466e38f;
     const float scale = cache_scale(finite ? a : 0.f);
-    const Divisor d = divisor_of(scale);
-    uint32_t w[4];
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+    constexpr float kGrid = 768.f; // 1.5 * 2^9: steps of 2^-14 about it
+    float f[8];
+    unpack8(in, f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float f[8];
-        unpack8(in[i], f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) // exact quotients: 16-bit inputs meet the middle of two values
-            f[e] = d.quotient<true>(f[e]);
-        w[i] = e2m1x8(f);
+    for (int e = 0; e < 8; e += 2) {
+        ffma2(f[e], f[e + 1], f[e], f[e + 1], inv, inv, kGrid, kGrid);
+        fadd2(f[e], f[e + 1], f[e], f[e + 1], -kGrid, -kGrid);
     }
-    q = make_uint4(w[0], w[1], w[2], w[3]);
+    word = e2m1x8(f);
     return finite ? __half_as_ushort(__float2half_rn(scale)) : kScaleNaN;
 }
 
+// blockIdx.y: keys, or values.
 template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32) cache_write_kernel(const __grid_constant__ RowsParams p) {
     using B = CacheBlock<D>;
     __shared__ __align__(16) uint8_t values[kWarps][8 * D];
@@ -106,21 +98,38 @@ template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32) cach
     if (page < 0)
         return;
     const int lane = threadIdx.x & 31;
+    const bool keys = blockIdx.y == 0;
     uint8_t *to = p.cache.block_at(page, w.head, within, B::BYTES), *mine = values[threadIdx.x >> 5];
-    const T *k = static_cast<const T *>(p.k) + w.b * p.ks[0] + w.head * p.ks[1];
-    const T *v = static_cast<const T *>(p.v) + w.b * p.vs[0] + w.head * p.vs[1];
-    uint16_t *k_scales = reinterpret_cast<uint16_t *>(to + B::KEY_SCALES);
-    uint16_t *v_scales = reinterpret_cast<uint16_t *>(to + B::VALUE_SCALES);
+    const long long *strides = keys ? p.ks : p.vs;
+    const T *from = static_cast<const T *>(keys ? p.k : p.v) + w.b * strides[0] + w.head * strides[1];
+    uint16_t *scales = reinterpret_cast<uint16_t *>(to + (keys ? B::KEY_SCALES : B::VALUE_SCALES));
+    uint8_t *rows = keys ? to + B::KEYS : mine;
     const int base = w.block * kCacheBlock, r0 = w.t0 - base, r1 = w.t1 - base;
-    for (int i = lane; i < (r1 - r0) * B::G; i += 32) {
-        const int r = r0 + i / B::G, g = i % B::G;
-        const long long row = base + r - w.zero;
-        uint4 q;
-        k_scales[B::key_scale(r, g)] = quantize_group(k + row * p.ks[2] + g * 32, p.hd - g * 32, q);
-        *reinterpret_cast<uint4 *>(to + B::KEYS + r * (D / 2) + g * 16) = q;
-        v_scales[B::value_scale(r, g)] = quantize_group(v + row * p.vs[2] + g * 32, p.hd - g * 32, q);
-        *reinterpret_cast<uint4 *>(mine + r * (D / 2) + g * 16) = q;
+    constexpr int WORDS = D / 8, STEPS = kCacheBlock * WORDS / 32, AT_ONCE = STEPS < 8 ? STEPS : 8;
+    const Vec8<T> none{};
+    for (int i0 = 0; i0 < (r1 - r0) * WORDS; i0 += 32 * AT_ONCE) {
+        Vec8<T> in[AT_ONCE];
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; ++x) {
+            const int i = i0 + 32 * x + lane, r = r0 + i / WORDS, col = i % WORDS * 8;
+            in[x] = r < r1 && col < p.hd ? load8(from + (base + r - w.zero) * strides[2] + col) : none;
+        }
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; ++x) {
+            if (i0 + 32 * x >= (r1 - r0) * WORDS)
+                break; // the same for all lanes
+            const int i = i0 + 32 * x + lane, r = r0 + i / WORDS, c = i % WORDS;
+            uint32_t word;
+            const uint16_t scale = quantize_words(in[x], word);
+            if (r < r1) {
+                *reinterpret_cast<uint32_t *>(rows + r * (D / 2) + c * 4) = word;
+                if (c % 4 == 0)
+                    scales[keys ? B::key_scale(r, c / 4) : B::value_scale(r, c / 4)] = scale;
+            }
+        }
     }
+    if (keys)
+        return;
     __syncwarp();
     // Words of the values: columns g and g + 8 of tokens 2c, 2c + 1, 2c + 8 and 2c + 9.
     const int g = lane >> 2, c = lane & 3;
@@ -133,42 +142,39 @@ template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32) cach
             if (t < r0 || t >= r1)
                 keep |= 0x0f0fu << (16 * half + 4 * odd);
         }
+    // Of two tokens' rows of eight columns: bytes with both tokens of columns g % 2, g % 2 + 2, ...
+    const int right = g & 1 ? 4 : 0, left = 4 - right;
+    auto both = [&](uint32_t even, uint32_t odd) { return ((even >> right) & 0x0f0f0f0fu) | ((odd << left) & 0xf0f0f0f0u); };
+    const uint32_t pick = (g >> 1) | (4 + (g >> 1)) << 4; // byte g / 2 of two words
 #pragma unroll
     for (int x = 0; x < D / 16; ++x) {
-        uint32_t word = 0;
+        uint2 row[4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int odd = 0; odd < 2; ++odd) {
-                const int t = 2 * c + 8 * half + odd;
-                const uint2 row = *reinterpret_cast<const uint2 *>(mine + t * (D / 2) + x * 8);
-                word |= (((row.x >> (4 * g)) & 15u) | ((row.y >> (4 * g)) & 15u) << 8) << (16 * half + 4 * odd);
-            }
+        for (int e = 0; e < 4; ++e)
+            row[e] = *reinterpret_cast<const uint2 *>(mine + (2 * c + 8 * (e >> 1) + (e & 1)) * (D / 2) + x * 8);
+        const uint32_t low = __byte_perm(both(row[0].x, row[1].x), both(row[0].y, row[1].y), pick);
+        const uint32_t high = __byte_perm(both(row[2].x, row[3].x), both(row[2].y, row[3].y), pick);
+        uint32_t word = __byte_perm(low, high, 0x5410);
         uint32_t *at = reinterpret_cast<uint32_t *>(to + B::VALUES + B::value_word(x, lane));
-        *at = keep ? (word & ~keep) | (*at & keep) : word;
+        if (keep)
+            word = (word & ~keep) | (*at & keep);
+        *at = word;
     }
 }
 
-// Stores 32 columns of a token, as many as there are.
-template <typename T> __device__ __forceinline__ void store_group(T *y, int cols, const uint4 &q, uint16_t scale) {
+// Stores eight columns, f16 pairs, times their scale.
+template <typename T> __device__ __forceinline__ void store_columns(T *y, const uint32_t (&h)[4], uint16_t scale) {
     const float s = __half2float(__ushort_as_half(scale));
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    float f[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t h[4];
-        f16x8(w[i], h);
-        float f[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&h[e]));
-            f[2 * e] = two.x * s;
-            f[2 * e + 1] = two.y * s;
-        }
-        if (i * 8 < cols)
-            store8(y + i * 8, pack8<T>(f));
+    for (int e = 0; e < 4; ++e) {
+        const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&h[e]));
+        fmul2(f[2 * e], f[2 * e + 1], two.x, two.y, s, s);
     }
+    store8(y, pack8<T>(f));
 }
 
+// blockIdx.y: keys, or values.
 template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32) cache_read_kernel(const __grid_constant__ RowsParams p) {
     using B = CacheBlock<D>;
     __shared__ __align__(16) uint8_t values[kWarps][8 * D];
@@ -183,44 +189,66 @@ template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32) cach
             return;
     }
     const int lane = threadIdx.x & 31;
+    const bool keys = blockIdx.y == 0;
     int within;
     const int page = p.cache.page_of(w.b, w.block, within);
-    T *k = static_cast<T *>(const_cast<void *>(p.k)) + w.b * p.ks[0] + w.head * p.ks[1];
-    T *v = static_cast<T *>(const_cast<void *>(p.v)) + w.b * p.vs[0] + w.head * p.vs[1];
+    const long long *strides = keys ? p.ks : p.vs;
+    T *to = static_cast<T *>(const_cast<void *>(keys ? p.k : p.v)) + w.b * strides[0] + w.head * strides[1];
     const uint8_t *from = page < 0 ? nullptr : p.cache.block_at(page, w.head, within, B::BYTES);
+    const int r0 = w.t0 - base, r1 = w.t1 - base;
+    constexpr int WORDS = D / 8, STEPS = kCacheBlock * WORDS / 32;
     uint8_t *mine = values[threadIdx.x >> 5];
-    if (from)
+    if (from && !keys) {
+#pragma unroll
         for (int i = lane; i < 8 * D / 16; i += 32)
             reinterpret_cast<uint4 *>(mine)[i] = reinterpret_cast<const uint4 *>(from + B::VALUES)[i];
+    }
     __syncwarp();
-    const int r0 = w.t0 - base, r1 = w.t1 - base;
-    for (int i = lane; i < (r1 - r0) * B::G; i += 32) {
-        const int r = r0 + i / B::G, g = i % B::G;
-        const long long row = base + r - w.zero;
-        uint16_t ks = kScaleNaN, vs = kScaleNaN; // a page that the cache does not have reads as NaN
-        uint4 q = make_uint4(0u, 0u, 0u, 0u), u = q;
-        if (from) {
-            ks = *reinterpret_cast<const uint16_t *>(from + B::KEY_SCALES + 2 * B::key_scale(r, g));
-            vs = *reinterpret_cast<const uint16_t *>(from + B::VALUE_SCALES + 2 * B::value_scale(r, g));
-            q = *reinterpret_cast<const uint4 *>(from + B::KEYS + r * (D / 2) + g * 16);
-            uint32_t word[4];
+    // All of a warp's reads, then its writes.  Keys: a word a step.  Values: eight bytes, each
+    // the column's nibbles of two tokens.
+    uint32_t words[STEPS][2] = {};
+    uint16_t scales[STEPS];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                uint32_t low = 0, high = 0; // columns 0 to 7 and 8 to 15 of the 16
+    for (int x = 0; x < STEPS; ++x) {
+        const int i = 32 * x + lane, r = r0 + i / WORDS, c = i % WORDS;
+        scales[x] = kScaleNaN; // a page that the cache does not have reads as NaN
+        if (!from || r >= r1)
+            continue;
+        if (keys) {
+            words[x][0] = *reinterpret_cast<const uint32_t *>(from + B::KEYS + r * (D / 2) + c * 4);
+            scales[x] = *reinterpret_cast<const uint16_t *>(from + B::KEY_SCALES + 2 * B::key_scale(r, c / 4));
+        } else {
+            scales[x] = *reinterpret_cast<const uint16_t *>(from + B::VALUE_SCALES + 2 * B::value_scale(r, c / 4));
+            const uint8_t *at = mine + B::value_word(c / 2, r % 8 / 2) + r / 8 * 2 + c % 2;
+            uint32_t b[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int from_lane = 4 * e + (r % 8) / 2;
-                    const uint32_t two = *reinterpret_cast<const uint16_t *>(mine + B::value_word(2 * g + x, from_lane) + r / 8 * 2);
-                    low |= ((two >> (r % 2 * 4)) & 15u) << (4 * e);
-                    high |= ((two >> (8 + r % 2 * 4)) & 15u) << (4 * e);
-                }
-                word[2 * x] = low;
-                word[2 * x + 1] = high;
-            }
-            u = make_uint4(word[0], word[1], word[2], word[3]);
+            for (int e = 0; e < 8; ++e) // columns 8 c + e, of lane 4 e + (r % 8) / 2
+                b[e] = at[16 * B::W * e];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) // nibbles of two columns in bytes 0 and 2
+                words[x][h] = __byte_perm(__byte_perm(b[4 * h], b[4 * h + 1], 0x0040), __byte_perm(b[4 * h + 2], b[4 * h + 3], 0x0040), 0x5410);
         }
-        store_group(k + row * p.ks[2] + g * 32, p.hd - g * 32, q, ks);
-        store_group(v + row * p.vs[2] + g * 32, p.hd - g * 32, u, vs);
+    }
+#pragma unroll
+    for (int x = 0; x < STEPS; ++x) {
+        const int i = 32 * x + lane, r = r0 + i / WORDS, c = i % WORDS;
+        if (r >= r1 || c * 8 >= p.hd)
+            continue;
+        uint32_t h[4];
+        if (keys) {
+            f16x8(words[x][0], h);
+        } else {
+            uint32_t two[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t w = (words[x][e] >> (r % 2 * 4)) & 0x0f0f0f0fu;
+                w |= w >> 4;
+                f16x8(w, two);
+                h[2 * e] = two[0];
+                h[2 * e + 1] = two[2];
+            }
+        }
+        store_columns(to + (base + r - w.zero) * strides[2] + c * 8, h, scales[x]);
     }
 }
 
@@ -256,9 +284,9 @@ template <typename T, int D> int launch_rows(RowsParams &p, int batch, bool read
     if (ctas > 0x7fffffffll)
         return static_cast<int>(cudaErrorInvalidValue);
     if (read)
-        cache_read_kernel<T, D><<<static_cast<unsigned>(ctas), kWarps * 32, 0, stream>>>(p);
+        cache_read_kernel<T, D><<<dim3(static_cast<unsigned>(ctas), 2), kWarps * 32, 0, stream>>>(p);
     else if constexpr (sizeof(T) == 2)
-        cache_write_kernel<T, D><<<static_cast<unsigned>(ctas), kWarps * 32, 0, stream>>>(p);
+        cache_write_kernel<T, D><<<dim3(static_cast<unsigned>(ctas), 2), kWarps * 32, 0, stream>>>(p);
     return static_cast<int>(cudaGetLastError());
 }
 template <typename T> int launch_width(RowsParams &p, int batch, bool read, cudaStream_t stream) {

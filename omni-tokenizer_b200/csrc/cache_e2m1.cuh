@@ -68,9 +68,13 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-// The scale of a group whose largest magnitude is amax (finite): six significant bits.
+// The scale of a group whose largest magnitude is amax (finite, of at most 11 significant bits):
+// six significant bits of amax / 6.  The product with 1/6 is within 2^-23 of it and may miss the
+// middle of two scales, from which any other quotient is 2^-11 away: rounded to 16 bits first,
+// it is the middle where the quotient is.
 __device__ __forceinline__ float cache_scale(float amax) {
-    uint32_t u = __float_as_uint(__fdiv_rn(amax, 6.f));
+    uint32_t u = __float_as_uint(amax * (1.f / 6.f));
+    u = (u + 0x80u) & ~0xffu;
     u = (u + 0x1ffffu + ((u >> 18) & 1u)) & ~0x3ffffu;
     return fminf(fmaxf(__uint_as_float(u), kScaleMin), kScaleMax);
 }
