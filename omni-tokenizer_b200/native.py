@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 import os
 from pathlib import Path
 
@@ -596,7 +597,7 @@ def rotary(q, k, positions, frequencies, axes=None, adjacent=False, inverse=Fals
     B, H, T, D = shape
     Hkv, k_ptr, k_to = 0, None, None
     if q_out is None:
-        q_out = q.new_empty(shape)
+        q_out = _t.empty_like(q)  # laid out as q is, where q's memory has no gaps
     elif q_out.shape != shape or q_out.dtype != dtype:
         _refuse("rotary: q_out must have q's shape and type")
     qb, qh, qt, qd = q.stride()
@@ -607,7 +608,7 @@ def rotary(q, k, positions, frequencies, axes=None, adjacent=False, inverse=Fals
         if k.shape != (B, Hkv, T, D) or Hkv == 0 or k.dtype != dtype:
             _refuse("rotary: k must be [B, Hkv, T, D] of q's type")
         if k_out is None:
-            k_out = k.new_empty(k.shape)
+            k_out = _t.empty_like(k)
         elif k_out.shape != k.shape or k_out.dtype != dtype:
             _refuse("rotary: k_out must have k's shape and type")
         kb, kh, kt, kd = k.stride()
@@ -759,6 +760,12 @@ def cache_read_e2m1(cache, head_dim, lengths, rows=None, q_lengths=None, table=N
     return k, v
 
 
+@functools.lru_cache(maxsize=4096)
+def _window_workspace(*sizes):
+    """Asked once for the sizes of a call: the question costs as much as a tensor."""
+    return library().lib.omni_b200_attention_window_e2m1_workspace(*sizes)
+
+
 def attention_window_e2m1(q, cache, lengths, q_lengths=None, table=None, window=0, sinks=0, right=0, scale=0.0,
                           kv_len=None, out=None, out_dtype=None, stream=None):
     """attention_window over a cache in 4 bits: q [B, H, T, D] (bfloat16 or float16, strides
@@ -779,7 +786,7 @@ def attention_window_e2m1(q, cache, lengths, q_lengths=None, table=None, window=
     if not (-_INT < window < _INT and -_INT < right < _INT and -_INT < sinks < _INT and 0 <= kv_len < _INT
             and max(B, H, T) < _INT):
         _refuse("attention_window_e2m1: sizes, window, right and sinks must be below 2^31")
-    size = library().lib.omni_b200_attention_window_e2m1_workspace(B, H, Hkv, T, kv_len, D, window, right, sinks)
+    size = _window_workspace(B, H, Hkv, T, kv_len, D, window, right, sinks)
     if stream is not None and (out is None or size):
         with _on("attention_window_e2m1", stream, q):
             return attention_window_e2m1(q, cache, lengths, q_lengths, table, window, sinks, right, scale, kv_len, out,

@@ -119,8 +119,8 @@ def _window(lib, cache=None, **k):
     (1, dict(scale=float("nan"))), (1, dict(scale=float("inf"))), (1, dict(dtype=F32)), (1, dict(out_dtype=F16)),
     (1, dict(q=K + 8)), (1, dict(out=KO + 1)), (1, dict(rows=2, strides=I6(512, 128, 60, 512, 128, 64))),
     (1, dict(strides=I6(256, 68, 64, 256, 64, 64))), (1, dict(strides=I6(256, 64, 64, 256, 0, 64))),
-    (1, dict(rows=96)), (1, dict(rows=96, workspace=Q, bytes=2 * 2 * 96 * 64 * 4 - 1)),
-    (1, dict(rows=96, workspace=Q + 8, bytes=1 << 20)), (1, dict(rows=1 << 30, batch=1 << 10)),
+    (1, dict(rows=600)), (1, dict(rows=600, workspace=Q, bytes=2 * 2 * 96 * 64 * 4 - 1)),
+    (1, dict(rows=600, workspace=Q + 8, bytes=1 << 20)), (1, dict(rows=1 << 30, batch=1 << 10)),
     (1, dict(cache="none")),
 ] + [(1, dict(cache=c)) for c in BAD_CACHES])
 def test_window_refuses(lib, status, bad):
@@ -204,15 +204,15 @@ NAMES = ["rotary", "rotary of q alone", "cache_read_e2m1", "attention_window_e2m
 
 def _calls(torch, device):
     g = torch.Generator().manual_seed(3)
-    q = torch.randn(2, 4, 200, 64, generator=g).to(torch.bfloat16).to(device)
-    where = torch.arange(200, dtype=torch.int32, device=device).expand(2, 200)
+    q = torch.randn(2, 4, 600, 64, generator=g).to(torch.bfloat16).to(device)
+    where = torch.arange(600, dtype=torch.int32, device=device).expand(2, 600)
     frequencies = torch.rand(32, generator=g).to(device)
-    cache = torch.zeros(2, 2, 208 // 16 * 1152, dtype=torch.uint8, device=device)
-    held = torch.full((2,), 200, dtype=torch.int32, device=device)
+    cache = torch.zeros(2, 2, 608 // 16 * 1152, dtype=torch.uint8, device=device)
+    held = torch.full((2,), 600, dtype=torch.int32, device=device)
     return {
         "rotary": lambda s: ob.rotary(q, q[:, :2], where, frequencies, stream=s),
         "rotary of q alone": lambda s: ob.rotary(q, None, where, frequencies, stream=s),
-        "cache_read_e2m1": lambda s: ob.cache_read_e2m1(cache, 64, held, rows=200, stream=s),
+        "cache_read_e2m1": lambda s: ob.cache_read_e2m1(cache, 64, held, rows=600, stream=s),
         "attention_window_e2m1": lambda s: ob.attention_window_e2m1(q[:, :, :1], cache, held, stream=s),
         "attention_window_e2m1 of a prompt": lambda s: ob.attention_window_e2m1(q, cache, held, stream=s),
         "attention_window_e2m1 of a prompt into a tensor":
@@ -233,16 +233,18 @@ def test_allocations_and_launch_are_the_streams(lib, monkeypatch, name):
         yield
         entered.pop()
 
-    new_empty = torch.Tensor.new_empty
+    def watched(make):
+        def call(*args, **kwargs):
+            made.append(bool(entered) and entered[-1] is stream)
+            return make(*args, **kwargs)
 
-    def watched(*args, **kwargs):
-        made.append(bool(entered) and entered[-1] is stream)
-        return new_empty(*args, **kwargs)
+        return call
 
     call = _calls(torch, "cpu")[name]
     native._t.codes  # looks torch's names up
     monkeypatch.setattr(native._t, "cuda", types.SimpleNamespace(stream=enter))
-    monkeypatch.setattr(torch.Tensor, "new_empty", watched)
+    monkeypatch.setattr(torch.Tensor, "new_empty", watched(torch.Tensor.new_empty))
+    monkeypatch.setattr(native._t, "empty_like", watched(torch.empty_like))
     monkeypatch.setattr(native, "_device_of", lambda *_: 0)
     monkeypatch.setattr(native, "_call", lambda *_: launched.append(bool(entered) and entered[-1] is stream))
     call(stream)
