@@ -8,9 +8,11 @@
 // becomes fp32 for sincospif (its error is below 2^-24 of a turn).
 //
 // The bound is the memory traffic: each element is read and written once.  A thread
-// holds the sines and cosines of V pairs of one token in registers and goes over heads,
-// so that they are computed once for `head_groups` heads' loads; neighbouring threads
-// take neighbouring columns, then tokens, so rows are read whole whatever the layout.
+// holds the sines and cosines of V pairs of one token in registers and goes over heads, so
+// that they are computed once for all heads of its group (gridDim.y groups); neighbouring
+// threads take neighbouring columns, then tokens, so rows are read whole whatever the layout.
+// 8192 tokens x 40 heads of 128 in bf16: 34 us, 4.9 TB/s with the launch; without angles it
+// would take 31.  fp32 angles would save nothing.
 #include "e4m3.cuh"
 #include "layer.h"
 
