@@ -759,7 +759,8 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
         int b = b0, of_head = listed_of<S::ROWS>(p, b);
         for (; b < b1 - 1 && from >= before + static_cast<long long>(of_head) * p.kv_heads; of_head = listed_of<S::ROWS>(p, b))
             before += static_cast<long long>(of_head) * p.kv_heads, ++b;
-        const int kvh = quotient(from - before, of_head);
+        // (Lengths that change under the kernel are a caller's mistake, but lead out of no array.)
+        const int kvh = max(0, min(quotient(from - before, max(of_head, 1)), p.kv_heads - 1));
         walk.tile = (static_cast<long long>(b) * p.kv_heads + kvh) * p.tiles;
         walk.at = before + static_cast<long long>(kvh) * of_head;
     }
@@ -846,7 +847,7 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
             }
             __syncthreads(); // the parts' place is free
         }
-    } while (walk.at < to);
+    } while (walk.at < to && walk.tile < static_cast<long long>(p.batch) * of_sequence);
 }
 
 // Joins the parts of the tiles that several CTAs share: a CTA for each of the list's, and two
@@ -971,26 +972,25 @@ template <int D, int NT, bool BF16> int launch_rows(const TokensParams &p, cudaS
     attr.val.programmaticStreamSerializationAllowed = 1;
     return static_cast<int>(cudaLaunchKernelEx(&cfg, window_e2m1_join_kernel<D, NT>, p));
 }
-template <int D> int launch_d(const TokensParams &p, bool bf16, cudaStream_t stream) {
-    const int rows = p.group * p.q_len;
-    if (rows <= 8)
+template <int D> int launch_d(const TokensParams &p, int rows, bool bf16, cudaStream_t stream) {
+    if (rows == 8)
         return bf16 ? launch_rows<D, 1, true>(p, stream) : launch_rows<D, 1, false>(p, stream);
-    if (rows <= 16)
+    if (rows == 16)
         return bf16 ? launch_rows<D, 2, true>(p, stream) : launch_rows<D, 2, false>(p, stream);
     return bf16 ? launch_rows<D, 3, true>(p, stream) : launch_rows<D, 3, false>(p, stream);
 }
 
-// How a call is split: CTAs of a cluster, or (parts 0) of the list.
+// How a call is split: rows of a tile, CTAs of a cluster, or (parts 0) of the list.
 struct Split {
     int rows, tiles, parts, ctas;
     size_t workspace;
     double us; // about what it takes
 };
-Split split_of(const WindowE2m1Args &a) {
+Split split_in(const WindowE2m1Args &a, int rows_of_tile) {
     const CacheArgs &c = a.cache;
     const long long rows = static_cast<long long>(a.heads / c.kv_heads) * c.q_len;
     Split s;
-    s.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 24;
+    s.rows = rows_of_tile;
     s.tiles = static_cast<int>((rows + s.rows - 1) / s.rows);
     long long keys = a.kv_len;
     if (a.window > 0)
@@ -1003,18 +1003,19 @@ Split split_of(const WindowE2m1Args &a) {
     const int most_parts = s.rows == 24 ? 8 : kMaxParts;
     while (s.parts < most_parts && tiles * s.parts * 2 <= most && of_tile >= 2ll * s.parts * 8)
         s.parts *= 2;
-    // In microseconds, as measured: a CTA's blocks one after another, slower the more CTAs share
-    // its SM; the list has its second kernel on top, but also evens out sequences that are
-    // shorter than kv_len, which is not known here, and gets a tenth for that.  Measured, cluster
-    // / list, 8 key heads of 128: 1 x 8192 10.5 / 13.5, 1 x
-    // 32768 22.7 / 19.9, 1 x 65536 39.6 / 25.7, 16 x 4096 15.9 / 22.1, 64 x 2048 26.0 / 32.0, 64
-    // x up to 4096 46.9 / 45.3, 64 x up to 16384 208 / 122.
-    const double sms = fmha_sm_count(), ctas = static_cast<double>(tiles) * s.parts, slow = (s.rows == 8 ? 1.0 : 1.6) * (0.1 + 0.9 * cache_width(c.hd) / 128);
+    // In microseconds, as measured: a CTA's blocks one after another, slower the more rows they
+    // meet and the more CTAs share its SM; the list has its second kernel on top, but also evens
+    // out sequences that are shorter than kv_len, which is not known here, and gets a tenth for
+    // that.  Measured, cluster / list, 8 key heads of 128, one row of four heads: 1 x 8192 keys
+    // 10.5 / 13.5, 1 x 32768 22.7 / 19.9, 1 x 65536 39.6 / 25.7, 16 x 4096 15.9 / 22.1, 64 x 2048
+    // 26.0 / 32.0, 64 x up to 4096 46.9 / 45.3, 64 x up to 16384 165 / 123.
+    const double sms = fmha_sm_count(), ctas = static_cast<double>(tiles) * s.parts;
+    const double block = (s.rows == 8 ? 1.0 : s.rows == 16 ? 1.3 : 1.7) * (0.1 + 0.9 * cache_width(c.hd) / 128);
     const double rounds = std::max(1.0, ctas / most);
-    const double cluster = 1 + 4 * rounds + slow * of_tile / s.parts * rounds * (0.11 + 0.028 * std::min(ctas, static_cast<double>(most)) / sms);
+    const double cluster = 1 + 4 * rounds + block * of_tile / s.parts * rounds * (0.11 + 0.028 * std::min(ctas, static_cast<double>(most)) / sms);
     const double total = static_cast<double>(tiles) * (of_tile + kTileCost);
     s.ctas = static_cast<int>(std::min<double>(most, std::ceil(total / 32)));
-    const double list = 13 + slow * total / s.ctas * (0.11 + 0.028 * s.ctas / sms);
+    const double list = 13 + block * total / s.ctas * (0.11 + 0.028 * s.ctas / sms);
     s.workspace = 0;
     s.us = std::min(list, cluster);
     if (list < 1.1 * cluster) {
@@ -1022,6 +1023,20 @@ Split split_of(const WindowE2m1Args &a) {
         s.workspace = s.ctas * (2ull * s.rows * (cache_width(c.hd) + 2) * 4 + sizeof(SharedTile));
     }
     return s;
+}
+// The cheapest height of a tile: high ones convert a block for more rows, low ones have more CTAs
+// and warps.  Measured, 8 / 16 / 24 rows: 1 x 8192 keys, 16 rows 11.8 / 13.3 us, 64 rows 20.1 /
+// 20.4 / 23.0; 2 x 2048, 20 rows 8.8 / 11.5 / 12.6; 16 x 4096 of 8192, 20 rows 47 / 52 / 40; 1 x
+// 131072, 16 rows 62 / 51.
+Split split_of(const WindowE2m1Args &a) {
+    const long long rows = static_cast<long long>(a.heads / a.cache.kv_heads) * a.cache.q_len;
+    Split best = split_in(a, 8);
+    for (int height = 16; height <= 24 && rows > height - 8; height += 8) {
+        const Split s = split_in(a, height);
+        if (s.us < best.us)
+            best = s;
+    }
+    return best;
 }
 
 } // namespace
@@ -1066,13 +1081,13 @@ int window_e2m1_tokens_launch(const WindowE2m1Args &a, cudaStream_t stream) {
     const bool bf16 = a.dtype == kBF16;
     switch (cache_width(c.hd)) {
     case 32:
-        return launch_d<32>(p, bf16, stream);
+        return launch_d<32>(p, split.rows, bf16, stream);
     case 64:
-        return launch_d<64>(p, bf16, stream);
+        return launch_d<64>(p, split.rows, bf16, stream);
     case 96:
-        return launch_d<96>(p, bf16, stream);
+        return launch_d<96>(p, split.rows, bf16, stream);
     default:
-        return launch_d<128>(p, bf16, stream);
+        return launch_d<128>(p, split.rows, bf16, stream);
     }
 }
 

@@ -40,25 +40,27 @@ def _names(call, tmp_path):
             for name, _, _ in launched(call, tmp_path)]
 
 
-# B, H, Hkv, T, D, page, lengths, window, sinks, kernels
+# B, H, Hkv, T, D, page, lengths, window, sinks, kernels, rows of a tile
 LIST, CLUSTER, PROMPT = ["e2m1_list", "e2m1_join"], ["e2m1_cluster"], ["cache_read", "window_prompt"]
 CASES = [
-    (1, 8, 2, 1, 64, 128, [65000], 0, 0, LIST),       # one tile for each key head, many parts
-    (1, 8, 2, 1, 128, 64, [20011], 0, 0, CLUSTER),
-    (2, 16, 1, 1, 128, 256, [33000, 7], 0, 0, LIST),  # 16 rows
-    (1, 40, 2, 1, 96, 64, [40000], 0, 0, LIST),       # 24 rows, of which 20 are there
-    (1, 8, 2, 40, 64, 48, [40000], 0, 0, LIST),       # seven tiles of rows
-    (1, 6, 2, 33, 80, 32, [3000], 700, 40, CLUSTER),
-    (1, 4, 4, 1, 32, 16, [120000], 0, 0, LIST),
-    (1, 8, 2, 300, 64, 64, [900], 0, 0, PROMPT),
-    (8, 16, 16, 128, 64, 64, [128] * 8, 0, 0, PROMPT),
+    (1, 8, 2, 1, 64, 128, [65000], 0, 0, LIST, 8),        # one tile for each key head, many parts
+    (1, 8, 2, 1, 128, 64, [20011], 0, 0, CLUSTER, 8),
+    (2, 16, 1, 1, 128, 256, [130000, 7], 0, 0, LIST, 16),
+    (1, 40, 2, 1, 96, 64, [100000], 0, 0, LIST, 24),      # of which 20 are there
+    (1, 8, 2, 40, 64, 48, [40000], 0, 0, LIST, 24),       # seven tiles of rows
+    (1, 6, 2, 33, 80, 32, [3000], 700, 40, CLUSTER, 8),
+    (1, 4, 4, 1, 32, 16, [120000], 0, 0, LIST, 8),
+    (64, 20, 2, 1, 64, 64, list(range(7, 1000, 16)) + [1000], 0, 0, CLUSTER, 16),
+    (16, 40, 2, 1, 64, 64, list(range(500, 2001, 100)), 1900, 5, CLUSTER, 24),
+    (1, 8, 2, 300, 64, 64, [900], 0, 0, PROMPT, None),
+    (8, 16, 16, 128, 64, 64, [128] * 8, 0, 0, PROMPT, None),
 ]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("case", CASES)
 def test_each_way(ob, tmp_path, case, dtype):  # noqa: F811
-    B, H, Hkv, T, D, page, lengths, window, sinks, kernels = case
+    B, H, Hkv, T, D, page, lengths, window, sinks, kernels, height = case
     cache, table, k, v = _paged(ob, B, Hkv, D, -(-max(lengths) // page), page, lengths, dtype, 60)
     q = _tensor((B, H, T, D), "tokens", dtype, 63)
     counts = [min(T, n) for n in lengths]
@@ -69,6 +71,8 @@ def test_each_way(ob, tmp_path, case, dtype):  # noqa: F811
         return ob.attention_window_e2m1(q, cache, held, q_lengths=m, table=table, window=window, sinks=sinks, out=out)
 
     assert _names(call, tmp_path) == kernels
+    if height:
+        assert all(f"ILi{-(-D // 32) * 32}ELi{height // 8}E" in name for name, _, _ in launched(call, tmp_path))
     call()
     _check(out, q, k, v, lengths, counts, window, 0, sinks, prompt=kernels == PROMPT)
     ob.library().sync_check()
