@@ -700,7 +700,7 @@ __device__ __forceinline__ long long share_of(long long total, int ctas) {
 // A tile that begins in a CTA's share of the list and ends in another's: for each CTA, behind
 // the parts' slots.  parts 0: there is none.
 struct alignas(16) SharedTile {
-    int b = 0, kvh = 0, tile = 0, slot = 0, parts = 0, unused[3] = {};
+    int b = 0, kvh = 0, tile = 0, slot = 0, parts = 0, n = 0, m = 0, unused = 0;
 };
 template <int D, int NT> __device__ __forceinline__ SharedTile *shared_tile(const TokensParams &p, int cta) {
     return reinterpret_cast<SharedTile *>(p.parts_at + 2ll * p.ctas * TokensShape<D, NT>::SLOT) + cta;
@@ -799,6 +799,8 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
                 t.kvh = s.kvh;
                 t.tile = in_b - s.kvh * p.tiles;
                 t.slot = s.slot;
+                t.n = s.tile.n;
+                t.m = s.tile.m;
                 t.parts = quotient(begin + size - 1, per) - static_cast<int>(blockIdx.x) + 1;
                 *shared_tile<D, NT>(p, blockIdx.x) = t;
             }
@@ -867,9 +869,7 @@ __global__ void __launch_bounds__(kJoinThreads) window_e2m1_join_kernel(const __
     const int parts = what.parts, row0 = blockIdx.y * kJoinRows;
     if (parts == 0)
         return;
-    int n, m;
-    lengths_of(p, what.b, n, m);
-    const Tile tile = tile_of<S::ROWS>(p, n, m, what.tile);
+    const Tile tile = tile_of<S::ROWS>(p, what.n, what.m, what.tile);
     const int rows = min(kJoinRows, tile.rows - row0), b = what.b, kvh = what.kvh;
     if (rows <= 0)
         return;
@@ -877,6 +877,16 @@ __global__ void __launch_bounds__(kJoinThreads) window_e2m1_join_kernel(const __
     const float *from = p.parts_at + static_cast<long long>(what.slot) * S::SLOT;
     const float *others = p.parts_at + 2ll * blockIdx.x * S::SLOT;
     auto slot = [&](int c) { return c ? others + 2ll * c * S::SLOT : from; };
+    // The first parts' columns are on their way while the weights are worked out.
+    constexpr int EARLY = 6;
+    const int of = threadIdx.x / FOURS, x = threadIdx.x % FOURS * 4, r = x / D, col = x % D;
+    const bool mine = of < SHARES && r < rows;
+    auto columns = [&](int c) { return *reinterpret_cast<const float4 *>(slot(c) + 2 * S::ROWS + row0 * D + x); };
+    float4 early[EARLY];
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i)
+        if (mine && of + i * SHARES < parts)
+            early[i] = columns(of + i * SHARES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp < rows) {
         float mx = -INFINITY, l = 0.f;
@@ -902,19 +912,21 @@ __global__ void __launch_bounds__(kJoinThreads) window_e2m1_join_kernel(const __
             total_l[warp] = l;
     }
     __syncthreads();
-    const int of = threadIdx.x / FOURS, x = threadIdx.x % FOURS * 4, r = x / D, col = x % D;
-    const bool mine = of < SHARES && r < rows;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (mine) {
-#pragma unroll 8
-        for (int c = of; c < parts; c += SHARES) {
-            const float4 o = *reinterpret_cast<const float4 *>(slot(c) + 2 * S::ROWS + row0 * D + x);
-            const float f = weight[r][c];
+        auto add = [&](const float4 &o, float f) {
             v[0] += f * o.x;
             v[1] += f * o.y;
             v[2] += f * o.z;
             v[3] += f * o.w;
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < EARLY; ++i)
+            if (of + i * SHARES < parts)
+                add(early[i], weight[r][of + i * SHARES]);
+#pragma unroll 4
+        for (int c = of + EARLY * SHARES; c < parts; c += SHARES)
+            add(columns(c), weight[r][c]);
         if (of)
             *reinterpret_cast<float4 *>(&share[of - 1][x]) = make_float4(v[0], v[1], v[2], v[3]);
     }
