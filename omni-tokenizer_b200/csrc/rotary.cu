@@ -30,7 +30,8 @@ struct RotaryParams {
     long long xs[2][3], ys[2][3]; // batch, head, token
     const void *positions, *frequencies;
     long long ps[3]; // axis, batch, token
-    long long items;
+    long long items, tail_items;
+    unsigned pair_blocks;
     int heads, all_heads; // of q; of q and k
     int tokens, hd, pairs, chunks, tail; // chunks: of V pairs; tail: of V columns that are copied
     int position_type;
@@ -59,20 +60,32 @@ __host__ __device__ constexpr int run_length(int v, bool adjacent, int size) {
 
 // V pairs a thread.
 template <typename T, int V, bool ADJACENT> __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-    const long long item = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
-    if (item >= p.items)
+    // The pairs' CTAs, then those of the columns behind them (in one warp they would wait for
+    // each other: 8192 tokens x 40 heads of 128 with 16 pairs 55 us, 36 so).
+    const bool behind = blockIdx.x >= p.pair_blocks;
+    const long long item = static_cast<long long>(blockIdx.x - (behind ? p.pair_blocks : 0)) * kThreads + threadIdx.x;
+    if (item >= (behind ? p.tail_items : p.items))
         return;
-    const int per_token = p.chunks + p.tail;
+    const int per_token = behind ? p.tail : p.chunks;
     const long long token = item / per_token; // of all sequences
     const int chunk = static_cast<int>(item - token * per_token);
     const long long b = token / p.tokens, t = token - b * p.tokens;
-    if (chunk >= p.chunks) { // columns behind the pairs
-        const int col = 2 * p.pairs + (chunk - p.chunks) * V;
-        for (int h = blockIdx.y; h < p.all_heads; h += gridDim.y) {
-            const int w = h >= p.heads, hh = h - (w ? p.heads : 0);
-            using R = Run<T, V>;
-            *reinterpret_cast<R *>(static_cast<T *>(p.y[w]) + b * p.ys[w][0] + hh * p.ys[w][1] + t * p.ys[w][2] + col) =
-                *reinterpret_cast<const R *>(static_cast<const T *>(p.x[w]) + b * p.xs[w][0] + hh * p.xs[w][1] + t * p.xs[w][2] + col);
+    if (behind) {
+        const int col = 2 * p.pairs + chunk * V;
+        using R = Run<T, V>;
+        for (int h0 = blockIdx.y * kRuns; h0 < p.all_heads; h0 += gridDim.y * kRuns) {
+            R r[kRuns];
+#pragma unroll
+            for (int u = 0; u < kRuns; ++u) {
+                const int h = min(h0 + u, p.all_heads - 1), w = h >= p.heads, hh = h - (w ? p.heads : 0);
+                r[u] = *reinterpret_cast<const R *>(static_cast<const T *>(p.x[w]) + b * p.xs[w][0] + hh * p.xs[w][1] + t * p.xs[w][2] + col);
+            }
+#pragma unroll
+            for (int u = 0; u < kRuns; ++u) {
+                const int h = h0 + u, w = h >= p.heads, hh = h - (w ? p.heads : 0);
+                if (h < p.all_heads)
+                    *reinterpret_cast<R *>(static_cast<T *>(p.y[w]) + b * p.ys[w][0] + hh * p.ys[w][1] + t * p.ys[w][2] + col) = r[u];
+            }
         }
         return;
     }
@@ -135,10 +148,13 @@ template <typename T, int V, bool ADJACENT> __global__ void __launch_bounds__(kT
 template <typename T, int V> int launch_v(RotaryParams &p, long long rows, bool adjacent, bool in_place, cudaStream_t stream) {
     p.chunks = p.pairs / V;
     p.tail = in_place ? 0 : (p.hd - 2 * p.pairs) / V;
-    p.items = rows * (p.chunks + p.tail);
-    const long long blocks = (p.items + kThreads - 1) / kThreads;
+    p.items = rows * p.chunks;
+    p.tail_items = rows * p.tail;
+    const long long pair_blocks = (p.items + kThreads - 1) / kThreads;
+    const long long blocks = pair_blocks + (p.tail_items + kThreads - 1) / kThreads;
     if (blocks > 0x7fffffffll)
         return static_cast<int>(cudaErrorInvalidValue);
+    p.pair_blocks = static_cast<unsigned>(pair_blocks);
     // Heads are split over CTAs until every SM has its threads.
     const long long full = kFull / kThreads * fmha_sm_count();
     const int groups = static_cast<int>(std::min<long long>(p.all_heads, std::max<long long>(1, (full + blocks - 1) / blocks)));
