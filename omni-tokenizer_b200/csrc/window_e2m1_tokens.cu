@@ -63,12 +63,14 @@ struct TokensParams {
     int *err;
 };
 
-// CTAs on an SM: as many as their registers allow.
-template <int NT> constexpr int kCtas = NT == 1 ? 4 : 2;
+// CTAs on an SM: as many as their registers allow without spills in the loop.  (More for narrow
+// heads do not help eight rows: 64 x up to 16384 keys of 64, 81 us with four, 82 with five; 16
+// rows of 64 columns 134 with two, 119 with three.)
+constexpr int ctas_of_sm(int width, int rows) { return rows == 8 ? 4 : rows == 16 && width <= 64 ? 3 : 2; }
 
 template <int D, int NT> struct TokensShape {
     static constexpr int BLOCK = CacheBlock<D>::BYTES;
-    static constexpr int WARPS = 4, CTAS = kCtas<NT>;
+    static constexpr int WARPS = 4, CTAS = ctas_of_sm(D, 8 * NT);
     static constexpr int STAGES = 2, STAGE = 2 * BLOCK; // a pair that is read, one on its way
     static constexpr int RING = WARPS * STAGES * STAGE;
     static constexpr int ROWS = 8 * NT;
@@ -1009,7 +1011,7 @@ Split split_in(const WindowE2m1Args &a, int rows_of_tile) {
         keys = std::min(keys, static_cast<long long>(a.window) + c.q_len + a.right + a.sinks);
     const long long of_tile = (keys + kCacheBlock - 1) / kCacheBlock + 1;
     const long long tiles = static_cast<long long>(s.tiles) * c.batch * c.kv_heads;
-    const long long most = std::min<long long>(kJoinParts, (s.rows == 8 ? kCtas<1> : kCtas<2>) * fmha_sm_count()); // CTAs at once
+    const long long most = std::min<long long>(kJoinParts, 1ll * ctas_of_sm(cache_width(c.hd), s.rows) * fmha_sm_count()); // CTAs at once
     s.parts = 1;
     // (Clusters of 16 with 24 rows do not all fit at once: 2 x 2048 keys, 20 rows, 23 us with 16, 12 with 8.)
     const int most_parts = s.rows == 24 ? 8 : kMaxParts;
@@ -1018,7 +1020,7 @@ Split split_in(const WindowE2m1Args &a, int rows_of_tile) {
     // In microseconds, as measured: a CTA's blocks one after another, slower the more rows they
     // meet and the more CTAs share its SM; the list has its second kernel on top, but also evens
     // out sequences that are shorter than kv_len, which is not known here, and gets a tenth for
-    // that.  Measured, cluster / list, 8 key heads of 128, one row of four heads: 1 x 8192 keys
+    // that (clusters of several rounds even them out themselves).  Measured, cluster / list, 8 key heads of 128, one row of four heads: 1 x 8192 keys
     // 10.5 / 13.5, 1 x 32768 22.7 / 19.9, 1 x 65536 39.6 / 25.7, 16 x 4096 15.9 / 22.1, 64 x 2048
     // 26.0 / 32.0, 64 x up to 4096 46.9 / 45.3, 64 x up to 16384 165 / 123.
     const double sms = fmha_sm_count(), ctas = static_cast<double>(tiles) * s.parts;
@@ -1030,7 +1032,7 @@ Split split_in(const WindowE2m1Args &a, int rows_of_tile) {
     const double list = 13 + block * total / s.ctas * (0.11 + 0.028 * s.ctas / sms);
     s.workspace = 0;
     s.us = std::min(list, cluster);
-    if (list < 1.1 * cluster) {
+    if (list < (rounds < 2 ? 1.1 : 1.0) * cluster) {
         s.parts = 0;
         s.workspace = s.ctas * (2ull * s.rows * (cache_width(c.hd) + 2) * 4 + sizeof(SharedTile));
     }

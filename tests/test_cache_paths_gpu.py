@@ -47,13 +47,13 @@ CASES = [
     (1, 8, 2, 1, 128, 64, [20011], 0, 0, CLUSTER, 8),
     (2, 16, 1, 1, 128, 256, [130000, 7], 0, 0, LIST, 16),
     (1, 40, 2, 1, 96, 64, [100000], 0, 0, LIST, 24),      # of which 20 are there
-    (1, 8, 2, 40, 64, 48, [40000], 0, 0, LIST, 24),       # seven tiles of rows
+    (1, 8, 2, 40, 128, 48, [40000], 0, 0, LIST, 24),      # seven tiles of rows
     (1, 6, 2, 33, 80, 32, [3000], 700, 40, CLUSTER, 8),
     (1, 4, 4, 1, 32, 16, [120000], 0, 0, LIST, 8),
     (64, 20, 2, 1, 64, 64, list(range(7, 1000, 16)) + [1000], 0, 0, CLUSTER, 16),
     (16, 40, 2, 1, 64, 64, list(range(500, 2001, 100)), 1900, 5, CLUSTER, 24),
     (1, 8, 2, 300, 64, 64, [900], 0, 0, PROMPT, None),
-    (8, 16, 16, 128, 64, 64, [128] * 8, 0, 0, PROMPT, None),
+    (8, 16, 16, 128, 128, 64, [128] * 8, 0, 0, PROMPT, None),
 ]
 
 
