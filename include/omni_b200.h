@@ -327,9 +327,11 @@ OMNI_B200_API int omni_b200_cache_read_e2m1(const omni_b200_cache_e2m1 *cache, v
  * contiguous.  Tokens from lengths[b] on are not used, whatever the cache holds there.
  * Sums, maxima and scores are fp32; the softmax's numerators are rounded to F16 (for prompts
  * to dtype) for the product with v.  workspace: 16-byte aligned, of at least
- * omni_b200_attention_window_e2m1_workspace bytes (0 for few queries: they read the cache
- * as it is; prompts put keys and values back to 16 bits there first).  Its contents do not
- * matter; calls that may overlap on the GPU must not share it. */
+ * omni_b200_attention_window_e2m1_workspace bytes for the same sizes (0 for many calls with few
+ * queries, some MB where their keys are split over many CTAs; prompts put keys and values back
+ * to 16 bits there, 4 * batch * kv_heads * kv_len * head_dim bytes).  Its contents do not
+ * matter; calls that may overlap on the GPU must not share it.  The same call gives the same
+ * bits. */
 OMNI_B200_API size_t omni_b200_attention_window_e2m1_workspace(int batch, int heads, int kv_heads,
                                                                int q_len, int kv_len, int head_dim,
                                                                int window, int right, int sinks);

@@ -17,9 +17,9 @@
 //
 // The bound is the cache's bytes.  A block of 16 tokens of a head (2304 bytes at 128 columns)
 // is one contiguous piece; each warp copies its own blocks, two at a time, to a ring in shared
-// memory (a bulk copy for a block, no barrier between warps) and keeps its own softmax state.  Converting
-// takes a conversion and a product for two elements, 128 instructions of a block's ~200; the
-// rest is kept short: a lane looks up the pages of 32 blocks at once, and the running maximum
+// memory (a bulk copy for a block, no barrier between warps) and keeps its own softmax state.
+// Converting takes a conversion and a product for two elements, 128 instructions of a block's
+// 248; the rest is kept short: a lane looks up the pages of 32 blocks at once, and the running maximum
 // is lazy (other lanes are asked only when some score is more than 2^8 above the reference).
 // 16 sequences of 65536 keys, 32/8 heads of 128: 198 us, 6.09 TB/s (copies alone 185, products
 // alone 176); 64 of up to 16384: 122 us, and 135 to 140 in a long run at the clock that the power
@@ -54,7 +54,7 @@ struct TokensParams {
     long long qs[3], os[3];
     const int *lengths, *q_lengths;
     int parts; // CTAs of a cluster, or 0: the list
-    int ctas;       // of the list
+    int ctas;  // of the list
     uint32_t group_inv; // ceil(2^20 / group): exact for quotients of numbers up to kMostRows by group up to it
     int batch, kv_heads, group, q_len, kv_len, hd, tiles; // tiles of rows that a sequence may have
     int window, right, sinks;
@@ -197,7 +197,7 @@ __device__ __forceinline__ void store_out(const TokensParams &p, const Tile &t, 
 }
 
 // What a CTA does at a time: pairs of blocks j0, j0 + step, ... below j1 of a tile.  slot: where
-// its part goes in the workspace, or -1: it is the whole tile.  b < 0: there is nothing.
+// its part goes in the workspace, or -1: it is the whole tile.
 struct Segment {
     Tile tile;
     int b, kvh, j0, j1, slot;
