@@ -380,6 +380,20 @@ def test_queries_of_any_size(ob, scale, power):
     _check(got, q, k, v, lengths, [1], scale=scale * 2.0**-power)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_queries_of_zeros_and_masks_past_everything(ob, dtype):
+    """Equal scores give means of the values; windows and first tokens beyond the sequence."""
+    B, H, Hkv, T, D, page, lengths = 2, 6, 2, 2, 72, 32, [90, 33]
+    q, cache, table, k, v = _case(ob, B, H, Hkv, T, D, page, lengths, [T] * B, dtype)
+    q = q.contiguous()
+    q[0, 1] = 0
+    for window, right, sinks, scale in ((0, 0, 0, 0.0), (1 << 30, 1 << 30, 1 << 30, 0.0), (5, 0, 1 << 30, 1e-30), (91, 2, 90, 3.0)):
+        out = torch.full(q.shape, KEPT, dtype=F32, device="cuda")
+        ob.attention_window_e2m1(q, cache, _i32(lengths), table=table, window=window, right=right, sinks=sinks,
+                                 scale=scale, out=out)
+        _check(out, q, k, v, lengths, [T] * B, min(window, 1000), min(right, 1000), min(sinks, 1000), scale)
+
+
 def test_queries_that_are_not_finite(ob):
     for T, case in ((1, TOKENS[2]), (2, TOKENS[4])):
         B, H, Hkv, _, D, page, lengths, counts, window, right, sinks = case

@@ -157,6 +157,14 @@ def test_back_and_gradients(ob):
     assert abs(left - right) <= 216 * 64 * 2.0**-19
 
 
+def test_new_outputs_are_laid_out_as_their_inputs(ob):
+    """So that a projection's rows stay rows."""
+    q, k = _tensor((2, 3, 5, 16), "tokens", BF16, 20), _tensor((2, 2, 5, 16), "heads", BF16, 21)
+    q_out, k_out = ob.rotary(q, k, torch.zeros(2, 5, dtype=torch.int32, device="cuda"), torch.ones(8, device="cuda"))
+    assert q_out.stride() == q.stride() and k_out.stride() == k.stride()
+    assert torch.equal(q_out, q) and torch.equal(k_out, k)  # position 0 turns nothing
+
+
 def test_not_finite(ob):
     q = _tensor((1, 1, 3, 8), "heads", F32, 12)
     where = torch.tensor([[0.0, float("inf"), float("nan")]], device="cuda")
