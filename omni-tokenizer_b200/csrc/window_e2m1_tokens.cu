@@ -173,9 +173,10 @@ template <int ROWS> __device__ __forceinline__ Tile tile_of(const TokensParams &
 // (3 us against 0.22 us for one; 64 x up to 16384 keys 124 us with 8 here, 122 with 16), so it counts for those as well.
 constexpr int kTileCost = 16;
 __device__ __forceinline__ int listed(const Tile &t) { return t.rows > 0 ? kTileCost + t.blocks : 0; }
-// Blocks of all tiles of a sequence's key head.
-template <int ROWS> __device__ __forceinline__ int listed_of(const TokensParams &p, int b) {
-    int n, m, sum = 0;
+// Blocks of all tiles of a sequence's key head: 2^31 and more of them where 32 tiles see 2^30 keys.
+template <int ROWS> __device__ __forceinline__ long long listed_of(const TokensParams &p, int b) {
+    int n, m;
+    long long sum = 0;
     lengths_of(p, b, n, m);
     for (int i = 0; i < p.tiles; ++i)
         sum += listed(tile_of<ROWS>(p, n, m, i));
@@ -758,13 +759,14 @@ __global__ void __launch_bounds__(TokensShape<D, NT>::WARPS * 32, TokensShape<D,
     if (from >= to)
         return;
     if (from >= before && from < before + mine) {
-        int b = b0, of_head = listed_of<S::ROWS>(p, b);
-        for (; b < b1 - 1 && from >= before + static_cast<long long>(of_head) * p.kv_heads; of_head = listed_of<S::ROWS>(p, b))
-            before += static_cast<long long>(of_head) * p.kv_heads, ++b;
+        int b = b0;
+        long long of_head = listed_of<S::ROWS>(p, b);
+        for (; b < b1 - 1 && from >= before + of_head * p.kv_heads; of_head = listed_of<S::ROWS>(p, b))
+            before += of_head * p.kv_heads, ++b;
         // (Lengths that change under the kernel are a caller's mistake, but lead out of no array.)
-        const int kvh = max(0, min(quotient(from - before, max(of_head, 1)), p.kv_heads - 1));
+        const int kvh = max(0, min(quotient(from - before, max(of_head, 1ll)), p.kv_heads - 1));
         walk.tile = (static_cast<long long>(b) * p.kv_heads + kvh) * p.tiles;
-        walk.at = before + static_cast<long long>(kvh) * of_head;
+        walk.at = before + kvh * of_head;
     }
     // A warp works out 32 tiles at once, those of them that this CTA has a share in.
     const int of_sequence = p.kv_heads * p.tiles;
