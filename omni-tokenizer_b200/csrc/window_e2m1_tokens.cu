@@ -209,7 +209,10 @@ struct Segment {
 template <int D, int NT> struct Parts {
     using S = TokensShape<D, NT>;
     float m[S::WARPS][S::ROWS];
-    float l[S::WARPS][S::ROWS];
+    union {
+        float l[S::WARPS][S::ROWS];
+        uint32_t lost[S::WARPS][S::ROWS]; // before: groups of columns that are NaN, a bit for each
+    };
     float cta_m[S::ROWS], cta_l[S::ROWS];
     float o[S::WARPS][S::ROWS][D + 4];
 };
@@ -369,9 +372,51 @@ template <int D, int NT, bool BF16> struct Worker {
         for (int t = 0; t < NT; ++t)
             none[t][0] = none[t][1] = true;
 
+        bool lost = false; // parts.lost holds what the masked pairs noted
         // One pair, at `at` in the ring.  (Two instances, so that pairs without a mask carry none of its instructions.)
         auto attend_pair = [&](auto masked, uint32_t at, int i0) {
             constexpr bool MASKED = decltype(masked)::value;
+            int key0 = 0, key1 = 0;
+            uint32_t bad = 0; // blocks whose page is none
+            if constexpr (MASKED) {
+                int within;
+                bad = (p.cache.page_of(seg.b, seg.block_of(i0), within) < 0 ? 1u : 0u) |
+                      (i0 + 1 < j1 && p.cache.page_of(seg.b, seg.block_of(i0 + 1), within) < 0 ? 2u : 0u);
+                key0 = seg.block_of(i0) * kCacheBlock;
+                key1 = i0 + 1 < j1 ? seg.block_of(i0 + 1) * kCacheBlock : tile.n; // no token is there
+                // Values that no row sees may be anything: their scales become zeros.  So do those that
+                // are not finite where the rows see different keys (0 * NaN would reach the others),
+                // and the rows that see one are noted: they get their NaN in the end.
+                const int u = lane / kCacheBlock, r = lane % kCacheBlock, token = (u ? key1 : key0) + r;
+                const bool unseen = (bad >> u & 1u) || token >= tile.high || (token < tile.low && token >= tile.sink);
+                uint32_t groups = 0;
+#pragma unroll
+                for (int group = 0; group < B::G; ++group) {
+                    const uint32_t scale_at = at + u * S::BLOCK + B::VALUE_SCALES + 2 * B::value_scale(r, group);
+                    bool clear = unseen;
+                    if (tile.first != tile.last && !unseen) {
+                        uint16_t scale;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(scale) : "r"(scale_at) : "memory");
+                        clear = (scale & 0x7c00) == 0x7c00;
+                        groups |= clear ? 1u << group : 0u;
+                    }
+                    if (clear)
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(scale_at), "h"(static_cast<uint16_t>(0)) : "memory");
+                }
+                if (__any_sync(0xffffffffu, groups)) {
+                    if (!lost && lane < ROWS)
+                        parts.lost[warp][lane] = 0;
+                    lost = true;
+                    __syncwarp();
+                    for (int row = 0; groups && row < tile.rows; ++row) {
+                        const int pos = tile.pos0 + query_of(p, tile.row0 + row);
+                        if (token <= pos + p.right && (p.window <= 0 || token > pos - p.window || token < p.sinks))
+                            atomicOr(&parts.lost[warp][row], groups);
+                    }
+                }
+                fence_proxy_async_smem(); // the next copy's writes come after these
+                __syncwarp();
+            }
             // S^T: tokens g (rows 0 to 7) and g + 8 of each block; the blocks' products take turns,
             // so that none waits for the one before it.
             float s[2][NT][4];
@@ -422,21 +467,6 @@ template <int D, int NT, bool BF16> struct Worker {
                                 mma16816(s[u][t], a[u][e], qb[t][2 * j + e][0], qb[t][2 * j + e][1]);
             }
             if constexpr (MASKED) {
-                int within;
-                const uint32_t bad = (p.cache.page_of(seg.b, seg.block_of(i0), within) < 0 ? 1u : 0u) |
-                                     (i0 + 1 < j1 && p.cache.page_of(seg.b, seg.block_of(i0 + 1), within) < 0 ? 2u : 0u);
-                const int key0 = seg.block_of(i0) * kCacheBlock;
-                const int key1 = i0 + 1 < j1 ? seg.block_of(i0 + 1) * kCacheBlock : tile.n; // no token is there
-                // Values that no row sees may be anything: their scales become zeros.
-                for (int x = lane; x < 2 * kCacheBlock * B::G; x += 32) {
-                    const int u = x / (kCacheBlock * B::G), r = x / B::G % kCacheBlock, token = (u ? key1 : key0) + r;
-                    if ((bad >> u & 1u) || token >= tile.high || (token < tile.low && token >= tile.sink))
-                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + u * S::BLOCK + B::VALUE_SCALES + 2 * B::value_scale(r, x % B::G)),
-                                     "h"(static_cast<uint16_t>(0))
-                                     : "memory");
-                }
-                fence_proxy_async_smem(); // the next copy's writes come after these
-                __syncwarp();
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -557,6 +587,8 @@ template <int D, int NT, bool BF16> struct Worker {
                 attend_pair(std::false_type(), at, i0);
         }
         __syncwarp();
+        const uint32_t groups = lost && lane < ROWS ? parts.lost[warp][lane] : 0u;
+        __syncwarp(); // their place is the sums'
 
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -576,6 +608,12 @@ template <int D, int NT, bool BF16> struct Worker {
                     parts.o[warp][r][16 * x + 8 + g] = o[t][x][2 + h];
                 }
             }
+        if (lost) {
+            __syncwarp();
+            for (int r = 0; r < ROWS; ++r)
+                for (uint32_t those = __shfl_sync(0xffffffffu, groups, r); those; those &= those - 1)
+                    parts.o[warp][r][(__ffs(those) - 1) * kCacheGroup + lane] = NAN;
+        }
     }
 
     // The warps' parts as one, m, l and four columns at a time of sum_i 2^(m_i - m) o_i, to
