@@ -282,8 +282,7 @@ OMNI_B200_API int omni_b200_rotary(const void *q, void *q_out, const void *k, vo
  * aligned.  table: DEVICE int32[batch, table_width], the pages of each sequence in their
  * order; NULL: page b is all that sequence b has.  Entries are read as far as a call needs
  * them.  An entry that is none of [0, pages) is not followed: nothing is written there, rows
- * read as NaN and queries that see a key there give NaN (for prompts, see below, other
- * queries of that sequence may, too).
+ * read as NaN and queries that see a key there give NaN.
  *
  * Columns share a scale in groups of 32 (the last may be smaller).  With amax the largest
  * magnitude of a group of a token,
@@ -324,7 +323,10 @@ OMNI_B200_API int omni_b200_cache_read_e2m1(const omni_b200_cache_e2m1 *cache, v
  * results, k and v being what the cache stands for.  kv_len is the most tokens that a
  * sequence holds, at most what its pages hold; lengths are clamped to [0, kv_len].  strides:
  * HOST int64[6], (batch, head, token) of q (multiples of 8) and out in elements; NULL:
- * contiguous.  Tokens from lengths[b] on are not used, whatever the cache holds there.
+ * contiguous.  Tokens from lengths[b] on are not used, whatever the cache holds there, and
+ * those that a query does not see do not matter to it, NaN among them.  A query that sees NaN
+ * in a token's keys gives NaN, in a group of its values NaN in the group's columns (prompts,
+ * see below: in all).
  * Sums, maxima and scores are fp32; the softmax's numerators are rounded to F16 (for prompts
  * to dtype) for the product with v.  workspace: 16-byte aligned, of at least
  * omni_b200_attention_window_e2m1_workspace bytes for the same sizes (0 for many calls with few

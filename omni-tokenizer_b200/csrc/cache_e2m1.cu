@@ -175,15 +175,17 @@ template <typename T> __device__ __forceinline__ void store_columns(T *y, const 
     store8(y, pack8<T>(f));
 }
 
-// blockIdx.y: keys, or values.
-template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32) cache_read_kernel(const __grid_constant__ RowsParams p) {
+// blockIdx.y: keys, or values.  WHOLE: for prompts, where what is not finite must not stand among
+// the values (0 * NaN would reach queries that do not see it): they get zeros there, and the
+// token's keys NaN, which a mask hides.
+template <typename T, int D, bool WHOLE> __global__ void __launch_bounds__(kWarps * 32) cache_read_kernel(const __grid_constant__ RowsParams p) {
     using B = CacheBlock<D>;
     __shared__ __align__(16) uint8_t values[kWarps][8 * D];
     Piece w;
     if (!piece_of(p, w))
         return;
     const int base = w.block * kCacheBlock;
-    if (p.window > 0) { // keys that no query of a prompt sees, nor stand near one that is seen
+    if (WHOLE && p.window > 0) { // keys that no query of a prompt sees, nor stand near one that is seen
         const long long n = min(max(p.lengths[w.b], 0), p.capacity);
         const long long m = p.q_lengths ? max(0, min(p.q_lengths[w.b], p.q_len)) : p.q_len;
         if (base + kCacheBlock <= n - m - p.window - 127 && base >= p.sinks + 128ll)
@@ -208,11 +210,15 @@ template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32) cach
     // All of a warp's reads, then its writes.  Keys: a word a step.  Values: eight bytes, each
     // the column's nibbles of two tokens.
     uint32_t words[STEPS][2] = {};
-    uint16_t scales[STEPS];
+    uint16_t scales[STEPS], value_scales[B::G] = {};
+    if (WHOLE && keys && from && lane < kCacheBlock)
+#pragma unroll
+        for (int g = 0; g < B::G; ++g)
+            value_scales[g] = *reinterpret_cast<const uint16_t *>(from + B::VALUE_SCALES + 2 * B::value_scale(lane, g));
 #pragma unroll
     for (int x = 0; x < STEPS; ++x) {
         const int i = 32 * x + lane, r = r0 + i / WORDS, c = i % WORDS;
-        scales[x] = kScaleNaN; // a page that the cache does not have reads as NaN
+        scales[x] = WHOLE && !keys ? 0 : kScaleNaN; // a page that the cache does not have reads as NaN
         if (!from || r >= r1)
             continue;
         if (keys) {
@@ -220,6 +226,8 @@ template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32) cach
             scales[x] = *reinterpret_cast<const uint16_t *>(from + B::KEY_SCALES + 2 * B::key_scale(r, c / 4));
         } else {
             scales[x] = *reinterpret_cast<const uint16_t *>(from + B::VALUE_SCALES + 2 * B::value_scale(r, c / 4));
+            if (WHOLE && not_finite(scales[x]))
+                scales[x] = 0;
             const uint8_t *at = mine + B::value_word(c / 2, r % 8 / 2) + r / 8 * 2 + c % 2;
             uint32_t b[8];
 #pragma unroll
@@ -230,6 +238,14 @@ template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32) cach
                 words[x][h] = __byte_perm(__byte_perm(b[4 * h], b[4 * h + 1], 0x0040), __byte_perm(b[4 * h + 2], b[4 * h + 3], 0x0040), 0x5410);
         }
     }
+    uint32_t lost = 0; // tokens of which some value is not finite
+    if (WHOLE && keys && from) {
+        bool mine = false;
+#pragma unroll
+        for (int g = 0; g < B::G; ++g)
+            mine |= not_finite(value_scales[g]);
+        lost = __ballot_sync(0xffffffffu, mine);
+    }
 #pragma unroll
     for (int x = 0; x < STEPS; ++x) {
         const int i = 32 * x + lane, r = r0 + i / WORDS, c = i % WORDS;
@@ -238,6 +254,8 @@ template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32) cach
         uint32_t h[4];
         if (keys) {
             f16x8(words[x][0], h);
+            if (lost >> r & 1u)
+                scales[x] = kScaleNaN;
         } else {
             uint32_t two[4];
 #pragma unroll
@@ -284,10 +302,15 @@ template <typename T, int D> int launch_rows(RowsParams &p, int batch, bool read
     const long long ctas = (p.warps + kWarps - 1) / kWarps;
     if (ctas > 0x7fffffffll)
         return static_cast<int>(cudaErrorInvalidValue);
-    if (read)
-        cache_read_kernel<T, D><<<dim3(static_cast<unsigned>(ctas), 2), kWarps * 32, 0, stream>>>(p);
-    else if constexpr (sizeof(T) == 2)
-        cache_write_kernel<T, D><<<dim3(static_cast<unsigned>(ctas), 2), kWarps * 32, 0, stream>>>(p);
+    const dim3 grid(static_cast<unsigned>(ctas), 2);
+    if (read && !p.whole)
+        cache_read_kernel<T, D, false><<<grid, kWarps * 32, 0, stream>>>(p);
+    else if constexpr (sizeof(T) == 2) {
+        if (read)
+            cache_read_kernel<T, D, true><<<grid, kWarps * 32, 0, stream>>>(p);
+        else
+            cache_write_kernel<T, D><<<grid, kWarps * 32, 0, stream>>>(p);
+    }
     return static_cast<int>(cudaGetLastError());
 }
 template <typename T> int launch_width(RowsParams &p, int batch, bool read, cudaStream_t stream) {

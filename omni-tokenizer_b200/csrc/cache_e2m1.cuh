@@ -26,6 +26,7 @@ namespace omni_b200 {
 constexpr int kCacheBlock = 16, kCacheGroup = 32;
 constexpr float kScaleMin = 6.103515625e-05f, kScaleMax = 10752.f; // 2^-14; 6 * 10752 is finite in f16
 constexpr uint16_t kScaleNaN = 0x7e00;
+__device__ __forceinline__ bool not_finite(uint16_t scale) { return (scale & 0x7c00u) == 0x7c00u; }
 
 __host__ __device__ constexpr int cache_width(int hd) { return (hd + 31) / 32 * 32; }
 template <int D> struct CacheBlock {

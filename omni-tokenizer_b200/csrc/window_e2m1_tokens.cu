@@ -397,7 +397,7 @@ template <int D, int NT, bool BF16> struct Worker {
                     if (tile.first != tile.last && !unseen) {
                         uint16_t scale;
                         asm volatile("ld.shared.u16 %0, [%1];" : "=h"(scale) : "r"(scale_at) : "memory");
-                        clear = (scale & 0x7c00) == 0x7c00;
+                        clear = not_finite(scale);
                         groups |= clear ? 1u << group : 0u;
                     }
                     if (clear)

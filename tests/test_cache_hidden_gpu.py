@@ -10,7 +10,7 @@ import math
 import pytest
 
 from tests.test_cache_gpu import BF16, F16, F32, KEPT, _i32, _made, _stored, _tensor, ob  # noqa: F401
-from tests.test_cache_paths_gpu import CLUSTER, LIST, _names
+from tests.test_cache_paths_gpu import CLUSTER, LIST, PROMPT, _names
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -34,14 +34,17 @@ def _attended(q, k, v, n, m, window, right, sinks):
     return (w @ vv).masked_fill(lost, math.nan), w @ vv.abs(), float(vv.abs().max())
 
 
-def _check(got, q, k, v, lengths, counts, window, right, sinks):
+def _check(got, q, k, v, lengths, counts, window, right, sinks, prompt):
+    eps = torch.finfo(q.dtype).eps if prompt else 2.0**-10
     for b, (n, m) in enumerate(zip(lengths, counts)):
         assert bool((got[b, :, m:] == KEPT).all())
         if n == 0 or m == 0:
             continue
         want, mean, most = _attended(q[b], k[b], v[b], n, m, window, right, sinks)
-        tol = mean * (2.0**-10 + 2.0**-12) + n * 2.0**-25 * most + want.abs() * 2.0**-23 + 1e-30
+        tol = mean * (eps + 2.0**-12) + n * 2.0**-25 * most + want.abs() * 2.0**-23 + 1e-30
         mine = got[b, :, :m].double()
+        if prompt:  # all columns of a query that sees a value which is none
+            want = want.masked_fill(want.isnan().any(dim=2, keepdim=True), math.nan)
         assert torch.equal(mine.isnan(), want.isnan())
         assert bool(((mine - want).abs() <= tol)[~want.isnan()].all())
 
@@ -83,14 +86,14 @@ def _go(ob, tmp_path, case, dtype, kernels):  # noqa: F811
         ob.cache_write_e2m1(kk, vv, cache, held, q_lengths=held, table=table)
         out.fill_(KEPT)
         call()
-        _check(out, q, _stored(kk), _stored(vv), lengths, counts, window, right, sinks)
+        _check(out, q, _stored(kk), _stored(vv), lengths, counts, window, right, sinks, kernels == PROMPT)
     kk, vv = k.clone(), v.clone()
     for b, t in bad:
         spoil(kk if t == lengths[b] - 1 else vv, b, t)
     ob.cache_write_e2m1(kk, vv, cache, held, q_lengths=held, table=table)
     out.fill_(KEPT)
     call()
-    _check(out, q, _stored(kk), _stored(vv), lengths, counts, window, right, sinks)
+    _check(out, q, _stored(kk), _stored(vv), lengths, counts, window, right, sinks, kernels == PROMPT)
     ob.library().sync_check()
 
 
@@ -110,3 +113,40 @@ FEW = [
 @pytest.mark.parametrize("case,kernels", FEW)
 def test_values_that_some_queries_do_not_see(ob, tmp_path, case, kernels, dtype):  # noqa: F811
     _go(ob, tmp_path, case, dtype, kernels)
+
+
+# B, H, Hkv, T, D, page, lengths, counts, window, right, sinks
+PROMPTS = [
+    (1, 4, 1, 600, 64, 16, [650], [600], 0, 0, 0),
+    (2, 8, 2, 300, 128, 64, [700, 300], [300, 299], 128, 0, 1),
+    (1, 8, 2, 200, 96, 48, [1000], [200], 77, 30, 70),
+    (3, 16, 4, 260, 32, 32, [260, 0, 500], [260, 0, 200], 40, 0, 130),
+    (1, 4, 1, 400, 72, 64, [3000], [400], 1500, 0, 20),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("case", PROMPTS)
+def test_values_that_some_queries_of_a_prompt_do_not_see(ob, tmp_path, case, dtype):  # noqa: F811
+    _go(ob, tmp_path, case, dtype, PROMPT)
+
+
+@pytest.mark.parametrize("case", PROMPTS)
+def test_missing_pages_that_some_queries_of_a_prompt_do_not_see(ob, case):  # noqa: F811
+    """A page that is none is NaN for the queries that see a key there, and for no others."""
+    B, H, Hkv, T, D, page, lengths, counts, window, right, sinks = case
+    cache, table = _made(ob, B, Hkv, D, max(lengths), page, 160)
+    k, v = (_tensor((B, Hkv, max(lengths), D), "heads", F16, s, 0.3) for s in (161, 162))
+    q = _tensor((B, H, T, D), "tokens", F16, 163)
+    held, m = _i32(lengths), _i32(counts)
+    ob.cache_write_e2m1(k, v, cache, held, q_lengths=held, table=table)
+    b = max(range(B), key=lambda b: lengths[b])
+    n = lengths[b]
+    for at in sorted({(n - 1) // page, (n - counts[b]) // page, max(n - counts[b] - window, 0) // page, sinks // page}):
+        some = table.clone()
+        some[b, at] = -1
+        kk, vv = _stored(k), _stored(v)
+        kk[b, :, at * page:(at + 1) * page] = math.nan
+        out = torch.full(q.shape, KEPT, dtype=F32, device="cuda")
+        ob.attention_window_e2m1(q, cache, held, q_lengths=m, table=some, window=window, right=right, sinks=sinks, out=out)
+        _check(out, q, kk, vv, lengths, counts, window, right, sinks, True)
