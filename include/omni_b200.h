@@ -328,7 +328,8 @@ OMNI_B200_API int omni_b200_cache_read_e2m1(const omni_b200_cache_e2m1 *cache, v
  * in a token's keys gives NaN, in a group of its values NaN in the group's columns (prompts,
  * see below: in all).
  * Sums, maxima and scores are fp32; the softmax's numerators are rounded to F16 (for prompts
- * to dtype) for the product with v.  workspace: 16-byte aligned, of at least
+ * to dtype) for the product with v: in F16 by half a step of 11 bits each, below 2^-21 of a
+ * row's largest by at most 2^-32 of that.  workspace: 16-byte aligned, of at least
  * omni_b200_attention_window_e2m1_workspace bytes for the same sizes (0 for many calls with few
  * queries, some MB where their keys are split over many CTAs; prompts put keys and values back
  * to 16 bits there, 4 * batch * kv_heads * kv_len * head_dim bytes).  Its contents do not

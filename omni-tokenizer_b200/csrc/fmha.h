@@ -100,6 +100,7 @@ struct WindowArgs {
     bool bf16 = true;
     int out_dtype = kOutBF16;
     float scale = 0.f; // 0: hd^-1/2
+    float lift = 0.f;  // prompts: log2 of the weight of a row's largest key, which grows to 2^8 times that
     int *err = nullptr;
 };
 int attention_window(const WindowArgs &a, cudaStream_t stream);

@@ -11,7 +11,7 @@
 //   O^T = V^T P^T: P^T's B operand is S^T's accumulators packed to f16 and turned by
 //     movmatrix.
 // Every product is f16 x f16 with fp32 sums whatever q's type is: the cache's values are
-// exact in f16, P <= 2^8 is rounded to 11 bits there (bf16: 8), and a bf16 row of q is
+// exact in f16, P <= 2^15 is rounded to 11 bits there (bf16: 8), and a bf16 row of q is
 // multiplied by the power of two that brings its largest element to [2^14, 2^15): elements
 // down to 2^-28 of it keep all their bits, what is below loses less than 2^-39 of it.
 //
@@ -20,7 +20,7 @@
 // memory (a bulk copy for a block, no barrier between warps) and keeps its own softmax state.
 // Converting takes a conversion and a product for two elements, 128 instructions of a block's
 // 248; the rest is kept short: a lane looks up the pages of 32 blocks at once, and the running maximum
-// is lazy (other lanes are asked only when some score is more than 2^8 above the reference).
+// is lazy (other lanes are asked only when some weight would be above 2^15).
 // 16 sequences of 65536 keys, 32/8 heads of 128: 198 us, 6.09 TB/s (copies alone 185, products
 // alone 176); 64 of up to 16384: 122 us, and 135 to 140 in a long run at the clock that the power
 // cap leaves.  248 instructions for a block of 16 tokens, issue slots 59 % busy, ALU 47 %.
@@ -44,7 +44,10 @@ namespace {
 
 constexpr int kMaxParts = 16;
 constexpr int kMostRows = 512; // of a key head, group * q_len
-constexpr float kLazy = 8.f; // log2 units a score may be above the reference
+// A row's largest key so far has the weight 2^kTop (log2 units, as scores), and a score may be
+// kLazy above it before the reference follows: weights reach 2^15 of f16's 2^16, and at the other
+// end lose at most 2^-25 / 2^kTop = 2^-32 of the largest each.
+constexpr float kTop = 7.f, kLazy = 8.f;
 
 struct TokensParams {
     CacheView cache;
@@ -495,12 +498,12 @@ template <int D, int NT, bool BF16> struct Worker {
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                         times[h] = 1.f;
-                        if (top > bar[t][h] || (!none[t][h] && top * factor[t][h] > ref[t][h])) {
-                            const float next = top * factor[t][h];
+                        const float next = fmaf(top, factor[t][h], -kTop);
+                        if (top > bar[t][h] || (!none[t][h] && next > ref[t][h])) {
                             times[h] = none[t][h] ? 0.f : ex2_approx(ref[t][h] - next);
                             none[t][h] = false;
                             ref[t][h] = next;
-                            bar[t][h] = (next + kLazy) / factor[t][h];
+                            bar[t][h] = (next + (kTop + kLazy)) / factor[t][h];
                         }
                         sum[t][h] *= times[h];
                     }
@@ -1203,6 +1206,7 @@ int window_e2m1_launch(const WindowE2m1Args &a, cudaStream_t stream) {
     w.bf16 = a.dtype == kBF16;
     w.out_dtype = a.out_dtype;
     w.scale = a.scale;
+    w.lift = a.dtype == kF16 ? kTop : 0.f;
     w.err = a.err;
     CacheReadRange range;
     range.whole = true;

@@ -25,8 +25,9 @@
 // loader publishes each block's description in shared memory, ahead of its use: the
 // divisions and the reads of the lengths stay off the other warps' path.
 // Exponentials are taken to base 2 with the scale folded in, statistics are fp32; a
-// row keeps a stale maximum until it grows by more than 2^8, so that P <= 2^8 and O
-// is rarely rescaled.  Steps take turns between two barriers where one side may
+// row keeps a stale maximum until it grows by more than 2^8, so that P <= 2^8 (times
+// 2^lift: 2^7 for the 4-bit cache's f16 weights, which so lose 2^-32 of a row's largest
+// where they leave f16's normal range, not 2^-25) and O is rarely rescaled.  Steps take turns between two barriers where one side may
 // be a step ahead of the other (P written, products done): one barrier's parity would
 // mistake the step before the last for the one awaited.
 //
@@ -55,7 +56,7 @@ struct PromptParams {
     int batch, heads, group, q_len, kv_len, hd;
     int window, right, sinks;
     int out_dtype, out_vec, table;
-    float scale_log2;
+    float scale_log2, lift;
     int *err;
 };
 
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(PromptShape<NC>::THREADS, 1) window_prompt_ker
                     m = next;
                 }
                 // A row that has seen no key yet: P = 0, not 2^NaN.
-                const float shift = m == -INFINITY ? 0.f : -m;
+                const float shift = m == -INFINITY ? 0.f : p.lift - m;
                 float a0 = 0.f, a1 = 0.f, b0 = 0.f, b1 = 0.f;
 #pragma unroll
                 for (int c = 0; c < kKeys / 2; c += 2) {
@@ -760,6 +761,7 @@ int window_prompt_launch(const WindowArgs &a, cudaStream_t stream) {
     p.table = (a.lengths || a.q_lengths) && a.batch > 1 && a.batch <= kMaxBatch;
     const double scale = a.scale > 0 ? a.scale : 1.0 / std::sqrt(static_cast<double>(a.hd));
     p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+    p.lift = a.lift;
     p.err = a.err;
     const int sms = fmha_sm_count();
     if (a.hd <= 64)

@@ -1,12 +1,52 @@
-"""attention_window_e2m1 at the ends of its ranges: as many keys as the entry point takes."""
+"""attention_window_e2m1 at the ends of its ranges: keys whose weights are far below the largest,
+and as many keys as the entry point takes."""
+
+import math
 
 import pytest
 
-from tests.test_cache_gpu import BF16, F32, KEPT, _check, _i32, _stored, _tensor, ob  # noqa: F401
-from tests.test_cache_paths_gpu import LIST, _names
+from tests.test_cache_gpu import BF16, F16, F32, KEPT, _check, _i32, _stored, _tensor, ob  # noqa: F401
+from tests.test_cache_paths_gpu import LIST, PROMPT, _names
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
+
+
+# A first token, and keys at 2^-below of its weight whose values alone are not 0: the result is
+# what they sum to.  The weights are rounded to multiples of 2^-24 where the largest is 2^7 or
+# more: each loses at most 2^-25 / 2^7 of it.  Sums run over the keys of a tile, in whatever
+# order, so with A the weighted mean of |v| the tolerance is A (2^-10 + 2^-12) + keys * 2^-32 * |v|.
+@pytest.mark.parametrize("below", [24.6, 25.5, 30.0])
+@pytest.mark.parametrize("B,T,keys,dtype", [
+    (1, 1, 131072, BF16), (600, 1, 4096, BF16), (600, 1, 4096, F16), (700, 3, 1000, F16),  # tiles of one CTA
+    (1, 600, 8192, F16), (1, 600, 8192, BF16),  # prompts
+])
+def test_keys_far_below_the_largest(ob, tmp_path, B, T, keys, dtype, below):  # noqa: F811
+    D = 32
+    k = torch.zeros(1, 1, keys, D, dtype=dtype, device="cuda")
+    v = torch.zeros_like(k)
+    k[..., 0], k[:, :, 0, 0] = -6.0, 6.0
+    v[:, :, 1:] = torch.rand(keys - 1, D, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) + 0.5
+    cache = ob.empty_cache_e2m1(-(-keys // 16), 1, 16, D)
+    pages = torch.arange(cache.shape[0], dtype=torch.int32, device="cuda")
+    ob.cache_write_e2m1(k, v, cache, _i32([keys]), table=pages[None])
+    table = pages.expand(B, -1).contiguous()  # a prefix that all sequences share
+    q = torch.zeros(B, 1, T, D, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    scale = below / (12 * math.log2(math.e))
+    held = _i32([keys] * B)
+
+    def call():
+        return ob.attention_window_e2m1(q, cache, held, table=table, right=T, scale=scale, out_dtype=F32)
+
+    assert (_names(call, tmp_path) == PROMPT) == (T == 600)
+    got = call().double()
+    e = torch.full((keys,), 2.0**-below, dtype=torch.float64, device="cuda")
+    e[0] = 1.0
+    want = (e / e.sum()) @ _stored(v)[0, 0]
+    eps = torch.finfo(BF16).eps if T == 600 and dtype == BF16 else 2.0**-10
+    tol = want * (eps + 2.0**-12) + keys * 2.0**-32 * 2.0
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
 
 
 def test_as_many_keys_as_there_may_be(ob, tmp_path):  # noqa: F811
