@@ -158,13 +158,13 @@ def _stream_ptr(stream):
 
 
 def _on(what, stream, t):
-    """The context in which a helper that was given a stream makes tensors: a call with
-    stream=s is the call made inside torch.cuda.stream(s).  Outputs and workspaces, those
+    """The context in which a helper that was given a stream makes tensors on t's device (t may
+    be its number): a call with stream=s is the call made inside torch.cuda.stream(s).  Outputs and workspaces, those
     that are dropped at once among them, are memory of that stream, so that no kernel
     pending on the current stream has it, and none there gets it before the call is over.
     (Entering the stream takes the host 8 us; calls that make no tensor are launched on it
     without.)"""
-    device = t.get_device()
+    device = t if isinstance(t, int) else t.get_device()
     if not hasattr(stream, "device_index"):  # another library's, known by its cuda_stream
         stream = _t.cuda.ExternalStream(stream.cuda_stream, device=device)
     if 0 <= device != stream.device_index:
@@ -306,7 +306,7 @@ class _Torch:
 
         self.codes = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
         self.e4m3, self.f32, self.bf16, self.i32 = torch.float8_e4m3fn, torch.float32, torch.bfloat16, torch.int32
-        self.u8, self.f64, self.zeros = torch.uint8, torch.float64, torch.zeros
+        self.u8, self.f64, self.zeros, self.device = torch.uint8, torch.float64, torch.zeros, torch.device
         self.position_codes = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
         self.empty_like, self.cuda, self.current_device = torch.empty_like, torch.cuda, torch.cuda.current_device
         self.raw_stream = torch._C._cuda_getCurrentRawStream
@@ -656,9 +656,11 @@ def empty_cache_e2m1(pages, kv_heads, page_tokens, head_dim, device="cuda", stre
     """A cache of keys and values in 4 bits, uint8 [pages, kv_heads, bytes of a page], all
     zeros.  A page holds page_tokens tokens (a multiple of 16) of one key head; head_dim is a
     multiple of 8 up to 128."""
-    if stream is not None:
-        with _t.cuda.stream(stream):
-            return empty_cache_e2m1(pages, kv_heads, page_tokens, head_dim, device)
+    if stream is not None and (place := _t.device(device)).type == "cuda":
+        if place.index is None:  # the stream's, or the current one where it does not say
+            place = _t.device("cuda", stream.device_index if hasattr(stream, "device_index") else _t.current_device())
+        with _on("empty_cache_e2m1", stream, place.index):
+            return empty_cache_e2m1(pages, kv_heads, page_tokens, head_dim, place)
     in_range = 0 <= page_tokens < _INT and 0 <= head_dim < _INT
     size = library().lib.omni_b200_cache_e2m1_bytes(page_tokens, head_dim) if in_range else 0
     if size == 0 or pages <= 0 or kv_heads <= 0:
