@@ -77,6 +77,8 @@ PROMPTS = [
     (2, 8, 1, 129, 120, 64, [129, 1000], [129, 129], 513, 65, 64),
     (1, 32, 1, 33, 64, 0, [400], [33], 0, 7, 0),
     (1, 4, 1, 400, 128, 64, [3000], [400], 1500, 0, 20),
+    (3, 8, 1, 200, 64, 32, [100, 0, 500], [200, 200, 200], 0, 0, 0),  # more queries than keys
+    (3, 8, 1, 200, 80, 32, [100, 1, 199], [200, 150, 200], 50, 30, 9),
 ]
 
 
@@ -126,3 +128,32 @@ def test_prompts_of_few_rows(ob, tmp_path, case, dtype):  # noqa: F811
     call()
     _check(out, q, k, v, lengths, counts, window, right, sinks)
     ob.library().sync_check()
+
+
+def test_a_captured_prompt_replayed_with_other_lengths_and_pages(ob, tmp_path):  # noqa: F811
+    """Lengths, pages and the workspace's old contents are the replay's own matter."""
+    B, H, Hkv, T, D, page = 2, 8, 1, 150, 64, 32
+    q, cache, table, k, v = _case(ob, B, H, Hkv, T, D, page, [400, 400], [T, T], F16)
+    held, m = _i32([400, 400]), _i32([T, T])
+    out = torch.full(q.shape, KEPT, dtype=F32, device="cuda")
+
+    def call():
+        return ob.attention_window_e2m1(q, cache, held, q_lengths=m, table=table, window=90, right=2, sinks=5, out=out)
+
+    assert _names(call, tmp_path) == PROMPT
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for lengths, counts in (([400, 37], [T, 37]), ([0, 399], [9, 100]), ([200, 1], [T, 0])):
+        held.copy_(_i32(lengths))
+        m.copy_(_i32(counts))
+        out.fill_(KEPT)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(out, q, k, v, lengths, counts, 90, 2, 5, prompt=True)
+    table.copy_(table.flip(0))  # the sequences change places
+    held.copy_(_i32([333, 400]))
+    m.copy_(_i32([T, T]))
+    graph.replay()
+    torch.cuda.synchronize()
+    _check(out, q, k.flip(0), v.flip(0), [333, 400], [T, T], 90, 2, 5, prompt=True)
