@@ -300,8 +300,9 @@ OMNI_B200_API int omni_b200_rotary(const void *q, void *q_out, const void *k, vo
  * into the cache; omni_b200_cache_read_e2m1 writes what the cache stands for to k and v (F32,
  * BF16 or F16).  strides: HOST int64[6], (batch, head, token) of k and v in elements, columns
  * contiguous, at least head_dim and multiples of 16 bytes; NULL: contiguous.  k and v are
- * 16-byte aligned.  head_dim is a multiple of 8 in [8, 128].  Two sequences of a call must not
- * write to the same page. */
+ * 16-byte aligned.  head_dim is a multiple of 8 in [8, 128].  A page that a call
+ * writes to stands once in the table, and no other call that may overlap on the GPU writes to
+ * it: tokens share bytes. */
 typedef struct omni_b200_cache_e2m1 {
     void *data;
     const int32_t *table;

@@ -22,8 +22,8 @@
 // 248; the rest is kept short: a lane looks up the pages of 32 blocks at once, and the running maximum
 // is lazy (other lanes are asked only when some weight would be above 2^15).
 // 16 sequences of 65536 keys, 32/8 heads of 128: 198 us, 6.09 TB/s (copies alone 185, products
-// alone 176); 64 of up to 16384: 122 us, and 135 to 140 in a long run at the clock that the power
-// cap leaves.  248 instructions for a block of 16 tokens, issue slots 59 % busy, ALU 47 %.
+// alone 176); 64 of up to 16384: 123 us, and 133 to 136 in a long run at the 1.81 GHz that the
+// power cap leaves.  248 instructions for a block of 16 tokens, issue slots 59 % busy, ALU 47 %.
 //
 // Two ways to split the keys over CTAs:
 //   * few tiles of rows: a cluster takes each; its parts meet in distributed shared memory, in
@@ -66,9 +66,11 @@ struct TokensParams {
     int *err;
 };
 
-// CTAs on an SM: as many as their registers allow without spills in the loop.  (More for narrow
-// heads do not help eight rows: 64 x up to 16384 keys of 64, 81 us with four, 82 with five; 16
-// rows of 64 columns 134 with two, 119 with three.)
+// CTAs on an SM, by registers; shared memory allows no more of 24 rows either (90 KB at 128
+// columns).  Some instances spill all the same, bytes stored and loaded: at 128 columns the list
+// 28 and 32 with 8 rows, 108 and 120 with 24, the f16 cluster of 24 rows 18 and 24; at 96 the list
+// of 8 rows up to 12 and 48.  (More for narrow heads do not help eight rows: 64 x up to 16384
+// keys of 64, 81 us with four, 82 with five; 16 rows of 64 columns 134 with two, 119 with three.)
 constexpr int ctas_of_sm(int width, int rows) { return rows == 8 ? 4 : rows == 16 && width <= 64 ? 3 : 2; }
 
 template <int D, int NT> struct TokensShape {
@@ -1065,7 +1067,9 @@ Split split_in(const WindowE2m1Args &a, int rows_of_tile) {
     // out sequences that are shorter than kv_len, which is not known here, and gets a tenth for
     // that (clusters of several rounds even them out themselves).  Measured, cluster / list, 8 key heads of 128, one row of four heads: 1 x 8192 keys
     // 10.5 / 13.5, 1 x 32768 22.7 / 19.9, 1 x 65536 39.6 / 25.7, 16 x 4096 15.9 / 22.1, 64 x 2048
-    // 26.0 / 32.0, 64 x up to 4096 46.9 / 45.3, 64 x up to 16384 165 / 123.
+    // 26.0 / 32.0, 64 x up to 4096 46.9 / 45.3, 64 x up to 16384 165 / 123.  Narrow heads with many
+    // rows are underrated: 8 x 128 queries over 128 keys, 16 heads of 64, take 18.9 us here and 13.6
+    // by the prompts' kernel, heads of 32 15.6 and 12.3 (heads of 128 15.2 either way).
     const double sms = fmha_sm_count(), ctas = static_cast<double>(tiles) * s.parts;
     const double block = (s.rows == 8 ? 1.0 : s.rows == 16 ? 1.3 : 1.7) * (0.1 + 0.9 * cache_width(c.hd) / 128);
     const double rounds = std::max(1.0, ctas / most);

@@ -712,7 +712,8 @@ def cache_write_e2m1(k, v, cache, lengths, q_lengths=None, table=None, stream=No
 
     Sequence b holds lengths[b] tokens when the call is over; k and v are its last
     q_lengths[b] of them (None: T), from row 0 on.  table [B, pages of a sequence] names the
-    pages (None: page b is sequence b).  lengths, q_lengths and table are CUDA int32
+    pages (None: page b is sequence b); those that are written to stand in it once, and in no
+    other call's that may run at the same time.  lengths, q_lengths and table are CUDA int32
     tensors."""
     shape, dtype = k.shape, k.dtype
     code = _t.codes.get(dtype, F32)
