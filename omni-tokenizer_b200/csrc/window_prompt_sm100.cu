@@ -27,9 +27,10 @@
 // Exponentials are taken to base 2 with the scale folded in, statistics are fp32; a
 // row keeps a stale maximum until it grows by more than 2^8, so that P <= 2^8 (times
 // 2^lift: 2^7 for the 4-bit cache's f16 weights, which so lose 2^-32 of a row's largest
-// where they leave f16's normal range, not 2^-25) and O is rarely rescaled.  Steps take turns between two barriers where one side may
-// be a step ahead of the other (P written, products done): one barrier's parity would
-// mistake the step before the last for the one awaited.
+// where they leave f16's normal range, not 2^-25) and O is rarely rescaled.  Steps
+// take turns between two barriers where one side may be a step ahead of the other (P
+// written, products done): one barrier's parity would mistake the step before the
+// last for the one awaited.
 //
 // Tiles hold 64 columns (128 bytes, 128-byte swizzle) per row and chunk; columns
 // past head_dim and rows past the tensor are TMA's zero fill.  Rows of v past a
